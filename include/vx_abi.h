@@ -347,6 +347,61 @@ size_t vx_nms_workspace_bytes(int32_t num_boxes);
 int32_t vx_nms_bev(const float* d_boxes, int32_t num_boxes, float thresh, int32_t rotated, int64_t* d_keep,
                    int64_t* h_num_keep, void* d_workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Dense layer with its epilogue, y = act(x w^T + bias + residual), and its backward pass: the 1x1 convolutions and
+ * feed-forward layers of the cross-view attention block (det3d/models/necks/attention.py:36-41,77-84,127-146). The activation
+ * comes after the residual, as in vx_spconv_fwd's epilogue. Every pointer but the workspace is of `dtype`
+ * (VX_F32: exact three-plane split on the bf16 matrix pipe, as vx_spconv_* with six products; VX_BF16); accumulation fp32.
+ *
+ * vx_linear_fwd  d_x [m][k] rows ldx apart, d_weight [n][k] rows ldw apart, d_bias [n] or NULL, d_residual [m][n] rows ldr
+ *                apart or NULL -> d_y [m][n]; d_pre [m][n] or NULL receives the sum before the activation
+ * vx_linear_bwd  d_dy [m][n] rows lddy apart; d_saved [m][n]: d_y of VX_ACT_RELU, d_pre of VX_ACT_GELU / _SILU, NULL of
+ *                VX_ACT_NONE. g = dy * act'(saved) -> d_dpre [m][n] (required with an activation: it is also the residual's
+ *                gradient; without one that is d_dy itself); d_dx [m][k] = g w, d_dw [n][k] = g^T x, d_dbias [n] = column
+ *                sums of g; each of the three may be NULL
+ * Row strides are in elements, >= 0 (0 repeats a row), the last dimension is contiguous. m < 2^31; n, k <= 2^20. m = 0 gives
+ * zero parameter gradients. No atomics: bitwise reproducible. VX_ACT_GELU is the erf form.
+ * ------------------------------------------------------------------------------------------- */
+#define VX_ACT_NONE 0
+#define VX_ACT_RELU 1
+#define VX_ACT_GELU 2
+#define VX_ACT_SILU 3
+int32_t vx_linear_fwd(const void* d_x, int64_t ldx, const void* d_weight, int64_t ldw, const void* d_bias,
+                      const void* d_residual, int64_t ldr, int64_t m, int32_t n, int32_t k, int32_t act, void* d_y,
+                      void* d_pre, int32_t dtype, void* stream);
+size_t vx_linear_bwd_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t dtype);
+int32_t vx_linear_bwd(const void* d_dy, int64_t lddy, const void* d_x, int64_t ldx, const void* d_weight, int64_t ldw,
+                      const void* d_saved, int64_t m, int32_t n, int32_t k, int32_t act, void* d_dpre, void* d_dx,
+                      void* d_dw, void* d_dbias, int32_t dtype, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Attention softmax(scale q k^T) v and its backward pass, which recomputes the probabilities (cross-view attention:
+ * det3d/models/necks/attention.py:55-124; its two read-outs of one value map are query / key heads that share a value head).
+ *
+ * shape    HOST int64[8] = {batch, q_len, k_len, heads, k_heads, v_heads, dim, v_dim}; query head h reads key head
+ *          h / (heads / k_heads) and value head h / (heads / v_heads); dim <= VX_ATTN_MAX_DIM, v_dim <= VX_ATTN_MAX_VDIM
+ * strides  HOST int64[10] in elements, >= 0: q (batch, position, head), k (same), v (same), key mask (batch); the last
+ *          dimension of each is contiguous
+ * d_key_mask  one byte per (batch, key) or NULL: a key whose byte is 0 has no part in anything, whatever its rows hold (its
+ *          gradients are 0). A query that is left without keys, and k_len = 0, give zeros
+ * vx_attn_fwd  d_out [batch][q_len][heads][v_dim]; d_stats f32[batch * heads][q_len][2] or NULL: what the backward pass
+ *          needs (maximum of log2(e) * scale * score, 1 / sum)
+ * vx_attn_bwd  d_dout with its own strides HOST int64[3] (batch, position, head), d_out and d_stats of the forward pass ->
+ *          d_dq [batch][q_len][heads][dim], d_dk [batch][k_len][k_heads][dim], d_dv [batch][k_len][v_heads][v_dim]
+ * Statistics, probabilities and sums are fp32; matrix arithmetic as in vx_linear_*. No atomics: bitwise reproducible.
+ * ------------------------------------------------------------------------------------------- */
+#define VX_ATTN_MAX_DIM 192
+#define VX_ATTN_MAX_VDIM 384
+size_t vx_attn_fwd_workspace_bytes(const int64_t* shape, int32_t dtype);
+int32_t vx_attn_fwd(const void* d_q, const void* d_k, const void* d_v, const uint8_t* d_key_mask, const int64_t* shape,
+                    const int64_t* strides, float scale, void* d_out, float* d_stats, int32_t dtype, void* d_workspace,
+                    size_t workspace_bytes, void* stream);
+size_t vx_attn_bwd_workspace_bytes(const int64_t* shape, int32_t dtype);
+int32_t vx_attn_bwd(const void* d_dout, const int64_t* dout_strides, const void* d_q, const void* d_k, const void* d_v,
+                    const uint8_t* d_key_mask, const int64_t* shape, const int64_t* strides, const void* d_out,
+                    const float* d_stats, float scale, void* d_dq, void* d_dk, void* d_dv, int32_t dtype,
+                    void* d_workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,106 @@
+"""CPU: refusals of the attention and dense-layer entry points, at the C-ABI (no launch happens) and in Python."""
+import ctypes
+
+import pytest
+import torch
+
+from vista_amd import _lib, dense_tail, fused_tail, ops
+
+ERR_ARG, ERR_WS = -1, -3
+FAKE = ctypes.c_void_p(256)          # never read: every call below is refused before a launch
+
+
+def i64(*v):
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+def fwd(shape, strides=(1,) * 10, q=FAKE, out=FAKE, dtype=0, ws=FAKE, wsb=1 << 40):
+    return _lib.lib().vx_attn_fwd(q, FAKE, FAKE, None, i64(*shape) if shape else None, i64(*strides) if strides else None, 1.0, out,
+                                  None, dtype, ws, wsb, None)
+
+
+GOOD = (2, 100, 50, 4, 2, 1, 64, 128)
+
+
+@pytest.mark.parametrize("at,value", [(0, -1), (1, -1), (2, -1), (1, 1 << 30), (2, 1 << 30), (3, 0), (4, 3), (5, 8), (4, 0), (6, 0),
+                                      (6, 193), (7, 0), (7, 385), (0, 1 << 24), (3, 1 << 16)])
+def test_attention_refuses_shapes(at, value):
+    bad = list(GOOD)
+    bad[at] = value
+    assert fwd(bad) == ERR_ARG
+    assert b"attn" in _lib.lib().vx_last_error()
+    lib = _lib.lib()
+    assert lib.vx_attn_fwd_workspace_bytes(i64(*bad), 0) == 0 and lib.vx_attn_bwd_workspace_bytes(i64(*bad), 0) == 0
+    rc = lib.vx_attn_bwd(FAKE, i64(1, 1, 1), FAKE, FAKE, FAKE, None, i64(*bad), i64(*(1,) * 10), FAKE, FAKE, 1.0, FAKE, FAKE, FAKE, 0,
+                         FAKE, 1 << 40, None)
+    assert rc == ERR_ARG
+
+
+def test_attention_refuses_arguments():
+    lib = _lib.lib()
+    assert fwd(None) == ERR_ARG and fwd(GOOD, strides=None) == ERR_ARG
+    assert fwd(GOOD, strides=(1,) * 9 + (-1,)) == ERR_ARG
+    assert fwd(GOOD, q=None) == ERR_ARG and fwd(GOOD, out=None) == ERR_ARG and fwd(GOOD, dtype=2) == ERR_ARG
+    few = (1, 1, 4096, 1, 1, 1, 64, 64)                    # one query: the keys are split, partial sums need room
+    need = lib.vx_attn_fwd_workspace_bytes(i64(*few), 0)
+    assert need > 0 and fwd(few, wsb=need - 1) == ERR_WS and fwd(few, ws=None, wsb=0) == ERR_WS
+    need = lib.vx_attn_bwd_workspace_bytes(i64(*GOOD), 0)
+    bwd = lambda ws, n, st: lib.vx_attn_bwd(FAKE, i64(*st), FAKE, FAKE, FAKE, None, i64(*GOOD), i64(*(1,) * 10), FAKE, FAKE, 1.0,  # noqa: E731
+                                            FAKE, FAKE, FAKE, 0, ws, n, None)
+    assert need > 0 and bwd(FAKE, need - 1, (1, 1, 1)) == ERR_WS and bwd(None, need, (1, 1, 1)) == ERR_WS
+    assert bwd(FAKE, need, (1, -1, 1)) == ERR_ARG
+
+
+def test_attention_workspace_is_bounded():
+    """Probabilities and score gradients of any number of queries stay within 256 MiB + what single tiles need."""
+    lib = _lib.lib()
+    for sq in (1000, 25600, 400000):
+        slabs_and_rows = 2 * (-(-sq // 64) + 1) * 1920 * 576 * 4
+        assert lib.vx_attn_bwd_workspace_bytes(i64(1, sq, 1920, 2, 2, 1, 192, 384), 0) < (300 << 20) + slabs_and_rows
+    for n in (0, 1):                                       # nothing to do: no workspace, no launch
+        assert lib.vx_attn_fwd_workspace_bytes(i64(n, 1 - n, 8, 1, 1, 1, 8, 8), 0) in (0, 0)
+
+
+def test_empty_calls_launch_nothing():
+    lib = _lib.lib()
+    assert fwd((0, 5, 5, 1, 1, 1, 8, 8)) == 0 and fwd((2, 0, 5, 1, 1, 1, 8, 8)) == 0
+    assert lib.vx_linear_fwd(None, 8, None, 8, None, None, 0, 0, 4, 8, 0, None, None, 0, None) == 0
+
+
+def test_linear_refuses_arguments():
+    lib = _lib.lib()
+    f = lambda x=FAKE, ldx=8, m=3, n=4, k=8, act=0, dtype=0: lib.vx_linear_fwd(x, ldx, FAKE, 8, None, None, 0, m, n, k, act, FAKE,  # noqa: E731
+                                                                              None, dtype, None)
+    for kw in (dict(x=None), dict(ldx=-1), dict(m=-1), dict(m=1 << 31), dict(n=0), dict(k=0), dict(n=(1 << 20) + 1), dict(act=4),
+               dict(act=-1), dict(dtype=2)):
+        assert f(**kw) == ERR_ARG, kw
+    need = lib.vx_linear_bwd_workspace_bytes(3, 4, 8, 0)
+    b = lambda ws=FAKE, n=need, act=0, saved=None, dpre=None, ld=4: lib.vx_linear_bwd(FAKE, ld, FAKE, 8, FAKE, 8, saved, 3, 4, 8,  # noqa: E731
+                                                                                      act, dpre, FAKE, FAKE, FAKE, 0, ws, n, None)
+    assert need > 0 and b(n=need - 1) == ERR_WS and b(ws=None) == ERR_WS and b(ld=-1) == ERR_ARG
+    assert b(act=1) == ERR_ARG and b(act=1, saved=FAKE) == ERR_ARG and b(act=2, dpre=FAKE) == ERR_ARG
+
+
+def test_python_refuses_cpu_tensors():
+    t = torch.zeros
+    with pytest.raises(_lib.VxError):
+        fused_tail.attention(t(1, 2, 1, 4), t(1, 2, 1, 4), t(1, 2, 1, 4))
+    with pytest.raises(_lib.VxError):
+        fused_tail.linear_act(t(2, 3), t(4, 3))
+    with pytest.raises(_lib.VxError):
+        ops.linear_bwd(t(2, 4), t(2, 3), t(4, 3))
+    with pytest.raises(ValueError):
+        fused_tail.linear_act(t(2, 5, 3), t(4, 3), None, t(2, 4))
+
+
+def test_fuse_cross_attention_keeps_keys_and_parameters():
+    m = dense_tail.Cross_Attention_Decouple(16, 16, 16, 2, (8, 8), (4, 4), (8, 4), (4, 4), 24)
+    sd = {k: v.data_ptr() for k, v in m.state_dict().items()}
+    out = fused_tail.fuse_cross_attention(m)
+    assert out is m and {k: v.data_ptr() for k, v in m.state_dict().items()} == sd
+    kinds = [type(c).__name__ for c in m.modules()]
+    assert kinds.count("FusedConvAttention") == 1 and kinds.count("FusedFeedForward") == 2
+    fused_tail.fuse_cross_attention(m)                      # again: nothing left to swap
+    assert [type(c).__name__ for c in m.modules()] == kinds
+    ffn = fused_tail.fuse_cross_attention(dense_tail.FeedFowardLayer(8, 16).eval())
+    assert isinstance(ffn, fused_tail.FusedFeedForward) and not ffn.training

@@ -1,0 +1,551 @@
+"""GPU tests of the attention and dense-layer kernels (vx_attn.hip, vx_linear.hip, vista_amd/fused_tail.py) against plain
+float64 evaluations of the same formulas.
+
+Tolerances are elementwise bounds worked out from the arithmetic, not fitted. u = 2^-24.
+  product     sum_k a_k b_k over K terms in fp32 accumulators. fp32 operands: three planes, h the top 16 bits of x, so
+              |m| < 2^-7 |x| and |l| < 2^-15 |x|; the dropped products m l, l m, l l are below 2^-21 |a||b|. 6 ceil(K/32) matrix
+              instructions (one for bf16) each add once to the accumulator and add up 32 products inside (5 levels), every
+              addition off by at most 2^-23 of the running magnitude. Error <= gamma(K) sum |a||b|,
+              gamma = [2^-21 +] 2^-23 (n + 5 n / ceil(K/32)), n = instructions of one element; a sum cut into slabs adds one
+              addition a slab, covered by 2^-23 * 64.
+  output      rounded once: finfo.eps / 2 of the value.
+  attention   a score is off by ds = scale gamma(D) sum |q||k| + 2^-22 |s|; p = exp(s - m) / l is off by 2 max ds + 2^-20
+              relative (statistics, exp2 and the division), for bf16 by another 2^-8 where it is a matrix operand; the rest
+              is products. Gradients carry these through their formulas, with |.| in the place of every factor.
+"""
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    return torch.device("cuda:0")
+
+
+def gamma(k, dtype):
+    steps = max(1, -(-k // 32))
+    n = steps * (6 if dtype == F32 else 1)
+    return (2.0 ** -21 if dtype == F32 else 0.0) + 2.0 ** -23 * (n + 5 * n / steps + 64)
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def within(got, want, bound, what):
+    d = (got.double() - want).abs()
+    assert got.shape == want.shape, what
+    assert torch.isfinite(got).all(), what
+    worst = (d / (bound + 1e-300)).max().item() if d.numel() else 0.0
+    assert worst <= 1.0, (what, worst, d.max().item())
+
+
+# ------------------------------------------------------------------------------------------------ dense layer
+def act64(a, act):
+    f = torch.nn.functional
+    return {"none": lambda t: t, "relu": torch.relu, "gelu": f.gelu, "silu": f.silu}[act](a)
+
+
+def slope64(a, act):
+    if act == "none":
+        return torch.ones_like(a)
+    if act == "relu":
+        return (a > 0).double()
+    if act == "gelu":
+        return torch.special.ndtr(a) + a * torch.exp(-a * a / 2) / math.sqrt(2 * math.pi)
+    s = torch.sigmoid(a)
+    return s * (1 + a * (1 - s))
+
+
+def make_linear(m, k, n, dtype, dev, seed, bias, residual):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g, device=dev)  # noqa: E731
+    return (r(m, k).to(dtype), (r(n, k) * k ** -0.5).to(dtype), (r(n) * 0.3).to(dtype) if bias else None,
+            r(m, n).to(dtype) if residual else None, r(m, n).to(dtype))
+
+
+LINEAR = [(1, 1, 1), (1, 384, 512), (7, 384, 512), (63, 33, 65), (64, 64, 64), (65, 31, 129), (130, 7, 3), (257, 100, 255),
+          (1600, 384, 384), (999, 511, 77), (16385, 64, 300), (20000, 72, 130)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("act,bias,residual", [("none", False, False), ("none", True, True), ("relu", True, False),
+                                               ("relu", True, True), ("gelu", True, True), ("silu", False, True)])
+@pytest.mark.parametrize("m,k,n", LINEAR)
+def test_linear_forward(m, k, n, act, bias, residual, dtype, dev):
+    from vista_amd import ops
+    x, w, b, r, _ = make_linear(m, k, n, dtype, dev, m + 7 * k + n, bias, residual)
+    y, pre = ops.linear_fwd(x, w, b, r, act, want_pre=True)
+    a = x.double() @ w.double().t()
+    size = x.double().abs() @ w.double().abs().t()
+    for t in (b, r):
+        if t is not None:
+            a, size = a + t.double(), size + t.double().abs()
+    off = gamma(k, dtype) * size
+    within(pre, a, off + half_step(dtype) * (a.abs() + off) + 1e-38, "pre")
+    want = act64(a, act)
+    # slopes of all four are at most 1.13; the activation itself is good to 2^-21 of its argument
+    off = 1.13 * off + 2.0 ** -21 * a.abs()
+    within(y, want, off + half_step(dtype) * (want.abs() + off) + 1e-38, "y")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("m,k,n", LINEAR)
+def test_linear_backward(m, k, n, act, dtype, dev):
+    from vista_amd import ops
+    x, w, _, s, dy = make_linear(m, k, n, dtype, dev, 3 * m + k + n, False, True)
+    saved = {"none": None, "relu": s.clamp(min=0)}.get(act, s)
+    dx, dw, db, dpre = ops.linear_bwd(dy, x, w, act, saved)
+    g = dy.double() * (slope64(s.double(), act) if act != "none" else 1.0)
+    # the slope is good to 2^-20 (exp and erf of a few), g is rounded to the tensors' type
+    goff = (2.0 ** -20 if act in ("gelu", "silu") else 0.0) * dy.double().abs() * (1 + s.double().abs())
+    goff = goff + (half_step(dtype) * g.abs() if act in ("gelu", "silu") else 0.0)
+    within(dpre, g, goff + 1e-38, "dpre")
+    wd, xd = w.double().abs(), x.double().abs()
+    want = g @ w.double()
+    off = gamma(n, dtype) * (g.abs() @ wd) + goff @ wd
+    within(dx, want, off + half_step(dtype) * (want.abs() + off) + 1e-38, "dx")
+    want = g.t() @ x.double()
+    off = gamma(m, dtype) * (g.abs().t() @ xd) + goff.t() @ xd
+    within(dw, want, off + half_step(dtype) * (want.abs() + off) + 1e-38, "dw")
+    want = g.sum(0)
+    # a thread's column sum runs over at most m / 8 rows one after the other, then over lanes and chunks
+    off = 2.0 ** -24 * (min(m, 8192) / 8 + 1100) * g.abs().sum(0) + goff.sum(0)
+    within(db, want, off + half_step(dtype) * (want.abs() + off) + 1e-38, "dbias")
+
+
+def test_linear_reads_strides_in_place(dev):
+    from vista_amd import ops
+    g = torch.Generator(device=dev).manual_seed(4)
+    wide = torch.randn((300, 2, 96), generator=g, device=dev)
+    big_w = torch.randn((70, 200), generator=g, device=dev)
+    row = torch.randn((1, 70), generator=g, device=dev)
+    x, w, r = wide[:, 1], big_w[:, 3:99], row.expand(300, 70)          # row strides 192, 200 and 0, bases off 16 bytes
+    want, _ = ops.linear_fwd(x.contiguous(), w.contiguous(), None, r.contiguous())
+    assert torch.equal(ops.linear_fwd(x, w, None, r)[0], want)
+    assert torch.equal(ops.linear_fwd(x.t().contiguous().t(), w, None, r)[0], want)       # last dimension strided: copied
+    dy = torch.randn((300, 140), generator=g, device=dev)[:, 1::2]
+    one, two = ops.linear_bwd(dy, x, w), ops.linear_bwd(dy.contiguous(), x.contiguous(), w.contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+
+
+def test_linear_without_rows(dev):
+    from vista_amd import ops
+    w = torch.randn(5, 9, device=dev)
+    y, _ = ops.linear_fwd(torch.empty(0, 9, device=dev), w)
+    assert y.shape == (0, 5)
+    dx, dw, db, _ = ops.linear_bwd(torch.empty(0, 5, device=dev), torch.empty(0, 9, device=dev), w)
+    assert dx.shape == (0, 9) and not dw.any() and not db.any() and dw.shape == (5, 9)
+
+
+def test_linear_nan_and_inf_stay_in_their_row(dev):
+    from vista_amd import ops
+    x, w, b, _, _ = make_linear(130, 64, 96, F32, dev, 1, True, False)
+    clean, _ = ops.linear_fwd(x, w, b, act="relu")
+    x[17, 3], x[99, 0] = math.nan, math.inf
+    y, _ = ops.linear_fwd(x, w, b, act="relu")
+    keep = torch.ones(130, dtype=torch.bool, device=dev)
+    keep[17] = keep[99] = False
+    assert torch.equal(y[keep], clean[keep]) and torch.isnan(y[17]).all()
+
+
+# ------------------------------------------------------------------------------------------------ attention
+# batch, q_len, k_len, heads, k_heads, v_heads, dim, v_dim
+ATTN = [(1, 1, 1, 1, 1, 1, 1, 1), (1, 1, 480, 2, 2, 1, 192, 384), (2, 65, 33, 4, 2, 1, 37, 53), (1, 130, 100, 2, 2, 1, 24, 48),
+        (2, 77, 129, 3, 1, 3, 96, 192), (1, 200, 65, 2, 2, 2, 128, 128), (3, 17, 64, 6, 3, 2, 64, 64), (2, 40, 31, 2, 1, 2, 33, 100),
+        (1, 64, 32, 1, 1, 1, 32, 64), (2, 150, 300, 2, 2, 1, 192, 384), (1, 3, 5000, 2, 1, 1, 48, 48), (5, 1, 7, 3, 3, 1, 130, 257)]
+# enough query tiles for the 128-query form, in the smallest and the largest tile
+ATTN_WIDE = [(2, 2048, 70, 8, 8, 8, 16, 24), (4, 4096, 40, 2, 2, 1, 192, 384), (2, 2050, 65, 8, 2, 4, 96, 130)]
+MASKS = ["none", "some", "blank", "all"]
+
+
+def make_attn(shape, dtype, dev, seed, mask, poison=False):
+    b, sq, sk, h, hk, hv, d, dv = shape
+    g = torch.Generator(device=dev).manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g, device=dev).to(dtype)  # noqa: E731
+    q, k, v, do = r(b, sq, h, d), r(b, sk, hk, d), r(b, sk, hv, dv), r(b, sq, h, dv)
+    km = None
+    if mask != "none":
+        km = torch.rand((b, sk), generator=g, device=dev) > 0.4
+        if mask == "blank":
+            km[0] = False
+        elif mask == "all":
+            km[:] = False
+        if poison:                      # what masked rows hold must not matter
+            bad = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(dtype).max], device=dev, dtype=dtype)
+            where = ~km
+            k[where] = bad[torch.randint(4, (int(where.sum()), hk, d), generator=g, device=dev)]
+            v[where] = bad[torch.randint(4, (int(where.sum()), hv, dv), generator=g, device=dev)]
+    return q, k, v, km, do
+
+
+def attn_reference(q, k, v, km, do, scale=None):
+    """float64 values and elementwise bounds of out, dq, dk, dv."""
+    dt = q.dtype
+    b, sq, h, d = q.shape
+    sk, hk, hv, dv = k.shape[1], k.shape[2], v.shape[2], v.shape[3]
+    scale = d ** -0.5 if scale is None else scale
+    gk, gv = h // hk, h // hv
+    live = torch.ones((b, sk), dtype=torch.bool, device=q.device) if km is None else km
+    z = lambda t: t.double().masked_fill(~live[:, :, None, None], 0.0)  # noqa: E731
+    Q, G = q.double().transpose(1, 2), do.double().transpose(1, 2)
+    K, V = z(k).transpose(1, 2).repeat_interleave(gk, 1), z(v).transpose(1, 2).repeat_interleave(gv, 1)
+    L = live[:, None, None, :]
+    s = (scale * (Q @ K.transpose(2, 3))).masked_fill(~L, -math.inf)
+    m = s.amax(-1, keepdim=True).clamp(min=-1e300) if sk else s.new_zeros((b, h, sq, 1))
+    p = torch.exp(s - m)
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+    out = p @ V
+    ds_ = abs(scale) * gamma(d, dt) * (Q.abs() @ K.abs().transpose(2, 3)) + 2.0 ** -22 * s.masked_fill(~L, 0.0).abs()
+    ds_ = ds_.masked_fill(~L, 0.0)
+    rel = 2 * (ds_.amax(-1, keepdim=True) if sk else s.new_zeros((b, h, sq, 1))) + 2.0 ** -20
+    r16 = 2.0 ** -8 if dt == BF16 else 0.0
+    hs = half_step(dt)
+    done = lambda val, off: off + hs * (val.abs() + off) + 1e-38  # noqa: E731
+    pv = p @ V.abs()
+    b_out = done(out, (rel * 1.01 + r16 + gamma(sk, dt)) * pv)
+    dV = p.transpose(2, 3) @ G
+    b_dV = (p * (rel * 1.01 + r16 + gamma(sq, dt))).transpose(2, 3) @ G.abs()
+    dP = G @ V.transpose(2, 3)
+    delta = (G * out).sum(-1, keepdim=True)
+    dS = scale * p * (dP - delta)
+    b_dP = gamma(dv, dt) * (G.abs() @ V.abs().transpose(2, 3))
+    b_delta = (G.abs() * b_out).sum(-1, keepdim=True) + 2.0 ** -24 * 16 * (G.abs() * out.abs()).sum(-1, keepdim=True)
+    e_dS = abs(scale) * p * ((rel * 1.01 + 2.0 ** -22) * (dP - delta).abs() + b_dP + b_delta)
+    e_dS = e_dS + r16 * (dS.abs() + e_dS)
+    dQ, dK = dS @ K, dS.transpose(2, 3) @ Q
+    b_dQ = e_dS @ K.abs() + gamma(sk, dt) * (dS.abs() @ K.abs())
+    b_dK = e_dS.transpose(2, 3) @ Q.abs() + gamma(sq, dt) * (dS.abs().transpose(2, 3) @ Q.abs())
+    fold = lambda t, g: t.view(b, h // g, g, *t.shape[2:]).sum(2).transpose(1, 2)  # noqa: E731
+    dK, b_dK, dV, b_dV = fold(dK, gk), fold(b_dK, gk), fold(dV, gv), fold(b_dV, gv)
+    t = lambda x: x.transpose(1, 2)  # noqa: E731
+    return {"out": (t(out), t(b_out)), "dq": (t(dQ), done(t(dQ), t(b_dQ))), "dk": (dK, done(dK, b_dK)), "dv": (dV, done(dV, b_dV))}
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("shape", ATTN)
+def test_attention_and_gradients(shape, mask, dtype, dev):
+    from vista_amd import ops
+    q, k, v, km, do = make_attn(shape, dtype, dev, sum(shape), mask, poison=True)
+    ref = attn_reference(q, k, v, km, do)
+    out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    within(out, *ref["out"], "out")
+    dq, dk, dv = ops.attn_bwd(do, q, k, v, out, stats, km)
+    within(dq, *ref["dq"], "dq")
+    within(dk, *ref["dk"], "dk")
+    within(dv, *ref["dv"], "dv")
+    if km is not None:
+        assert not dk[~km].any() and not dv[~km].any()
+        assert not out[~km.any(1)].any() and not dq[~km.any(1)].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", ATTN_WIDE)
+def test_attention_many_queries(shape, dtype, dev):
+    from vista_amd import ops
+    q, k, v, km, do = make_attn(shape, dtype, dev, 5, "blank", poison=True)
+    ref = attn_reference(q, k, v, km, do)
+    out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    within(out, *ref["out"], "out")
+    for name, got in zip(("dq", "dk", "dv"), ops.attn_bwd(do, q, k, v, out, stats, km)):
+        within(got, *ref[name], name)
+
+
+def test_attention_gradients_in_chunks_of_queries(dev):
+    """Probabilities of 2 x 20000 x 2000 pairs do not fit the workspace at once: several chunks, one slab each and more."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((1, 20000, 2000, 2, 2, 1, 16, 24), F32, dev, 6, "some", poison=True)
+    ref = attn_reference(q, k, v, km, do)
+    out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    within(out, *ref["out"], "out")
+    for name, got in zip(("dq", "dk", "dv"), ops.attn_bwd(do, q, k, v, out, stats, km)):
+        within(got, *ref[name], name)
+
+
+def test_attention_of_large_scores(dev):
+    """Scores of some hundreds: the running maximum keeps every exponent in range; scale 0 and below zero are scales too."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((2, 70, 90, 2, 2, 1, 64, 64), F32, dev, 9, "some")
+    for scale in (40.0, -3.0, 0.0):
+        ref = attn_reference(q, k, v, km, do, scale)
+        out, stats = ops.attn_fwd(q, k, v, km, scale, want_stats=True)
+        within(out, *ref["out"], "out")
+        for name, got in zip(("dq", "dk", "dv"), ops.attn_bwd(do, q, k, v, out, stats, km, scale)):
+            within(got, *ref[name], name)
+
+
+def test_attention_without_keys_or_queries(dev):
+    from vista_amd import ops
+    q, k, v = (torch.randn(2, n, 2, 16, device=dev) for n in (5, 0, 0))
+    out, stats = ops.attn_fwd(q, k, v, want_stats=True)
+    assert out.shape == (2, 5, 2, 16) and not out.any()
+    dq, dk, dv = ops.attn_bwd(torch.ones_like(out), q, k, v, out, stats)
+    assert not dq.any() and dk.shape == k.shape and dv.shape == v.shape
+    q, k, v = (torch.randn(2, n, 2, 16, device=dev) for n in (0, 5, 5))
+    out, stats = ops.attn_fwd(q, k, v, want_stats=True)
+    assert out.shape == (2, 0, 2, 16)
+    dq, dk, dv = ops.attn_bwd(out, q, k, v, out, stats)
+    assert dq.shape == q.shape and not dk.any() and not dv.any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_reads_strides_in_place(dtype, dev):
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((2, 70, 50, 4, 2, 2, 24, 40), dtype, dev, 2, "some")
+    want, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    grads = ops.attn_bwd(do, q, k, v, want, stats, km)
+    heads_first = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    kv = torch.cat([torch.zeros_like(k[..., :1]), k, v], -1)[..., 1:]             # one buffer, rows off 16 bytes
+    mask_rows = torch.stack([~km, km], 1)[:, 1]
+    q2, k2, v2, do2 = heads_first(q), kv[..., :24], kv[..., 24:], heads_first(do)
+    out, st = ops.attn_fwd(q2, k2, v2, mask_rows, want_stats=True)
+    assert torch.equal(out, want) and torch.equal(st, stats)
+    for a, b in zip(ops.attn_bwd(do2, q2, k2, v2, out, st, mask_rows), grads):
+        assert torch.equal(a, b)
+    one = torch.ones((1, 1, 1, 1), dtype=dtype, device=dev).expand_as(do)         # a sum's gradient: all strides 0
+    for a, b in zip(ops.attn_bwd(one, q, k, v, want, stats, km), ops.attn_bwd(one.contiguous(), q, k, v, want, stats, km)):
+        assert torch.equal(a, b)
+
+
+def test_attention_offsets_past_32_bits(dev):
+    """Two batches of keys and values whose elements lie more than 2^31 apart."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((2, 40, 50, 2, 2, 1, 32, 48), BF16, dev, 3, "some")
+    far = (1 << 31) + 64
+    buf = torch.empty(far + 50 * 2 * 32 + 50 * 48, dtype=BF16, device=dev)
+    k2 = buf.as_strided((2, 50, 2, 32), (far, 64, 32, 1))
+    v2 = buf.as_strided((2, 50, 1, 48), (far, 48, 48, 1), storage_offset=50 * 64)
+    k2.copy_(k)
+    v2.copy_(v)
+    out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    out2, stats2 = ops.attn_fwd(q, k2, v2, km, want_stats=True)
+    assert torch.equal(out, out2)
+    for a, b in zip(ops.attn_bwd(do, q, k, v, out, stats, km), ops.attn_bwd(do, q, k2, v2, out2, stats2, km)):
+        assert torch.equal(a, b)
+
+
+def test_same_inputs_same_bits(dev):
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((2, 300, 200, 2, 2, 1, 192, 384), F32, dev, 8, "some")
+    runs = []
+    for _ in range(3):
+        out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+        runs.append((out, *ops.attn_bwd(do, q, k, v, out, stats, km)))
+    assert all(torch.equal(a, b) for r in runs[1:] for a, b in zip(runs[0], r))
+    x, w, _, s, dy = make_linear(5000, 130, 70, F32, dev, 1, False, True)
+    a, b = ops.linear_bwd(dy, x, w, "gelu", s), ops.linear_bwd(dy, x, w, "gelu", s)
+    assert all(torch.equal(i, j) for i, j in zip(a, b))
+
+
+# ------------------------------------------------------------------------------------------------ autograd, streams, graphs
+def test_gradients_against_differences(dev):
+    """<gradient, direction> of attention and of a gelu layer against central differences of the float64 formulas: the
+    difference quotient of a smooth function is off by h^2 / 6 of its third derivative (some 1e-7 here), the gradients by
+    1e-5 of their size at most."""
+    from vista_amd.fused_tail import attention, linear_act
+    q, k, v, km, do = make_attn((1, 9, 12, 2, 1, 2, 8, 8), F32, dev, 11, "some")
+    x, w, b, r, dy = make_linear(9, 16, 12, F32, dev, 12, True, True)
+
+    def attn64(q, k, v):
+        K, V = k.transpose(1, 2).repeat_interleave(2, 1), v.transpose(1, 2)
+        s = (q.transpose(1, 2) @ K.transpose(2, 3) * 8 ** -0.5).masked_fill(~km[:, None, None], -math.inf)
+        return ((torch.softmax(s, -1) @ V).transpose(1, 2) * do.double()).sum()
+
+    def lin64(x, w, b, r):
+        return (torch.nn.functional.gelu(x @ w.t() + b + r) * dy.double()).sum()
+
+    for args, f, g in (((q, k, v), attn64, lambda *a: (attention(*a, key_mask=km) * do).sum()),
+                       ((x, w, b, r), lin64, lambda *a: (linear_act(*a, act="gelu") * dy).sum())):
+        leaves = [a.clone().requires_grad_(True) for a in args]
+        grads = torch.autograd.grad(g(*leaves), leaves)
+        for i, grad in enumerate(grads):
+            dirn = torch.randn(args[i].shape, dtype=torch.float64, device=dev)
+            h = 1e-4
+            at = [a.double() for a in args]
+            up, down = list(at), list(at)
+            up[i], down[i] = at[i] + h * dirn, at[i] - h * dirn
+            want = (f(*up) - f(*down)).item() / (2 * h)
+            size = (grad.double().norm() * dirn.norm()).item()
+            assert abs((grad.double() * dirn).sum().item() - want) <= 1e-5 * size + 1e-6, i
+
+
+def test_autograd_returns_what_is_asked(dev):
+    from vista_amd.fused_tail import attention, linear_act
+    q, k, v, km, do = make_attn((2, 20, 30, 2, 2, 1, 16, 32), F32, dev, 1, "some")
+    k.requires_grad_(True)
+    out = attention(q, k, v, km)
+    out.backward(do)
+    assert k.grad is not None and q.grad is None
+    with torch.no_grad():
+        assert not attention(q, k, v, km).requires_grad
+    x, w, b, r, dy = make_linear(6, 8, 10, F32, dev, 1, True, True)
+    x3, r3 = x.view(2, 3, 8), r.view(2, 3, 10)
+    w.requires_grad_(True)
+    r3.requires_grad_(True)
+    y = linear_act(x3, w, b, r3, "silu")
+    assert y.shape == (2, 3, 10)
+    y.backward(dy.view(2, 3, 10))
+    assert w.grad.shape == w.shape and r3.grad.shape == r3.shape and b.grad is None
+    out = attention(q, k, v, km)
+    (gk,) = torch.autograd.grad(out.sum(), k, create_graph=True)
+    with pytest.raises(RuntimeError):                      # once differentiable
+        gk.sum().backward()
+
+
+def test_on_another_stream(dev):
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((2, 200, 100, 2, 2, 1, 48, 96), F32, dev, 1, "some")
+    want, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    grads = ops.attn_bwd(do, q, k, v, want, stats, km)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out, st = ops.attn_fwd(q, k, v, km, want_stats=True)
+        got = ops.attn_bwd(do, q, k, v, out, st, km)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(got, grads))
+
+
+def test_captured_and_replayed(dev):
+    """Forward and backward calls in one graph, another graph of the same calls beside it, replays on new inputs between eager work."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((2, 130, 70, 2, 2, 1, 48, 96), F32, dev, 1, "some")
+    x, w, b, r, dy = make_linear(700, 64, 96, F32, dev, 2, True, True)
+
+    def step():
+        out, st = ops.attn_fwd(q, k, v, km, want_stats=True)
+        y, pre = ops.linear_fwd(x, w, b, r, "gelu", want_pre=True)
+        return (out, *ops.attn_bwd(do, q, k, v, out, st, km), y, *ops.linear_bwd(dy, x, w, "gelu", pre))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            held = step()
+        graphs.append((gr, held))
+    gen = torch.Generator(device=dev).manual_seed(77)
+    for i in range(4):
+        for t in (q, k, v, do, x, dy):
+            t.copy_(torch.randn(t.shape, generator=gen, device=dev))
+        want = [t.clone() for t in step()]
+        for gr, held in graphs:
+            gr.replay()
+        torch.cuda.synchronize()
+        for gr, held in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(held, want)), i
+
+
+# ------------------------------------------------------------------------------------------------ the block
+def block(dev, heads=1):
+    from vista_amd import dense_tail as dt
+    torch.manual_seed(3)
+    m = dt.Cross_Attention_Decouple(48, 48, 48, heads, (40, 40), (10, 10), (40, 12), (10, 12), 64)
+    bev, rv = torch.randn(3, 48, 40, 40), torch.randn(3, 48, 40, 12)
+    return m, bev, rv
+
+
+@pytest.mark.parametrize("heads", [1, 2])
+def test_fused_block_runs_the_operators_together(heads, dev):
+    """The neck with its attention block on the kernels against the stock module in float64, outputs and every gradient: 1e-4 of
+    each tensor's largest value, the bar of this path's fp32 parity."""
+    from vista_amd.fused_tail import FusedConvAttention, FusedFeedForward, fuse_cross_attention
+    m, bev, rv = block(dev, heads)
+    import copy
+    stock = copy.deepcopy(m).double()
+    keys = list(m.state_dict())
+    fused = fuse_cross_attention(m).to(dev)
+    assert list(fused.state_dict()) == keys
+    kinds = [type(c) for c in fused.modules()]
+    assert kinds.count(FusedConvAttention) == 1 and kinds.count(FusedFeedForward) == 2
+    bev64, rv64 = bev.double().requires_grad_(True), rv.double().requires_grad_(True)
+    bevg, rvg = bev.to(dev).requires_grad_(True), rv.to(dev).requires_grad_(True)
+    want, _ = stock((bev64, rv64), need_maps=False)
+    got, maps = fused((bevg, rvg), need_maps=False)
+    assert maps == [None, None]
+    cot = [torch.randn(t.shape, dtype=torch.float64, generator=torch.Generator().manual_seed(i)) for i, t in enumerate(want)]
+    sum((w * c).sum() for w, c in zip(want, cot)).backward()
+    sum((g * c.float().to(dev)).sum() for g, c in zip(got, cot)).backward()
+
+    def close(a, b, what):
+        err = (a.detach().cpu().double() - b.detach()).abs().max().item() / max(b.detach().abs().max().item(), 1e-12)
+        assert err <= 1e-4, (what, err)
+
+    for g, w in zip(got, want):
+        close(g, w, "out")
+    close(bevg.grad, bev64.grad, "bev")
+    close(rvg.grad, rv64.grad, "rv")
+    for (name, a), (_, b) in zip(fused.named_parameters(), stock.named_parameters()):
+        if ".k_" in name and name.endswith("bias"):        # softmax is blind to a shift of a query's scores: exactly zero
+            assert a.grad.abs().max().item() <= 1e-4 * b.grad.abs().max().clamp(min=1.0).item(), name
+        else:
+            close(a.grad, b.grad, name)
+
+
+def test_fused_block_with_maps_runs_the_stock_path(dev):
+    from vista_amd.fused_tail import fuse_cross_attention
+    m, bev, rv = block(dev)
+    m, bev, rv = m.to(dev).eval(), bev.to(dev), rv.to(dev)
+    with torch.no_grad():
+        want, maps = m((bev, rv))
+        layer = m.cross_atten.cross_atten
+        fuse_cross_attention(m)
+        blk = m.cross_atten.cross_atten
+        assert blk is not layer and blk.q_sem_conv is layer.q_sem_conv
+        q = torch.randn(2, 48, 5, 5, device=dev)
+        kv = torch.randn(2, 48, 5, 3, device=dev)
+        a, ma = layer(q, kv, kv)
+        b, mb = blk(q, kv, kv)
+        assert all(torch.equal(x, y) for x, y in zip(a + ma, b + mb))
+        mask = torch.ones(2, 15, dtype=torch.bool, device=dev)
+        c, none = blk(q, kv, kv, need_maps=False, key_mask=mask)
+        assert none == [None, None] and torch.equal(c[0], blk(q, kv, kv, need_maps=False)[0][0])
+        with pytest.raises(ValueError):
+            blk(q, kv, kv, key_mask=mask)
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_refusals(dev):
+    from vista_amd import ops
+    from vista_amd._lib import VxError
+    z = lambda *s, dtype=F32, device=dev: torch.zeros(s, dtype=dtype, device=device)  # noqa: E731
+    q, k, v = z(2, 3, 4, 8), z(2, 5, 2, 8), z(2, 5, 1, 16)
+    bad = [dict(q=z(2, 3, 4, 8, dtype=torch.float16)), dict(k=z(2, 5, 2, 8, dtype=BF16)), dict(k=z(2, 5, 3, 8)), dict(k=z(2, 5, 2, 9)),
+           dict(k=z(2, 6, 2, 8)), dict(k=z(1, 5, 2, 8)), dict(q=z(2, 3, 8)), dict(q=z(2, 3, 4, 193), k=z(2, 5, 2, 193)),
+           dict(v=z(2, 5, 1, 385)), dict(v=z(2, 5, 0, 16)), dict(q=z(2, 3, 4, 0), k=z(2, 5, 2, 0)),
+           dict(key_mask=z(2, 5)), dict(key_mask=z(2, 4, dtype=torch.bool)), dict(key_mask=z(2, 1, 1, 5, dtype=torch.bool))]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            ops.attn_fwd(**dict(dict(q=q, k=k, v=v), **kw))
+    with pytest.raises(VxError):
+        ops.attn_fwd(q, k.cpu(), v)
+    out, stats = ops.attn_fwd(q, k, v, want_stats=True)
+    for kw in (dict(dout=z(2, 3, 4, 8)), dict(dout=z(2, 3, 4, 16, dtype=BF16)), dict(out=z(2, 4, 3, 16).transpose(1, 2)),
+               dict(stats=stats[:1]), dict(stats=stats.double())):
+        with pytest.raises(ValueError):
+            ops.attn_bwd(**dict(dict(dout=out, q=q, k=k, v=v, out=out, stats=stats), **kw))
+    x, w = z(4, 6), z(5, 6)
+    for kw in (dict(act="tanh"), dict(act=None), dict(weight=z(5, 7)), dict(x=z(4, 6, dtype=torch.float64)), dict(bias=z(6)),
+               dict(bias=z(5, dtype=BF16)), dict(residual=z(4, 6)), dict(residual=z(1, 5)), dict(x=z(2, 4, 6)), dict(x=z(4, 0), weight=z(5, 0))):
+        with pytest.raises(ValueError):
+            ops.linear_fwd(**dict(dict(x=x, weight=w), **kw))
+    for kw in (dict(act="relu"), dict(act="gelu", saved=z(4, 6)), dict(dy=z(5, 4)), dict(act="swish", saved=z(4, 5))):
+        with pytest.raises(ValueError):
+            ops.linear_bwd(**dict(dict(dy=z(4, 5), x=x, weight=w), **kw))

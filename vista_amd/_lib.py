@@ -15,6 +15,8 @@ c_i64p = ctypes.POINTER(ctypes.c_int64)
 
 VX_F32, VX_BF16 = 0, 1
 VX_EPI_RELU = 1
+VX_ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+VX_ATTN_MAX_DIM, VX_ATTN_MAX_VDIM = 192, 384
 VX_CONV_NO_COMPACT = 0x100
 VX_CONV_NO_SPLIT_TAIL = 0x200
 VX_CONV_F32_MFMA, VX_CONV_F32_PRODUCTS6, VX_CONV_F32_PRODUCTS9 = 0x1000, 0x2000, 0x3000
@@ -97,6 +99,17 @@ SIGNATURES = {
     "vx_nms_workspace_bytes": (c_size_t, [c_int32]),
     "vx_nms_bev": (c_int32, [c_void_p, c_int32, ctypes.c_float, c_int32, c_void_p, c_i64p, c_void_p, c_size_t,
                              c_void_p]),
+    "vx_linear_fwd": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32,
+                                c_int32, c_void_p, c_void_p, c_int32, c_void_p]),
+    "vx_linear_bwd_workspace_bytes": (c_size_t, [c_int64, c_int32, c_int32, c_int32]),
+    "vx_linear_bwd": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32,
+                                c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),
+    "vx_attn_fwd_workspace_bytes": (c_size_t, [c_i64p, c_int32]),
+    "vx_attn_fwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_i64p, c_i64p, ctypes.c_float, c_void_p, c_void_p,
+                              c_int32, c_void_p, c_size_t, c_void_p]),
+    "vx_attn_bwd_workspace_bytes": (c_size_t, [c_i64p, c_int32]),
+    "vx_attn_bwd": (c_int32, [c_void_p, c_i64p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64p, c_i64p, c_void_p, c_void_p,
+                              ctypes.c_float, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,676 @@
+// Attention softmax(scale q k^T) v with a key mask, and its backward pass (cross-view attention:
+// det3d/models/necks/attention.py:55-124, two read-outs -- query / key heads -- over one value map).
+//
+// Forward: one pass over the keys with a running maximum and sum per query; probabilities never leave the registers.
+// Backward: probabilities recomputed from the saved (maximum, 1 / sum); see attn_pds below.
+// fp32 operands run as three exact bf16 planes (six products, fp32 accumulation), bf16 ones directly (vx_tile.h). Softmax
+// statistics, probabilities and sums over queries are fp32; for bf16 tensors the probabilities and score gradients are rounded
+// to bf16 where they become matrix operands (at most half a step, 2^-8 of each value: independent errors, so that their sum is off
+// by about as much as the output's own rounding).
+// A masked key has no part in anything, whatever its rows hold; a query without keys gives zeros. No atomics: bitwise
+// reproducible.
+#include "vx_tile.h"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <typename T>
+struct AttnArgs {
+  const T *q, *k, *v;
+  const uint8_t* mask;                       // [batch][mask_b] bytes, or null
+  long long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h, mask_b;
+  int sq, sk, h, gk, gv, d, dv;              // gk, gv: query heads per key / value head
+  float scale2;                              // scale * log2(e)
+};
+
+template <typename T>
+struct FwdArgs : AttnArgs<T> {
+  T* out;                                    // [b][sq][h][dv]
+  float2* stats;                             // [b*h][sq] {max of scale2 * score, 1 / sum} or null
+  float* part;                               // [splits][b*h][sq][dv] when the keys are split
+  float2* part_ml;                           // [splits][b*h][sq]
+  int tiles_q, splits, span;                 // span: key tiles of one split
+};
+
+template <typename T>
+struct AttnTile {
+  static constexpr int KT = VxType<T>::BK;   // keys per staged tile
+};
+
+// bits: which keys of tile t take part (lane l < KT speaks for key t * KT + l)
+template <typename T>
+__device__ __forceinline__ bool attn_key_live(const AttnArgs<T>& a, const uint8_t* mask, int t, int lane) {
+  const int key = t * AttnTile<T>::KT + lane;
+  return lane < AttnTile<T>::KT && key < a.sk && (mask == nullptr || mask[key] != 0);
+}
+
+// A workgroup (4 waves) owns 64 * RT queries of one head, wave w 16 * RT of them; everything is kept transposed --
+// S^T = K Q^T, O^T = V^T P^T -- so that a lane holds ONE query (c = lane & 15) and the softmax statistics, the rescaling
+// and the operand form of P are lane-local. A lane's S values are keys {16 t + 4 g + i}; as an operand they are the eight
+// k's of its group g in the order (t, i), and the V^T image is staged in that order of keys.
+template <typename T, int DP, int DVP, int RT>
+__global__ __launch_bounds__(kTileThreads, (DVP > 192 || (DVP > 64 && VxType<T>::NPL == 3)) ? 1 : 2) void attn_fwd(const FwdArgs<T> a) {
+  constexpr int NPL = VxType<T>::NPL, KT = AttnTile<T>::KT, NS = KT / 32;     // NS: 32-key steps of a tile
+  constexpr int KD = DP / 32, NV = DVP / 16;
+  constexpr int K_FRAGS = KT / 16 * KD, V_FRAGS = NV * NS;
+  constexpr int K_PLANE = K_FRAGS * kFragBytes, V_PLANE = V_FRAGS * kFragBytes;
+  constexpr int KI = (K_FRAGS + 3) / 4;                                        // K fragments staged per wave
+  constexpr int VW = (DVP % 128 == 0 || sizeof(T) == 2) ? 2 : 1;               // V columns per staged item
+  constexpr int V_ITEMS = DVP / VW * (KT / 8), VI = (V_ITEMS + kTileThreads - 1) / kTileThreads;
+  __shared__ __attribute__((aligned(16))) char lds[(K_PLANE + V_PLANE) * NPL];
+  char *ik = lds, *iv = lds + K_PLANE * NPL;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+  unsigned w = vx_xcd_tile(blockIdx.x, gridDim.x);
+  const int tile_q = (int)(w % a.tiles_q);
+  w /= a.tiles_q;
+  const int split = (int)(w % a.splits);
+  const int bh = (int)(w / a.splits), b = bh / a.h, h = bh % a.h;
+  const int tiles_k = (a.sk + KT - 1) / KT;
+  const int t0 = split * a.span, t1 = t0 + a.span < tiles_k ? t0 + a.span : tiles_k;
+  const T* kp = a.k + b * a.k_b + (h / a.gk) * a.k_h;
+  const T* vp = a.v + b * a.v_b + (h / a.gv) * a.v_h;
+  const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  const int q0 = tile_q * (64 * RT) + wave * (16 * RT);
+
+  VxFrag<NPL> qf[RT][KD];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = q0 + rt * 16 + c;
+    const T* qp = a.q + b * a.q_b + row * a.q_s + h * a.q_h;
+#pragma unroll
+    for (int kd = 0; kd < KD; ++kd) {
+      VxRow8<T> x;
+      x.load(qp + kd * 32 + g * 8, row < a.sq ? a.d - kd * 32 - g * 8 : 0);
+      x.planes(qf[rt][kd]);
+    }
+  }
+  float m[RT], l[RT];
+  vx_f32x4 o[RT][NV];
+  vx_acc_zero(o);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -INFINITY;
+    l[rt] = 0.0f;
+  }
+
+  VxRow8<T> ks[KI];
+  VxCol8<T, VW> vs[VI];
+  auto load = [&](int t, unsigned long long live) {
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int frag = i * 4 + wave, key = t * KT + frag / KD * 16 + c, d = frag % KD * 32 + g * 8;
+      ks[i].load(kp + key * a.k_s + d, frag < K_FRAGS && key < a.sk ? a.d - d : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int item = i * kTileThreads + tid, n = item % (DVP / VW) * VW, kg = item / (DVP / VW);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int kk = kg / 4 * 32 + (j >> 2) * 16 + kg % 4 * 4 + (j & 3);     // operand order of the keys, see above
+        vs[i].load(j, vp + (t * KT + kk) * a.v_s + n, item < V_ITEMS && (live >> kk & 1) ? a.dv - n : 0);
+      }
+    }
+  };
+  auto store = [&]() {
+    VxFrag<NPL> f;
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int frag = i * 4 + wave;
+      if (frag < K_FRAGS) {
+        ks[i].planes(f);
+        vx_frag_store(ik, K_PLANE, frag, frag / KD, lane, f);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int item = i * kTileThreads + tid, n = item % (DVP / VW) * VW, kg = item / (DVP / VW);
+      if (item < V_ITEMS) {
+#pragma unroll
+        for (int j = 0; j < VW; ++j) {
+          vs[i].planes(j, f);
+          vx_frag_store(iv, V_PLANE, ((n + j) >> 4) * NS + kg / 4, n >> 4, ((n + j) & 15) + 16 * (kg % 4), f);
+        }
+      }
+    }
+  };
+
+  const bool any = q0 < a.sq;                  // a wave without queries only stages
+  unsigned long long cur = t0 < t1 ? __ballot(attn_key_live(a, mask, t0, lane)) : 0;
+  unsigned long long nxt = t0 + 1 < t1 ? __ballot(attn_key_live(a, mask, t0 + 1, lane)) : 0;
+  if (cur) load(t0, cur);
+  for (int t = t0; t < t1; ++t) {
+    if (cur) store();                          // a tile without keys is neither loaded nor multiplied
+    const bool ahead = t + 2 < t1 && attn_key_live(a, mask, t + 2, lane);
+    __syncthreads();
+    if (nxt) load(t + 1, nxt);
+    if (cur && any) {
+      vx_f32x4 s[RT][KT / 16];
+      vx_acc_zero(s);
+#pragma unroll
+      for (int kt = 0; kt < KT / 16; ++kt)
+#pragma unroll
+        for (int kd = 0; kd < KD; ++kd) {
+          VxFrag<NPL> kf;
+          vx_frag_load(ik, K_PLANE, kt * KD + kd, kt, lane, kf);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[rt][kt] = vx_mma(kf, qf[rt][kd], s[rt][kt]);
+        }
+      VxFrag<NPL> pf[RT][NS];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < KT / 16; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool live = cur >> (kt * 16 + g * 4 + i) & 1;
+            s[rt][kt][i] = live ? s[rt][kt][i] * a.scale2 : -INFINITY;
+            mx = fmaxf(mx, s[rt][kt][i]);
+          }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mn = fmaxf(m[rt], mx), ref = mn == -INFINITY ? 0.0f : mn;
+        const float alpha = exp2f(m[rt] - ref);
+        m[rt] = mn;
+        float sum = 0.0f;
+#pragma unroll
+        for (int ns = 0; ns < NS; ++ns) {
+          float p[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            p[j] = exp2f(s[rt][ns * 2 + (j >> 2)][j & 3] - ref);
+            sum += p[j];
+          }
+          vx_planes(p, pf[rt][ns]);
+        }
+        l[rt] = l[rt] * alpha + sum;
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+          for (int nv = 0; nv < NV; ++nv) o[rt][nv] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv)
+#pragma unroll
+        for (int ns = 0; ns < NS; ++ns) {
+          VxFrag<NPL> vf;
+          vx_frag_load(iv, V_PLANE, nv * NS + ns, nv, lane, vf);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) o[rt][nv] = vx_mma(vf, pf[rt][ns], o[rt][nv]);
+        }
+    }
+    __syncthreads();
+    cur = nxt;
+    nxt = __ballot(ahead);
+  }
+
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    float sum = l[rt];
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    const int row = q0 + rt * 16 + c;
+    if (row >= a.sq) continue;
+    if (a.splits > 1) {
+      const long long at = ((long long)split * gridDim.x / (a.tiles_q * a.splits) + bh) * a.sq + row;
+      if (g == 0) a.part_ml[at] = make_float2(m[rt], sum);
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv) vx_store4(a.part + at * a.dv + nv * 16 + g * 4, o[rt][nv], a.dv - nv * 16 - g * 4);
+    } else {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      if (a.stats && g == 0) a.stats[(long long)bh * a.sq + row] = make_float2(m[rt], inv);
+      T* op = a.out + (((long long)b * a.sq + row) * a.h + h) * a.dv;
+#pragma unroll
+      for (int nv = 0; nv < NV; ++nv) vx_store4(op + nv * 16 + g * 4, o[rt][nv] * inv, a.dv - nv * 16 - g * 4);
+    }
+  }
+}
+
+// joins the splits of a row: weights 2^(m_s - m), in order of the splits. One thread per four output values.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join(const FwdArgs<T> a, long long items, int quads) {
+  const long long it = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (it >= items) return;
+  const long long rowid = it / quads;               // bh * sq + row
+  const int n = (int)(it % quads) * 4;
+  const long long rows = items / quads;
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[s * rows + rowid].x);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  vx_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = a.part_ml[s * rows + rowid];
+    const float wgt = exp2f(ml.x - ref);
+    l += wgt * ml.y;
+    o += vx_load4(a.part + (s * rows + rowid) * a.dv + n, a.dv - n) * wgt;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int bh = (int)(rowid / a.sq), row = (int)(rowid % a.sq), b = bh / a.h, h = bh % a.h;
+  vx_store4(a.out + (((long long)b * a.sq + row) * a.h + h) * a.dv + n, o * inv, a.dv - n);
+  if (a.stats && n == 0) a.stats[rowid] = make_float2(m, inv);
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------
+template <typename T>
+struct BwdArgs : AttnArgs<T> {
+  const T *out, *go;                         // out [b][sq][h][dv]; go by strides
+  long long go_b, go_s, go_h;
+  const float2* stats;
+  float* delta;                              // [b*h][sq]
+  T *p, *ds;                                 // [b*h][rows][skp] of the present chunk of queries
+  T *dq, *dk, *dvv;                          // [b][sq][h][d], [b][sk][h/gk][d], [b][sk][h/gv][dv]
+  float *slab_k, *slab_v;                    // [splits][b*h][sk][d], [splits][b*h][sk][dv]
+  float scale;
+  int q0, rows, skp;                         // present chunk: queries [q0, q0 + rows); skp: sk rounded up to 8
+  int bh, split0, span;                      // first split of the chunk, queries of one split
+  int tq, td, tkd, tkv, tk;                  // tiles of attn_grads
+  unsigned n_v, n_k, n_q;                    // workgroups per problem
+};
+
+// delta = sum_n go * out per query: one wave per row
+template <typename T>
+__global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long rows) {
+  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const int lane = threadIdx.x & 63;
+  const int bh = (int)(r / a.sq), row = (int)(r % a.sq), b = bh / a.h, h = bh % a.h;
+  const T* go = a.go + b * a.go_b + row * a.go_s + h * a.go_h;
+  const T* o = a.out + (((long long)b * a.sq + row) * a.h + h) * a.dv;
+  float s = 0.0f;
+  for (int n = lane * 4; n < a.dv; n += 256) {
+    const vx_f32x4 x = vx_load4(go + n, a.dv - n) * vx_load4(o + n, a.dv - n);
+    s += (x[0] + x[1]) + (x[2] + x[3]);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
+  if (lane == 0) a.delta[r] = s;
+}
+
+// P and dS of a TM-query x TN-key tile: scores and dP = go v^T are two products with one epilogue,
+// P = 2^(scale2 s - max) / sum, dS = scale P (dP - delta).
+template <typename T, int TM, int TN>
+__global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) {
+  __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
+  unsigned w = vx_xcd_tile(blockIdx.x, gridDim.x);
+  const int n0 = (int)(w % a.tk) * TN;
+  w /= a.tk;
+  const int m0 = (int)(w % a.tq) * TM;
+  const int bh = (int)(w / a.tq), b = bh / a.h, h = bh % a.h;
+  const int rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = a.sk - n0 < TN ? a.sk - n0 : TN;
+  const long long q = a.q0 + m0;
+  vx_f32x4 s[TM / 32][TN / 32], dp[TM / 32][TN / 32];
+  vx_acc_zero(s);
+  vx_acc_zero(dp);
+  vx_gemm_loop<T, KC, KC, TM, TN>({a.q + b * a.q_b + q * a.q_s + h * a.q_h, a.q_s, rows_m, nullptr},
+                                  {a.k + b * a.k_b + (h / a.gk) * a.k_h + n0 * a.k_s, a.k_s, rows_n, nullptr}, 0, a.d, lds, s);
+  vx_gemm_loop<T, KC, KC, TM, TN>({a.go + b * a.go_b + q * a.go_s + h * a.go_h, a.go_s, rows_m, nullptr},
+                                  {a.v + b * a.v_b + (h / a.gv) * a.v_h + n0 * a.v_s, a.v_s, rows_n, nullptr}, 0, a.dv, lds, dp);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+#pragma unroll
+  for (int ni = 0; ni < TN / 32; ++ni) {
+    const int n = n0 + wn * (TN / 2) + ni * 16 + (lane >> 4) * 4;
+    bool live[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) live[i] = n + i < a.sk && (mask == nullptr || mask[n + i] != 0);
+#pragma unroll
+    for (int mi = 0; mi < TM / 32; ++mi) {
+      const int m = m0 + wm * (TM / 2) + mi * 16 + (lane & 15);
+      if (m >= a.rows || n >= a.skp) continue;
+      const long long r = (long long)bh * a.sq + a.q0 + m;
+      const float2 st = a.stats[r];
+      const float delta = a.delta[r];
+      vx_f32x4 p, d;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = live[i] ? exp2f(s[mi][ni][i] * a.scale2 - st.x) * st.y : 0.0f;
+        d[i] = live[i] ? p[i] * (dp[mi][ni][i] - delta) * a.scale : 0.0f;
+      }
+      const long long at = ((long long)bh * a.rows + m) * a.skp + n;
+      vx_store4(a.p + at, p, 4);
+      vx_store4(a.ds + at, d, 4);
+    }
+  }
+}
+
+// the three gradients of a chunk in one launch: dV slabs = P^T go, dK slabs = dS^T q (reduction over the queries of a split),
+// dQ = dS k (reduction over the keys)
+template <typename T, int TM, int TN>
+__global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a) {
+  __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
+  vx_f32x4 acc[TM / 32][TN / 32];
+  vx_acc_zero(acc);
+  if (blockIdx.x < a.n_v + a.n_k) {
+    const bool is_v = blockIdx.x < a.n_v;
+    const int tn = is_v ? a.tkv : a.tkd, width = is_v ? a.dv : a.d;
+    unsigned w = is_v ? vx_xcd_tile(blockIdx.x, a.n_v) : vx_xcd_tile(blockIdx.x - a.n_v, a.n_k);
+    const int n0 = (int)(w % tn) * TN;
+    w /= tn;
+    const int m0 = (int)(w % a.tk) * TM;
+    w /= a.tk;
+    const int bh = (int)(w % a.bh), sp = (int)(w / a.bh), b = bh / a.h, h = bh % a.h;
+    const int r0 = sp * a.span, len = a.rows - r0 < a.span ? a.rows - r0 : a.span;
+    const int rows_m = a.sk - m0 < TM ? a.sk - m0 : TM, rows_n = width - n0 < TN ? width - n0 : TN;
+    const long long q = a.q0 + r0;
+    const VxOperand<T> X{(is_v ? a.p : a.ds) + ((long long)bh * a.rows + r0) * a.skp + m0, a.skp, rows_m, nullptr};
+    const VxOperand<T> W{is_v ? a.go + b * a.go_b + q * a.go_s + h * a.go_h + n0 : a.q + b * a.q_b + q * a.q_s + h * a.q_h + n0,
+                         is_v ? a.go_s : a.q_s, rows_n, nullptr};
+    vx_gemm_loop<T, KS, KS, TM, TN>(X, W, 0, len, lds, acc);
+    float* slab = (is_v ? a.slab_v : a.slab_k) + ((long long)(a.split0 + sp) * a.bh + bh) * a.sk * width;
+    vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
+      if (m < rows_m && n < rows_n) vx_store4(slab + (long long)(m0 + m) * width + n0 + n, v, rows_n - n);
+    });
+  } else {
+    unsigned w = vx_xcd_tile(blockIdx.x - a.n_v - a.n_k, a.n_q);
+    const int n0 = (int)(w % a.td) * TN;
+    w /= a.td;
+    const int m0 = (int)(w % a.tq) * TM;
+    const int bh = (int)(w / a.tq), b = bh / a.h, h = bh % a.h;
+    const int rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = a.d - n0 < TN ? a.d - n0 : TN;
+    const VxOperand<T> X{a.ds + ((long long)bh * a.rows + m0) * a.skp, a.skp, rows_m, nullptr};
+    const VxOperand<T> W{a.k + b * a.k_b + (h / a.gk) * a.k_h + n0, a.k_s, rows_n, a.mask ? a.mask + b * a.mask_b : nullptr};
+    vx_gemm_loop<T, KC, KS, TM, TN>(X, W, 0, a.sk, lds, acc);
+    vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
+      if (m < rows_m && n < rows_n)
+        vx_store4(a.dq + (((long long)b * a.sq + a.q0 + m0 + m) * a.h + h) * a.d + n0 + n, v, rows_n - n);
+    });
+  }
+}
+
+// dk, dv = sums of the slabs over a head's query heads and the splits, in that order; masked keys get zeros
+template <typename T>
+__global__ __launch_bounds__(256) void attn_slab_sum(const BwdArgs<T> a, int splits, unsigned blocks_v, long long items_v,
+                                                     long long items_k) {
+  const bool is_v = blockIdx.x < blocks_v;
+  const int width = is_v ? a.dv : a.d, group = is_v ? a.gv : a.gk, quads = (width + 3) / 4;
+  const long long it = (long long)(is_v ? blockIdx.x : blockIdx.x - blocks_v) * 256 + threadIdx.x;
+  if (it >= (is_v ? items_v : items_k)) return;
+  const int n = (int)(it % quads) * 4, left = width - n;
+  long long r = it / quads;                        // (b * heads + head) * sk + key
+  const int key = (int)(r % a.sk);
+  r /= a.sk;
+  const int heads = a.h / group, head = (int)(r % heads), b = (int)(r / heads);
+  vx_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (a.mask == nullptr || a.mask[b * a.mask_b + key]) {
+    const float* slab = is_v ? a.slab_v : a.slab_k;
+    for (int j = 0; j < group; ++j)
+      for (int sp = 0; sp < splits; ++sp)
+        s += vx_load4(slab + (((long long)sp * a.bh + b * a.h + head * group + j) * a.sk + key) * width + n, left);
+  }
+  vx_store4((is_v ? a.dvv : a.dk) + (((long long)b * a.sk + key) * heads + head) * width + n, s, left);
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+struct Shape {
+  int64_t b, sq, sk, h, hk, hv, d, dv;
+};
+Shape shape_of(const int64_t* s) { return {s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]}; }
+
+int32_t check(const char* who, const int64_t* shape, int32_t dtype) {
+  VX_REQUIRE(shape, "%s: null shape", who);
+  const Shape s = shape_of(shape);
+  VX_REQUIRE(dtype == VX_F32 || dtype == VX_BF16, "%s: dtype must be VX_F32 or VX_BF16", who);
+  VX_REQUIRE(s.b >= 0 && s.sq >= 0 && s.sk >= 0 && s.b < (1 << 24) && s.sq < (1LL << 30) && s.sk < (1LL << 30), "%s: bad lengths", who);
+  VX_REQUIRE(s.h >= 1 && s.hk >= 1 && s.hv >= 1 && s.h % s.hk == 0 && s.h % s.hv == 0 && s.h < (1 << 16),
+             "%s: key and value heads must divide the query heads", who);
+  VX_REQUIRE(s.d >= 1 && s.d <= VX_ATTN_MAX_DIM && s.dv >= 1 && s.dv <= VX_ATTN_MAX_VDIM, "%s: dim must be in [1, %d], v_dim in [1, %d]",
+             who, VX_ATTN_MAX_DIM, VX_ATTN_MAX_VDIM);
+  VX_REQUIRE(s.b * s.h < (1LL << 24), "%s: too many heads", who);
+  return VX_OK;
+}
+
+// strides: q, k, v (batch, position, head), mask (batch)
+template <typename T>
+void fill_args(AttnArgs<T>& a, const Shape& s, const int64_t* st, const void* q, const void* k, const void* v, const uint8_t* mask,
+               float scale) {
+  a.q = (const T*)q; a.k = (const T*)k; a.v = (const T*)v; a.mask = mask;
+  a.q_b = st[0]; a.q_s = st[1]; a.q_h = st[2];
+  a.k_b = st[3]; a.k_s = st[4]; a.k_h = st[5];
+  a.v_b = st[6]; a.v_s = st[7]; a.v_h = st[8];
+  a.mask_b = st[9];
+  a.sq = (int)s.sq; a.sk = (int)s.sk; a.h = (int)s.h;
+  a.gk = (int)(s.h / s.hk); a.gv = (int)(s.h / s.hv); a.d = (int)s.d; a.dv = (int)s.dv;
+  a.scale2 = scale * kLog2e;
+}
+
+struct FwdPlan {
+  int rt;
+  int64_t tiles_q, splits, span;
+};
+FwdPlan fwd_plan(const Shape& s, int32_t dtype) {
+  FwdPlan p;
+  const int64_t cus = vx_tile_cus(), bh = s.b * s.h, kt = dtype == VX_F32 ? 32 : 64, tiles_k = vx_cdiv(s.sk, kt);
+  p.rt = vx_cdiv(s.sq, 128) * bh >= cus ? 2 : 1;
+  p.tiles_q = vx_cdiv(s.sq, 64 * p.rt);
+  // few workgroups: split the keys so that every CU has one
+  int64_t splits = p.tiles_q * bh > 0 ? cus / (p.tiles_q * bh) : 1;
+  if (splits > tiles_k) splits = tiles_k;
+  if (splits < 1) splits = 1;
+  p.span = tiles_k ? vx_cdiv(tiles_k, splits) : 1;
+  p.splits = tiles_k ? vx_cdiv(tiles_k, p.span) : 1;
+  return p;
+}
+size_t fwd_bytes(const Shape& s, int32_t dtype) {
+  const FwdPlan p = fwd_plan(s, dtype);
+  if (p.splits <= 1) return 0;
+  const size_t rows = (size_t)p.splits * s.b * s.h * s.sq;
+  return vx_align(rows * s.dv * 4) + vx_align(rows * 8);
+}
+
+template <typename T, int DP, int DVP>
+void launch_fwd(const FwdArgs<T>& a, int rt, unsigned grid, hipStream_t s) {
+  if (rt == 2)
+    attn_fwd<T, DP, DVP, 2><<<grid, kTileThreads, 0, s>>>(a);
+  else
+    attn_fwd<T, DP, DVP, 1><<<grid, kTileThreads, 0, s>>>(a);
+}
+
+template <typename T>
+int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStream_t s) {
+  const FwdPlan p = fwd_plan(sh, dtype);
+  const int64_t bh = sh.b * sh.h, grid = p.tiles_q * p.splits * bh;
+  VX_REQUIRE(grid < (1LL << 31), "attn_fwd: too many tiles");
+  a.tiles_q = (int)p.tiles_q;
+  a.splits = (int)p.splits;
+  a.span = (int)p.span;
+  const size_t rows = (size_t)p.splits * bh * sh.sq;
+  a.part = (float*)ws;
+  a.part_ml = (float2*)(ws + vx_align(rows * sh.dv * 4));
+  // the smallest tile that holds both widths
+  if (a.d <= 32 && a.dv <= 64) launch_fwd<T, 32, 64>(a, p.rt, (unsigned)grid, s);
+  else if (a.d <= 64 && a.dv <= 64) launch_fwd<T, 64, 64>(a, p.rt, (unsigned)grid, s);
+  else if (a.d <= 64 && a.dv <= 128) launch_fwd<T, 64, 128>(a, p.rt, (unsigned)grid, s);
+  else if (a.d <= 128 && a.dv <= 128) launch_fwd<T, 128, 128>(a, p.rt, (unsigned)grid, s);
+  else if (a.d <= 96 && a.dv <= 192) launch_fwd<T, 96, 192>(a, p.rt, (unsigned)grid, s);
+  else launch_fwd<T, 192, 384>(a, p.rt, (unsigned)grid, s);
+  VX_LAUNCH_CHECK();
+  if (p.splits > 1) {
+    const int quads = (a.dv + 3) / 4;
+    const int64_t items = bh * sh.sq * quads;
+    attn_join<T><<<(unsigned)vx_cdiv(items, 256), 256, 0, s>>>(a, items, quads);
+    VX_LAUNCH_CHECK();
+  }
+  return VX_OK;
+}
+
+struct BwdPlan {
+  int64_t tm, skp, span, per_chunk, splits, chunk;      // queries per split, splits per chunk, all splits, queries per chunk
+  size_t delta, pds, slab_k, slab_v;                    // bytes
+  size_t total() const { return delta + 2 * pds + slab_k + slab_v; }
+};
+// queries are cut into splits (one slab each) and the splits into chunks, whose probabilities and score gradients are in
+// memory at a time (at most kChunkBytes of both)
+constexpr size_t kChunkBytes = (size_t)256 << 20;
+BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
+  BwdPlan p;
+  const int64_t cus = vx_tile_cus(), bh = s.b * s.h, e = dtype == VX_F32 ? 4 : 2, bk = dtype == VX_F32 ? 32 : 64;
+  p.skp = vx_cdiv(s.sk, 8) * 8;
+  p.tm = vx_cdiv(s.sq, 128) * vx_cdiv(s.sk, 128) * bh >= 2 * cus ? 128 : 64;
+  const int64_t tiles = vx_cdiv(s.sk, p.tm) * (vx_cdiv(s.dv, p.tm) + vx_cdiv(s.d, p.tm)) * bh;
+  int64_t splits = vx_cdiv(2 * cus, tiles > 0 ? tiles : 1);
+  const int64_t most = vx_cdiv(s.sq, 4 * bk);
+  if (splits > most) splits = most;
+  int64_t fit = (int64_t)(kChunkBytes / 2) / (bh * p.skp * e);       // queries of a chunk
+  if (fit < p.tm) fit = p.tm;
+  if (splits < vx_cdiv(s.sq, fit)) splits = vx_cdiv(s.sq, fit);
+  p.span = vx_cdiv(vx_cdiv(s.sq, splits), p.tm) * p.tm;
+  p.splits = vx_cdiv(s.sq, p.span);
+  p.per_chunk = fit / p.span < 1 ? 1 : fit / p.span;
+  if (p.per_chunk > p.splits) p.per_chunk = p.splits;
+  p.chunk = p.per_chunk * p.span < s.sq ? p.per_chunk * p.span : s.sq;
+  p.delta = vx_align((size_t)bh * s.sq * 4);
+  p.pds = vx_align((size_t)bh * p.chunk * p.skp * e);
+  p.slab_k = vx_align((size_t)p.splits * bh * s.sk * s.d * 4);
+  p.slab_v = vx_align((size_t)p.splits * bh * s.sk * s.dv * 4);
+  return p;
+}
+
+template <typename T, int TM>
+int32_t bwd_chunk(const BwdArgs<T>& a, int64_t pds, int64_t grads, hipStream_t s) {
+  attn_pds<T, TM, TM><<<(unsigned)pds, kTileThreads, 0, s>>>(a);
+  VX_LAUNCH_CHECK();
+  attn_grads<T, TM, TM><<<(unsigned)grads, kTileThreads, 0, s>>>(a);
+  VX_LAUNCH_CHECK();
+  return VX_OK;
+}
+
+template <typename T>
+int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStream_t s) {
+  const BwdPlan p = bwd_plan(sh, dtype);
+  const int64_t bh = sh.b * sh.h, rows = bh * sh.sq;
+  a.delta = (float*)ws;
+  a.p = (T*)(ws + p.delta);
+  a.ds = (T*)(ws + p.delta + p.pds);
+  a.slab_k = (float*)(ws + p.delta + 2 * p.pds);
+  a.slab_v = (float*)(ws + p.delta + 2 * p.pds + p.slab_k);
+  a.skp = (int)p.skp;
+  a.bh = (int)bh;
+  a.span = (int)p.span;
+  a.tk = (int)vx_cdiv(p.skp, p.tm);
+  a.td = a.tkd = (int)vx_cdiv(sh.d, p.tm);
+  a.tkv = (int)vx_cdiv(sh.dv, p.tm);
+  VX_REQUIRE(vx_cdiv(rows, 4) < (1LL << 31), "attn_bwd: too many queries");
+  attn_delta<T><<<(unsigned)vx_cdiv(rows, 4), 256, 0, s>>>(a, rows);
+  VX_LAUNCH_CHECK();
+  for (int64_t q0 = 0, split = 0; q0 < sh.sq; q0 += p.chunk, split += p.per_chunk) {
+    a.q0 = (int)q0;
+    a.rows = (int)(sh.sq - q0 < p.chunk ? sh.sq - q0 : p.chunk);
+    a.split0 = (int)split;
+    a.tq = (int)vx_cdiv(a.rows, p.tm);
+    const int64_t here = vx_cdiv(a.rows, p.span), tkeys = vx_cdiv(sh.sk, p.tm);
+    a.tk = (int)vx_cdiv(p.skp, p.tm);
+    const int64_t pds = (int64_t)a.tk * a.tq * bh;
+    const int64_t nv = here * bh * tkeys * a.tkv, nk = here * bh * tkeys * a.tkd, nq = (int64_t)a.tq * a.td * bh;
+    VX_REQUIRE(pds < (1LL << 31) && nv + nk + nq < (1LL << 31), "attn_bwd: too many tiles");
+    a.n_v = (unsigned)nv;
+    a.n_k = (unsigned)nk;
+    a.n_q = (unsigned)nq;
+    const int32_t rc = p.tm == 128 ? bwd_chunk<T, 128>(a, pds, nv + nk + nq, s) : bwd_chunk<T, 64>(a, pds, nv + nk + nq, s);
+    if (rc) return rc;
+  }
+  const int64_t iv = sh.b * sh.hv * sh.sk * vx_cdiv(sh.dv, 4), ik = sh.b * sh.hk * sh.sk * vx_cdiv(sh.d, 4);
+  const int64_t gv = vx_cdiv(iv, 256), gk = vx_cdiv(ik, 256);
+  VX_REQUIRE(gv + gk < (1LL << 31), "attn_bwd: too many keys");
+  attn_slab_sum<T><<<(unsigned)(gv + gk), 256, 0, s>>>(a, (int)p.splits, (unsigned)gv, iv, ik);
+  VX_LAUNCH_CHECK();
+  return VX_OK;
+}
+
+}  // namespace
+
+extern "C" size_t vx_attn_fwd_workspace_bytes(const int64_t* shape, int32_t dtype) {
+  if (check("attn_fwd", shape, dtype)) return 0;
+  const Shape s = shape_of(shape);
+  return s.b && s.sq ? fwd_bytes(s, dtype) : 0;
+}
+
+extern "C" int32_t vx_attn_fwd(const void* d_q, const void* d_k, const void* d_v, const uint8_t* d_key_mask, const int64_t* shape,
+                               const int64_t* strides, float scale, void* d_out, float* d_stats, int32_t dtype, void* d_workspace,
+                               size_t workspace_bytes, void* stream) {
+  if (int32_t rc = check("attn_fwd", shape, dtype)) return rc;
+  const Shape s = shape_of(shape);
+  if (s.b == 0 || s.sq == 0) return VX_OK;
+  VX_REQUIRE(strides && d_q && d_out && (s.sk == 0 || (d_k && d_v)), "attn_fwd: null pointer");
+  for (int i = 0; i < 10; ++i) VX_REQUIRE(strides[i] >= 0, "attn_fwd: negative stride");
+  const size_t need = fwd_bytes(s, dtype);
+  if (workspace_bytes < need || (need && !d_workspace)) {
+    vx_set_error("attn_fwd: workspace too small");
+    return VX_ERR_WORKSPACE;
+  }
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == VX_F32) {
+    FwdArgs<float> a{};
+    fill_args(a, s, strides, d_q, d_k, d_v, d_key_mask, scale);
+    a.out = (float*)d_out;
+    a.stats = (float2*)d_stats;
+    return fwd_impl(a, s, dtype, (char*)d_workspace, st);
+  }
+  FwdArgs<__bf16> a{};
+  fill_args(a, s, strides, d_q, d_k, d_v, d_key_mask, scale);
+  a.out = (__bf16*)d_out;
+  a.stats = (float2*)d_stats;
+  return fwd_impl(a, s, dtype, (char*)d_workspace, st);
+}
+
+extern "C" size_t vx_attn_bwd_workspace_bytes(const int64_t* shape, int32_t dtype) {
+  if (check("attn_bwd", shape, dtype)) return 0;
+  const Shape s = shape_of(shape);
+  return s.b && s.sq && s.sk ? bwd_plan(s, dtype).total() : 0;
+}
+
+template <typename T>
+static int32_t attn_bwd_typed(const Shape& s, const void* d_dout, const int64_t* dout_strides, const void* d_q, const void* d_k,
+                              const void* d_v, const uint8_t* d_key_mask, const int64_t* strides, const void* d_out,
+                              const float* d_stats, float scale, void* d_dq, void* d_dk, void* d_dv, int32_t dtype, void* ws,
+                              hipStream_t st) {
+  BwdArgs<T> a{};
+  fill_args(a, s, strides, d_q, d_k, d_v, d_key_mask, scale);
+  a.out = (const T*)d_out;
+  a.go = (const T*)d_dout;
+  a.go_b = dout_strides[0];
+  a.go_s = dout_strides[1];
+  a.go_h = dout_strides[2];
+  a.stats = (const float2*)d_stats;
+  a.dq = (T*)d_dq;
+  a.dk = (T*)d_dk;
+  a.dvv = (T*)d_dv;
+  a.scale = scale;
+  return bwd_impl(a, s, dtype, (char*)ws, st);
+}
+
+extern "C" int32_t vx_attn_bwd(const void* d_dout, const int64_t* dout_strides, const void* d_q, const void* d_k, const void* d_v,
+                               const uint8_t* d_key_mask, const int64_t* shape, const int64_t* strides, const void* d_out,
+                               const float* d_stats, float scale, void* d_dq, void* d_dk, void* d_dv, int32_t dtype,
+                               void* d_workspace, size_t workspace_bytes, void* stream) {
+  if (int32_t rc = check("attn_bwd", shape, dtype)) return rc;
+  const Shape s = shape_of(shape);
+  const hipStream_t st = (hipStream_t)stream;
+  const size_t e = dtype == VX_F32 ? 4 : 2;
+  if (s.b == 0 || s.sq == 0 || s.sk == 0) {          // nothing attends: zero gradients
+    const size_t nq = (size_t)s.b * s.sq * s.h * s.d * e, nk = (size_t)s.b * s.sk * s.hk * s.d * e,
+                 nv = (size_t)s.b * s.sk * s.hv * s.dv * e;
+    if (nq)
+      if (int32_t rc = vx_fill_async(d_dq, 0, nq, st)) return rc;
+    if (nk)
+      if (int32_t rc = vx_fill_async(d_dk, 0, nk, st)) return rc;
+    if (nv)
+      if (int32_t rc = vx_fill_async(d_dv, 0, nv, st)) return rc;
+    return VX_OK;
+  }
+  VX_REQUIRE(strides && dout_strides && d_dout && d_q && d_k && d_v && d_out && d_stats && d_dq && d_dk && d_dv,
+             "attn_bwd: null pointer");
+  for (int i = 0; i < 10; ++i) VX_REQUIRE(strides[i] >= 0, "attn_bwd: negative stride");
+  for (int i = 0; i < 3; ++i) VX_REQUIRE(dout_strides[i] >= 0, "attn_bwd: negative stride");
+  if (workspace_bytes < bwd_plan(s, dtype).total() || !d_workspace) {
+    vx_set_error("attn_bwd: workspace too small");
+    return VX_ERR_WORKSPACE;
+  }
+  if (dtype == VX_F32)
+    return attn_bwd_typed<float>(s, d_dout, dout_strides, d_q, d_k, d_v, d_key_mask, strides, d_out, d_stats, scale, d_dq, d_dk, d_dv,
+                                 dtype, d_workspace, st);
+  return attn_bwd_typed<__bf16>(s, d_dout, dout_strides, d_q, d_k, d_v, d_key_mask, strides, d_out, d_stats, scale, d_dq, d_dk, d_dv,
+                                dtype, d_workspace, st);
+}

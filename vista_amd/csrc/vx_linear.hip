@@ -1,0 +1,315 @@
+// Dense layer with its epilogue: y = act(x w^T + bias + residual), and its backward pass (1x1 convolutions and
+// feed-forward layers of the cross-view attention block: det3d/models/necks/attention.py:36-41, :77-84, :127-146).
+// The activation comes after the residual, as in the epilogue of the sparse convolutions.
+//
+// fp32 operands run as three exact bf16 planes (six products, fp32 accumulation), bf16 ones directly; both in the tiles of
+// vx_tile.h. A reduction split over workgroups leaves fp32 slabs that one kernel adds in a fixed order: no atomics, bitwise
+// reproducible.
+#include "vx_tile.h"
+
+namespace {
+
+constexpr int kActNone = VX_ACT_NONE, kActRelu = VX_ACT_RELU, kActGelu = VX_ACT_GELU, kActSilu = VX_ACT_SILU;
+
+__device__ __forceinline__ float act_value(float a, int act) {
+  if (act == kActRelu) return a > 0.0f ? a : (a != a ? a : 0.0f);      // NaN stays NaN
+  if (act == kActGelu) return 0.5f * a * (1.0f + erff(a * 0.70710678118654752f));
+  if (act == kActSilu) return a / (1.0f + expf(-a));
+  return a;
+}
+// slope at the saved value: relu's output, the others' pre-activation
+__device__ __forceinline__ float act_slope(float a, int act) {
+  if (act == kActRelu) return a > 0.0f ? 1.0f : 0.0f;
+  if (act == kActGelu)
+    return 0.5f * (1.0f + erff(a * 0.70710678118654752f)) + a * 0.39894228040143268f * expf(-0.5f * a * a);
+  if (act == kActSilu) {
+    const float e = 1.0f / (1.0f + expf(-a));
+    return e * (1.0f + a * (1.0f - e));
+  }
+  return 1.0f;
+}
+
+template <typename T>
+struct FwdArgs {
+  const T *x, *w, *bias, *res;
+  T *y, *pre;
+  long long ldx, ldw, ldr, m;
+  int n, k, act, tiles_n;
+};
+
+template <typename T, int TM, int TN>
+__global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a) {
+  __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
+  const unsigned t = vx_xcd_tile(blockIdx.x, gridDim.x);
+  const long long m0 = (long long)(t / a.tiles_n) * TM;
+  const int n0 = (int)(t % a.tiles_n) * TN;
+  const int rows_m = (int)(a.m - m0 < TM ? a.m - m0 : TM), rows_n = a.n - n0 < TN ? a.n - n0 : TN;
+  vx_f32x4 acc[TM / 32][TN / 32];
+  vx_acc_zero(acc);
+  const VxOperand<T> X{a.x + m0 * a.ldx, a.ldx, rows_m, nullptr}, W{a.w + (long long)n0 * a.ldw, a.ldw, rows_n, nullptr};
+  vx_gemm_loop<T, KC, KC, TM, TN>(X, W, 0, a.k, lds, acc);
+  vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
+    const int left = rows_n - n;
+    if (m >= rows_m || left <= 0) return;
+    if (a.bias) v += vx_load4(a.bias + n0 + n, left);
+    if (a.res) v += vx_load4(a.res + (m0 + m) * a.ldr + n0 + n, left);
+    const long long at = (m0 + m) * a.n + n0 + n;
+    if (a.pre) vx_store4(a.pre + at, v, left);
+    if (a.act != kActNone) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = act_value(v[i], a.act);
+    }
+    vx_store4(a.y + at, v, left);
+  });
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------
+// g = dy * act'(saved) (written where there is an activation) and the column sums of g per row chunk. A workgroup owns 128
+// columns (32 lanes x 4) and a chunk of rows (8 row lanes); sums in fp32 per thread, then over the 8 row lanes in order.
+constexpr int kActCols = 128, kActRowLanes = 8;
+template <typename T>
+__global__ __launch_bounds__(256) void act_bwd(const T* __restrict__ dy, long long ldy, const T* __restrict__ saved, long long m,
+                                               int n, int act, long long chunk, T* __restrict__ g, float* __restrict__ part) {
+  __shared__ vx_f32x4 sh[kActRowLanes][32];
+  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
+  const int c = blockIdx.x * kActCols + cl * 4;
+  const long long r0 = (long long)blockIdx.y * chunk, r1 = r0 + chunk < m ? r0 + chunk : m;
+  vx_f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < n) {
+    for (long long r = r0 + rl; r < r1; r += kActRowLanes) {
+      vx_f32x4 v = vx_load4(dy + r * ldy + c, n - c);
+      if (act != kActNone) {
+        const vx_f32x4 s = vx_load4(saved + r * n + c, n - c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = act == kActRelu ? (s[i] > 0.0f ? v[i] : 0.0f) : v[i] * act_slope(s[i], act);
+        vx_store4(g + r * n + c, v, n - c);
+      }
+      sum += v;
+    }
+  }
+  if (!part) return;
+  sh[rl][cl] = sum;
+  __syncthreads();
+  if (rl == 0 && c < n) {
+#pragma unroll
+    for (int i = 1; i < kActRowLanes; ++i) sum += sh[i][cl];
+    vx_store4(part + (long long)blockIdx.y * n + c, sum, n - c);
+  }
+}
+
+template <typename T>
+struct BwdArgs {
+  const T *g, *x, *w;
+  T *dx, *dw;
+  float* slab;          // [splits][n][k] when splits > 1
+  long long ldg, ldx, ldw, m, span;   // span: rows of one split
+  int n, k, tiles_w, tiles_wk, tiles_xk;   // dw: tiles_w = all tiles of one split, tiles_wk along k; dx: tiles along k
+  unsigned blocks_w, blocks_x;
+};
+
+// one launch for both gradients: workgroups [0, blocks_w) are tiles of dw = g^T x (reduction over the rows, split), the rest
+// tiles of dx = g w (reduction over n)
+template <typename T, int TM, int TN>
+__global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a) {
+  __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
+  vx_f32x4 acc[TM / 32][TN / 32];
+  vx_acc_zero(acc);
+  if (blockIdx.x < a.blocks_w) {
+    const unsigned t = vx_xcd_tile(blockIdx.x, a.blocks_w);
+    const int split = (int)(t / a.tiles_w), tile = (int)(t % a.tiles_w);
+    const int n0 = tile / a.tiles_wk * TM, k0 = tile % a.tiles_wk * TN;
+    const long long r0 = split * a.span;
+    const int rows = (int)(a.m - r0 < a.span ? a.m - r0 : a.span);
+    const int rows_n = a.n - n0 < TM ? a.n - n0 : TM, rows_k = a.k - k0 < TN ? a.k - k0 : TN;
+    const VxOperand<T> X{a.g + r0 * a.ldg + n0, a.ldg, rows_n, nullptr}, W{a.x + r0 * a.ldx + k0, a.ldx, rows_k, nullptr};
+    vx_gemm_loop<T, KS, KS, TM, TN>(X, W, 0, rows, lds, acc);
+    float* slab = a.slab ? a.slab + (long long)split * a.n * a.k : nullptr;
+    vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
+      const int left = rows_k - n;
+      if (m >= rows_n || left <= 0) return;
+      const long long at = (long long)(n0 + m) * a.k + k0 + n;
+      if (slab) vx_store4(slab + at, v, left); else vx_store4(a.dw + at, v, left);
+    });
+  } else {
+    const unsigned t = vx_xcd_tile(blockIdx.x - a.blocks_w, a.blocks_x);
+    const long long m0 = (long long)(t / a.tiles_xk) * TM;
+    const int k0 = (int)(t % a.tiles_xk) * TN;
+    const int rows_m = (int)(a.m - m0 < TM ? a.m - m0 : TM), rows_k = a.k - k0 < TN ? a.k - k0 : TN;
+    const VxOperand<T> X{a.g + m0 * a.ldg, a.ldg, rows_m, nullptr}, W{a.w + k0, a.ldw, rows_k, nullptr};
+    vx_gemm_loop<T, KC, KS, TM, TN>(X, W, 0, a.n, lds, acc);
+    vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
+      const int left = rows_k - n;
+      if (m < rows_m && left > 0) vx_store4(a.dx + (m0 + m) * a.k + k0 + n, v, left);
+    });
+  }
+}
+
+// out[i] = sum over `count` slabs of slab[s * len + i], in order of s; two such sums in one launch (dw, dbias)
+template <typename T>
+__global__ __launch_bounds__(256) void slab_sum(const float* __restrict__ a, int count_a, long long len_a, T* __restrict__ out_a,
+                                                const float* __restrict__ b, int count_b, long long len_b,
+                                                T* __restrict__ out_b, unsigned blocks_a) {
+  const bool first = blockIdx.x < blocks_a;
+  const float* src = first ? a : b;
+  const int count = first ? count_a : count_b;
+  const long long len = first ? len_a : len_b;
+  T* out = first ? out_a : out_b;
+  const long long i = ((long long)(first ? blockIdx.x : blockIdx.x - blocks_a) * 256 + threadIdx.x) * 4;
+  if (i >= len) return;
+  const int left = len - i < 4 ? (int)(len - i) : 4;
+  vx_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int c = 0; c < count; ++c) s += vx_load4(src + c * len + i, left);
+  vx_store4(out + i, s, left);
+}
+
+struct BwdPlan {
+  bool big;
+  int64_t splits, span, chunks, chunk;
+};
+BwdPlan bwd_plan(int64_t m, int64_t n, int64_t k, int32_t dtype) {
+  BwdPlan p;
+  const int64_t cus = vx_tile_cus(), bk = dtype == VX_F32 ? 32 : 64;
+  p.big = vx_cdiv(m, 128) * vx_cdiv(k, 128) >= cus;
+  const int64_t t = p.big ? 128 : 64, tiles = vx_cdiv(n, t) * vx_cdiv(k, t);
+  int64_t splits = vx_cdiv(2 * cus, tiles);
+  const int64_t most = vx_cdiv(m, 8 * bk);
+  if (splits > most) splits = most;
+  if (splits < 1) splits = 1;
+  p.span = vx_cdiv(vx_cdiv(m, splits), bk) * bk;
+  p.splits = vx_cdiv(m, p.span);
+  p.chunk = vx_cdiv(vx_cdiv(m, vx_cdiv(4 * cus, vx_cdiv(n, kActCols))), kActRowLanes) * kActRowLanes;
+  if (p.chunk < 4 * kActRowLanes) p.chunk = 4 * kActRowLanes;
+  p.chunks = vx_cdiv(m, p.chunk);
+  return p;
+}
+
+template <typename T>
+int32_t fwd_impl(const FwdArgs<T>& args, hipStream_t s) {
+  FwdArgs<T> a = args;
+  const int64_t big = vx_cdiv(a.m, 128) * vx_cdiv(a.n, 128);
+  const bool use_big = big >= vx_tile_cus();
+  const int64_t t = use_big ? 128 : 64;
+  a.tiles_n = (int)vx_cdiv(a.n, t);
+  const int64_t grid = vx_cdiv(a.m, t) * a.tiles_n;
+  VX_REQUIRE(grid < (1LL << 31), "linear_fwd: too many rows");
+  if (use_big)
+    linear_fwd<T, 128, 128><<<(unsigned)grid, kTileThreads, 0, s>>>(a);
+  else
+    linear_fwd<T, 64, 64><<<(unsigned)grid, kTileThreads, 0, s>>>(a);
+  VX_LAUNCH_CHECK();
+  return VX_OK;
+}
+
+template <typename T>
+int32_t bwd_impl(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w, int64_t ldw, const T* saved, int64_t m, int32_t n,
+                 int32_t k, int32_t act, T* dpre, T* dx, T* dw, T* dbias, char* ws, int32_t dtype, hipStream_t s) {
+  const BwdPlan p = bwd_plan(m, n, k, dtype);
+  float* slab = (float*)ws;
+  float* part = (float*)(ws + vx_align(p.splits > 1 ? (size_t)p.splits * n * k * 4 : 0));
+  const T* g = dy;
+  int64_t ldg = lddy;
+  if (act != VX_ACT_NONE || dbias) {
+    const dim3 grid((unsigned)vx_cdiv(n, kActCols), (unsigned)p.chunks);
+    act_bwd<T><<<grid, 256, 0, s>>>(dy, lddy, saved, m, n, act, p.chunk, dpre, dbias ? part : nullptr);
+    VX_LAUNCH_CHECK();
+    if (act != VX_ACT_NONE) {
+      g = dpre;
+      ldg = n;
+    }
+  }
+  const int64_t t = p.big ? 128 : 64;
+  BwdArgs<T> a{};
+  a.g = g; a.x = x; a.w = w; a.dx = dx; a.dw = dw;
+  a.slab = p.splits > 1 ? slab : nullptr;
+  a.ldg = ldg; a.ldx = ldx; a.ldw = ldw; a.m = m; a.span = p.span; a.n = n; a.k = k;
+  a.tiles_wk = (int)vx_cdiv(k, t);
+  a.tiles_w = (int)(vx_cdiv(n, t) * a.tiles_wk);
+  a.tiles_xk = a.tiles_wk;
+  const int64_t bw = dw ? a.tiles_w * p.splits : 0, bx = dx ? vx_cdiv(m, t) * a.tiles_xk : 0;
+  VX_REQUIRE(bw + bx < (1LL << 31), "linear_bwd: too many rows");
+  a.blocks_w = (unsigned)bw;
+  a.blocks_x = (unsigned)bx;
+  if (bw + bx) {
+    if (p.big)
+      linear_bwd<T, 128, 128><<<(unsigned)(bw + bx), kTileThreads, 0, s>>>(a);
+    else
+      linear_bwd<T, 64, 64><<<(unsigned)(bw + bx), kTileThreads, 0, s>>>(a);
+    VX_LAUNCH_CHECK();
+  }
+  const int64_t len_w = dw && p.splits > 1 ? (int64_t)n * k : 0, len_b = dbias ? n : 0;
+  const unsigned ga = (unsigned)vx_cdiv(len_w, 1024), gb = (unsigned)vx_cdiv(len_b, 1024);
+  if (ga + gb) {
+    slab_sum<T><<<ga + gb, 256, 0, s>>>(slab, (int)p.splits, len_w, dw, part, (int)p.chunks, len_b, dbias, ga);
+    VX_LAUNCH_CHECK();
+  }
+  return VX_OK;
+}
+
+}  // namespace
+
+int vx_tile_cus() {
+  static int cached[64];       // benign race: every writer stores the same value
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (!cached[dev]) {
+    int n = 0;
+    cached[dev] = hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && n > 0 ? n : 256;
+  }
+  return cached[dev];
+}
+
+static int32_t linear_check(const char* who, int64_t m, int32_t n, int32_t k, int32_t act, int32_t dtype) {
+  VX_REQUIRE(dtype == VX_F32 || dtype == VX_BF16, "%s: dtype must be VX_F32 or VX_BF16", who);
+  VX_REQUIRE(act >= VX_ACT_NONE && act <= VX_ACT_SILU, "%s: unknown activation %d", who, act);
+  VX_REQUIRE(m >= 0 && m < (1LL << 31) && n >= 1 && k >= 1 && n <= (1 << 20) && k <= (1 << 20), "%s: bad sizes", who);
+  return VX_OK;
+}
+
+extern "C" int32_t vx_linear_fwd(const void* d_x, int64_t ldx, const void* d_weight, int64_t ldw, const void* d_bias,
+                                 const void* d_residual, int64_t ldr, int64_t m, int32_t n, int32_t k, int32_t act, void* d_y,
+                                 void* d_pre, int32_t dtype, void* stream) {
+  if (int32_t rc = linear_check("linear_fwd", m, n, k, act, dtype)) return rc;
+  if (m == 0) return VX_OK;
+  VX_REQUIRE(d_x && d_weight && d_y, "linear_fwd: null pointer");
+  VX_REQUIRE(ldx >= 0 && ldw >= 0 && ldr >= 0, "linear_fwd: negative row stride");
+  if (dtype == VX_F32)
+    return fwd_impl<float>({(const float*)d_x, (const float*)d_weight, (const float*)d_bias, (const float*)d_residual, (float*)d_y,
+                            (float*)d_pre, ldx, ldw, ldr, m, n, k, act, 0}, (hipStream_t)stream);
+  return fwd_impl<__bf16>({(const __bf16*)d_x, (const __bf16*)d_weight, (const __bf16*)d_bias, (const __bf16*)d_residual,
+                           (__bf16*)d_y, (__bf16*)d_pre, ldx, ldw, ldr, m, n, k, act, 0}, (hipStream_t)stream);
+}
+
+extern "C" size_t vx_linear_bwd_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t dtype) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const BwdPlan p = bwd_plan(m, n, k, dtype);
+  return vx_align(p.splits > 1 ? (size_t)p.splits * n * k * 4 : 0) + vx_align((size_t)p.chunks * n * 4);
+}
+
+extern "C" int32_t vx_linear_bwd(const void* d_dy, int64_t lddy, const void* d_x, int64_t ldx, const void* d_weight, int64_t ldw,
+                                 const void* d_saved, int64_t m, int32_t n, int32_t k, int32_t act, void* d_dpre, void* d_dx,
+                                 void* d_dw, void* d_dbias, int32_t dtype, void* d_workspace, size_t workspace_bytes,
+                                 void* stream) {
+  if (int32_t rc = linear_check("linear_bwd", m, n, k, act, dtype)) return rc;
+  const hipStream_t s = (hipStream_t)stream;
+  if (m == 0) {       // sums over no rows
+    const int64_t nk = d_dw ? (int64_t)n * k : 0, nb = d_dbias ? n : 0;
+    const size_t e = dtype == VX_F32 ? 4 : 2;
+    if (nk)
+      if (int32_t rc = vx_fill_async(d_dw, 0, nk * e, s)) return rc;
+    if (nb)
+      if (int32_t rc = vx_fill_async(d_dbias, 0, nb * e, s)) return rc;
+    return VX_OK;
+  }
+  VX_REQUIRE(d_dy && d_x && d_weight, "linear_bwd: null pointer");
+  VX_REQUIRE(lddy >= 0 && ldx >= 0 && ldw >= 0, "linear_bwd: negative row stride");
+  VX_REQUIRE(act == VX_ACT_NONE || (d_saved && d_dpre), "linear_bwd: an activation needs d_saved and d_dpre");
+  if (workspace_bytes < vx_linear_bwd_workspace_bytes(m, n, k, dtype) || !d_workspace) {
+    vx_set_error("linear_bwd: workspace too small");
+    return VX_ERR_WORKSPACE;
+  }
+  if (dtype == VX_F32)
+    return bwd_impl<float>((const float*)d_dy, lddy, (const float*)d_x, ldx, (const float*)d_weight, ldw, (const float*)d_saved, m, n,
+                           k, act, (float*)d_dpre, (float*)d_dx, (float*)d_dw, (float*)d_dbias, (char*)d_workspace, dtype, s);
+  return bwd_impl<__bf16>((const __bf16*)d_dy, lddy, (const __bf16*)d_x, ldx, (const __bf16*)d_weight, ldw, (const __bf16*)d_saved, m,
+                          n, k, act, (__bf16*)d_dpre, (__bf16*)d_dx, (__bf16*)d_dw, (__bf16*)d_dbias, (char*)d_workspace, dtype, s);
+}

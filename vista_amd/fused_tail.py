@@ -1,0 +1,152 @@
+"""The cross-view attention block of the dense tail on hand-written kernels, forward and backward.
+
+`attention` and `linear_act` are differentiable torch functions over the libvx kernels of vista_amd/csrc/vx_attn.hip and
+vx_linear.hip (HIP tensors, float32 or bfloat16, no CPU path); `fuse_cross_attention(module)` rewrites the
+ConvAttentionLayer_Decouple and FeedFowardLayer of a module to run on them:
+  attention   det3d/models/necks/attention.py:55-124   both read-outs as two query / key heads over one value head
+  linear_act  attention.py:36-41 (1x1 value / out convolutions, identity added in the epilogue), :127-146 (feed-forward)
+Gradients are exact formulas of the saved tensors (once differentiable). Both run on the caller's stream, allocate through
+torch's caching allocator only, and can be captured in a HIP graph.
+"""
+import torch
+from torch import nn
+
+from . import ops
+from .dense_tail import ConvAttentionLayer_Decouple, FeedFowardLayer
+
+
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, key_mask, scale):
+        out, stats = ops.attn_fwd(q, k, v, key_mask, scale, want_stats=True)
+        ctx.save_for_backward(q, k, v, key_mask, out, stats)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, key_mask, out, stats = ctx.saved_tensors
+        grads = ops.attn_bwd(dout, q, k, v, out, stats, key_mask, ctx.scale)
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None)
+
+
+def attention(q, k, v, key_mask=None, scale=None):
+    """softmax(scale q k^T) v. q [b, sq, heads, dim], k [b, sk, k_heads, dim], v [b, sk, v_heads, v_dim] -> [b, sq, heads, v_dim];
+    key and value heads are shared by consecutive query heads. key_mask: bool [b, sk], True where the key takes part; a masked key
+    has no part in the output or any gradient, whatever it holds, and a query without keys gives zeros. scale defaults to
+    dim ** -0.5; dim <= 192, v_dim <= 384."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+        return _AttentionFn.apply(q, k, v, key_mask, scale)
+    return ops.attn_fwd(q, k, v, key_mask, scale)[0]
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        y, pre = ops.linear_fwd(x, weight, bias, residual, act, want_pre=act in ("gelu", "silu"))
+        ctx.save_for_backward(x, weight, y if act == "relu" else pre)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, saved = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db, dpre = ops.linear_bwd(dy, x, weight, ctx.act, saved, *need[:3])
+        return dx, dw, db, dpre if need[3] else None, None
+
+
+def linear_act(x, weight, bias=None, residual=None, act="none"):
+    """act(x w^T + bias + residual) over the last dimension of x [..., fin]; weight [fout, fin], bias [fout], residual
+    [..., fout]. act: none, relu, gelu (erf form), silu; it comes after the residual, as in the sparse convolutions' epilogue."""
+    if x.dim() < 1 or (residual is not None and residual.shape[:-1] != x.shape[:-1]):
+        raise ValueError("x must be [..., fin] and residual [..., fout] with the same leading dimensions")
+    lead = x.shape[:-1]
+    x2 = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    r2 = residual.reshape(-1, residual.shape[-1]) if residual is not None and residual.dim() != 2 else residual
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        y = _LinearFn.apply(x2, weight, bias, r2, act)
+    else:
+        y = ops.linear_fwd(x2, weight, bias, r2, act)[0]
+    return y if x.dim() == 2 else y.view(*lead, weight.shape[0])
+
+
+def _conv1x1(conv, x, residual=None):
+    """A 1x1 nn.Conv2d over tokens [..., c] instead of a map [b, c, h, w]."""
+    return linear_act(x, conv.weight.flatten(1), conv.bias, residual)
+
+
+class FusedConvAttention(nn.Module):
+    """ConvAttentionLayer_Decouple on `attention` and `linear_act`; shares the layer's submodules, so parameters and
+    state_dict keys are the layer's. The attention maps are not formed: need_maps=True runs the layer's own forward."""
+
+    def __init__(self, layer):
+        super().__init__()
+        for name, child in layer.named_children():
+            self.add_module(name, child)
+        self.channels, self.numhead, self.head_dim = layer.channels, layer.numhead, layer.head_dim
+
+    def forward(self, query, key, value, q_pos_emb=None, k_pos_emb=None, need_maps=True, key_mask=None):
+        """-> ([tokens[HW_q, B, C]] x2, [None, None]); key_mask bool [B, HW_kv], True where the key block takes part."""
+        if need_maps:
+            if key_mask is not None:
+                raise ValueError("key_mask is supported without attention maps only (need_maps=False)")
+            return ConvAttentionLayer_Decouple.forward(self, query, key, value, q_pos_emb, k_pos_emb, True)
+        identity = query
+        if q_pos_emb is not None:
+            query = query + q_pos_emb
+        if k_pos_emb is not None:
+            shared = value is key            # the embedding reaches the value path too (attention.py:64-65, :206)
+            key = key + k_pos_emb
+            if shared:
+                value = key
+        b, c, hq, wq = identity.shape
+        n, sq = self.numhead, hq * wq
+
+        def tokens(t):                       # [B, c, H, W] -> [B, H*W, c]
+            return t.flatten(2).transpose(1, 2).contiguous()
+
+        def heads(sem, geo):                 # two maps -> [B, H*W, 2 n, d], a head's read-outs side by side
+            s = torch.stack([sem.flatten(2), geo.flatten(2)], 1).view(b, 2, n, self.head_dim, -1)
+            return s.permute(0, 4, 2, 1, 3).reshape(b, -1, 2 * n, self.head_dim)
+
+        v = _conv1x1(self.v_conv, tokens(value)).view(b, -1, n, c // n)
+        r = attention(heads(self.q_sem_conv(query), self.q_geo_conv(query)), heads(self.k_sem_conv(key), self.k_geo_conv(key)),
+                      v, key_mask, float(self.head_dim) ** -0.5).view(b, sq, n, 2, c // n)
+        rows = tokens(identity)
+        outs = []
+        for i, (conv, norm) in enumerate(((self.out_sem_conv, self.sem_norm), (self.out_geo_conv, self.geo_norm))):
+            y = norm(_conv1x1(conv, r[:, :, :, i].reshape(b, sq, c), rows))
+            outs.append(y.transpose(0, 1))
+        return outs, [None, None]
+
+
+class FusedFeedForward(nn.Module):
+    """FeedFowardLayer on `linear_act`: ReLU in the first product's epilogue, the residual in the second's."""
+
+    def __init__(self, layer):
+        super().__init__()
+        for name, child in layer.named_children():
+            self.add_module(name, child)
+
+    def forward(self, view):
+        flip = view.dim() == 3 and not view.is_contiguous()     # FusedConvAttention's tokens: rows in memory order
+        x = view.transpose(0, 1) if flip else view
+        h = linear_act(x, self.linear1.weight, self.linear1.bias, act="relu")
+        y = self.norm(linear_act(h, self.linear2.weight, self.linear2.bias, x))
+        return y.transpose(0, 1) if flip else y
+
+
+def fuse_cross_attention(module):
+    """Rewrite `module` in place: every ConvAttentionLayer_Decouple and FeedFowardLayer in it runs on the fused kernels
+    (inference and training; HIP tensors only from then on, unless attention maps are asked for). Parameters, buffers and
+    state_dict keys are unchanged. Returns `module`, or its replacement when it is such a layer itself."""
+    swap = {ConvAttentionLayer_Decouple: FusedConvAttention, FeedFowardLayer: FusedFeedForward}
+    if type(module) in swap:
+        return swap[type(module)](module).train(module.training)
+    for name, child in list(module._modules.items()):
+        if child is not None:
+            module._modules[name] = fuse_cross_attention(child)
+    return module

@@ -591,3 +591,176 @@ def bn_bwd_apply(dy, x, mask, mean, invstd, gamma, sums, count, want_dres=False)
                                      _ptr(sums), _ptr(count), _ptr(dx), _ptr(dres), _stream())
     L.check(rc, "vx_bn_bwd_apply")
     return dx, dres
+
+
+# ------------------------------------------------------------------------------------------------
+# dense layer with its epilogue, attention
+# ------------------------------------------------------------------------------------------------
+def _on_one_device(first, **tensors):
+    _need_gpu(first[1], first[0])
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        _need_gpu(t, name)
+        if t.device != first[1].device:
+            raise ValueError(f"{name} is on {t.device}, {first[0]} on {first[1].device}")
+
+
+def _same_dtype(first, **tensors):
+    if first[1].dtype not in _DT:
+        raise ValueError(f"unsupported {first[0]} dtype {first[1].dtype}: float32 or bfloat16")
+    for name, t in tensors.items():
+        if t is not None and t.dtype != first[1].dtype:
+            raise ValueError(f"{name} is {t.dtype}, {first[0]} {first[1].dtype}: they must share a dtype")
+
+
+def _act_code(act):
+    try:
+        return L.VX_ACT[act]
+    except (KeyError, TypeError):
+        raise ValueError(f"act must be one of {sorted(L.VX_ACT)}, got {act!r}") from None
+
+
+def _rows(t):
+    """A 2-D tensor whose last dimension is contiguous (a copy only when it is not)."""
+    return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _linear_check(x, weight):
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} must be [rows, fin] and [fout, fin]")
+    if weight.shape[0] < 1 or weight.shape[1] < 1 or max(weight.shape) > 1 << 20 or x.shape[0] >= 1 << 31:
+        raise ValueError(f"sizes out of range: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
+
+
+def linear_fwd(x, weight, bias=None, residual=None, act="none", want_pre=False):
+    """x [m, k], weight [n, k], bias [n], residual [m, n] -> (y [m, n], pre [m, n] | None): y = act(x w^T + bias + residual),
+    pre (want_pre) = the sum before the activation. One dtype (float32 or bfloat16); act: none, relu, gelu (erf form), silu."""
+    _on_one_device(("x", x), weight=weight, bias=bias, residual=residual)
+    _same_dtype(("x", x), weight=weight, bias=bias, residual=residual)
+    code = _act_code(act)
+    _linear_check(x, weight)
+    (m, k), n = x.shape, weight.shape[0]
+    if bias is not None and tuple(bias.shape) != (n,):
+        raise ValueError(f"bias must be [{n}], got {tuple(bias.shape)}")
+    if residual is not None and tuple(residual.shape) != (m, n):
+        raise ValueError(f"residual must be [{m}, {n}], got {tuple(residual.shape)}")
+    x, weight = _rows(x), _rows(weight)
+    bias = bias.contiguous() if bias is not None else None
+    residual = _rows(residual) if residual is not None else None
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    pre = torch.empty_like(y) if want_pre else None
+    with torch.cuda.device(x.device), _Timed("linear", m=m, n=n, k=k, esize=x.element_size()):
+        rc = L.lib().vx_linear_fwd(_ptr(x), x.stride(0), _ptr(weight), weight.stride(0), _ptr(bias), _ptr(residual),
+                                   residual.stride(0) if residual is not None else 0, m, n, k, code, _ptr(y), _ptr(pre),
+                                   _DT[x.dtype], _stream())
+    L.check(rc, "vx_linear_fwd")
+    return y, pre
+
+
+def linear_bwd(dy, x, weight, act="none", saved=None, want_dx=True, want_dw=True, want_dbias=True):
+    """Gradients of linear_fwd -> (dx [m, k], dw [n, k], dbias [n], dpre [m, n]); an unwanted one is None. saved = y of relu,
+    pre of gelu / silu, unused without an activation. dpre = dy * act'(saved) is the residual's gradient (dy itself
+    without an activation)."""
+    _on_one_device(("dy", dy), x=x, weight=weight, saved=saved)
+    _same_dtype(("dy", dy), x=x, weight=weight, saved=saved)
+    code = _act_code(act)
+    _linear_check(x, weight)
+    (m, k), n = x.shape, weight.shape[0]
+    if tuple(dy.shape) != (m, n):
+        raise ValueError(f"dy must be [{m}, {n}], got {tuple(dy.shape)}")
+    if code and (saved is None or tuple(saved.shape) != (m, n)):
+        raise ValueError(f"act={act!r} needs saved [{m}, {n}]: relu's output, the pre-activation of gelu / silu")
+    x, weight, g = _rows(x), _rows(weight), _rows(dy)
+    saved = saved.contiguous() if code else None
+    dev, dt = x.device, x.dtype
+    dpre = torch.empty((m, n), dtype=dt, device=dev) if code else dy
+    dx = torch.empty((m, k), dtype=dt, device=dev) if want_dx else None
+    dw = torch.empty((n, k), dtype=dt, device=dev) if want_dw else None
+    db = torch.empty((n,), dtype=dt, device=dev) if want_dbias else None
+    lib = L.lib()
+    with torch.cuda.device(dev):
+        wsb = lib.vx_linear_bwd_workspace_bytes(m, n, k, _DT[dt])
+        ws = _ws(wsb, dev)
+        rc = lib.vx_linear_bwd(_ptr(g), g.stride(0), _ptr(x), x.stride(0), _ptr(weight), weight.stride(0), _ptr(saved), m, n, k,
+                               code, _ptr(dpre) if code else None, _ptr(dx), _ptr(dw), _ptr(db), _DT[dt], _ptr(ws), wsb, _stream())
+    L.check(rc, "vx_linear_bwd")
+    return dx, dw, db, dpre
+
+
+def _heads_last(t):
+    """[batch, position, head, width] with a contiguous last dimension (a copy only when it is not)."""
+    return t if t.shape[3] == 1 or t.stride(3) == 1 else t.contiguous()
+
+
+def _attn_args(q, k, v, key_mask):
+    _on_one_device(("q", q), k=k, v=v, key_mask=key_mask)
+    _same_dtype(("q", q), k=k, v=v)
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("q, k and v must be [batch, length, heads, width]")
+    b, sq, h, d = q.shape
+    sk, hk, hv, dv = k.shape[1], k.shape[2], v.shape[2], v.shape[3]
+    if k.shape[0] != b or v.shape[0] != b or v.shape[1] != sk or k.shape[3] != d:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+    if h < 1 or hk < 1 or hv < 1 or h % hk or h % hv:
+        raise ValueError(f"key heads ({hk}) and value heads ({hv}) must divide the query heads ({h})")
+    if not (1 <= d <= L.VX_ATTN_MAX_DIM and 1 <= dv <= L.VX_ATTN_MAX_VDIM):
+        raise ValueError(f"head width must be in [1, {L.VX_ATTN_MAX_DIM}], value width in [1, {L.VX_ATTN_MAX_VDIM}], got {d}, {dv}")
+    if b >= 1 << 24 or sq >= 1 << 30 or sk >= 1 << 30 or h >= 1 << 16 or b * h >= 1 << 24:
+        raise ValueError("attention sizes out of range")
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (b, sk):
+            raise ValueError(f"key_mask must be bool [{b}, {sk}] (True: the key takes part), got {key_mask.dtype} "
+                             f"{tuple(key_mask.shape)}")
+        key_mask = key_mask if sk <= 1 or key_mask.stride(1) == 1 else key_mask.contiguous()
+    q, k, v = _heads_last(q), _heads_last(k), _heads_last(v)
+    shape = (ctypes.c_int64 * 8)(b, sq, sk, h, hk, hv, d, dv)
+    strides = (ctypes.c_int64 * 10)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                                    key_mask.stride(0) if key_mask is not None else 0)
+    return q, k, v, key_mask, shape, strides
+
+
+def attn_fwd(q, k, v, key_mask=None, scale=None, want_stats=False):
+    """softmax(scale q k^T) v over q [b, sq, h, d], k [b, sk, hk, d], v [b, sk, hv, dv] -> (out [b, sq, h, dv], stats | None).
+    Query head i reads key head i // (h / hk) and value head i // (h / hv); key_mask bool [b, sk], True where the key takes part;
+    a query without keys gives zeros. scale defaults to d ** -0.5. stats (want_stats) is what attn_bwd needs. Any strides with
+    a contiguous last dimension are read in place."""
+    q, k, v, key_mask, shape, strides = _attn_args(q, k, v, key_mask)
+    b, sq, h, d = q.shape
+    scale = d ** -0.5 if scale is None else float(scale)
+    out = torch.empty((b, sq, h, v.shape[3]), dtype=q.dtype, device=q.device)
+    stats = torch.empty((b * h, sq, 2), dtype=torch.float32, device=q.device) if want_stats else None
+    lib = L.lib()
+    with torch.cuda.device(q.device), _Timed("attn", b=b, sq=sq, sk=k.shape[1], h=h, d=d, dv=v.shape[3], esize=q.element_size()):
+        wsb = lib.vx_attn_fwd_workspace_bytes(shape, _DT[q.dtype])
+        ws = _ws(wsb, q.device) if wsb else None
+        rc = lib.vx_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(key_mask), shape, strides, scale, _ptr(out), _ptr(stats),
+                             _DT[q.dtype], _ptr(ws), wsb, _stream())
+    L.check(rc, "vx_attn_fwd")
+    return out, stats
+
+
+def attn_bwd(dout, q, k, v, out, stats, key_mask=None, scale=None):
+    """Gradients of attn_fwd from its own out and stats -> (dq, dk, dv), shaped as q, k and v; the probabilities are recomputed.
+    Gradients of masked keys are 0."""
+    q, k, v, key_mask, shape, strides = _attn_args(q, k, v, key_mask)
+    b, sq, h, d = q.shape
+    dv_ = v.shape[3]
+    _on_one_device(("q", q), dout=dout, out=out, stats=stats)
+    _same_dtype(("q", q), dout=dout, out=out)
+    if tuple(dout.shape) != (b, sq, h, dv_) or tuple(out.shape) != (b, sq, h, dv_) or not out.is_contiguous():
+        raise ValueError(f"dout and out must be [{b}, {sq}, {h}, {dv_}], out contiguous (attn_fwd's own)")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (b * h, sq, 2) or not stats.is_contiguous():
+        raise ValueError("stats must be what attn_fwd(want_stats=True) returned")
+    scale = d ** -0.5 if scale is None else float(scale)
+    dout = _heads_last(dout)
+    dout_strides = (ctypes.c_int64 * 3)(*dout.stride()[:3])
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    lib = L.lib()
+    with torch.cuda.device(q.device):
+        wsb = lib.vx_attn_bwd_workspace_bytes(shape, _DT[q.dtype])
+        ws = _ws(wsb, q.device)
+        rc = lib.vx_attn_bwd(_ptr(dout), dout_strides, _ptr(q), _ptr(k), _ptr(v), _ptr(key_mask), shape, strides, _ptr(out),
+                             _ptr(stats), scale, _ptr(dq), _ptr(dk), _ptr(dv), _DT[q.dtype], _ptr(ws), wsb, _stream())
+    L.check(rc, "vx_attn_bwd")
+    return dq, dk, dv
