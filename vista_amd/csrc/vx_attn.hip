@@ -45,23 +45,31 @@ __device__ __forceinline__ bool attn_key_live(const AttnArgs<T>& a, const uint8_
   return lane < AttnTile<T>::KT && key < a.sk && (mask == nullptr || mask[key] != 0);
 }
 
-// A workgroup (4 waves) owns 64 * RT queries of one head, wave w 16 * RT of them; everything is kept transposed --
-// S^T = K Q^T, O^T = V^T P^T -- so that a lane holds ONE query (c = lane & 15) and the softmax statistics, the rescaling
-// and the operand form of P are lane-local. A lane's S values are keys {16 t + 4 g + i}; as an operand they are the eight
-// k's of its group g in the order (t, i), and the V^T image is staged in that order of keys.
-template <typename T, int DP, int DVP, int RT>
-__global__ __launch_bounds__(kTileThreads, (DVP > 192 || (DVP > 64 && VxType<T>::NPL == 3)) ? 1 : 2) void attn_fwd(const FwdArgs<T> a) {
+// A workgroup owns 16 * RT * QG queries of one head: QG groups of 16 * RT, each with CS waves. Everything is kept transposed --
+// S^T = K Q^T, O^T = V^T P^T -- so that a lane holds ONE query per block (c = lane & 15) and the softmax statistics, the
+// rescaling and the operand form of P are lane-local. A lane's S values are keys {16 t + 4 g + i}; as an operand they are the
+// eight k's of its group g in the order (t, i), and the V^T image is staged in that order of keys.
+// CS = 2 (wide heads): the two waves of a group hold one half of the output columns each, compute the scores of one half of a
+// tile's keys each, and swap them through LDS as they are (a lane reads what the same lane of the other wave wrote).
+// A tile: V(t) travels to registers under S(t), then to LDS; K(t + 1) under O += P V(t). So at most one of the two is held in
+// registers, and each image is rewritten only after the barrier behind its last reader.
+template <typename T, int DP, int DVP, int RT, int QG, int CS, bool FAST>
+__global__ __launch_bounds__(64 * QG * CS, (DVP > 192 && QG * CS == 4) || (DVP > 64 && VxType<T>::NPL == 3) ? 1 : 2)
+void attn_fwd(const FwdArgs<T> a) {
   constexpr int NPL = VxType<T>::NPL, KT = AttnTile<T>::KT, NS = KT / 32;     // NS: 32-key steps of a tile
-  constexpr int KD = DP / 32, NV = DVP / 16;
-  constexpr int K_FRAGS = KT / 16 * KD, V_FRAGS = NV * NS;
-  constexpr int K_PLANE = K_FRAGS * kFragBytes, V_PLANE = V_FRAGS * kFragBytes;
-  constexpr int KI = (K_FRAGS + 3) / 4;                                        // K fragments staged per wave
-  constexpr int VW = (DVP % 128 == 0 || sizeof(T) == 2) ? 2 : 1;               // V columns per staged item
-  constexpr int V_ITEMS = DVP / VW * (KT / 8), VI = (V_ITEMS + kTileThreads - 1) / kTileThreads;
-  __shared__ __attribute__((aligned(16))) char lds[(K_PLANE + V_PLANE) * NPL];
-  char *ik = lds, *iv = lds + K_PLANE * NPL;
+  constexpr int KD = DP / 32, NV = DVP / 16 / CS, NK = KT / 16, OWN = NK / CS, E = sizeof(T), NW = QG * CS;
+  constexpr int K_FRAGS = NK * KD;
+  constexpr int K_PLANE = NK * vx_image_block<KD>(), V_PLANE = DVP / 16 * vx_image_block<NS>();
+  constexpr int KI = (K_FRAGS + NW - 1) / NW;                                  // K fragments staged per wave
+  constexpr int CB = DVP % 128 == 0 ? 128 : 64, VW = E == 2 ? CB / 32 : CB / 64;   // columns of a staged block and of a lane
+  constexpr int LR = CB / VW, LG = 64 / LR;                                    // lanes of a row, key groups of a wave
+  constexpr int V_UNITS = DVP / CB * (KT / 8) / LG, VI = (V_UNITS + NW - 1) / NW;
+  constexpr int SWAP = CS == 2 ? NW * OWN * RT * kFragBytes : 0;
+  __shared__ __attribute__((aligned(16))) char lds[(K_PLANE + V_PLANE) * NPL + SWAP];
+  char *ik = lds, *iv = lds + K_PLANE * NPL, *swap = iv + V_PLANE * NPL;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const int half = wave % CS;
   unsigned w = vx_xcd_tile(blockIdx.x, gridDim.x);
   const int tile_q = (int)(w % a.tiles_q);
   w /= a.tiles_q;
@@ -72,21 +80,25 @@ __global__ __launch_bounds__(kTileThreads, (DVP > 192 || (DVP > 64 && VxType<T>:
   const T* kp = a.k + b * a.k_b + (h / a.gk) * a.k_h;
   const T* vp = a.v + b * a.v_b + (h / a.gv) * a.v_h;
   const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
-  const int q0 = tile_q * (64 * RT) + wave * (16 * RT);
+  const int q0 = (tile_q * QG + wave / CS) * (16 * RT);
 
   VxFrag<NPL> qf[RT][KD];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int row = q0 + rt * 16 + c;
-    const T* qp = a.q + b * a.q_b + row * a.q_s + h * a.q_h;
+    const T* qp = a.q + b * a.q_b + q0 * a.q_s + h * a.q_h;
 #pragma unroll
     for (int kd = 0; kd < KD; ++kd) {
       VxRow8<T> x;
-      x.load(qp + kd * 32 + g * 8, row < a.sq ? a.d - kd * 32 - g * 8 : 0);
+      const int d = kd * 32 + g * 8;
+      if constexpr (FAST)
+        x.load(vx_buffer(qp), row < a.sq && d < a.d ? (rt * 16 + c) * (int)a.q_s * E + d * E : kVxOut);
+      else
+        x.load(qp + (rt * 16 + c) * a.q_s + d, row < a.sq ? a.d - d : 0);
       x.planes(qf[rt][kd]);
     }
   }
-  float m[RT], l[RT];
+  float m[RT], l[RT];                          // reference of the exponents (log2), sum of this lane's keys
   vx_f32x4 o[RT][NV];
   vx_acc_zero(o);
 #pragma unroll
@@ -95,115 +107,192 @@ __global__ __launch_bounds__(kTileThreads, (DVP > 192 || (DVP > 64 && VxType<T>:
     l[rt] = 0.0f;
   }
 
-  VxRow8<T> ks[KI];
-  VxCol8<T, VW> vs[VI];
-  auto load = [&](int t, unsigned long long live) {
+  // fragment (key block, k step) i of a wave: lane offsets are loop constants, the rest of an address is wave-uniform
+  const int k_lane = c * (int)a.k_s * E + g * 8 * E;
+  auto load_k = [&](VxRow8<T> (&ks)[KI], int t) {
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
-      const int frag = i * 4 + wave, key = t * KT + frag / KD * 16 + c, d = frag % KD * 32 + g * 8;
-      ks[i].load(kp + key * a.k_s + d, frag < K_FRAGS && key < a.sk ? a.d - d : 0);
-    }
-#pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      const int item = i * kTileThreads + tid, n = item % (DVP / VW) * VW, kg = item / (DVP / VW);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int kk = kg / 4 * 32 + (j >> 2) * 16 + kg % 4 * 4 + (j & 3);     // operand order of the keys, see above
-        vs[i].load(j, vp + (t * KT + kk) * a.v_s + n, item < V_ITEMS && (live >> kk & 1) ? a.dv - n : 0);
-      }
+      const int frag = i * NW + wave, kt = frag / KD, kd = frag % KD;
+      const bool here = frag < K_FRAGS && t * KT + kt * 16 + c < a.sk && kd * 32 + g * 8 < a.d;
+      const T* base = kp + (t * KT + kt * 16) * a.k_s + kd * 32;
+      if constexpr (FAST)
+        ks[i].load(vx_buffer(base), here ? k_lane : kVxOut);
+      else
+        ks[i].load(base + c * a.k_s + g * 8, here ? a.d - kd * 32 - g * 8 : 0);
     }
   };
-  auto store = [&]() {
+  auto store_k = [&](const VxRow8<T> (&ks)[KI]) {
     VxFrag<NPL> f;
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
-      const int frag = i * 4 + wave;
-      if (frag < K_FRAGS) {
+      const int frag = i * NW + wave;
+      if (K_FRAGS % NW == 0 || frag < K_FRAGS) {
         ks[i].planes(f);
-        vx_frag_store(ik, K_PLANE, frag, frag / KD, lane, f);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      const int item = i * kTileThreads + tid, n = item % (DVP / VW) * VW, kg = item / (DVP / VW);
-      if (item < V_ITEMS) {
-#pragma unroll
-        for (int j = 0; j < VW; ++j) {
-          vs[i].planes(j, f);
-          vx_frag_store(iv, V_PLANE, ((n + j) >> 4) * NS + kg / 4, n >> 4, ((n + j) & 15) + 16 * (kg % 4), f);
-        }
+        vx_frag_store(ik + vx_image_at<KD>(frag / KD, frag % KD, lane), K_PLANE, f);
       }
     }
   };
-
-  const bool any = q0 < a.sq;                  // a wave without queries only stages
-  unsigned long long cur = t0 < t1 ? __ballot(attn_key_live(a, mask, t0, lane)) : 0;
-  unsigned long long nxt = t0 + 1 < t1 ? __ballot(attn_key_live(a, mask, t0 + 1, lane)) : 0;
-  if (cur) load(t0, cur);
-  for (int t = t0; t < t1; ++t) {
-    if (cur) store();                          // a tile without keys is neither loaded nor multiplied
-    const bool ahead = t + 2 < t1 && attn_key_live(a, mask, t + 2, lane);
-    __syncthreads();
-    if (nxt) load(t + 1, nxt);
-    if (cur && any) {
-      vx_f32x4 s[RT][KT / 16];
-      vx_acc_zero(s);
+  // V unit i of a wave: a block of CB columns and LG key groups of eight (operand order of the keys, see above)
+  const int vl = lane % LR * VW, vg = lane / LR;
+  const int v_lane = vg * 4 * (int)a.v_s * E + vl * E;
+  auto load_v = [&](VxCol8<T, VW> (&vs)[VI], int t, unsigned long long live) {
+    const unsigned long long bits = live >> (vg * 4);
 #pragma unroll
-      for (int kt = 0; kt < KT / 16; ++kt)
+    for (int i = 0; i < VI; ++i) {
+      const int u = i * NW + wave, nb = u % (DVP / CB) * CB, kg = u / (DVP / CB) * LG;
+      const int at = u < V_UNITS && nb + vl < a.dv ? v_lane : kVxOut;
 #pragma unroll
-        for (int kd = 0; kd < KD; ++kd) {
-          VxFrag<NPL> kf;
-          vx_frag_load(ik, K_PLANE, kt * KD + kd, kt, lane, kf);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[rt][kt] = vx_mma(kf, qf[rt][kd], s[rt][kt]);
-        }
-      VxFrag<NPL> pf[RT][NS];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int kt = 0; kt < KT / 16; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool live = cur >> (kt * 16 + g * 4 + i) & 1;
-            s[rt][kt][i] = live ? s[rt][kt][i] * a.scale2 : -INFINITY;
-            mx = fmaxf(mx, s[rt][kt][i]);
-          }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mn = fmaxf(m[rt], mx), ref = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = exp2f(m[rt] - ref);
-        m[rt] = mn;
-        float sum = 0.0f;
-#pragma unroll
-        for (int ns = 0; ns < NS; ++ns) {
-          float p[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            p[j] = exp2f(s[rt][ns * 2 + (j >> 2)][j & 3] - ref);
-            sum += p[j];
-          }
-          vx_planes(p, pf[rt][ns]);
-        }
-        l[rt] = l[rt] * alpha + sum;
-        if (__any(alpha != 1.0f)) {
-#pragma unroll
-          for (int nv = 0; nv < NV; ++nv) o[rt][nv] *= alpha;
-        }
+      for (int j = 0; j < 8; ++j) {
+        const int kk = kg / 4 * 32 + (j >> 2) * 16 + kg % 4 * 4 + (j & 3);
+        const bool here = bits >> kk & 1;
+        const T* base = vp + (t * KT + kk) * a.v_s + nb;
+        if constexpr (FAST)
+          vs[i].load(j, vx_buffer(base), here ? at : kVxOut, 0);
+        else
+          vs[i].load(j, base + vg * 4 * a.v_s + vl, here && u < V_UNITS ? a.dv - nb - vl : 0);
       }
+    }
+  };
+  auto store_v = [&](const VxCol8<T, VW> (&vs)[VI]) {
+    VxFrag<NPL> f;
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv)
+    for (int i = 0; i < VI; ++i) {
+      const int u = i * NW + wave, nb = u % (DVP / CB) * CB, kg = u / (DVP / CB) * LG;
+      if (V_UNITS % NW != 0 && u >= V_UNITS) continue;
 #pragma unroll
-        for (int ns = 0; ns < NS; ++ns) {
-          VxFrag<NPL> vf;
-          vx_frag_load(iv, V_PLANE, nv * NS + ns, nv, lane, vf);
+      for (int j = 0; j < VW; ++j) {
+        vs[i].planes(j, f);
+        vx_frag_store(iv + nb / 16 * vx_image_block<NS>() + vx_image_at<NS>((vl + j) >> 4, kg / 4, ((vl + j) & 15) + 16 * (kg % 4 + vg)),
+                      V_PLANE, f);
+      }
+    }
+  };
+  // the first tile from t on that has a key that takes part, and which of its keys do
+  auto find = [&](int t, unsigned long long& live) {
+    for (live = 0; t < t1; ++t) {
+      live = __ballot(attn_key_live(a, mask, t, lane));
+      if (live) break;
+    }
+    return t;
+  };
+
+  unsigned long long cur, nxt = 0;
+  int t = find(t0, cur), tn = t1;
+  if (cur) {
+    tn = find(t + 1, nxt);
+    VxRow8<T> ks[KI];
+    load_k(ks, t);
+    store_k(ks);
+  }
+  __syncthreads();
+  while (cur) {
+    const bool ahead = tn + 1 < t1 && attn_key_live(a, mask, tn + 1, lane);
+    vx_f32x4 s[RT][NK];
+    {
+      VxCol8<T, VW> vs[VI];
+      load_v(vs, t, cur);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) o[rt][nv] = vx_mma(vf, pf[rt][ns], o[rt][nv]);
-        }
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) s[rt][k] = vx_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int kd = 0; kd < KD; ++kd) {
+        VxFrag<NPL> kf[OWN];
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) vx_frag_load(ik + vx_image_at<KD>(half * OWN + k, kd, lane), K_PLANE, kf[k]);
+#pragma unroll
+        for (int pr = 0; pr < VxProducts<NPL>::N; ++pr)
+#pragma unroll
+          for (int k = 0; k < OWN; ++k)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) s[rt][k] = vx_mma(pr, kf[k], qf[rt][kd], s[rt][k]);
+        if constexpr (DVP > 128) __builtin_amdgcn_sched_barrier(0);   // keeps later fragment reads out of the registers
+      }
+      if constexpr (CS == 2) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int k = 0; k < OWN; ++k)
+            *reinterpret_cast<vx_f32x4*>(swap + (wave * OWN * RT + rt * OWN + k) * kFragBytes + lane * 16) = s[rt][k];
+      }
+      store_v(vs);
     }
     __syncthreads();
+    VxRow8<T> ks[KI];
+    if (nxt) load_k(ks, tn);
+    if constexpr (CS == 2) {                   // both halves, in the order of the keys
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+          s[rt][k] = *reinterpret_cast<const vx_f32x4*>(swap + (((wave & ~1) + k / OWN) * OWN * RT + rt * OWN + k % OWN) * kFragBytes + lane * 16);
+    }
+    VxFrag<NPL> pf[RT][NS];
+    float alpha[RT];
+    bool moved = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool live = cur >> (k * 16 + g * 4 + i) & 1;
+          s[rt][k][i] = live ? s[rt][k][i] * a.scale2 : -INFINITY;
+          mx = fmaxf(mx, s[rt][k][i]);
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      // the reference follows the maximum only when it is 2^8 behind: values stay below 2^8, far from any limit of fp32, and the
+      // accumulators are hardly ever rescaled
+      const bool far = mx > m[rt] + 8.0f;
+      alpha[rt] = far ? __builtin_amdgcn_exp2f(m[rt] - mx) : 1.0f;
+      m[rt] = far ? mx : m[rt];
+      moved |= far;
+      const float ref = m[rt] == -INFINITY ? 0.0f : m[rt];
+      float sum = 0.0f;
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns) {
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          p[j] = __builtin_amdgcn_exp2f(s[rt][ns * 2 + (j >> 2)][j & 3] - ref);
+          sum += p[j];
+        }
+        vx_planes(p, pf[rt][ns]);
+      }
+      l[rt] = l[rt] * alpha[rt] + sum;
+    }
+    if (__any(moved)) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int nv = 0; nv < NV; ++nv) o[rt][nv] *= alpha[rt];
+    }
+    constexpr int G = 2;                       // column blocks at a time: independent accumulators
+#pragma unroll
+    for (int nv = 0; nv < NV; nv += G) {
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns) {
+        VxFrag<NPL> vf[G];
+#pragma unroll
+        for (int u = 0; u < G; ++u) vx_frag_load(iv + vx_image_at<NS>(half * NV + nv + u, ns, lane), V_PLANE, vf[u]);
+#pragma unroll
+        for (int pr = 0; pr < VxProducts<NPL>::N; ++pr)
+#pragma unroll
+          for (int u = 0; u < G; ++u)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) o[rt][nv + u] = vx_mma(pr, vf[u], pf[rt][ns], o[rt][nv + u]);
+      }
+      if (nv % 4 == 2) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (nxt) store_k(ks);
+    __syncthreads();
+    t = tn;
     cur = nxt;
+    tn = tn + 1;
     nxt = __ballot(ahead);
+    if (cur && !nxt) tn = find(tn + 1, nxt);
   }
 
 #pragma unroll
@@ -213,17 +302,18 @@ __global__ __launch_bounds__(kTileThreads, (DVP > 192 || (DVP > 64 && VxType<T>:
     sum += __shfl_xor(sum, 32, 64);
     const int row = q0 + rt * 16 + c;
     if (row >= a.sq) continue;
+    const int n0 = half * NV * 16 + g * 4;
     if (a.splits > 1) {
       const long long at = ((long long)split * gridDim.x / (a.tiles_q * a.splits) + bh) * a.sq + row;
-      if (g == 0) a.part_ml[at] = make_float2(m[rt], sum);
+      if (g == 0 && half == 0) a.part_ml[at] = make_float2(m[rt], sum);
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv) vx_store4(a.part + at * a.dv + nv * 16 + g * 4, o[rt][nv], a.dv - nv * 16 - g * 4);
+      for (int nv = 0; nv < NV; ++nv) vx_store4(a.part + at * a.dv + n0 + nv * 16, o[rt][nv], a.dv - n0 - nv * 16);
     } else {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      if (a.stats && g == 0) a.stats[(long long)bh * a.sq + row] = make_float2(m[rt], inv);
+      if (a.stats && g == 0 && half == 0) a.stats[(long long)bh * a.sq + row] = make_float2(m[rt], inv);
       T* op = a.out + (((long long)b * a.sq + row) * a.h + h) * a.dv;
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv) vx_store4(op + nv * 16 + g * 4, o[rt][nv] * inv, a.dv - nv * 16 - g * 4);
+      for (int nv = 0; nv < NV; ++nv) vx_store4(op + n0 + nv * 16, o[rt][nv] * inv, a.dv - n0 - nv * 16);
     }
   }
 }
@@ -243,7 +333,7 @@ __global__ __launch_bounds__(256) void attn_join(const FwdArgs<T> a, long long i
   vx_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int s = 0; s < a.splits; ++s) {
     const float2 ml = a.part_ml[s * rows + rowid];
-    const float wgt = exp2f(ml.x - ref);
+    const float wgt = __builtin_amdgcn_exp2f(ml.x - ref);
     l += wgt * ml.y;
     o += vx_load4(a.part + (s * rows + rowid) * a.dv + n, a.dv - n) * wgt;
   }
@@ -291,7 +381,7 @@ __global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long 
 
 // P and dS of a TM-query x TN-key tile: scores and dP = go v^T are two products with one epilogue,
 // P = 2^(scale2 s - max) / sum, dS = scale P (dP - delta).
-template <typename T, int TM, int TN>
+template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) {
   __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
   unsigned w = vx_xcd_tile(blockIdx.x, gridDim.x);
@@ -304,9 +394,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) 
   vx_f32x4 s[TM / 32][TN / 32], dp[TM / 32][TN / 32];
   vx_acc_zero(s);
   vx_acc_zero(dp);
-  vx_gemm_loop<T, KC, KC, TM, TN>({a.q + b * a.q_b + q * a.q_s + h * a.q_h, a.q_s, rows_m, nullptr},
+  vx_gemm_loop<T, KC, KC, TM, TN, FAST>({a.q + b * a.q_b + q * a.q_s + h * a.q_h, a.q_s, rows_m, nullptr},
                                   {a.k + b * a.k_b + (h / a.gk) * a.k_h + n0 * a.k_s, a.k_s, rows_n, nullptr}, 0, a.d, lds, s);
-  vx_gemm_loop<T, KC, KC, TM, TN>({a.go + b * a.go_b + q * a.go_s + h * a.go_h, a.go_s, rows_m, nullptr},
+  vx_gemm_loop<T, KC, KC, TM, TN, FAST>({a.go + b * a.go_b + q * a.go_s + h * a.go_h, a.go_s, rows_m, nullptr},
                                   {a.v + b * a.v_b + (h / a.gv) * a.v_h + n0 * a.v_s, a.v_s, rows_n, nullptr}, 0, a.dv, lds, dp);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
   const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
@@ -326,7 +416,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) 
       vx_f32x4 p, d;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[i] = live[i] ? exp2f(s[mi][ni][i] * a.scale2 - st.x) * st.y : 0.0f;
+        p[i] = live[i] ? __builtin_amdgcn_exp2f(s[mi][ni][i] * a.scale2 - st.x) * st.y : 0.0f;
         d[i] = live[i] ? p[i] * (dp[mi][ni][i] - delta) * a.scale : 0.0f;
       }
       const long long at = ((long long)bh * a.rows + m) * a.skp + n;
@@ -338,7 +428,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) 
 
 // the three gradients of a chunk in one launch: dV slabs = P^T go, dK slabs = dS^T q (reduction over the queries of a split),
 // dQ = dS k (reduction over the keys)
-template <typename T, int TM, int TN>
+template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a) {
   __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
   vx_f32x4 acc[TM / 32][TN / 32];
@@ -355,10 +445,10 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
     const int r0 = sp * a.span, len = a.rows - r0 < a.span ? a.rows - r0 : a.span;
     const int rows_m = a.sk - m0 < TM ? a.sk - m0 : TM, rows_n = width - n0 < TN ? width - n0 : TN;
     const long long q = a.q0 + r0;
-    const VxOperand<T> X{(is_v ? a.p : a.ds) + ((long long)bh * a.rows + r0) * a.skp + m0, a.skp, rows_m, nullptr};
+    const VxOperand<T> X{(is_v ? a.p : a.ds) + ((long long)bh * a.rows + r0) * a.skp + m0, a.skp, a.skp - m0, nullptr};
     const VxOperand<T> W{is_v ? a.go + b * a.go_b + q * a.go_s + h * a.go_h + n0 : a.q + b * a.q_b + q * a.q_s + h * a.q_h + n0,
                          is_v ? a.go_s : a.q_s, rows_n, nullptr};
-    vx_gemm_loop<T, KS, KS, TM, TN>(X, W, 0, len, lds, acc);
+    vx_gemm_loop<T, KS, KS, TM, TN, FAST>(X, W, 0, len, lds, acc);
     float* slab = (is_v ? a.slab_v : a.slab_k) + ((long long)(a.split0 + sp) * a.bh + bh) * a.sk * width;
     vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
       if (m < rows_m && n < rows_n) vx_store4(slab + (long long)(m0 + m) * width + n0 + n, v, rows_n - n);
@@ -372,7 +462,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
     const int rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = a.d - n0 < TN ? a.d - n0 : TN;
     const VxOperand<T> X{a.ds + ((long long)bh * a.rows + m0) * a.skp, a.skp, rows_m, nullptr};
     const VxOperand<T> W{a.k + b * a.k_b + (h / a.gk) * a.k_h + n0, a.k_s, rows_n, a.mask ? a.mask + b * a.mask_b : nullptr};
-    vx_gemm_loop<T, KC, KS, TM, TN>(X, W, 0, a.sk, lds, acc);
+    vx_gemm_loop<T, KC, KS, TM, TN, FAST>(X, W, 0, a.sk, lds, acc);   // the pad of dS is 0
     vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
       if (m < rows_m && n < rows_n)
         vx_store4(a.dq + (((long long)b * a.sq + a.q0 + m0 + m) * a.h + h) * a.d + n0 + n, v, rows_n - n);
@@ -436,15 +526,34 @@ void fill_args(AttnArgs<T>& a, const Shape& s, const int64_t* st, const void* q,
   a.scale2 = scale * kLog2e;
 }
 
+// whether every row of a [batch, position, head, width] tensor can be read by buffer loads
+bool heads_fast(const void* p, int64_t b, int64_t s, int64_t h, int64_t width, int64_t e) {
+  return vx_fast(p, s, width, e) && b * e % 16 == 0 && h * e % 16 == 0;
+}
+template <typename T>
+bool args_fast(const AttnArgs<T>& a) {
+  return heads_fast(a.q, a.q_b, a.q_s, a.q_h, a.d, sizeof(T)) && heads_fast(a.k, a.k_b, a.k_s, a.k_h, a.d, sizeof(T)) &&
+         heads_fast(a.v, a.v_b, a.v_s, a.v_h, a.dv, sizeof(T));
+}
+
+// the smallest tile that holds both widths
+constexpr int kClasses = 6;
+constexpr int kDims[kClasses][2] = {{32, 64}, {64, 64}, {64, 128}, {128, 128}, {96, 192}, {192, 384}};
+int class_of(int64_t d, int64_t dv) {
+  int i = 0;
+  while (d > kDims[i][0] || dv > kDims[i][1]) ++i;
+  return i;
+}
+
 struct FwdPlan {
-  int rt;
+  bool many;                 // 128 queries per workgroup instead of 64
   int64_t tiles_q, splits, span;
 };
 FwdPlan fwd_plan(const Shape& s, int32_t dtype) {
   FwdPlan p;
   const int64_t cus = vx_tile_cus(), bh = s.b * s.h, kt = dtype == VX_F32 ? 32 : 64, tiles_k = vx_cdiv(s.sk, kt);
-  p.rt = vx_cdiv(s.sq, 128) * bh >= cus ? 2 : 1;
-  p.tiles_q = vx_cdiv(s.sq, 64 * p.rt);
+  p.many = vx_cdiv(s.sq, 128) * bh >= cus && !(dtype == VX_F32 && class_of(s.d, s.dv) == kClasses - 1);
+  p.tiles_q = vx_cdiv(s.sq, p.many ? 128 : 64);
   // few workgroups: split the keys so that every CU has one
   int64_t splits = p.tiles_q * bh > 0 ? cus / (p.tiles_q * bh) : 1;
   if (splits > tiles_k) splits = tiles_k;
@@ -460,12 +569,23 @@ size_t fwd_bytes(const Shape& s, int32_t dtype) {
   return vx_align(rows * s.dv * 4) + vx_align(rows * 8);
 }
 
-template <typename T, int DP, int DVP>
-void launch_fwd(const FwdArgs<T>& a, int rt, unsigned grid, hipStream_t s) {
-  if (rt == 2)
-    attn_fwd<T, DP, DVP, 2><<<grid, kTileThreads, 0, s>>>(a);
-  else
-    attn_fwd<T, DP, DVP, 1><<<grid, kTileThreads, 0, s>>>(a);
+template <typename T, int C>
+void launch_fwd(const FwdArgs<T>& a, bool many, unsigned grid, hipStream_t s) {
+  constexpr int DP = kDims[C][0], DVP = kDims[C][1];
+  const bool fast = args_fast(a);
+  if constexpr (C == kClasses - 1) {       // 64 queries: 2 groups of 32; 128 (bf16 only): 4 groups, two waves a SIMD
+    if (sizeof(T) == 2 && many) {
+      const auto kernel = fast ? attn_fwd<T, DP, DVP, 2, sizeof(T) == 2 ? 4 : 2, 2, true> : attn_fwd<T, DP, DVP, 2, sizeof(T) == 2 ? 4 : 2, 2, false>;
+      kernel<<<grid, 512, 0, s>>>(a);
+    } else {
+      const auto kernel = fast ? attn_fwd<T, DP, DVP, 2, 2, 2, true> : attn_fwd<T, DP, DVP, 2, 2, 2, false>;
+      kernel<<<grid, 256, 0, s>>>(a);
+    }
+  } else {
+    const auto kernel = many ? (fast ? attn_fwd<T, DP, DVP, 2, 4, 1, true> : attn_fwd<T, DP, DVP, 2, 4, 1, false>)
+                             : (fast ? attn_fwd<T, DP, DVP, 1, 4, 1, true> : attn_fwd<T, DP, DVP, 1, 4, 1, false>);
+    kernel<<<grid, 256, 0, s>>>(a);
+  }
 }
 
 template <typename T>
@@ -479,13 +599,14 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   const size_t rows = (size_t)p.splits * bh * sh.sq;
   a.part = (float*)ws;
   a.part_ml = (float2*)(ws + vx_align(rows * sh.dv * 4));
-  // the smallest tile that holds both widths
-  if (a.d <= 32 && a.dv <= 64) launch_fwd<T, 32, 64>(a, p.rt, (unsigned)grid, s);
-  else if (a.d <= 64 && a.dv <= 64) launch_fwd<T, 64, 64>(a, p.rt, (unsigned)grid, s);
-  else if (a.d <= 64 && a.dv <= 128) launch_fwd<T, 64, 128>(a, p.rt, (unsigned)grid, s);
-  else if (a.d <= 128 && a.dv <= 128) launch_fwd<T, 128, 128>(a, p.rt, (unsigned)grid, s);
-  else if (a.d <= 96 && a.dv <= 192) launch_fwd<T, 96, 192>(a, p.rt, (unsigned)grid, s);
-  else launch_fwd<T, 192, 384>(a, p.rt, (unsigned)grid, s);
+  switch (class_of(sh.d, sh.dv)) {
+    case 0: launch_fwd<T, 0>(a, p.many, (unsigned)grid, s); break;
+    case 1: launch_fwd<T, 1>(a, p.many, (unsigned)grid, s); break;
+    case 2: launch_fwd<T, 2>(a, p.many, (unsigned)grid, s); break;
+    case 3: launch_fwd<T, 3>(a, p.many, (unsigned)grid, s); break;
+    case 4: launch_fwd<T, 4>(a, p.many, (unsigned)grid, s); break;
+    default: launch_fwd<T, 5>(a, p.many, (unsigned)grid, s); break;
+  }
   VX_LAUNCH_CHECK();
   if (p.splits > 1) {
     const int quads = (a.dv + 3) / 4;
@@ -528,11 +649,11 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   return p;
 }
 
-template <typename T, int TM>
+template <typename T, int TM, bool FAST>
 int32_t bwd_chunk(const BwdArgs<T>& a, int64_t pds, int64_t grads, hipStream_t s) {
-  attn_pds<T, TM, TM><<<(unsigned)pds, kTileThreads, 0, s>>>(a);
+  attn_pds<T, TM, TM, FAST><<<(unsigned)pds, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
-  attn_grads<T, TM, TM><<<(unsigned)grads, kTileThreads, 0, s>>>(a);
+  attn_grads<T, TM, TM, FAST><<<(unsigned)grads, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
   return VX_OK;
 }
@@ -555,6 +676,7 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   VX_REQUIRE(vx_cdiv(rows, 4) < (1LL << 31), "attn_bwd: too many queries");
   attn_delta<T><<<(unsigned)vx_cdiv(rows, 4), 256, 0, s>>>(a, rows);
   VX_LAUNCH_CHECK();
+  const bool fast = args_fast(a) && heads_fast(a.go, a.go_b, a.go_s, a.go_h, sh.dv, sizeof(T));
   for (int64_t q0 = 0, split = 0; q0 < sh.sq; q0 += p.chunk, split += p.per_chunk) {
     a.q0 = (int)q0;
     a.rows = (int)(sh.sq - q0 < p.chunk ? sh.sq - q0 : p.chunk);
@@ -568,7 +690,8 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
     a.n_v = (unsigned)nv;
     a.n_k = (unsigned)nk;
     a.n_q = (unsigned)nq;
-    const int32_t rc = p.tm == 128 ? bwd_chunk<T, 128>(a, pds, nv + nk + nq, s) : bwd_chunk<T, 64>(a, pds, nv + nk + nq, s);
+    const int32_t rc = p.tm == 128 ? (fast ? bwd_chunk<T, 128, true>(a, pds, nv + nk + nq, s) : bwd_chunk<T, 128, false>(a, pds, nv + nk + nq, s))
+                                   : (fast ? bwd_chunk<T, 64, true>(a, pds, nv + nk + nq, s) : bwd_chunk<T, 64, false>(a, pds, nv + nk + nq, s));
     if (rc) return rc;
   }
   const int64_t iv = sh.b * sh.hv * sh.sk * vx_cdiv(sh.dv, 4), ik = sh.b * sh.hk * sh.sk * vx_cdiv(sh.d, 4);

@@ -37,7 +37,7 @@ struct FwdArgs {
   int n, k, act, tiles_n;
 };
 
-template <typename T, int TM, int TN>
+template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a) {
   __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
   const unsigned t = vx_xcd_tile(blockIdx.x, gridDim.x);
@@ -47,7 +47,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a
   vx_f32x4 acc[TM / 32][TN / 32];
   vx_acc_zero(acc);
   const VxOperand<T> X{a.x + m0 * a.ldx, a.ldx, rows_m, nullptr}, W{a.w + (long long)n0 * a.ldw, a.ldw, rows_n, nullptr};
-  vx_gemm_loop<T, KC, KC, TM, TN>(X, W, 0, a.k, lds, acc);
+  vx_gemm_loop<T, KC, KC, TM, TN, FAST>(X, W, 0, a.k, lds, acc);
   vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
     const int left = rows_n - n;
     if (m >= rows_m || left <= 0) return;
@@ -109,7 +109,7 @@ struct BwdArgs {
 
 // one launch for both gradients: workgroups [0, blocks_w) are tiles of dw = g^T x (reduction over the rows, split), the rest
 // tiles of dx = g w (reduction over n)
-template <typename T, int TM, int TN>
+template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a) {
   __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
   vx_f32x4 acc[TM / 32][TN / 32];
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a
     const int rows = (int)(a.m - r0 < a.span ? a.m - r0 : a.span);
     const int rows_n = a.n - n0 < TM ? a.n - n0 : TM, rows_k = a.k - k0 < TN ? a.k - k0 : TN;
     const VxOperand<T> X{a.g + r0 * a.ldg + n0, a.ldg, rows_n, nullptr}, W{a.x + r0 * a.ldx + k0, a.ldx, rows_k, nullptr};
-    vx_gemm_loop<T, KS, KS, TM, TN>(X, W, 0, rows, lds, acc);
+    vx_gemm_loop<T, KS, KS, TM, TN, FAST>(X, W, 0, rows, lds, acc);
     float* slab = a.slab ? a.slab + (long long)split * a.n * a.k : nullptr;
     vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
       const int left = rows_k - n;
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a
     const int k0 = (int)(t % a.tiles_xk) * TN;
     const int rows_m = (int)(a.m - m0 < TM ? a.m - m0 : TM), rows_k = a.k - k0 < TN ? a.k - k0 : TN;
     const VxOperand<T> X{a.g + m0 * a.ldg, a.ldg, rows_m, nullptr}, W{a.w + k0, a.ldw, rows_k, nullptr};
-    vx_gemm_loop<T, KC, KS, TM, TN>(X, W, 0, a.n, lds, acc);
+    vx_gemm_loop<T, KC, KS, TM, TN, FAST>(X, W, 0, a.n, lds, acc);
     vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
       const int left = rows_k - n;
       if (m < rows_m && left > 0) vx_store4(a.dx + (m0 + m) * a.k + k0 + n, v, left);
@@ -144,21 +144,28 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a
   }
 }
 
-// out[i] = sum over `count` slabs of slab[s * len + i], in order of s; two such sums in one launch (dw, dbias)
+// out[i] = sum over the slabs of slab[s * len + i], in a fixed order: lane group j of a workgroup (16 of 16 lanes, four values a
+// lane) adds the slabs j, j + 16, ..., then the 16 groups are added in order. Two such sums in one launch (dw, dbias).
 template <typename T>
 __global__ __launch_bounds__(256) void slab_sum(const float* __restrict__ a, int count_a, long long len_a, T* __restrict__ out_a,
                                                 const float* __restrict__ b, int count_b, long long len_b,
                                                 T* __restrict__ out_b, unsigned blocks_a) {
+  __shared__ vx_f32x4 sh[16][17];
   const bool first = blockIdx.x < blocks_a;
   const float* src = first ? a : b;
-  const int count = first ? count_a : count_b;
+  const int count = first ? count_a : count_b, cl = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const long long len = first ? len_a : len_b;
   T* out = first ? out_a : out_b;
-  const long long i = ((long long)(first ? blockIdx.x : blockIdx.x - blocks_a) * 256 + threadIdx.x) * 4;
-  if (i >= len) return;
+  const long long i = ((long long)(first ? blockIdx.x : blockIdx.x - blocks_a) * 16 + cl) * 4;
   const int left = len - i < 4 ? (int)(len - i) : 4;
   vx_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int c = 0; c < count; ++c) s += vx_load4(src + c * len + i, left);
+  if (left > 0)
+    for (int c = grp; c < count; c += 16) s += vx_load4(src + c * len + i, left);
+  sh[grp][cl] = s;
+  __syncthreads();
+  if (grp || left <= 0) return;
+#pragma unroll
+  for (int j = 1; j < 16; ++j) s += sh[j][cl];
   vx_store4(out + i, s, left);
 }
 
@@ -192,10 +199,10 @@ int32_t fwd_impl(const FwdArgs<T>& args, hipStream_t s) {
   a.tiles_n = (int)vx_cdiv(a.n, t);
   const int64_t grid = vx_cdiv(a.m, t) * a.tiles_n;
   VX_REQUIRE(grid < (1LL << 31), "linear_fwd: too many rows");
-  if (use_big)
-    linear_fwd<T, 128, 128><<<(unsigned)grid, kTileThreads, 0, s>>>(a);
-  else
-    linear_fwd<T, 64, 64><<<(unsigned)grid, kTileThreads, 0, s>>>(a);
+  const bool fast = vx_fast(a.x, a.ldx, a.k, sizeof(T)) && vx_fast(a.w, a.ldw, a.k, sizeof(T));
+  const auto kernel = use_big ? (fast ? linear_fwd<T, 128, 128, true> : linear_fwd<T, 128, 128, false>)
+                              : (fast ? linear_fwd<T, 64, 64, true> : linear_fwd<T, 64, 64, false>);
+  kernel<<<(unsigned)grid, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
   return VX_OK;
 }
@@ -230,14 +237,14 @@ int32_t bwd_impl(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w,
   a.blocks_w = (unsigned)bw;
   a.blocks_x = (unsigned)bx;
   if (bw + bx) {
-    if (p.big)
-      linear_bwd<T, 128, 128><<<(unsigned)(bw + bx), kTileThreads, 0, s>>>(a);
-    else
-      linear_bwd<T, 64, 64><<<(unsigned)(bw + bx), kTileThreads, 0, s>>>(a);
+    const bool fast = vx_fast(a.g, a.ldg, n, sizeof(T)) && vx_fast(a.x, a.ldx, k, sizeof(T)) && vx_fast(a.w, a.ldw, k, sizeof(T));
+    const auto kernel = p.big ? (fast ? linear_bwd<T, 128, 128, true> : linear_bwd<T, 128, 128, false>)
+                              : (fast ? linear_bwd<T, 64, 64, true> : linear_bwd<T, 64, 64, false>);
+    kernel<<<(unsigned)(bw + bx), kTileThreads, 0, s>>>(a);
     VX_LAUNCH_CHECK();
   }
   const int64_t len_w = dw && p.splits > 1 ? (int64_t)n * k : 0, len_b = dbias ? n : 0;
-  const unsigned ga = (unsigned)vx_cdiv(len_w, 1024), gb = (unsigned)vx_cdiv(len_b, 1024);
+  const unsigned ga = (unsigned)vx_cdiv(len_w, 64), gb = (unsigned)vx_cdiv(len_b, 64);
   if (ga + gb) {
     slab_sum<T><<<ga + gb, 256, 0, s>>>(slab, (int)p.splits, len_w, dw, part, (int)p.chunks, len_b, dbias, ga);
     VX_LAUNCH_CHECK();

@@ -7,8 +7,9 @@
 //
 // LDS image of an operand tile: fragments of 16 rows x 32 k, 1 KB each and one per plane, in lane order -- lane (c, g) of a
 // fragment read takes the 16 bytes {k = 8 g .. 8 g + 7} of row c with one ds_read_b128, 64 lanes over 1 KB: no bank
-// conflicts. The 16-byte pieces of a fragment are XOR-ed by its row block (& 7), which also spreads the writes of a
-// k-strided operand, whose lanes each own a few rows (16 lanes over 16 different pieces of the 256-byte bank row).
+// conflicts. Two more rules keep the writes free of them: the 16-byte pieces of a fragment are XOR-ed by their k group
+// (a wave that writes whole 128-byte rows spreads a row's eight pieces over eight bank groups), and every block of 16 rows
+// starts 16 bytes later (a k-strided operand's lanes each own a few rows: 16 lanes over 16 different pieces).
 #pragma once
 #include "vx_common.h"
 #include "vx_split.h"
@@ -19,6 +20,7 @@ typedef unsigned vx_u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned vx_u32x2u __attribute__((ext_vector_type(2), aligned(2)));
 typedef unsigned vx_u32x1u __attribute__((aligned(2)));
 typedef unsigned vx_u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned vx_u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTileThreads = 256;
 constexpr int kFragBytes = 1024;
@@ -47,17 +49,21 @@ struct VxFrag {
   bf16x8 p[NPL];
 };
 
-// c += w * x; fp32: the six plane products down to 2^-24 of the largest, smallest first
-__device__ __forceinline__ vx_f32x4 vx_mma(const VxFrag<1>& w, const VxFrag<1>& x, vx_f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[0], x.p[0], c, 0, 0, 0);
-}
-__device__ __forceinline__ vx_f32x4 vx_mma(const VxFrag<3>& w, const VxFrag<3>& x, vx_f32x4 c) {
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[2], x.p[0], c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[0], x.p[2], c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[1], x.p[1], c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[1], x.p[0], c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[0], x.p[1], c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[0], x.p[0], c, 0, 0, 0);
+// the plane products of c += w * x, in order (fp32: six, down to 2^-21 of |w x|, smallest first). Callers loop over independent
+// accumulators inside a product, so that no matrix instruction waits for the one before it.
+template <int NPL>
+struct VxProducts;
+template <>
+struct VxProducts<1> {
+  static constexpr int N = 1, W[1] = {0}, X[1] = {0};
+};
+template <>
+struct VxProducts<3> {
+  static constexpr int N = 6, W[6] = {2, 0, 1, 1, 0, 0}, X[6] = {0, 2, 1, 0, 1, 0};
+};
+template <int NPL>
+__device__ __forceinline__ vx_f32x4 vx_mma(int product, const VxFrag<NPL>& w, const VxFrag<NPL>& x, vx_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[VxProducts<NPL>::W[product]], x.p[VxProducts<NPL>::X[product]], c, 0, 0, 0);
 }
 
 // eight fp32 values -> operand planes (bf16: rounded to nearest even)
@@ -70,6 +76,16 @@ __device__ __forceinline__ void vx_planes(const float (&v)[8], VxFrag<3>& f) {
 __device__ __forceinline__ void vx_planes(const float (&v)[8], VxFrag<1>& f) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) f.p[0][i] = (__bf16)v[i];
+}
+
+// ---- buffer loads -------------------------------------------------------------------------------------------------
+// 32-bit offsets from a wave-uniform base, with a range check that returns 0: masked lanes and tails need no branch (a branch
+// around a load whose other side writes zeros makes the load wait). kVxOut is past every range.
+constexpr unsigned kVxRange = 0x80000000u;
+constexpr int kVxOut = (int)0x80000000u;
+typedef __amdgpu_buffer_rsrc_t vx_rsrc;
+__device__ __forceinline__ vx_rsrc vx_buffer(const void* base, unsigned range = kVxRange) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)range, 0x00020000);   // raw, 32-bit data format
 }
 
 // ---- eight k-consecutive values of one row ---------------------------------------------------------------------
@@ -92,6 +108,14 @@ struct VxRow8<float> {
       for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
     }
   }
+  __device__ __forceinline__ void load(vx_rsrc b, int at) {
+    const vx_u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0), y = __builtin_amdgcn_raw_buffer_load_b128(b, at, 16, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = __uint_as_float(x[i]);
+      v[4 + i] = __uint_as_float(y[i]);
+    }
+  }
   __device__ __forceinline__ void planes(VxFrag<3>& f) const { vx_planes(v, f); }
 };
 template <>
@@ -109,6 +133,7 @@ struct VxRow8<__bf16> {
       }
     }
   }
+  __device__ __forceinline__ void load(vx_rsrc b, int at) { v = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0); }
   __device__ __forceinline__ void planes(VxFrag<1>& f) const { f.p[0] = __builtin_bit_cast(bf16x8, v); }
 };
 
@@ -137,6 +162,23 @@ struct VxCol8<float, W> {
       for (int j = 0; j < W; ++j) v[k][j] = j < n ? p[j] : 0.0f;
     }
   }
+  __device__ __forceinline__ void load(int k, vx_rsrc b, int at, int uniform) {
+    if constexpr (W == 4) {
+      const vx_u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(b, at, uniform, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[k][j] = __uint_as_float(a[j]);
+    } else if constexpr (W == 2) {
+      const vx_u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(b, at, uniform, 0);
+      v[k][0] = __uint_as_float(a[0]);
+      v[k][1] = __uint_as_float(a[1]);
+    } else {
+      v[k][0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, at, uniform, 0));
+    }
+  }
+  __device__ __forceinline__ void clear(int k) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[k][j] = 0.0f;
+  }
   __device__ __forceinline__ void planes(int j, VxFrag<3>& f) const {
     const float x[8] = {v[0][j], v[1][j], v[2][j], v[3][j], v[4][j], v[5][j], v[6][j], v[7][j]};
     vx_planes(x, f);
@@ -164,6 +206,19 @@ struct VxCol8<__bf16, W> {
       }
     }
   }
+  __device__ __forceinline__ void load(int k, vx_rsrc b, int at, int uniform) {
+    if constexpr (W == 4) {
+      const vx_u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(b, at, uniform, 0);
+      v[k][0] = a[0];
+      v[k][1] = a[1];
+    } else {
+      v[k][0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, uniform, 0);
+    }
+  }
+  __device__ __forceinline__ void clear(int k) {
+#pragma unroll
+    for (int j = 0; j < W / 2; ++j) v[k][j] = 0u;
+  }
   __device__ __forceinline__ void planes(int j, VxFrag<1>& f) const {
     vx_u32x4 o;
     const unsigned sel = j & 1 ? 0x07060302u : 0x05040100u;
@@ -174,16 +229,20 @@ struct VxCol8<__bf16, W> {
 };
 
 // ---- LDS image --------------------------------------------------------------------------------------------------
-// fragment (row block rb, k step ks) of an image with NK k steps per row block; planes are `plane` bytes apart
+// byte of (row block rb, k step ks, slot) of an image with NK k steps; slot = row & 15 + 16 * k group
+template <int NK>
+constexpr int vx_image_block() { return NK * kFragBytes + 16; }
+template <int NK>
+__device__ __forceinline__ int vx_image_at(int rb, int ks, int slot) {
+  return rb * vx_image_block<NK>() + ks * kFragBytes + ((slot ^ (slot >> 4 & 3) ^ (ks & 1) << 2) << 4);
+}
 template <int NPL>
-__device__ __forceinline__ void vx_frag_store(char* img, int plane, int frag, int key, int slot, const VxFrag<NPL>& f) {
-  char* p = img + frag * kFragBytes + ((slot ^ (key & 7)) << 4);
+__device__ __forceinline__ void vx_frag_store(char* p, int plane, const VxFrag<NPL>& f) {
 #pragma unroll
   for (int i = 0; i < NPL; ++i) *reinterpret_cast<bf16x8*>(p + i * plane) = f.p[i];
 }
 template <int NPL>
-__device__ __forceinline__ void vx_frag_load(const char* img, int plane, int frag, int key, int lane, VxFrag<NPL>& f) {
-  const char* p = img + frag * kFragBytes + ((lane ^ (key & 7)) << 4);
+__device__ __forceinline__ void vx_frag_load(const char* p, int plane, VxFrag<NPL>& f) {
 #pragma unroll
   for (int i = 0; i < NPL; ++i) f.p[i] = *reinterpret_cast<const bf16x8*>(p + i * plane);
 }
@@ -191,7 +250,10 @@ __device__ __forceinline__ void vx_frag_load(const char* img, int plane, int fra
 // ---- GEMM ---------------------------------------------------------------------------------------------------------
 // operand tile: p points at (first row of the tile, k = 0)
 //   KC (k contiguous): element (r, k) at p[r * ld + k];  KS (k strided): element (r, k) at p[k * ld + r]
-// rows: rows that exist from the tile's first on; kmask (KS only): k's whose byte is 0 read as 0, whatever they hold
+// rows: rows that exist from the tile's first on; kmask (KS only): k's whose byte is 0 read as 0, whatever they hold.
+// FAST operands are read by buffer loads: 16-byte aligned base and row stride, and (vx_fast) rows (KS) or the reduction (KC) in
+// multiples of 8, ld no smaller than a row, the offsets of a tile in 31 bits. The others are read element by element at
+// their edges, and every load waits for its own branch: measured 1.7 to 6 times the time of a FAST call.
 constexpr int KC = 0, KS = 1;
 template <typename T>
 struct VxOperand {
@@ -200,56 +262,88 @@ struct VxOperand {
   int rows;
   const uint8_t* kmask;
 };
+static inline bool vx_fast(const void* p, int64_t ld, int64_t width, int64_t esize) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * esize % 16 == 0 && width % 8 == 0 && ld >= width && ld < (1 << 21);
+}
 
 // stages R rows x BK k's with 256 threads: registers first (load), then the LDS image (store)
-template <typename T, int MODE, int R>
+template <typename T, int MODE, int R, bool FAST>
 struct VxStage {
-  static constexpr int BK = VxType<T>::BK, NPL = VxType<T>::NPL, NK = BK / 32;
-  static constexpr int PLANE = (R / 16) * NK * kFragBytes;
+  static constexpr int BK = VxType<T>::BK, NPL = VxType<T>::NPL, NK = BK / 32, E = sizeof(T);
+  static constexpr int PLANE = (R / 16) * vx_image_block<NK>();
   static constexpr int BYTES = PLANE * NPL;
-  static constexpr int NI = R * BK / 8 / kTileThreads;            // 8-value items per thread (KC)
-  static constexpr int W = R * BK / 8 / kTileThreads;             // rows per thread (KS)
+  static constexpr int NI = R * BK / 8 / kTileThreads;            // KC: 8-value items per thread; KS: rows per thread
+  static constexpr int W = NI;
   static_assert(R * BK / 8 % kTileThreads == 0, "every thread stages the same amount");
-  struct Empty {};
   VxRow8<T> a[MODE == KC ? NI : 1];
   VxCol8<T, MODE == KS ? W : 2> b;
+  unsigned dead;                                                   // KS with a mask: bit i = k i of the eight reads as 0
 
+  // KC item i of a thread: row (of the tile) and k group. bf16: eight lanes read a row's 128 bytes; fp32: a lane's eight
+  // values are two loads, four lanes a row
+  static __device__ __forceinline__ void item(int i, int tid, int& row, int& kc) {
+    const int wave = tid >> 6, l = tid & 63, blk = i * (kTileThreads / 64) + wave;
+    if constexpr (NK == 2) {
+      row = (blk >> 1) * 16 + (l >> 3 & 1) * 8 + (blk & 1) * 4 + (l >> 4);
+      kc = l & 7;
+    } else {
+      row = blk * 16 + (l & 15);
+      kc = l >> 4;
+    }
+  }
   __device__ __forceinline__ void load(const VxOperand<T>& o, int k0, int kend, int tid) {
     if constexpr (MODE == KC) {
-      const int wave = tid >> 6, lane = tid & 63;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int frag = i * (kTileThreads / 64) + wave, r = frag / NK * 16 + (lane & 15);
-        const int k = k0 + frag % NK * 32 + (lane >> 4) * 8;
-        a[i].load(o.p + r * o.ld + k, r < o.rows ? kend - k : 0);
+        int row, kc;
+        item(i, tid, row, kc);
+        if constexpr (FAST)
+          a[i].load(vx_buffer(o.p + k0), row < o.rows && kc * 8 < kend - k0 ? row * (int)o.ld * E + kc * 8 * E : kVxOut);
+        else
+          a[i].load(o.p + row * o.ld + k0 + kc * 8, row < o.rows ? kend - k0 - kc * 8 : 0);
       }
     } else {
-      const int r = tid % (R / W) * W, k = k0 + tid / (R / W) * 8;
-      const T* p = o.p + k * o.ld + r;
+      const int r = tid % (R / W) * W, kg = tid / (R / W) * 8;
+      if (o.kmask != nullptr) {
+        dead = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool live = k + i < kend && (o.kmask == nullptr || o.kmask[k + i]);
-        b.load(i, p + i * o.ld, live ? o.rows - r : 0);
+        for (int i = 0; i < 8; ++i) dead |= k0 + kg + i < kend && o.kmask[k0 + kg + i] ? 0u : 1u << i;
+      }
+      if constexpr (FAST) {
+        // the range ends with the reduction: k's past it read as 0
+        const long long left = (long long)(kend - k0) * o.ld * E;
+        const vx_rsrc buf = vx_buffer(o.p + (long long)k0 * o.ld, left < (long long)kVxRange ? (unsigned)left : kVxRange);
+        const int at = r < o.rows ? kg * (int)o.ld * E + r * E : kVxOut;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b.load(i, buf, at, i * (int)o.ld * E);
+      } else {
+        const T* p = o.p + (long long)(k0 + kg) * o.ld + r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b.load(i, p + i * o.ld, k0 + kg + i < kend ? o.rows - r : 0);
       }
     }
   }
-  __device__ __forceinline__ void store(char* img, int tid) const {
+  __device__ __forceinline__ void store(const VxOperand<T>& o, char* img, int tid) {
     VxFrag<NPL> f;
     if constexpr (MODE == KC) {
-      const int wave = tid >> 6, lane = tid & 63;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int frag = i * (kTileThreads / 64) + wave;
+        int row, kc;
+        item(i, tid, row, kc);
         a[i].planes(f);
-        vx_frag_store(img, PLANE, frag, frag / NK, lane, f);
+        vx_frag_store(img + vx_image_at<NK>(row >> 4, kc >> 2, (row & 15) + 16 * (kc & 3)), PLANE, f);
       }
     } else {
       const int r = tid % (R / W) * W, kg = tid / (R / W);
+      if (o.kmask != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (dead >> i & 1) b.clear(i);
+      }
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         b.planes(j, f);
-        const int rr = r + j, rb = rr >> 4;
-        vx_frag_store(img, PLANE, rb * NK + (kg >> 2), rb, (rr & 15) + 16 * (kg & 3), f);
+        vx_frag_store(img + vx_image_at<NK>((r + j) >> 4, kg >> 2, ((r + j) & 15) + 16 * (kg & 3)), PLANE, f);
       }
     }
   }
@@ -258,18 +352,18 @@ struct VxStage {
 // LDS bytes of vx_gemm_loop
 template <typename T, int TM, int TN>
 constexpr int vx_gemm_lds() {
-  return (TM + TN) * VxType<T>::BK * 2 * VxType<T>::NPL;
+  return (TM + TN) / 16 * vx_image_block<VxType<T>::BK / 32>() * VxType<T>::NPL;
 }
 
 // acc[mi][ni] += the TM x TN tile's product over k in [k0, kend); wave (wm, wn) of 2 x 2 owns TM/2 x TN/2. One LDS image,
 // two barriers per step: the next step's operands travel to registers while this one's are multiplied, and the two or
 // three workgroups of a CU cover each other's barriers. Ends with a barrier: the caller may reuse the LDS.
-template <typename T, int XM, int WM, int TM, int TN>
+template <typename T, int XM, int WM, int TM, int TN, bool FAST>
 __device__ __forceinline__ void vx_gemm_loop(const VxOperand<T>& X, const VxOperand<T>& W, int k0, int kend, char* lds,
                                              vx_f32x4 (&acc)[TM / 32][TN / 32]) {
   constexpr int BK = VxType<T>::BK, NPL = VxType<T>::NPL, NK = BK / 32;
-  using SX = VxStage<T, XM, TM>;
-  using SW = VxStage<T, WM, TN>;
+  using SX = VxStage<T, XM, TM, FAST>;
+  using SW = VxStage<T, WM, TN, FAST>;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   char *ix = lds, *iw = lds + SX::BYTES;
   SX sx;
@@ -279,8 +373,8 @@ __device__ __forceinline__ void vx_gemm_loop(const VxOperand<T>& X, const VxOper
     sw.load(W, k0, kend, tid);
   }
   for (int k = k0; k < kend; k += BK) {
-    sx.store(ix, tid);
-    sw.store(iw, tid);
+    sx.store(X, ix, tid);
+    sw.store(W, iw, tid);
     __syncthreads();
     if (k + BK < kend) {
       sx.load(X, k + BK, kend, tid);
@@ -288,19 +382,19 @@ __device__ __forceinline__ void vx_gemm_loop(const VxOperand<T>& X, const VxOper
     }
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks) {
+      const char* px = ix + vx_image_at<NK>(wm * (TM / 32), ks, lane);
+      const char* pw = iw + vx_image_at<NK>(wn * (TN / 32), ks, lane);
       VxFrag<NPL> fx[TM / 32];
 #pragma unroll
-      for (int mi = 0; mi < TM / 32; ++mi) {
-        const int rb = wm * (TM / 32) + mi;
-        vx_frag_load(ix, SX::PLANE, rb * NK + ks, rb, lane, fx[mi]);
-      }
+      for (int mi = 0; mi < TM / 32; ++mi) vx_frag_load(px + mi * vx_image_block<NK>(), SX::PLANE, fx[mi]);
 #pragma unroll
       for (int ni = 0; ni < TN / 32; ++ni) {
-        const int rb = wn * (TN / 32) + ni;
         VxFrag<NPL> fw;
-        vx_frag_load(iw, SW::PLANE, rb * NK + ks, rb, lane, fw);
+        vx_frag_load(pw + ni * vx_image_block<NK>(), SW::PLANE, fw);
 #pragma unroll
-        for (int mi = 0; mi < TM / 32; ++mi) acc[mi][ni] = vx_mma(fw, fx[mi], acc[mi][ni]);
+        for (int pr = 0; pr < VxProducts<NPL>::N; ++pr)
+#pragma unroll
+          for (int mi = 0; mi < TM / 32; ++mi) acc[mi][ni] = vx_mma(pr, fw, fx[mi], acc[mi][ni]);
       }
     }
     __syncthreads();
