@@ -9,6 +9,8 @@
 // by about as much as the output's own rounding).
 // A masked key has no part in anything, whatever its rows hold; a query without keys gives zeros. No atomics: bitwise
 // reproducible.
+#include <stdlib.h>
+
 #include "vx_tile.h"
 
 namespace {
@@ -26,6 +28,7 @@ struct AttnArgs {
 
 template <typename T>
 struct FwdArgs : AttnArgs<T> {
+  const char *k_img, *v_img;                 // attn_pack's images, tile after tile of each key / value head
   T* out;                                    // [b][sq][h][dv]
   float2* stats;                             // [b*h][sq] {max of scale2 * score, 1 / sum} or null
   float* part;                               // [splits][b*h][sq][dv] when the keys are split
@@ -51,15 +54,17 @@ __device__ __forceinline__ bool attn_key_live(const AttnArgs<T>& a, const uint8_
 // eight k's of its group g in the order (t, i), and the V^T image is staged in that order of keys.
 // CS = 2 (wide heads): the two waves of a group hold one half of the output columns each, compute the scores of one half of a
 // tile's keys each, and swap them through LDS as they are (a lane reads what the same lane of the other wave wrote).
-// A tile: V(t) travels to registers under S(t), then to LDS; K(t + 1) under O += P V(t). So at most one of the two is held in
-// registers, and each image is rewritten only after the barrier behind its last reader.
-template <typename T, int DP, int DVP, int RT, int QG, int CS, bool FAST>
+// A tile: V(t) travels under S(t), K(t + 1) under O += P V(t); each LDS image is rewritten only after the barrier behind its last
+// reader. IMG: both come as finished images (attn_pack) and go straight to LDS; else (few queries) through registers, where
+// they are split and V is transposed.
+template <typename T, int DP, int DVP, int RT, int QG, int CS, bool IMG, bool FAST>
 __global__ __launch_bounds__(64 * QG * CS, (DVP > 192 && QG * CS == 4) || (DVP > 64 && VxType<T>::NPL == 3) ? 1 : 2)
 void attn_fwd(const FwdArgs<T> a) {
   constexpr int NPL = VxType<T>::NPL, KT = AttnTile<T>::KT, NS = KT / 32;     // NS: 32-key steps of a tile
   constexpr int KD = DP / 32, NV = DVP / 16 / CS, NK = KT / 16, OWN = NK / CS, E = sizeof(T), NW = QG * CS;
   constexpr int K_FRAGS = NK * KD;
-  constexpr int K_PLANE = NK * vx_image_block<KD>(), V_PLANE = DVP / 16 * vx_image_block<NS>();
+  constexpr int K_BLOCK = IMG ? KD * kFragBytes : vx_image_block<KD>(), V_BLOCK = IMG ? NS * kFragBytes : vx_image_block<NS>();
+  constexpr int K_PLANE = NK * K_BLOCK, V_PLANE = DVP / 16 * V_BLOCK;
   constexpr int KI = (K_FRAGS + NW - 1) / NW;                                  // K fragments staged per wave
   constexpr int CB = DVP % 128 == 0 ? 128 : 64, VW = E == 2 ? CB / 32 : CB / 64;   // columns of a staged block and of a lane
   constexpr int LR = CB / VW, LG = 64 / LR;                                    // lanes of a row, key groups of a wave
@@ -167,6 +172,17 @@ void attn_fwd(const FwdArgs<T> a) {
       }
     }
   };
+  // IMG: whole fragments, in the order of the images
+  auto copy = [&](const char* from, char* to, int frags) {
+#pragma unroll
+    for (int i = wave; i < frags; i += NW) vx_copy_frag(from + i * kFragBytes, to + i * kFragBytes, lane);
+  };
+  const long long k_head = IMG ? ((long long)b * (a.h / a.gk) + h / a.gk) * tiles_k : 0;
+  const long long v_head = IMG ? ((long long)b * (a.h / a.gv) + h / a.gv) * tiles_k : 0;
+  const char *k_img = a.k_img + k_head * (K_PLANE * NPL), *v_img = a.v_img + v_head * (V_PLANE * NPL);
+  auto frag_at = [&](int block, int rb, int ks) {
+    return rb * block + ks * kFragBytes + (IMG ? lane : lane ^ (lane >> 4) ^ (ks & 1) << 2) * 16;
+  };
   // the first tile from t on that has a key that takes part, and which of its keys do
   auto find = [&](int t, unsigned long long& live) {
     for (live = 0; t < t1; ++t) {
@@ -180,9 +196,14 @@ void attn_fwd(const FwdArgs<T> a) {
   int t = find(t0, cur), tn = t1;
   if (cur) {
     tn = find(t + 1, nxt);
-    VxRow8<T> ks[KI];
-    load_k(ks, t);
-    store_k(ks);
+    if constexpr (IMG) {
+      copy(k_img + (long long)t * (K_PLANE * NPL), ik, K_PLANE * NPL / kFragBytes);
+      vx_arrived();
+    } else {
+      VxRow8<T> ks[KI];
+      load_k(ks, t);
+      store_k(ks);
+    }
   }
   __syncthreads();
   while (cur) {
@@ -190,7 +211,10 @@ void attn_fwd(const FwdArgs<T> a) {
     vx_f32x4 s[RT][NK];
     {
       VxCol8<T, VW> vs[VI];
-      load_v(vs, t, cur);
+      if constexpr (IMG)
+        copy(v_img + (long long)t * (V_PLANE * NPL), iv, V_PLANE * NPL / kFragBytes);
+      else
+        load_v(vs, t, cur);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -199,7 +223,7 @@ void attn_fwd(const FwdArgs<T> a) {
       for (int kd = 0; kd < KD; ++kd) {
         VxFrag<NPL> kf[OWN];
 #pragma unroll
-        for (int k = 0; k < OWN; ++k) vx_frag_load(ik + vx_image_at<KD>(half * OWN + k, kd, lane), K_PLANE, kf[k]);
+        for (int k = 0; k < OWN; ++k) vx_frag_load(ik + frag_at(K_BLOCK, half * OWN + k, kd), K_PLANE, kf[k]);
 #pragma unroll
         for (int pr = 0; pr < VxProducts<NPL>::N; ++pr)
 #pragma unroll
@@ -215,11 +239,16 @@ void attn_fwd(const FwdArgs<T> a) {
           for (int k = 0; k < OWN; ++k)
             *reinterpret_cast<vx_f32x4*>(swap + (wave * OWN * RT + rt * OWN + k) * kFragBytes + lane * 16) = s[rt][k];
       }
-      store_v(vs);
+      if constexpr (IMG) vx_arrived(); else store_v(vs);
     }
     __syncthreads();
     VxRow8<T> ks[KI];
-    if (nxt) load_k(ks, tn);
+    if (nxt) {
+      if constexpr (IMG)
+        copy(k_img + (long long)tn * (K_PLANE * NPL), ik, K_PLANE * NPL / kFragBytes);
+      else
+        load_k(ks, tn);
+    }
     if constexpr (CS == 2) {                   // both halves, in the order of the keys
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -276,7 +305,7 @@ void attn_fwd(const FwdArgs<T> a) {
       for (int ns = 0; ns < NS; ++ns) {
         VxFrag<NPL> vf[G];
 #pragma unroll
-        for (int u = 0; u < G; ++u) vx_frag_load(iv + vx_image_at<NS>(half * NV + nv + u, ns, lane), V_PLANE, vf[u]);
+        for (int u = 0; u < G; ++u) vx_frag_load(iv + frag_at(V_BLOCK, half * NV + nv + u, ns), V_PLANE, vf[u]);
 #pragma unroll
         for (int pr = 0; pr < VxProducts<NPL>::N; ++pr)
 #pragma unroll
@@ -286,7 +315,10 @@ void attn_fwd(const FwdArgs<T> a) {
       }
       if (nv % 4 == 2) __builtin_amdgcn_sched_barrier(0);
     }
-    if (nxt) store_k(ks);
+    if constexpr (IMG)
+      vx_arrived();
+    else if (nxt)
+      store_k(ks);
     __syncthreads();
     t = tn;
     cur = nxt;
@@ -318,6 +350,50 @@ void attn_fwd(const FwdArgs<T> a) {
   }
 }
 
+// K and V as operand images: per head and tile of KT keys, planes of 1 KB fragments -- K: key block, 32-d step; V^T: column block,
+// 32-key step in the operand order of the keys. A thread makes one lane's 16 bytes of a fragment (all planes). Widths are padded
+// with 0 to the tile's, masked and missing keys are 0. It costs one pass over k and v; each tile of queries then saves the split
+// and the transposition.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_pack(const AttnArgs<T> a, char* __restrict__ k_img, char* __restrict__ v_img, int tiles,
+                                                 int kd, int nv, long long k_slots, long long slots) {
+  constexpr int NPL = VxType<T>::NPL, KT = AttnTile<T>::KT, NS = KT / 32, NK = KT / 16;
+  long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= slots) return;
+  const bool is_k = i < k_slots;
+  if (!is_k) i -= k_slots;
+  const int lane = (int)(i & 63), c = lane & 15, g = lane >> 4;
+  const int frags = is_k ? NK * kd : nv * NS;
+  const long long ft = i >> 6, tile_id = ft / frags;
+  const int frag = (int)(ft % frags), t = (int)(tile_id % tiles);
+  const long long head_id = tile_id / tiles;
+  const int heads = is_k ? a.h / a.gk : a.h / a.gv, b = (int)(head_id / heads), head = (int)(head_id % heads);
+  const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  VxFrag<NPL> f;
+  if (is_k) {
+    const int key = t * KT + frag / kd * 16 + c, d = frag % kd * 32 + g * 8;
+    const bool live = key < a.sk && (mask == nullptr || mask[key]);
+    VxRow8<T> x;
+    x.load(a.k + b * a.k_b + head * a.k_h + key * a.k_s + d, live ? a.d - d : 0);
+    x.planes(f);
+  } else {
+    const int n = frag / NS * 16 + c, k0 = t * KT + frag % NS * 32 + g * 4;
+    const T* p = a.v + b * a.v_b + head * a.v_h + (n < a.dv ? n : 0);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int key = k0 + (j >> 2) * 16 + (j & 3);
+      const bool live = key < a.sk && n < a.dv && (mask == nullptr || mask[key]);
+      const float y = (float)p[(key < a.sk ? key : 0) * a.v_s];
+      x[j] = live ? y : 0.0f;
+    }
+    vx_planes(x, f);
+  }
+  char* to = (is_k ? k_img : v_img) + tile_id * frags * (NPL * kFragBytes) + frag * kFragBytes + lane * 16;
+#pragma unroll
+  for (int q = 0; q < NPL; ++q) *reinterpret_cast<bf16x8*>(to + (long long)q * frags * kFragBytes) = f.p[q];
+}
+
 // joins the splits of a row: weights 2^(m_s - m), in order of the splits. One thread per four output values.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join(const FwdArgs<T> a, long long items, int quads) {
@@ -326,16 +402,35 @@ __global__ __launch_bounds__(256) void attn_join(const FwdArgs<T> a, long long i
   const long long rowid = it / quads;               // bh * sq + row
   const int n = (int)(it % quads) * 4;
   const long long rows = items / quads;
+  constexpr int U = 8;                              // splits in flight: what a row costs is latency
+  const int last = a.splits - 1;
   float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[s * rows + rowid].x);
+  for (int s0 = 0; s0 < a.splits; s0 += U) {
+    float x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = a.part_ml[(s0 + u < last ? s0 + u : last) * rows + rowid].x;
+#pragma unroll
+    for (int u = 0; u < U; ++u) m = fmaxf(m, x[u]);
+  }
   const float ref = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
   vx_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = a.part_ml[s * rows + rowid];
-    const float wgt = __builtin_amdgcn_exp2f(ml.x - ref);
-    l += wgt * ml.y;
-    o += vx_load4(a.part + (s * rows + rowid) * a.dv + n, a.dv - n) * wgt;
+  for (int s0 = 0; s0 < a.splits; s0 += U) {
+    float2 ml[U];
+    vx_f32x4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long at = (s0 + u < last ? s0 + u : last) * rows + rowid;
+      ml[u] = a.part_ml[at];
+      v[u] = vx_load4(a.part + at * a.dv + n, a.dv - n);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u > last) break;
+      const float wgt = __builtin_amdgcn_exp2f(ml[u].x - ref);
+      l += wgt * ml[u].y;
+      o += v[u] * wgt;
+    }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int bh = (int)(rowid / a.sq), row = (int)(rowid % a.sq), b = bh / a.h, h = bh % a.h;
@@ -546,13 +641,14 @@ int class_of(int64_t d, int64_t dv) {
 }
 
 struct FwdPlan {
-  bool many;                 // 128 queries per workgroup instead of 64
-  int64_t tiles_q, splits, span;
+  bool many, img;            // 128 queries per workgroup instead of 64; operand images
+  int64_t tiles_q, splits, span, tiles_k;
+  size_t k_img, v_img;       // bytes
 };
 FwdPlan fwd_plan(const Shape& s, int32_t dtype) {
   FwdPlan p;
   const int64_t cus = vx_tile_cus(), bh = s.b * s.h, kt = dtype == VX_F32 ? 32 : 64, tiles_k = vx_cdiv(s.sk, kt);
-  p.many = vx_cdiv(s.sq, 128) * bh >= cus && !(dtype == VX_F32 && class_of(s.d, s.dv) == kClasses - 1);
+  p.many = vx_cdiv(s.sq, 128) * bh >= cus && s.sq > 64 && !(dtype == VX_F32 && class_of(s.d, s.dv) == kClasses - 1);
   p.tiles_q = vx_cdiv(s.sq, p.many ? 128 : 64);
   // few workgroups: split the keys so that every CU has one
   int64_t splits = p.tiles_q * bh > 0 ? cus / (p.tiles_q * bh) : 1;
@@ -560,31 +656,34 @@ FwdPlan fwd_plan(const Shape& s, int32_t dtype) {
   if (splits < 1) splits = 1;
   p.span = tiles_k ? vx_cdiv(tiles_k, splits) : 1;
   p.splits = tiles_k ? vx_cdiv(tiles_k, p.span) : 1;
+  p.tiles_k = tiles_k;
+  static const char* env = getenv("VX_IMG");
+  p.img = p.tiles_q * (s.h / s.hk) > (env ? atoi(env) : 1);
+  const int c = class_of(s.d, s.dv);
+  const size_t row = dtype == VX_F32 ? 6 : 2;      // bytes of a value's planes
+  p.k_img = p.img ? (size_t)s.b * s.hk * tiles_k * kt * kDims[c][0] * row : 0;
+  p.v_img = p.img ? (size_t)s.b * s.hv * tiles_k * kt * kDims[c][1] * row : 0;
   return p;
 }
 size_t fwd_bytes(const Shape& s, int32_t dtype) {
   const FwdPlan p = fwd_plan(s, dtype);
-  if (p.splits <= 1) return 0;
-  const size_t rows = (size_t)p.splits * s.b * s.h * s.sq;
-  return vx_align(rows * s.dv * 4) + vx_align(rows * 8);
+  const size_t rows = p.splits > 1 ? (size_t)p.splits * s.b * s.h * s.sq : 0;
+  return p.k_img + p.v_img + vx_align(rows * s.dv * 4) + vx_align(rows * 8);
 }
 
 template <typename T, int C>
-void launch_fwd(const FwdArgs<T>& a, bool many, unsigned grid, hipStream_t s) {
+void launch_fwd(const FwdArgs<T>& a, const FwdPlan& p, unsigned grid, hipStream_t s) {
   constexpr int DP = kDims[C][0], DVP = kDims[C][1];
-  const bool fast = args_fast(a);
-  if constexpr (C == kClasses - 1) {       // 64 queries: 2 groups of 32; 128 (bf16 only): 4 groups, two waves a SIMD
-    if (sizeof(T) == 2 && many) {
-      const auto kernel = fast ? attn_fwd<T, DP, DVP, 2, sizeof(T) == 2 ? 4 : 2, 2, true> : attn_fwd<T, DP, DVP, 2, sizeof(T) == 2 ? 4 : 2, 2, false>;
-      kernel<<<grid, 512, 0, s>>>(a);
-    } else {
-      const auto kernel = fast ? attn_fwd<T, DP, DVP, 2, 2, 2, true> : attn_fwd<T, DP, DVP, 2, 2, 2, false>;
-      kernel<<<grid, 256, 0, s>>>(a);
-    }
+  constexpr bool WIDE = C == kClasses - 1;       // two waves a query group
+  constexpr int RT = WIDE ? 2 : 1, QG = WIDE ? 2 : 4, CS = WIDE ? 2 : 1;       // 64 queries
+  // 128: twice the query groups (two waves a SIMD), or twice the queries of a wave
+  constexpr int RT2 = 2, QG2 = sizeof(T) == 4 && WIDE ? 2 : 4;
+  if (p.img) {
+    const auto kernel = p.many ? attn_fwd<T, DP, DVP, RT2, QG2, CS, true, false> : attn_fwd<T, DP, DVP, RT, QG, CS, true, false>;
+    kernel<<<grid, 64 * CS * (p.many ? QG2 : QG), 0, s>>>(a);
   } else {
-    const auto kernel = many ? (fast ? attn_fwd<T, DP, DVP, 2, 4, 1, true> : attn_fwd<T, DP, DVP, 2, 4, 1, false>)
-                             : (fast ? attn_fwd<T, DP, DVP, 1, 4, 1, true> : attn_fwd<T, DP, DVP, 1, 4, 1, false>);
-    kernel<<<grid, 256, 0, s>>>(a);
+    const auto kernel = args_fast(a) ? attn_fwd<T, DP, DVP, RT, QG, CS, false, true> : attn_fwd<T, DP, DVP, RT, QG, CS, false, false>;
+    kernel<<<grid, 64 * CS * QG, 0, s>>>(a);
   }
 }
 
@@ -597,15 +696,24 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   a.splits = (int)p.splits;
   a.span = (int)p.span;
   const size_t rows = (size_t)p.splits * bh * sh.sq;
-  a.part = (float*)ws;
-  a.part_ml = (float2*)(ws + vx_align(rows * sh.dv * 4));
+  a.k_img = ws;
+  a.v_img = ws + p.k_img;
+  a.part = (float*)(ws + p.k_img + p.v_img);
+  a.part_ml = (float2*)(ws + p.k_img + p.v_img + vx_align(rows * sh.dv * 4));
+  if (p.img && p.tiles_k) {
+    const int c = class_of(sh.d, sh.dv), kd = kDims[c][0] / 32, nv = kDims[c][1] / 16, kt = AttnTile<T>::KT;
+    const int64_t ks = sh.b * sh.hk * p.tiles_k * (kt / 16) * kd * 64, all = ks + sh.b * sh.hv * p.tiles_k * nv * (kt / 32) * 64;
+    VX_REQUIRE(vx_cdiv(all, 256) < (1LL << 31), "attn_fwd: too many keys");
+    attn_pack<T><<<(unsigned)vx_cdiv(all, 256), 256, 0, s>>>(a, ws, ws + p.k_img, (int)p.tiles_k, kd, nv, ks, all);
+    VX_LAUNCH_CHECK();
+  }
   switch (class_of(sh.d, sh.dv)) {
-    case 0: launch_fwd<T, 0>(a, p.many, (unsigned)grid, s); break;
-    case 1: launch_fwd<T, 1>(a, p.many, (unsigned)grid, s); break;
-    case 2: launch_fwd<T, 2>(a, p.many, (unsigned)grid, s); break;
-    case 3: launch_fwd<T, 3>(a, p.many, (unsigned)grid, s); break;
-    case 4: launch_fwd<T, 4>(a, p.many, (unsigned)grid, s); break;
-    default: launch_fwd<T, 5>(a, p.many, (unsigned)grid, s); break;
+    case 0: launch_fwd<T, 0>(a, p, (unsigned)grid, s); break;
+    case 1: launch_fwd<T, 1>(a, p, (unsigned)grid, s); break;
+    case 2: launch_fwd<T, 2>(a, p, (unsigned)grid, s); break;
+    case 3: launch_fwd<T, 3>(a, p, (unsigned)grid, s); break;
+    case 4: launch_fwd<T, 4>(a, p, (unsigned)grid, s); break;
+    default: launch_fwd<T, 5>(a, p, (unsigned)grid, s); break;
   }
   VX_LAUNCH_CHECK();
   if (p.splits > 1) {

@@ -37,6 +37,20 @@ struct FwdArgs {
   int n, k, act, tiles_n;
 };
 
+// y[m][n .. n + 3] from the product v: `left` of the four exist
+template <typename T>
+__device__ __forceinline__ void linear_finish(const FwdArgs<T>& a, long long m, int n, int left, vx_f32x4 v) {
+  if (a.bias) v += vx_load4(a.bias + n, left);
+  if (a.res) v += vx_load4(a.res + m * a.ldr + n, left);
+  const long long at = m * a.n + n;
+  if (a.pre) vx_store4(a.pre + at, v, left);
+  if (a.act != kActNone) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = act_value(v[i], a.act);
+  }
+  vx_store4(a.y + at, v, left);
+}
+
 template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a) {
   __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
@@ -49,18 +63,51 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a
   const VxOperand<T> X{a.x + m0 * a.ldx, a.ldx, rows_m, nullptr}, W{a.w + (long long)n0 * a.ldw, a.ldw, rows_n, nullptr};
   vx_gemm_loop<T, KC, KC, TM, TN, FAST>(X, W, 0, a.k, lds, acc);
   vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
-    const int left = rows_n - n;
-    if (m >= rows_m || left <= 0) return;
-    if (a.bias) v += vx_load4(a.bias + n0 + n, left);
-    if (a.res) v += vx_load4(a.res + (m0 + m) * a.ldr + n0 + n, left);
-    const long long at = (m0 + m) * a.n + n0 + n;
-    if (a.pre) vx_store4(a.pre + at, v, left);
-    if (a.act != kActNone) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = act_value(v[i], a.act);
-    }
-    vx_store4(a.y + at, v, left);
+    if (m < rows_m && n < rows_n) linear_finish(a, m0 + m, n0 + n, rows_n - n, v);
   });
+}
+
+// Few rows: what counts is latency. A workgroup owns 16 x 16 outputs, its four waves every fourth 32-k step each, with operands
+// straight from memory in fragment order and four steps of loads in flight; the four partial sums meet in LDS, added in order.
+template <typename T, bool FAST>
+__global__ __launch_bounds__(kTileThreads) void linear_few(const FwdArgs<T> a) {
+  constexpr int NPL = VxType<T>::NPL, U = 4, E = sizeof(T);
+  __shared__ vx_f32x4 sh[kTileThreads / 64][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const long long m0 = (long long)(blockIdx.x / a.tiles_n) * 16;
+  const int n0 = (int)(blockIdx.x % a.tiles_n) * 16;
+  const bool row_m = m0 + c < a.m, row_n = n0 + c < a.n;
+  const T *px = a.x + m0 * a.ldx, *pw = a.w + (long long)n0 * a.ldw;
+  vx_f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k0 = wave * 32; k0 < a.k; k0 += U * 128) {
+    VxRow8<T> x[U], w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * 128, left = a.k - k - g * 8;
+      if constexpr (FAST) {
+        x[u].load(vx_buffer(px + k), row_m && left > 0 ? (c * (int)a.ldx + g * 8) * E : kVxOut);
+        w[u].load(vx_buffer(pw + k), row_n && left > 0 ? (c * (int)a.ldw + g * 8) * E : kVxOut);
+      } else {
+        x[u].load(px + c * a.ldx + k + g * 8, row_m ? left : 0);
+        w[u].load(pw + c * a.ldw + k + g * 8, row_n ? left : 0);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      VxFrag<NPL> fx, fw;
+      x[u].planes(fx);
+      w[u].planes(fw);
+#pragma unroll
+      for (int pr = 0; pr < VxProducts<NPL>::N; ++pr) acc = vx_mma(pr, fw, fx, acc);
+    }
+  }
+  sh[wave][lane] = acc;
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int i = 1; i < kTileThreads / 64; ++i) acc += sh[i][lane];
+  const int n = n0 + g * 4;
+  if (row_m && n < a.n) linear_finish(a, m0 + c, n, a.n - n, acc);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------
@@ -190,18 +237,24 @@ BwdPlan bwd_plan(int64_t m, int64_t n, int64_t k, int32_t dtype) {
   return p;
 }
 
+// linear_few instead of 64 x 64 tiles: time of a call in a graph, us, few / 64 x 64, 384 -> 512 and 640 -> 640: fp32 1 row 3.0 / 9.7,
+// 4.1 / 14.9; 512 rows 8.2 / 10.6, 15.9 / 16.0 (1024, 1280 workgroups); 1024 rows 14.1 / 10.9. bf16 1 row 2.3 / 4.0; 256 rows
+// 3.5 / 4.5, 5.8 / 5.9 (512, 640 workgroups); 512 rows 5.0 / 4.5.
+bool few_rule(int64_t m, int64_t n, int64_t cus, bool f32) { return vx_cdiv(m, 16) * vx_cdiv(n, 16) <= (f32 ? 4 : 2) * cus; }
+
 template <typename T>
 int32_t fwd_impl(const FwdArgs<T>& args, hipStream_t s) {
   FwdArgs<T> a = args;
-  const int64_t big = vx_cdiv(a.m, 128) * vx_cdiv(a.n, 128);
-  const bool use_big = big >= vx_tile_cus();
-  const int64_t t = use_big ? 128 : 64;
+  const int64_t cus = vx_tile_cus();
+  const bool few = few_rule(a.m, a.n, cus, sizeof(T) == 4), use_big = vx_cdiv(a.m, 128) * vx_cdiv(a.n, 128) >= cus;
+  const int64_t t = few ? 16 : use_big ? 128 : 64;
   a.tiles_n = (int)vx_cdiv(a.n, t);
   const int64_t grid = vx_cdiv(a.m, t) * a.tiles_n;
   VX_REQUIRE(grid < (1LL << 31), "linear_fwd: too many rows");
   const bool fast = vx_fast(a.x, a.ldx, a.k, sizeof(T)) && vx_fast(a.w, a.ldw, a.k, sizeof(T));
-  const auto kernel = use_big ? (fast ? linear_fwd<T, 128, 128, true> : linear_fwd<T, 128, 128, false>)
-                              : (fast ? linear_fwd<T, 64, 64, true> : linear_fwd<T, 64, 64, false>);
+  const auto kernel = few ? (fast ? linear_few<T, true> : linear_few<T, false>)
+                          : use_big ? (fast ? linear_fwd<T, 128, 128, true> : linear_fwd<T, 128, 128, false>)
+                                    : (fast ? linear_fwd<T, 64, 64, true> : linear_fwd<T, 64, 64, false>);
   kernel<<<(unsigned)grid, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
   return VX_OK;

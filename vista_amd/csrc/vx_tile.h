@@ -228,6 +228,14 @@ struct VxCol8<__bf16, W> {
   }
 };
 
+// ---- copies from memory to LDS ----------------------------------------------------------------------------------
+// one fragment (1 KB, in lane order in memory too) straight to LDS, without registers; vx_arrived() waits for all of a wave's
+__device__ __forceinline__ void vx_copy_frag(const void* from, char* to, int lane) {
+  __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(const_cast<char*>((const char*)from) + lane * 16),
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+__device__ __forceinline__ void vx_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // ---- LDS image --------------------------------------------------------------------------------------------------
 // byte of (row block rb, k step ks, slot) of an image with NK k steps; slot = row & 15 + 16 * k group
 template <int NK>
@@ -357,7 +365,8 @@ constexpr int vx_gemm_lds() {
 
 // acc[mi][ni] += the TM x TN tile's product over k in [k0, kend); wave (wm, wn) of 2 x 2 owns TM/2 x TN/2. One LDS image,
 // two barriers per step: the next step's operands travel to registers while this one's are multiplied, and the two or
-// three workgroups of a CU cover each other's barriers. Ends with a barrier: the caller may reuse the LDS.
+// three workgroups of a CU cover each other's barriers (two images, or two and three steps in flight, were no faster at any
+// size: the steps are bound by the splitting and the LDS, not by latency). Ends with a barrier: the caller may reuse the LDS.
 template <typename T, int XM, int WM, int TM, int TN, bool FAST>
 __device__ __forceinline__ void vx_gemm_loop(const VxOperand<T>& X, const VxOperand<T>& W, int k0, int kend, char* lds,
                                              vx_f32x4 (&acc)[TM / 32][TN / 32]) {

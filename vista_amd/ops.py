@@ -4,6 +4,7 @@ PyTorch is plumbing here: it owns device memory (caching allocator) and streams.
 requires CUDA(HIP) tensors and raises otherwise: there is no CPU path.
 """
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -596,22 +597,36 @@ def bn_bwd_apply(dy, x, mask, mean, invstd, gamma, sums, count, want_dres=False)
 # ------------------------------------------------------------------------------------------------
 # dense layer with its epilogue, attention
 # ------------------------------------------------------------------------------------------------
-def _on_one_device(first, **tensors):
-    _need_gpu(first[1], first[0])
-    for name, t in tensors.items():
+# These calls take some microseconds on the device, so the host side is kept short: raw pointers and the raw stream go straight to
+# ctypes, and what follows from sizes and strides alone (argument arrays, workspace sizes) is worked out once per geometry.
+def _at(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _launch(dev, fn, *args):
+    """fn(*args, the current stream of `dev`) with `dev` current."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _check_tensors(first, name, others, names):
+    """`first` is a float32 / bfloat16 HIP tensor; the `others` (None: absent) share its device and dtype."""
+    if not isinstance(first, torch.Tensor) or not first.is_cuda:
+        _need_gpu(first, name)
+    if first.dtype not in _DT:
+        raise ValueError(f"unsupported {name} dtype {first.dtype}: float32 or bfloat16")
+    for t, n in zip(others, names):
         if t is None:
             continue
-        _need_gpu(t, name)
-        if t.device != first[1].device:
-            raise ValueError(f"{name} is on {t.device}, {first[0]} on {first[1].device}")
-
-
-def _same_dtype(first, **tensors):
-    if first[1].dtype not in _DT:
-        raise ValueError(f"unsupported {first[0]} dtype {first[1].dtype}: float32 or bfloat16")
-    for name, t in tensors.items():
-        if t is not None and t.dtype != first[1].dtype:
-            raise ValueError(f"{name} is {t.dtype}, {first[0]} {first[1].dtype}: they must share a dtype")
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            _need_gpu(t, n)
+        if t.device != first.device:
+            raise ValueError(f"{n} is on {t.device}, {name} on {first.device}")
+        if t.dtype != first.dtype:
+            raise ValueError(f"{n} is {t.dtype}, {name} {first.dtype}: they must share a dtype")
 
 
 def _act_code(act):
@@ -626,35 +641,44 @@ def _rows(t):
     return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
 
 
-def _linear_check(x, weight):
+def _linear_sizes(x, weight):
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} must be [rows, fin] and [fout, fin]")
-    if weight.shape[0] < 1 or weight.shape[1] < 1 or max(weight.shape) > 1 << 20 or x.shape[0] >= 1 << 31:
+    (m, k), n = x.shape, weight.shape[0]
+    if n < 1 or k < 1 or n > 1 << 20 or k > 1 << 20 or m >= 1 << 31:
         raise ValueError(f"sizes out of range: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    return m, k, n
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_bwd_bytes(device, m, n, k, dtype):
+    with torch.cuda.device(device):
+        return L.lib().vx_linear_bwd_workspace_bytes(m, n, k, dtype)
 
 
 def linear_fwd(x, weight, bias=None, residual=None, act="none", want_pre=False):
     """x [m, k], weight [n, k], bias [n], residual [m, n] -> (y [m, n], pre [m, n] | None): y = act(x w^T + bias + residual),
     pre (want_pre) = the sum before the activation. One dtype (float32 or bfloat16); act: none, relu, gelu (erf form), silu."""
-    _on_one_device(("x", x), weight=weight, bias=bias, residual=residual)
-    _same_dtype(("x", x), weight=weight, bias=bias, residual=residual)
+    _check_tensors(x, "x", (weight, bias, residual), ("weight", "bias", "residual"))
     code = _act_code(act)
-    _linear_check(x, weight)
-    (m, k), n = x.shape, weight.shape[0]
-    if bias is not None and tuple(bias.shape) != (n,):
-        raise ValueError(f"bias must be [{n}], got {tuple(bias.shape)}")
-    if residual is not None and tuple(residual.shape) != (m, n):
-        raise ValueError(f"residual must be [{m}, {n}], got {tuple(residual.shape)}")
+    m, k, n = _linear_sizes(x, weight)
     x, weight = _rows(x), _rows(weight)
-    bias = bias.contiguous() if bias is not None else None
-    residual = _rows(residual) if residual is not None else None
+    if bias is not None:
+        if bias.shape != (n,):
+            raise ValueError(f"bias must be [{n}], got {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    ldr = 0
+    if residual is not None:
+        if residual.shape != (m, n):
+            raise ValueError(f"residual must be [{m}, {n}], got {tuple(residual.shape)}")
+        residual = _rows(residual)
+        ldr = residual.stride(0)
     y = torch.empty((m, n), dtype=x.dtype, device=x.device)
     pre = torch.empty_like(y) if want_pre else None
-    with torch.cuda.device(x.device), _Timed("linear", m=m, n=n, k=k, esize=x.element_size()):
-        rc = L.lib().vx_linear_fwd(_ptr(x), x.stride(0), _ptr(weight), weight.stride(0), _ptr(bias), _ptr(residual),
-                                   residual.stride(0) if residual is not None else 0, m, n, k, code, _ptr(y), _ptr(pre),
-                                   _DT[x.dtype], _stream())
-    L.check(rc, "vx_linear_fwd")
+    rc = _launch(x.device, L.lib().vx_linear_fwd, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), _at(bias),
+                 _at(residual), ldr, m, n, k, code, y.data_ptr(), _at(pre), _DT[x.dtype])
+    if rc:
+        L.check(rc, "vx_linear_fwd")
     return y, pre
 
 
@@ -662,30 +686,54 @@ def linear_bwd(dy, x, weight, act="none", saved=None, want_dx=True, want_dw=True
     """Gradients of linear_fwd -> (dx [m, k], dw [n, k], dbias [n], dpre [m, n]); an unwanted one is None. saved = y of relu,
     pre of gelu / silu, unused without an activation. dpre = dy * act'(saved) is the residual's gradient (dy itself
     without an activation)."""
-    _on_one_device(("dy", dy), x=x, weight=weight, saved=saved)
-    _same_dtype(("dy", dy), x=x, weight=weight, saved=saved)
+    _check_tensors(dy, "dy", (x, weight, saved), ("x", "weight", "saved"))
     code = _act_code(act)
-    _linear_check(x, weight)
-    (m, k), n = x.shape, weight.shape[0]
-    if tuple(dy.shape) != (m, n):
+    m, k, n = _linear_sizes(x, weight)
+    if dy.shape != (m, n):
         raise ValueError(f"dy must be [{m}, {n}], got {tuple(dy.shape)}")
-    if code and (saved is None or tuple(saved.shape) != (m, n)):
-        raise ValueError(f"act={act!r} needs saved [{m}, {n}]: relu's output, the pre-activation of gelu / silu")
+    if code:
+        if saved is None or saved.shape != (m, n):
+            raise ValueError(f"act={act!r} needs saved [{m}, {n}]: relu's output, the pre-activation of gelu / silu")
+        saved = saved.contiguous()
     x, weight, g = _rows(x), _rows(weight), _rows(dy)
-    saved = saved.contiguous() if code else None
     dev, dt = x.device, x.dtype
     dpre = torch.empty((m, n), dtype=dt, device=dev) if code else dy
     dx = torch.empty((m, k), dtype=dt, device=dev) if want_dx else None
     dw = torch.empty((n, k), dtype=dt, device=dev) if want_dw else None
     db = torch.empty((n,), dtype=dt, device=dev) if want_dbias else None
-    lib = L.lib()
-    with torch.cuda.device(dev):
-        wsb = lib.vx_linear_bwd_workspace_bytes(m, n, k, _DT[dt])
-        ws = _ws(wsb, dev)
-        rc = lib.vx_linear_bwd(_ptr(g), g.stride(0), _ptr(x), x.stride(0), _ptr(weight), weight.stride(0), _ptr(saved), m, n, k,
-                               code, _ptr(dpre) if code else None, _ptr(dx), _ptr(dw), _ptr(db), _DT[dt], _ptr(ws), wsb, _stream())
-    L.check(rc, "vx_linear_bwd")
+    wsb = _linear_bwd_bytes(dev.index, m, n, k, _DT[dt])
+    ws = _ws(wsb, dev)
+    rc = _launch(dev, L.lib().vx_linear_bwd, g.data_ptr(), g.stride(0), x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0),
+                 _at(saved) if code else None, m, n, k, code, dpre.data_ptr() if code else None, _at(dx), _at(dw), _at(db), _DT[dt],
+                 ws.data_ptr(), wsb)
+    if rc:
+        L.check(rc, "vx_linear_bwd")
     return dx, dw, db, dpre
+
+
+class _AttnGeometry:
+    """What vx_attn_* need that follows from sizes and strides alone."""
+
+    def __init__(self, device, qs, ks, vs, q_st, k_st, v_st, mask_st, dtype):
+        (b, sq, h, d), (bk, sk, hk, dk), (bv, sv, hv, dv) = qs, ks, vs
+        if bk != b or bv != b or sv != sk or dk != d:
+            raise ValueError(f"q {qs}, k {ks} and v {vs} do not match")
+        if h < 1 or hk < 1 or hv < 1 or h % hk or h % hv:
+            raise ValueError(f"key heads ({hk}) and value heads ({hv}) must divide the query heads ({h})")
+        if not (1 <= d <= L.VX_ATTN_MAX_DIM and 1 <= dv <= L.VX_ATTN_MAX_VDIM):
+            raise ValueError(f"head width must be in [1, {L.VX_ATTN_MAX_DIM}], value width in [1, {L.VX_ATTN_MAX_VDIM}], got {d}, {dv}")
+        if b >= 1 << 24 or sq >= 1 << 30 or sk >= 1 << 30 or h >= 1 << 16 or b * h >= 1 << 24:
+            raise ValueError("attention sizes out of range")
+        self.shape = (ctypes.c_int64 * 8)(b, sq, sk, h, hk, hv, d, dv)
+        self.strides = (ctypes.c_int64 * 10)(*q_st[:3], *k_st[:3], *v_st[:3], mask_st)
+        self.scale = d ** -0.5
+        self.out, self.stats = (b, sq, h, dv), (b * h, sq, 2)
+        with torch.cuda.device(device):
+            self.fwd_bytes = L.lib().vx_attn_fwd_workspace_bytes(self.shape, dtype)
+            self.bwd_bytes = L.lib().vx_attn_bwd_workspace_bytes(self.shape, dtype)
+
+
+_attn_geometry = functools.lru_cache(maxsize=1024)(_AttnGeometry)
 
 
 def _heads_last(t):
@@ -694,30 +742,22 @@ def _heads_last(t):
 
 
 def _attn_args(q, k, v, key_mask):
-    _on_one_device(("q", q), k=k, v=v, key_mask=key_mask)
-    _same_dtype(("q", q), k=k, v=v)
+    _check_tensors(q, "q", (k, v), ("k", "v"))
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("q, k and v must be [batch, length, heads, width]")
-    b, sq, h, d = q.shape
-    sk, hk, hv, dv = k.shape[1], k.shape[2], v.shape[2], v.shape[3]
-    if k.shape[0] != b or v.shape[0] != b or v.shape[1] != sk or k.shape[3] != d:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
-    if h < 1 or hk < 1 or hv < 1 or h % hk or h % hv:
-        raise ValueError(f"key heads ({hk}) and value heads ({hv}) must divide the query heads ({h})")
-    if not (1 <= d <= L.VX_ATTN_MAX_DIM and 1 <= dv <= L.VX_ATTN_MAX_VDIM):
-        raise ValueError(f"head width must be in [1, {L.VX_ATTN_MAX_DIM}], value width in [1, {L.VX_ATTN_MAX_VDIM}], got {d}, {dv}")
-    if b >= 1 << 24 or sq >= 1 << 30 or sk >= 1 << 30 or h >= 1 << 16 or b * h >= 1 << 24:
-        raise ValueError("attention sizes out of range")
+    mask_st = 0
     if key_mask is not None:
-        if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (b, sk):
-            raise ValueError(f"key_mask must be bool [{b}, {sk}] (True: the key takes part), got {key_mask.dtype} "
-                             f"{tuple(key_mask.shape)}")
-        key_mask = key_mask if sk <= 1 or key_mask.stride(1) == 1 else key_mask.contiguous()
+        _need_gpu(key_mask, "key_mask")
+        if key_mask.dtype != torch.bool or key_mask.shape != (q.shape[0], k.shape[1]) or key_mask.device != q.device:
+            raise ValueError(f"key_mask must be bool [{q.shape[0]}, {k.shape[1]}] on {q.device} (True: the key takes part), got "
+                             f"{key_mask.dtype} {tuple(key_mask.shape)} on {key_mask.device}")
+        if key_mask.shape[1] > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+        mask_st = key_mask.stride(0)
     q, k, v = _heads_last(q), _heads_last(k), _heads_last(v)
-    shape = (ctypes.c_int64 * 8)(b, sq, sk, h, hk, hv, d, dv)
-    strides = (ctypes.c_int64 * 10)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-                                    key_mask.stride(0) if key_mask is not None else 0)
-    return q, k, v, key_mask, shape, strides
+    geo = _attn_geometry(q.device.index, tuple(q.shape), tuple(k.shape), tuple(v.shape), q.stride(), k.stride(), v.stride(), mask_st,
+                         _DT[q.dtype])
+    return q, k, v, key_mask, geo
 
 
 def attn_fwd(q, k, v, key_mask=None, scale=None, want_stats=False):
@@ -725,42 +765,36 @@ def attn_fwd(q, k, v, key_mask=None, scale=None, want_stats=False):
     Query head i reads key head i // (h / hk) and value head i // (h / hv); key_mask bool [b, sk], True where the key takes part;
     a query without keys gives zeros. scale defaults to d ** -0.5. stats (want_stats) is what attn_bwd needs. Any strides with
     a contiguous last dimension are read in place."""
-    q, k, v, key_mask, shape, strides = _attn_args(q, k, v, key_mask)
-    b, sq, h, d = q.shape
-    scale = d ** -0.5 if scale is None else float(scale)
-    out = torch.empty((b, sq, h, v.shape[3]), dtype=q.dtype, device=q.device)
-    stats = torch.empty((b * h, sq, 2), dtype=torch.float32, device=q.device) if want_stats else None
-    lib = L.lib()
-    with torch.cuda.device(q.device), _Timed("attn", b=b, sq=sq, sk=k.shape[1], h=h, d=d, dv=v.shape[3], esize=q.element_size()):
-        wsb = lib.vx_attn_fwd_workspace_bytes(shape, _DT[q.dtype])
-        ws = _ws(wsb, q.device) if wsb else None
-        rc = lib.vx_attn_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(key_mask), shape, strides, scale, _ptr(out), _ptr(stats),
-                             _DT[q.dtype], _ptr(ws), wsb, _stream())
-    L.check(rc, "vx_attn_fwd")
+    q, k, v, key_mask, geo = _attn_args(q, k, v, key_mask)
+    dev = q.device
+    out = torch.empty(geo.out, dtype=q.dtype, device=dev)
+    stats = torch.empty(geo.stats, dtype=torch.float32, device=dev) if want_stats else None
+    ws = _ws(geo.fwd_bytes, dev) if geo.fwd_bytes else None
+    rc = _launch(dev, L.lib().vx_attn_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(key_mask), geo.shape, geo.strides,
+                 geo.scale if scale is None else float(scale), out.data_ptr(), _at(stats), _DT[q.dtype], _at(ws), geo.fwd_bytes)
+    if rc:
+        L.check(rc, "vx_attn_fwd")
     return out, stats
 
 
 def attn_bwd(dout, q, k, v, out, stats, key_mask=None, scale=None):
     """Gradients of attn_fwd from its own out and stats -> (dq, dk, dv), shaped as q, k and v; the probabilities are recomputed.
     Gradients of masked keys are 0."""
-    q, k, v, key_mask, shape, strides = _attn_args(q, k, v, key_mask)
-    b, sq, h, d = q.shape
-    dv_ = v.shape[3]
-    _on_one_device(("q", q), dout=dout, out=out, stats=stats)
-    _same_dtype(("q", q), dout=dout, out=out)
-    if tuple(dout.shape) != (b, sq, h, dv_) or tuple(out.shape) != (b, sq, h, dv_) or not out.is_contiguous():
-        raise ValueError(f"dout and out must be [{b}, {sq}, {h}, {dv_}], out contiguous (attn_fwd's own)")
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (b * h, sq, 2) or not stats.is_contiguous():
+    q, k, v, key_mask, geo = _attn_args(q, k, v, key_mask)
+    _check_tensors(q, "q", (dout, out), ("dout", "out"))
+    dev = q.device
+    if dout.shape != geo.out or out.shape != geo.out or not out.is_contiguous():
+        raise ValueError(f"dout and out must be {list(geo.out)}, out contiguous (attn_fwd's own)")
+    _need_gpu(stats, "stats")
+    if stats.dtype != torch.float32 or stats.shape != geo.stats or not stats.is_contiguous() or stats.device != dev:
         raise ValueError("stats must be what attn_fwd(want_stats=True) returned")
-    scale = d ** -0.5 if scale is None else float(scale)
     dout = _heads_last(dout)
     dout_strides = (ctypes.c_int64 * 3)(*dout.stride()[:3])
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    lib = L.lib()
-    with torch.cuda.device(q.device):
-        wsb = lib.vx_attn_bwd_workspace_bytes(shape, _DT[q.dtype])
-        ws = _ws(wsb, q.device)
-        rc = lib.vx_attn_bwd(_ptr(dout), dout_strides, _ptr(q), _ptr(k), _ptr(v), _ptr(key_mask), shape, strides, _ptr(out),
-                             _ptr(stats), scale, _ptr(dq), _ptr(dk), _ptr(dv), _DT[q.dtype], _ptr(ws), wsb, _stream())
-    L.check(rc, "vx_attn_bwd")
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+    ws = _ws(geo.bwd_bytes, dev)
+    rc = _launch(dev, L.lib().vx_attn_bwd, dout.data_ptr(), dout_strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(key_mask),
+                 geo.shape, geo.strides, out.data_ptr(), stats.data_ptr(), geo.scale if scale is None else float(scale), dq.data_ptr(),
+                 dk.data_ptr(), dv.data_ptr(), _DT[q.dtype], ws.data_ptr(), geo.bwd_bytes)
+    if rc:
+        L.check(rc, "vx_attn_bwd")
     return dq, dk, dv
