@@ -9,8 +9,6 @@
 // by about as much as the output's own rounding).
 // A masked key has no part in anything, whatever its rows hold; a query without keys gives zeros. No atomics: bitwise
 // reproducible.
-#include <stdlib.h>
-
 #include "vx_tile.h"
 
 namespace {
@@ -23,7 +21,8 @@ struct AttnArgs {
   const uint8_t* mask;                       // [batch][mask_b] bytes, or null
   long long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h, mask_b;
   int sq, sk, h, gk, gv, d, dv;              // gk, gv: query heads per key / value head
-  float scale2;                              // scale * log2(e)
+  float scale2, sign;                        // scale * log2(e) as scale2 > 0 (1 for scale 0) and a sign of 1, -1 or 0, so that the
+                                             // maximum of the scores is that of the scaled ones and masked ones stay -inf
 };
 
 template <typename T>
@@ -58,7 +57,7 @@ __device__ __forceinline__ bool attn_key_live(const AttnArgs<T>& a, const uint8_
 // reader. IMG: both come as finished images (attn_pack) and go straight to LDS; else (few queries) through registers, where
 // they are split and V is transposed.
 template <typename T, int DP, int DVP, int RT, int QG, int CS, bool IMG, bool FAST>
-__global__ __launch_bounds__(64 * QG * CS, (DVP > 192 && QG * CS == 4) || (DVP > 64 && VxType<T>::NPL == 3) ? 1 : 2)
+__global__ __launch_bounds__(64 * QG * CS, QG * CS == 8 ? 2 : DVP > 192 || (DVP > 64 && VxType<T>::NPL == 3) ? 1 : 2)
 void attn_fwd(const FwdArgs<T> a) {
   constexpr int NPL = VxType<T>::NPL, KT = AttnTile<T>::KT, NS = KT / 32;     // NS: 32-key steps of a tile
   constexpr int KD = DP / 32, NV = DVP / 16 / CS, NK = KT / 16, OWN = NK / CS, E = sizeof(T), NW = QG * CS;
@@ -101,6 +100,10 @@ void attn_fwd(const FwdArgs<T> a) {
       else
         x.load(qp + (rt * 16 + c) * a.q_s + d, row < a.sq ? a.d - d : 0);
       x.planes(qf[rt][kd]);
+      if (a.sign != 1.0f) {                    // exact: -1 and 0 times the planes
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) qf[rt][kd].p[i] = a.sign == 0.0f ? bf16x8{} : -qf[rt][kd].p[i];
+      }
     }
   }
   float m[RT], l[RT];                          // reference of the exponents (log2), sum of this lane's keys
@@ -257,6 +260,15 @@ void attn_fwd(const FwdArgs<T> a) {
           s[rt][k] = *reinterpret_cast<const vx_f32x4*>(swap + (((wave & ~1) + k / OWN) * OWN * RT + rt * OWN + k % OWN) * kFragBytes + lane * 16);
     }
     VxFrag<NPL> pf[RT][NS];
+    if (cur != ~0ull >> (64 - KT)) {           // some keys take no part
+      const unsigned long long bits = cur >> (g * 4);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[rt][k][i] = bits >> (k * 16 + i) & 1 ? s[rt][k][i] : -INFINITY;
+    }
     float alpha[RT];
     bool moved = false;
 #pragma unroll
@@ -265,13 +277,9 @@ void attn_fwd(const FwdArgs<T> a) {
 #pragma unroll
       for (int k = 0; k < NK; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool live = cur >> (k * 16 + g * 4 + i) & 1;
-          s[rt][k][i] = live ? s[rt][k][i] * a.scale2 : -INFINITY;
-          mx = fmaxf(mx, s[rt][k][i]);
-        }
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][k][i]);
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale2;   // the maximum of the scaled scores
       // the reference follows the maximum only when it is 2^8 behind: values stay below 2^8, far from any limit of fp32, and the
       // accumulators are hardly ever rescaled
       const bool far = mx > m[rt] + 8.0f;
@@ -285,7 +293,7 @@ void attn_fwd(const FwdArgs<T> a) {
         float p[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          p[j] = __builtin_amdgcn_exp2f(s[rt][ns * 2 + (j >> 2)][j & 3] - ref);
+          p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][ns * 2 + (j >> 2)][j & 3], a.scale2, -ref));
           sum += p[j];
         }
         vx_planes(p, pf[rt][ns]);
@@ -394,44 +402,58 @@ __global__ __launch_bounds__(256) void attn_pack(const AttnArgs<T> a, char* __re
   for (int q = 0; q < NPL; ++q) *reinterpret_cast<bf16x8*>(to + (long long)q * frags * kFragBytes) = f.p[q];
 }
 
-// joins the splits of a row: weights 2^(m_s - m), in order of the splits. One thread per four output values.
-template <typename T>
+// joins the splits of a row: weights 2^(m_s - m). A workgroup has 256 / J quads of output values, J lanes each: lane j adds the
+// splits j, j + J, ..., four of them in flight (few rows: what counts is latency), then the J sums are added in order.
+template <typename T, int J>
 __global__ __launch_bounds__(256) void attn_join(const FwdArgs<T> a, long long items, int quads) {
-  const long long it = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (it >= items) return;
-  const long long rowid = it / quads;               // bh * sq + row
-  const int n = (int)(it % quads) * 4;
-  const long long rows = items / quads;
-  constexpr int U = 8;                              // splits in flight: what a row costs is latency
-  const int last = a.splits - 1;
+  constexpr int U = 4, Q = 256 / J;
+  __shared__ vx_f32x4 sh_o[J][Q];
+  __shared__ float sh_l[J][Q];
+  const int lane = threadIdx.x % Q, j = threadIdx.x / Q;
+  const long long it = (long long)blockIdx.x * Q + lane;
+  const bool here = it < items;
+  const long long rowid = here ? it / quads : 0, rows = items / quads;      // bh * sq + row
+  const int n = here ? (int)(it % quads) * 4 : 0, last = a.splits - 1;
   float m = -INFINITY;
-  for (int s0 = 0; s0 < a.splits; s0 += U) {
-    float x[U];
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    float x[8];
 #pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = a.part_ml[(s0 + u < last ? s0 + u : last) * rows + rowid].x;
+    for (int u = 0; u < 8; ++u) x[u] = a.part_ml[(s0 + u < last ? s0 + u : last) * rows + rowid].x;
 #pragma unroll
-    for (int u = 0; u < U; ++u) m = fmaxf(m, x[u]);
+    for (int u = 0; u < 8; ++u) m = fmaxf(m, x[u]);
   }
   const float ref = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
   vx_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s0 = 0; s0 < a.splits; s0 += U) {
+  for (int s0 = j; s0 < a.splits; s0 += U * J) {
     float2 ml[U];
     vx_f32x4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long at = (s0 + u < last ? s0 + u : last) * rows + rowid;
+      const long long at = (s0 + u * J < last ? s0 + u * J : last) * rows + rowid;
       ml[u] = a.part_ml[at];
       v[u] = vx_load4(a.part + at * a.dv + n, a.dv - n);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (s0 + u > last) break;
+      if (s0 + u * J > last) break;
       const float wgt = __builtin_amdgcn_exp2f(ml[u].x - ref);
       l += wgt * ml[u].y;
       o += v[u] * wgt;
     }
   }
+  if constexpr (J > 1) {
+    sh_o[j][lane] = o;
+    sh_l[j][lane] = l;
+    __syncthreads();
+    if (j) return;
+#pragma unroll
+    for (int i = 1; i < J; ++i) {
+      l += sh_l[i][lane];
+      o += sh_o[i][lane];
+    }
+  }
+  if (!here) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int bh = (int)(rowid / a.sq), row = (int)(rowid % a.sq), b = bh / a.h, h = bh % a.h;
   vx_store4(a.out + (((long long)b * a.sq + row) * a.h + h) * a.dv + n, o * inv, a.dv - n);
@@ -511,7 +533,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) 
       vx_f32x4 p, d;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[i] = live[i] ? __builtin_amdgcn_exp2f(s[mi][ni][i] * a.scale2 - st.x) * st.y : 0.0f;
+        p[i] = live[i] ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[mi][ni][i] * a.sign, a.scale2, -st.x)) * st.y : 0.0f;
         d[i] = live[i] ? p[i] * (dp[mi][ni][i] - delta) * a.scale : 0.0f;
       }
       const long long at = ((long long)bh * a.rows + m) * a.skp + n;
@@ -618,7 +640,8 @@ void fill_args(AttnArgs<T>& a, const Shape& s, const int64_t* st, const void* q,
   a.mask_b = st[9];
   a.sq = (int)s.sq; a.sk = (int)s.sk; a.h = (int)s.h;
   a.gk = (int)(s.h / s.hk); a.gv = (int)(s.h / s.hv); a.d = (int)s.d; a.dv = (int)s.dv;
-  a.scale2 = scale * kLog2e;
+  a.scale2 = scale == 0.0f ? 1.0f : fabsf(scale) * kLog2e;
+  a.sign = scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f;
 }
 
 // whether every row of a [batch, position, head, width] tensor can be read by buffer loads
@@ -632,7 +655,7 @@ bool args_fast(const AttnArgs<T>& a) {
 }
 
 // the smallest tile that holds both widths
-constexpr int kClasses = 6;
+constexpr int kClasses = 6, kWideF32 = 3;
 constexpr int kDims[kClasses][2] = {{32, 64}, {64, 64}, {64, 128}, {128, 128}, {96, 192}, {192, 384}};
 int class_of(int64_t d, int64_t dv) {
   int i = 0;
@@ -648,7 +671,17 @@ struct FwdPlan {
 FwdPlan fwd_plan(const Shape& s, int32_t dtype) {
   FwdPlan p;
   const int64_t cus = vx_tile_cus(), bh = s.b * s.h, kt = dtype == VX_F32 ? 32 : 64, tiles_k = vx_cdiv(s.sk, kt);
-  p.many = vx_cdiv(s.sq, 128) * bh >= cus && s.sq > 64 && !(dtype == VX_F32 && class_of(s.d, s.dv) == kClasses - 1);
+  // 128 queries a workgroup share a staged tile, 64 fill the CUs sooner. us of 64 / 128 at 1024 keys, 8 heads, n 128-query tiles:
+  // 192 / 384 wide, fp32: n = 128 125 / 180, 256 239 / 206, 2048 1887 / 1489; bf16: 50 / 64, 87 / 68, 633 / 480: a tile takes 1.45
+  // times as long, so whole rounds over the CUs decide. 64 / 64, fp32: 256 70 / 76, 512 104 / 101, 2048 358 / 317; bf16: 28 / 31,
+  // 38 / 37, 117 / 109: two workgroups of 64 fit a CU. 96 / 192 and 128 / 128, fp32: 128 loses everywhere (831 / 973, 746 / 845:
+  // one wave a SIMD) and is not built.
+  const int64_t n128 = vx_cdiv(s.sq, 128) * bh, n64 = vx_cdiv(s.sq, 64) * bh;
+  const int c = class_of(s.d, s.dv);
+  if (c == kClasses - 1)
+    p.many = 1.45 * vx_cdiv(n128, cus) < vx_cdiv(n64, cus);
+  else
+    p.many = n128 >= 2 * cus && !(dtype == VX_F32 && c >= kWideF32);
   p.tiles_q = vx_cdiv(s.sq, p.many ? 128 : 64);
   // few workgroups: split the keys so that every CU has one
   int64_t splits = p.tiles_q * bh > 0 ? cus / (p.tiles_q * bh) : 1;
@@ -657,9 +690,9 @@ FwdPlan fwd_plan(const Shape& s, int32_t dtype) {
   p.span = tiles_k ? vx_cdiv(tiles_k, splits) : 1;
   p.splits = tiles_k ? vx_cdiv(tiles_k, p.span) : 1;
   p.tiles_k = tiles_k;
-  static const char* env = getenv("VX_IMG");
-  p.img = p.tiles_q * (s.h / s.hk) > (env ? atoi(env) : 1);
-  const int c = class_of(s.d, s.dv);
+  // images pay from about five tiles of queries on; us with / without, 480 and 4096 keys, 4 x 2 heads of 192 / 384 fp32: 64 queries
+  // 31 / 25, 58 / 42; 256 32 / 34, 93 / 92; 512 38 / 44, 145 / 164; 2 x 8 heads of 64 / 64 bf16: 64 13 / 10, 23 / 15; 512 16 / 14, 49 / 48
+  p.img = p.tiles_q > 4;
   const size_t row = dtype == VX_F32 ? 6 : 2;      // bytes of a value's planes
   p.k_img = p.img ? (size_t)s.b * s.hk * tiles_k * kt * kDims[c][0] * row : 0;
   p.v_img = p.img ? (size_t)s.b * s.hv * tiles_k * kt * kDims[c][1] * row : 0;
@@ -674,13 +707,14 @@ size_t fwd_bytes(const Shape& s, int32_t dtype) {
 template <typename T, int C>
 void launch_fwd(const FwdArgs<T>& a, const FwdPlan& p, unsigned grid, hipStream_t s) {
   constexpr int DP = kDims[C][0], DVP = kDims[C][1];
-  constexpr bool WIDE = C == kClasses - 1;       // two waves a query group
-  constexpr int RT = WIDE ? 2 : 1, QG = WIDE ? 2 : 4, CS = WIDE ? 2 : 1;       // 64 queries
-  // 128: twice the query groups (two waves a SIMD), or twice the queries of a wave
-  constexpr int RT2 = 2, QG2 = sizeof(T) == 4 && WIDE ? 2 : 4;
-  if (p.img) {
-    const auto kernel = p.many ? attn_fwd<T, DP, DVP, RT2, QG2, CS, true, false> : attn_fwd<T, DP, DVP, RT, QG, CS, true, false>;
-    kernel<<<grid, 64 * CS * (p.many ? QG2 : QG), 0, s>>>(a);
+  constexpr bool WIDE = C == kClasses - 1, F32 = sizeof(T) == 4, MANY = WIDE || !F32 || C < kWideF32;
+  constexpr int RT = 1, QG = 4, CS = WIDE ? 2 : 1;       // 64 queries; wide heads: two waves a query group
+  // 128 queries: 32 a wave, but 16 and twice the waves for wide fp32 heads, whose registers hold no more
+  constexpr int RT2 = WIDE && F32 ? 1 : 2, QG2 = WIDE && F32 ? 8 : 4, CS2 = WIDE && F32 ? 1 : CS;
+  if (p.img && p.many) {
+    if constexpr (MANY) attn_fwd<T, DP, DVP, RT2, QG2, CS2, true, false><<<grid, 64 * QG2 * CS2, 0, s>>>(a);
+  } else if (p.img) {
+    attn_fwd<T, DP, DVP, RT, QG, CS, true, false><<<grid, 64 * QG * CS, 0, s>>>(a);
   } else {
     const auto kernel = args_fast(a) ? attn_fwd<T, DP, DVP, RT, QG, CS, false, true> : attn_fwd<T, DP, DVP, RT, QG, CS, false, false>;
     kernel<<<grid, 64 * CS * QG, 0, s>>>(a);
@@ -719,7 +753,10 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   if (p.splits > 1) {
     const int quads = (a.dv + 3) / 4;
     const int64_t items = bh * sh.sq * quads;
-    attn_join<T><<<(unsigned)vx_cdiv(items, 256), 256, 0, s>>>(a, items, quads);
+    if (p.splits > 8)
+      attn_join<T, 8><<<(unsigned)vx_cdiv(items, 32), 256, 0, s>>>(a, items, quads);
+    else
+      attn_join<T, 1><<<(unsigned)vx_cdiv(items, 256), 256, 0, s>>>(a, items, quads);
     VX_LAUNCH_CHECK();
   }
   return VX_OK;
