@@ -515,32 +515,40 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) 
                                   {a.k + b * a.k_b + (h / a.gk) * a.k_h + n0 * a.k_s, a.k_s, rows_n, nullptr}, 0, a.d, lds, s);
   vx_gemm_loop<T, KC, KC, TM, TN, FAST>({a.go + b * a.go_b + q * a.go_s + h * a.go_h, a.go_s, rows_m, nullptr},
                                   {a.v + b * a.v_b + (h / a.gv) * a.v_h + n0 * a.v_s, a.v_s, rows_n, nullptr}, 0, a.dv, lds, dp);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
   const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  unsigned live[TN / 64];                      // of this lane's eight keys
+  vx_acc_each<TM, TN>(s, [&](int mi, int, int j, int n, const vx_f32x4&, const vx_f32x4&) {
+    if (mi) return;
+    live[j] = 0;
 #pragma unroll
-  for (int ni = 0; ni < TN / 32; ++ni) {
-    const int n = n0 + wn * (TN / 2) + ni * 16 + (lane >> 4) * 4;
-    bool live[4];
+    for (int i = 0; i < 8; ++i) live[j] |= n + i < rows_n && (mask == nullptr || mask[n0 + n + i] != 0) ? 1u << i : 0u;
+  });
+  float2 st[TM / 32];
+  float delta[TM / 32];
+  vx_acc_each<TM, TN>(s, [&](int mi, int m, int j, int, const vx_f32x4&, const vx_f32x4&) {
+    if (j) return;
+    const long long r = (long long)bh * a.sq + a.q0 + m0 + (m < rows_m ? m : 0);
+    st[mi] = a.stats[r];
+    delta[mi] = a.delta[r];
+  });
+  const long long at0 = ((long long)bh * a.rows + m0) * a.skp + n0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) live[i] = n + i < a.sk && (mask == nullptr || mask[n + i] != 0);
+  for (int mi = 0; mi < TM / 32; ++mi)
 #pragma unroll
-    for (int mi = 0; mi < TM / 32; ++mi) {
-      const int m = m0 + wm * (TM / 2) + mi * 16 + (lane & 15);
-      if (m >= a.rows || n >= a.skp) continue;
-      const long long r = (long long)bh * a.sq + a.q0 + m;
-      const float2 st = a.stats[r];
-      const float delta = a.delta[r];
-      vx_f32x4 p, d;
+    for (int ni = 0; ni < TN / 32; ++ni)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[i] = live[i] ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[mi][ni][i] * a.sign, a.scale2, -st.x)) * st.y : 0.0f;
-        d[i] = live[i] ? p[i] * (dp[mi][ni][i] - delta) * a.scale : 0.0f;
+        const bool on = live[ni / 2] >> (ni % 2 * 4 + i) & 1;
+        const float p = on ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[mi][ni][i] * a.sign, a.scale2, -st[mi].x)) * st[mi].y : 0.0f;
+        dp[mi][ni][i] = on ? p * (dp[mi][ni][i] - delta[mi]) * a.scale : 0.0f;
+        s[mi][ni][i] = p;
       }
-      const long long at = ((long long)bh * a.rows + m) * a.skp + n;
-      vx_store4(a.p + at, p, 4);
-      vx_store4(a.ds + at, d, 4);
-    }
-  }
+  vx_acc_each<TM, TN>(s, [&](int mi, int m, int j, int n, const vx_f32x4& v, const vx_f32x4& w) {
+    if (m >= rows_m || n0 + n >= a.skp) return;
+    const long long at = at0 + (long long)m * a.skp + n;
+    vx_store8(a.p + at, v, w, 8);
+    vx_store8(a.ds + at, dp[mi][2 * j], dp[mi][2 * j + 1], 8);
+  });
 }
 
 // the three gradients of a chunk in one launch: dV slabs = P^T go, dK slabs = dS^T q (reduction over the queries of a split),
@@ -567,8 +575,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
                          is_v ? a.go_s : a.q_s, rows_n, nullptr};
     vx_gemm_loop<T, KS, KS, TM, TN, FAST>(X, W, 0, len, lds, acc);
     float* slab = (is_v ? a.slab_v : a.slab_k) + ((long long)(a.split0 + sp) * a.bh + bh) * a.sk * width;
-    vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
-      if (m < rows_m && n < rows_n) vx_store4(slab + (long long)(m0 + m) * width + n0 + n, v, rows_n - n);
+    vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
+      if (m < rows_m && n < rows_n) vx_store8(slab + (long long)(m0 + m) * width + n0 + n, v, w, rows_n - n);
     });
   } else {
     unsigned w = vx_xcd_tile(blockIdx.x - a.n_v - a.n_k, a.n_q);
@@ -580,9 +588,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
     const VxOperand<T> X{a.ds + ((long long)bh * a.rows + m0) * a.skp, a.skp, rows_m, nullptr};
     const VxOperand<T> W{a.k + b * a.k_b + (h / a.gk) * a.k_h + n0, a.k_s, rows_n, a.mask ? a.mask + b * a.mask_b : nullptr};
     vx_gemm_loop<T, KC, KS, TM, TN, FAST>(X, W, 0, a.sk, lds, acc);   // the pad of dS is 0
-    vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
+    vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
       if (m < rows_m && n < rows_n)
-        vx_store4(a.dq + (((long long)b * a.sq + a.q0 + m0 + m) * a.h + h) * a.d + n0 + n, v, rows_n - n);
+        vx_store8(a.dq + (((long long)b * a.sq + a.q0 + m0 + m) * a.h + h) * a.d + n0 + n, v, w, rows_n - n);
     });
   }
 }

@@ -12,7 +12,7 @@ namespace {
 constexpr int kActNone = VX_ACT_NONE, kActRelu = VX_ACT_RELU, kActGelu = VX_ACT_GELU, kActSilu = VX_ACT_SILU;
 
 __device__ __forceinline__ float act_value(float a, int act) {
-  if (act == kActRelu) return a > 0.0f ? a : (a != a ? a : 0.0f);      // NaN stays NaN
+  if (act == kActRelu) return a < 0.0f ? 0.0f : a;      // NaN stays NaN
   if (act == kActGelu) return 0.5f * a * (1.0f + erff(a * 0.70710678118654752f));
   if (act == kActSilu) return a / (1.0f + expf(-a));
   return a;
@@ -62,8 +62,43 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a
   vx_acc_zero(acc);
   const VxOperand<T> X{a.x + m0 * a.ldx, a.ldx, rows_m, nullptr}, W{a.w + (long long)n0 * a.ldw, a.ldw, rows_n, nullptr};
   vx_gemm_loop<T, KC, KC, TM, TN, FAST>(X, W, 0, a.k, lds, acc);
-  vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
-    if (m < rows_m && n < rows_n) linear_finish(a, m0 + m, n0 + n, rows_n - n, v);
+  vx_f32x4 bias[TN / 64][2];                   // of this lane's columns
+  if (a.bias) {
+    vx_acc_each<TM, TN>(acc, [&](int mi, int, int j, int n, const vx_f32x4&, const vx_f32x4&) {
+      if (mi) return;
+      bias[j][0] = vx_load4(a.bias + n0 + n, rows_n - n);
+      bias[j][1] = vx_load4(a.bias + n0 + n + 4, rows_n - n - 4);
+    });
+  }
+  const long long at0 = m0 * a.n + n0;
+  vx_acc_each<TM, TN>(acc, [&](int, int m, int j, int n, vx_f32x4 v, vx_f32x4 w) {
+    const int left = rows_n - n;
+    if (m >= rows_m || left <= 0) return;
+    if (a.bias) {
+      v += bias[j][0];
+      w += bias[j][1];
+    }
+    if (a.res) {
+      const T* r = a.res + (m0 + m) * a.ldr + n0 + n;
+      v += vx_load4(r, left);
+      w += vx_load4(r + 4, left - 4);
+    }
+    const long long at = at0 + (long long)m * a.n + n;
+    if (a.pre) vx_store8(a.pre + at, v, w, left);
+    if (a.act == kActRelu) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = act_value(v[i], kActRelu);
+        w[i] = act_value(w[i], kActRelu);
+      }
+    } else if (a.act != kActNone) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = act_value(v[i], a.act);
+        w[i] = act_value(w[i], a.act);
+      }
+    }
+    vx_store8(a.y + at, v, w, left);
   });
 }
 
@@ -171,11 +206,11 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a
     const VxOperand<T> X{a.g + r0 * a.ldg + n0, a.ldg, rows_n, nullptr}, W{a.x + r0 * a.ldx + k0, a.ldx, rows_k, nullptr};
     vx_gemm_loop<T, KS, KS, TM, TN, FAST>(X, W, 0, rows, lds, acc);
     float* slab = a.slab ? a.slab + (long long)split * a.n * a.k : nullptr;
-    vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
+    vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
       const int left = rows_k - n;
       if (m >= rows_n || left <= 0) return;
       const long long at = (long long)(n0 + m) * a.k + k0 + n;
-      if (slab) vx_store4(slab + at, v, left); else vx_store4(a.dw + at, v, left);
+      if (slab) vx_store8(slab + at, v, w, left); else vx_store8(a.dw + at, v, w, left);
     });
   } else {
     const unsigned t = vx_xcd_tile(blockIdx.x - a.blocks_w, a.blocks_x);
@@ -184,9 +219,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a
     const int rows_m = (int)(a.m - m0 < TM ? a.m - m0 : TM), rows_k = a.k - k0 < TN ? a.k - k0 : TN;
     const VxOperand<T> X{a.g + m0 * a.ldg, a.ldg, rows_m, nullptr}, W{a.w + k0, a.ldw, rows_k, nullptr};
     vx_gemm_loop<T, KC, KS, TM, TN, FAST>(X, W, 0, a.n, lds, acc);
-    vx_acc_each<TM, TN>(acc, [&](int m, int n, vx_f32x4 v) {
-      const int left = rows_k - n;
-      if (m < rows_m && left > 0) vx_store4(a.dx + (m0 + m) * a.k + k0 + n, v, left);
+    const long long at0 = m0 * a.k + k0;
+    vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
+      if (m < rows_m && n < rows_k) vx_store8(a.dx + at0 + (long long)m * a.k + n, v, w, rows_k - n);
     });
   }
 }

@@ -2,8 +2,9 @@
 // v_mfma_f32_16x16x32_bf16 reads its fragments, for fp32 (exact three-plane bf16 split, six products) and bf16.
 //
 // A product is C[m][n] = sum_k X[m][k] * W[n][k]. The matrix instruction takes W as its row operand and X as its column
-// operand, so that lane (c = lane & 15, g = lane >> 4) holds C[m0 + c][n0 + 4 g + 0..3]: four neighbours of one output row,
-// one 16- or 8-byte store.
+// operand, so that lane (c = lane & 15, g = lane >> 4) holds four neighbours of row m0 + c. The GEMMs deal the rows of W to
+// the blocks of a 32-row group four at a time (vx_row_w), so that a lane's two accumulators of a group are eight neighbours
+// C[m0 + c][n0 + 8 g + 0..7], and the four lanes of a row store 64 (bf16) or 128 (fp32) bytes in one piece.
 //
 // LDS image of an operand tile: fragments of 16 rows x 32 k, 1 KB each and one per plane, in lane order -- lane (c, g) of a
 // fragment read takes the 16 bytes {k = 8 g .. 8 g + 7} of row c with one ds_read_b128, 64 lanes over 1 KB: no bank
@@ -274,8 +275,11 @@ static inline bool vx_fast(const void* p, int64_t ld, int64_t width, int64_t esi
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * esize % 16 == 0 && width % 8 == 0 && ld >= width && ld < (1 << 21);
 }
 
+// row n of a W tile -> its row in the image (block * 16 + row of the block)
+__device__ __forceinline__ int vx_row_w(int n) { return (n & ~31) + (n & 4) * 4 + (n >> 1 & 12) + (n & 3); }
+
 // stages R rows x BK k's with 256 threads: registers first (load), then the LDS image (store)
-template <typename T, int MODE, int R, bool FAST>
+template <typename T, int MODE, int R, bool FAST, bool IS_W>
 struct VxStage {
   static constexpr int BK = VxType<T>::BK, NPL = VxType<T>::NPL, NK = BK / 32, E = sizeof(T);
   static constexpr int PLANE = (R / 16) * vx_image_block<NK>();
@@ -299,6 +303,12 @@ struct VxStage {
       kc = l >> 4;
     }
   }
+  // KS: k group of a thread. Where a wave's halves have a group each, the two are two apart: LDS serves lanes of both halves
+  // together, and the XOR then keeps their pieces apart
+  static __device__ __forceinline__ int group(int tid) {
+    const int i = tid / (R / W);
+    return R / W == 32 ? (i & 1) * 2 + (i >> 1 & 1) + (i & 4) : i;
+  }
   __device__ __forceinline__ void load(const VxOperand<T>& o, int k0, int kend, int tid) {
     if constexpr (MODE == KC) {
 #pragma unroll
@@ -311,7 +321,7 @@ struct VxStage {
           a[i].load(o.p + row * o.ld + k0 + kc * 8, row < o.rows ? kend - k0 - kc * 8 : 0);
       }
     } else {
-      const int r = tid % (R / W) * W, kg = tid / (R / W) * 8;
+      const int r = tid % (R / W) * W, kg = group(tid) * 8;
       if (o.kmask != nullptr) {
         dead = 0;
 #pragma unroll
@@ -339,10 +349,11 @@ struct VxStage {
         int row, kc;
         item(i, tid, row, kc);
         a[i].planes(f);
+        if constexpr (IS_W) row = vx_row_w(row);
         vx_frag_store(img + vx_image_at<NK>(row >> 4, kc >> 2, (row & 15) + 16 * (kc & 3)), PLANE, f);
       }
     } else {
-      const int r = tid % (R / W) * W, kg = tid / (R / W);
+      const int r = tid % (R / W) * W, kg = group(tid);
       if (o.kmask != nullptr) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -351,7 +362,8 @@ struct VxStage {
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         b.planes(j, f);
-        vx_frag_store(img + vx_image_at<NK>((r + j) >> 4, kg >> 2, ((r + j) & 15) + 16 * (kg & 3)), PLANE, f);
+        const int row = IS_W ? vx_row_w(r + j) : r + j;
+        vx_frag_store(img + vx_image_at<NK>(row >> 4, kg >> 2, (row & 15) + 16 * (kg & 3)), PLANE, f);
       }
     }
   }
@@ -371,8 +383,8 @@ template <typename T, int XM, int WM, int TM, int TN, bool FAST>
 __device__ __forceinline__ void vx_gemm_loop(const VxOperand<T>& X, const VxOperand<T>& W, int k0, int kend, char* lds,
                                              vx_f32x4 (&acc)[TM / 32][TN / 32]) {
   constexpr int BK = VxType<T>::BK, NPL = VxType<T>::NPL, NK = BK / 32;
-  using SX = VxStage<T, XM, TM, FAST>;
-  using SW = VxStage<T, WM, TN, FAST>;
+  using SX = VxStage<T, XM, TM, FAST, false>;
+  using SW = VxStage<T, WM, TN, FAST, true>;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   char *ix = lds, *iw = lds + SX::BYTES;
   SX sx;
@@ -418,15 +430,16 @@ __device__ __forceinline__ void vx_acc_zero(vx_f32x4 (&acc)[A][B]) {
     for (int j = 0; j < B; ++j) acc[i][j] = vx_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
-// f(m, n, value4) for every accumulator of this lane: m, n relative to the tile, n a multiple of 4
+// f(mi, m, j, n, first, second) for every pair of accumulators of this lane: the values n .. n + 7 of row m, relative to the tile;
+// mi and j are their compile-time numbers
 template <int TM, int TN, typename F>
 __device__ __forceinline__ void vx_acc_each(const vx_f32x4 (&acc)[TM / 32][TN / 32], F&& f) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
 #pragma unroll
   for (int mi = 0; mi < TM / 32; ++mi)
 #pragma unroll
-    for (int ni = 0; ni < TN / 32; ++ni)
-      f(wm * (TM / 2) + mi * 16 + (lane & 15), wn * (TN / 2) + ni * 16 + (lane >> 4) * 4, acc[mi][ni]);
+    for (int j = 0; j < TN / 64; ++j)
+      f(mi, wm * (TM / 2) + mi * 16 + (lane & 15), j, wn * (TN / 2) + j * 32 + (lane >> 4) * 8, acc[mi][2 * j], acc[mi][2 * j + 1]);
 }
 
 // ---- up to four neighbours of a row -------------------------------------------------------------------------------
@@ -470,6 +483,26 @@ __device__ __forceinline__ void vx_store4(__bf16* p, const vx_f32x4& v, int n) {
 #pragma unroll
   for (int i = 0; i < 3; ++i)
     if (i < n) p[i] = (__bf16)v[i];
+}
+
+// eight neighbours, `n` of which exist
+__device__ __forceinline__ void vx_store8(float* p, const vx_f32x4& a, const vx_f32x4& b, int n) {
+  vx_store4(p, a, n);
+  vx_store4(p + 4, b, n - 4);
+}
+__device__ __forceinline__ void vx_store8(__bf16* p, const vx_f32x4& a, const vx_f32x4& b, int n) {
+  if (n >= 8) {
+    bf16x8 h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[i] = (__bf16)a[i];
+      h[4 + i] = (__bf16)b[i];
+    }
+    *reinterpret_cast<vx_u32x4u*>(p) = __builtin_bit_cast(vx_u32x4u, h);
+    return;
+  }
+  vx_store4(p, a, n);
+  vx_store4(p + 4, b, n - 4);
 }
 
 // compute units of the current device (cached per device; 256 if it cannot be asked)
