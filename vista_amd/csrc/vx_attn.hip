@@ -473,7 +473,7 @@ struct BwdArgs : AttnArgs<T> {
   float scale;
   int q0, rows, skp;                         // present chunk: queries [q0, q0 + rows); skp: sk rounded up to 8
   int bh, split0, span;                      // first split of the chunk, queries of one split
-  int tq, td, tkd, tkv, tk;                  // tiles of attn_grads
+  int tq, tkp, tk, td, tdv;                  // tiles: queries; keys of attn_pds, of attn_grads; columns of dK and dQ, of dV
   unsigned n_v, n_k, n_q;                    // workgroups per problem
 };
 
@@ -496,14 +496,15 @@ __global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long 
   if (lane == 0) a.delta[r] = s;
 }
 
+constexpr int kPdsN = 128;                   // keys of an attn_pds tile
 // P and dS of a TM-query x TN-key tile: scores and dP = go v^T are two products with one epilogue,
 // P = 2^(scale2 s - max) / sum, dS = scale P (dP - delta).
 template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) {
   __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
   unsigned w = vx_xcd_tile(blockIdx.x, gridDim.x);
-  const int n0 = (int)(w % a.tk) * TN;
-  w /= a.tk;
+  const int n0 = (int)(w % a.tkp) * TN;
+  w /= a.tkp;
   const int m0 = (int)(w % a.tq) * TM;
   const int bh = (int)(w / a.tq), b = bh / a.h, h = bh % a.h;
   const int rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = a.sk - n0 < TN ? a.sk - n0 : TN;
@@ -560,7 +561,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
   vx_acc_zero(acc);
   if (blockIdx.x < a.n_v + a.n_k) {
     const bool is_v = blockIdx.x < a.n_v;
-    const int tn = is_v ? a.tkv : a.tkd, width = is_v ? a.dv : a.d;
+    const int tn = is_v ? a.tdv : a.td, width = is_v ? a.dv : a.d;
     unsigned w = is_v ? vx_xcd_tile(blockIdx.x, a.n_v) : vx_xcd_tile(blockIdx.x - a.n_v, a.n_k);
     const int n0 = (int)(w % tn) * TN;
     w /= tn;
@@ -771,25 +772,28 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
 }
 
 struct BwdPlan {
-  int64_t tm, skp, span, per_chunk, splits, chunk;      // queries per split, splits per chunk, all splits, queries per chunk
+  int64_t tm, tn, skp, span, per_chunk, splits, chunk;  // queries per split, splits per chunk, all splits, queries per chunk
   size_t delta, pds, slab_k, slab_v;                    // bytes
   size_t total() const { return delta + 2 * pds + slab_k + slab_v; }
 };
 // queries are cut into splits (one slab each) and the splits into chunks, whose probabilities and score gradients are in
 // memory at a time (at most kChunkBytes of both)
-constexpr size_t kChunkBytes = (size_t)256 << 20;
+constexpr size_t kChunkBytes = (size_t)1 << 30;
 BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   BwdPlan p;
   const int64_t cus = vx_tile_cus(), bh = s.b * s.h, e = dtype == VX_F32 ? 4 : 2, bk = dtype == VX_F32 ? 32 : 64;
   p.skp = vx_cdiv(s.sk, 8) * 8;
   p.tm = vx_cdiv(s.sq, 128) * vx_cdiv(s.sk, 128) * bh >= 2 * cus ? 128 : 64;
-  const int64_t tiles = vx_cdiv(s.sk, p.tm) * (vx_cdiv(s.dv, p.tm) + vx_cdiv(s.d, p.tm)) * bh;
-  int64_t splits = vx_cdiv(2 * cus, tiles > 0 ? tiles : 1);
+  p.tn = s.d > 128 ? 192 : p.tm;           // wide heads: 192 and 384 columns without a ragged tile, and less staging per product
+  const int64_t tiles = vx_cdiv(s.sk, p.tm) * (vx_cdiv(s.dv, p.tn) + vx_cdiv(s.d, p.tn)) * bh;
+  int64_t splits = 2 * cus / (tiles > 0 ? tiles : 1);
+  if (splits < vx_cdiv(s.sq, 2 * s.sk)) splits = vx_cdiv(s.sq, 2 * s.sk);       // no workgroup much longer than those of dQ
   const int64_t most = vx_cdiv(s.sq, 4 * bk);
   if (splits > most) splits = most;
   int64_t fit = (int64_t)(kChunkBytes / 2) / (bh * p.skp * e);       // queries of a chunk
   if (fit < p.tm) fit = p.tm;
   if (splits < vx_cdiv(s.sq, fit)) splits = vx_cdiv(s.sq, fit);
+  if (splits < 1) splits = 1;
   p.span = vx_cdiv(vx_cdiv(s.sq, splits), p.tm) * p.tm;
   p.splits = vx_cdiv(s.sq, p.span);
   p.per_chunk = fit / p.span < 1 ? 1 : fit / p.span;
@@ -802,13 +806,18 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   return p;
 }
 
-template <typename T, int TM, bool FAST>
+template <typename T, int TM, int TN, bool FAST>
 int32_t bwd_chunk(const BwdArgs<T>& a, int64_t pds, int64_t grads, hipStream_t s) {
-  attn_pds<T, TM, TM, FAST><<<(unsigned)pds, kTileThreads, 0, s>>>(a);
+  attn_pds<T, TM, kPdsN, FAST><<<(unsigned)pds, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
-  attn_grads<T, TM, TM, FAST><<<(unsigned)grads, kTileThreads, 0, s>>>(a);
+  attn_grads<T, TM, TN, FAST><<<(unsigned)grads, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
   return VX_OK;
+}
+template <typename T, bool FAST>
+int32_t bwd_chunk(const BwdArgs<T>& a, const BwdPlan& p, int64_t pds, int64_t grads, hipStream_t s) {
+  if (p.tm == 128) return p.tn == 192 ? bwd_chunk<T, 128, 192, FAST>(a, pds, grads, s) : bwd_chunk<T, 128, 128, FAST>(a, pds, grads, s);
+  return p.tn == 192 ? bwd_chunk<T, 64, 192, FAST>(a, pds, grads, s) : bwd_chunk<T, 64, 64, FAST>(a, pds, grads, s);
 }
 
 template <typename T>
@@ -823,9 +832,10 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   a.skp = (int)p.skp;
   a.bh = (int)bh;
   a.span = (int)p.span;
-  a.tk = (int)vx_cdiv(p.skp, p.tm);
-  a.td = a.tkd = (int)vx_cdiv(sh.d, p.tm);
-  a.tkv = (int)vx_cdiv(sh.dv, p.tm);
+  a.tkp = (int)vx_cdiv(p.skp, kPdsN);
+  a.tk = (int)vx_cdiv(sh.sk, p.tm);
+  a.td = (int)vx_cdiv(sh.d, p.tn);
+  a.tdv = (int)vx_cdiv(sh.dv, p.tn);
   VX_REQUIRE(vx_cdiv(rows, 4) < (1LL << 31), "attn_bwd: too many queries");
   attn_delta<T><<<(unsigned)vx_cdiv(rows, 4), 256, 0, s>>>(a, rows);
   VX_LAUNCH_CHECK();
@@ -835,16 +845,14 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
     a.rows = (int)(sh.sq - q0 < p.chunk ? sh.sq - q0 : p.chunk);
     a.split0 = (int)split;
     a.tq = (int)vx_cdiv(a.rows, p.tm);
-    const int64_t here = vx_cdiv(a.rows, p.span), tkeys = vx_cdiv(sh.sk, p.tm);
-    a.tk = (int)vx_cdiv(p.skp, p.tm);
-    const int64_t pds = (int64_t)a.tk * a.tq * bh;
-    const int64_t nv = here * bh * tkeys * a.tkv, nk = here * bh * tkeys * a.tkd, nq = (int64_t)a.tq * a.td * bh;
+    const int64_t here = vx_cdiv(a.rows, p.span);
+    const int64_t pds = (int64_t)a.tkp * a.tq * bh;
+    const int64_t nv = here * bh * a.tk * a.tdv, nk = here * bh * a.tk * a.td, nq = (int64_t)a.tq * a.td * bh;
     VX_REQUIRE(pds < (1LL << 31) && nv + nk + nq < (1LL << 31), "attn_bwd: too many tiles");
     a.n_v = (unsigned)nv;
     a.n_k = (unsigned)nk;
     a.n_q = (unsigned)nq;
-    const int32_t rc = p.tm == 128 ? (fast ? bwd_chunk<T, 128, true>(a, pds, nv + nk + nq, s) : bwd_chunk<T, 128, false>(a, pds, nv + nk + nq, s))
-                                   : (fast ? bwd_chunk<T, 64, true>(a, pds, nv + nk + nq, s) : bwd_chunk<T, 64, false>(a, pds, nv + nk + nq, s));
+    const int32_t rc = fast ? bwd_chunk<T, true>(a, p, pds, nv + nk + nq, s) : bwd_chunk<T, false>(a, p, pds, nv + nk + nq, s);
     if (rc) return rc;
   }
   const int64_t iv = sh.b * sh.hv * sh.sk * vx_cdiv(sh.dv, 4), ik = sh.b * sh.hk * sh.sk * vx_cdiv(sh.d, 4);

@@ -22,6 +22,7 @@ typedef unsigned vx_u32x2u __attribute__((ext_vector_type(2), aligned(2)));
 typedef unsigned vx_u32x1u __attribute__((aligned(2)));
 typedef unsigned vx_u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned vx_u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned vx_u32x3 __attribute__((ext_vector_type(3)));
 
 constexpr int kTileThreads = 256;
 constexpr int kFragBytes = 1024;
@@ -156,7 +157,8 @@ struct VxCol8<float, W> {
         v[k][0] = a[0];
         v[k][1] = a[1];
       } else {
-        v[k][0] = p[0];
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[k][j] = p[j];
       }
     } else {
 #pragma unroll
@@ -168,6 +170,10 @@ struct VxCol8<float, W> {
       const vx_u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(b, at, uniform, 0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[k][j] = __uint_as_float(a[j]);
+    } else if constexpr (W == 3) {
+      const vx_u32x3 a = __builtin_amdgcn_raw_buffer_load_b96(b, at, uniform, 0);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) v[k][j] = __uint_as_float(a[j]);
     } else if constexpr (W == 2) {
       const vx_u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(b, at, uniform, 0);
       v[k][0] = __uint_as_float(a[0]);
@@ -187,7 +193,7 @@ struct VxCol8<float, W> {
 };
 template <int W>
 struct VxCol8<__bf16, W> {
-  static_assert(W == 2 || W == 4, "pairs of 16-bit rows");
+  static_assert(W == 2 || W == 4 || W == 6, "pairs of 16-bit rows");
   unsigned v[8][W / 2];
   __device__ __forceinline__ void load(int k, const __bf16* p, int n) {
     if (n >= W) {
@@ -196,7 +202,8 @@ struct VxCol8<__bf16, W> {
         v[k][0] = a[0];
         v[k][1] = a[1];
       } else {
-        v[k][0] = *reinterpret_cast<const vx_u32x1u*>(p);
+#pragma unroll
+        for (int j = 0; j < W / 2; ++j) v[k][j] = reinterpret_cast<const vx_u32x1u*>(p)[j];
       }
     } else {
       const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
@@ -212,6 +219,10 @@ struct VxCol8<__bf16, W> {
       const vx_u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(b, at, uniform, 0);
       v[k][0] = a[0];
       v[k][1] = a[1];
+    } else if constexpr (W == 6) {
+      const vx_u32x3 a = __builtin_amdgcn_raw_buffer_load_b96(b, at, uniform, 0);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) v[k][j] = a[j];
     } else {
       v[k][0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, uniform, 0);
     }
