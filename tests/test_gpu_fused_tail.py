@@ -264,10 +264,11 @@ def test_attention_many_queries(shape, dtype, dev):
         within(got, *ref[name], name)
 
 
-def test_attention_gradients_in_chunks_of_queries(dev):
-    """Probabilities of 2 x 20000 x 2000 pairs do not fit the workspace at once: several chunks, one slab each and more."""
+@pytest.mark.parametrize("k_len", [2000, 5001])
+def test_attention_gradients_in_chunks_of_queries(k_len, dev):
+    """Many queries: one chunk of several splits (2000 keys), and more probabilities than the workspace holds at once (5001)."""
     from vista_amd import ops
-    q, k, v, km, do = make_attn((1, 20000, 2000, 2, 2, 1, 16, 24), F32, dev, 6, "some", poison=True)
+    q, k, v, km, do = make_attn((1, 20000, k_len, 2, 2, 1, 16, 24), F32, dev, 6, "some", poison=True)
     ref = attn_reference(q, k, v, km, do)
     out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
     within(out, *ref["out"], "out")

@@ -473,7 +473,8 @@ struct BwdArgs : AttnArgs<T> {
   float scale;
   int q0, rows, skp;                         // present chunk: queries [q0, q0 + rows); skp: sk rounded up to 8
   int bh, split0, span;                      // first split of the chunk, queries of one split
-  int tq, tkp, tk, td, tdv;                  // tiles: queries; keys of attn_pds, of attn_grads; columns of dK and dQ, of dV
+  int tqp, tkp;                              // tiles of attn_pds: queries, keys
+  int tq, tk, td, tdv;                       // tiles of attn_grads: queries, keys, columns of dK and dQ, columns of dV
   unsigned n_v, n_k, n_q;                    // workgroups per problem
 };
 
@@ -501,20 +502,21 @@ constexpr int kPdsN = 128;                   // keys of an attn_pds tile
 // P = 2^(scale2 s - max) / sum, dS = scale P (dP - delta).
 template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) {
-  __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
+  constexpr int BK = TM <= 64 ? 64 : VxType<T>::BK;
+  __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN, BK>()];
   unsigned w = vx_xcd_tile(blockIdx.x, gridDim.x);
   const int n0 = (int)(w % a.tkp) * TN;
   w /= a.tkp;
-  const int m0 = (int)(w % a.tq) * TM;
-  const int bh = (int)(w / a.tq), b = bh / a.h, h = bh % a.h;
+  const int m0 = (int)(w % a.tqp) * TM;
+  const int bh = (int)(w / a.tqp), b = bh / a.h, h = bh % a.h;
   const int rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = a.sk - n0 < TN ? a.sk - n0 : TN;
   const long long q = a.q0 + m0;
   vx_f32x4 s[TM / 32][TN / 32], dp[TM / 32][TN / 32];
   vx_acc_zero(s);
   vx_acc_zero(dp);
-  vx_gemm_loop<T, KC, KC, TM, TN, FAST>({a.q + b * a.q_b + q * a.q_s + h * a.q_h, a.q_s, rows_m, nullptr},
+  vx_gemm_loop<T, KC, KC, TM, TN, FAST, BK>({a.q + b * a.q_b + q * a.q_s + h * a.q_h, a.q_s, rows_m, nullptr},
                                   {a.k + b * a.k_b + (h / a.gk) * a.k_h + n0 * a.k_s, a.k_s, rows_n, nullptr}, 0, a.d, lds, s);
-  vx_gemm_loop<T, KC, KC, TM, TN, FAST>({a.go + b * a.go_b + q * a.go_s + h * a.go_h, a.go_s, rows_m, nullptr},
+  vx_gemm_loop<T, KC, KC, TM, TN, FAST, BK>({a.go + b * a.go_b + q * a.go_s + h * a.go_h, a.go_s, rows_m, nullptr},
                                   {a.v + b * a.v_b + (h / a.gv) * a.v_h + n0 * a.v_s, a.v_s, rows_n, nullptr}, 0, a.dv, lds, dp);
   const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
   unsigned live[TN / 64];                      // of this lane's eight keys
@@ -772,7 +774,7 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
 }
 
 struct BwdPlan {
-  int64_t tm, tn, skp, span, per_chunk, splits, chunk;  // queries per split, splits per chunk, all splits, queries per chunk
+  int64_t tp, tm, tn, skp, span, per_chunk, splits, chunk;  // queries per split, splits per chunk, all splits, queries per chunk
   size_t delta, pds, slab_k, slab_v;                    // bytes
   size_t total() const { return delta + 2 * pds + slab_k + slab_v; }
 };
@@ -783,7 +785,11 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   BwdPlan p;
   const int64_t cus = vx_tile_cus(), bh = s.b * s.h, e = dtype == VX_F32 ? 4 : 2, bk = dtype == VX_F32 ? 32 : 64;
   p.skp = vx_cdiv(s.sk, 8) * 8;
-  p.tm = vx_cdiv(s.sq, 128) * vx_cdiv(s.sk, 128) * bh >= 2 * cus ? 128 : 64;
+  // query rows of a tile; 4 x 2 heads, 1600 x 480, 192 / 384 wide, fp32 (416 tiles of 128): attn_pds 71 us with 64, 62 with 128,
+  // attn_grads 82 and 84
+  const int64_t t128 = vx_cdiv(s.sq, 128) * vx_cdiv(s.sk, 128) * bh;
+  p.tp = 2 * t128 >= 3 * cus ? 128 : 64;
+  p.tm = t128 >= 2 * cus ? 128 : 64;
   p.tn = s.d > 128 ? 192 : p.tm;           // wide heads: 192 and 384 columns without a ragged tile, and less staging per product
   const int64_t tiles = vx_cdiv(s.sk, p.tm) * (vx_cdiv(s.dv, p.tn) + vx_cdiv(s.d, p.tn)) * bh;
   int64_t splits = 2 * cus / (tiles > 0 ? tiles : 1);
@@ -806,18 +812,16 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   return p;
 }
 
-template <typename T, int TM, int TN, bool FAST>
-int32_t bwd_chunk(const BwdArgs<T>& a, int64_t pds, int64_t grads, hipStream_t s) {
-  attn_pds<T, TM, kPdsN, FAST><<<(unsigned)pds, kTileThreads, 0, s>>>(a);
+template <typename T, bool FAST>
+int32_t bwd_chunk(const BwdArgs<T>& a, const BwdPlan& p, unsigned pds, unsigned grads, hipStream_t s) {
+  const auto probs = p.tp == 128 ? attn_pds<T, 128, kPdsN, FAST> : attn_pds<T, 64, kPdsN, FAST>;
+  probs<<<pds, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
-  attn_grads<T, TM, TN, FAST><<<(unsigned)grads, kTileThreads, 0, s>>>(a);
+  const auto sums = p.tm == 128 ? (p.tn == 192 ? attn_grads<T, 128, 192, FAST> : attn_grads<T, 128, 128, FAST>)
+                                : (p.tn == 192 ? attn_grads<T, 64, 192, FAST> : attn_grads<T, 64, 64, FAST>);
+  sums<<<grads, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
   return VX_OK;
-}
-template <typename T, bool FAST>
-int32_t bwd_chunk(const BwdArgs<T>& a, const BwdPlan& p, int64_t pds, int64_t grads, hipStream_t s) {
-  if (p.tm == 128) return p.tn == 192 ? bwd_chunk<T, 128, 192, FAST>(a, pds, grads, s) : bwd_chunk<T, 128, 128, FAST>(a, pds, grads, s);
-  return p.tn == 192 ? bwd_chunk<T, 64, 192, FAST>(a, pds, grads, s) : bwd_chunk<T, 64, 64, FAST>(a, pds, grads, s);
 }
 
 template <typename T>
@@ -846,13 +850,15 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
     a.split0 = (int)split;
     a.tq = (int)vx_cdiv(a.rows, p.tm);
     const int64_t here = vx_cdiv(a.rows, p.span);
-    const int64_t pds = (int64_t)a.tkp * a.tq * bh;
     const int64_t nv = here * bh * a.tk * a.tdv, nk = here * bh * a.tk * a.td, nq = (int64_t)a.tq * a.td * bh;
-    VX_REQUIRE(pds < (1LL << 31) && nv + nk + nq < (1LL << 31), "attn_bwd: too many tiles");
+    const int64_t pds = (int64_t)a.tkp * vx_cdiv(a.rows, p.tp) * bh, grads = nv + nk + nq;
+    VX_REQUIRE(pds < (1LL << 31) && grads < (1LL << 31), "attn_bwd: too many tiles");
     a.n_v = (unsigned)nv;
     a.n_k = (unsigned)nk;
     a.n_q = (unsigned)nq;
-    const int32_t rc = fast ? bwd_chunk<T, true>(a, p, pds, nv + nk + nq, s) : bwd_chunk<T, false>(a, p, pds, nv + nk + nq, s);
+    a.tqp = (int)vx_cdiv(a.rows, p.tp);
+    const int32_t rc = fast ? bwd_chunk<T, true>(a, p, (unsigned)pds, (unsigned)grads, s)
+                            : bwd_chunk<T, false>(a, p, (unsigned)pds, (unsigned)grads, s);
     if (rc) return rc;
   }
   const int64_t iv = sh.b * sh.hv * sh.sk * vx_cdiv(sh.dv, 4), ik = sh.b * sh.hk * sh.sk * vx_cdiv(sh.d, 4);

@@ -38,7 +38,7 @@ struct VxType;
 template <>
 struct VxType<float> {
   static constexpr int NPL = 3;   // bf16 planes per value
-  static constexpr int BK = 32;   // reduction values per staged step of a GEMM
+  static constexpr int BK = 32;   // reduction values per staged step of a GEMM (64: small tiles of k-contiguous operands)
 };
 template <>
 struct VxType<__bf16> {
@@ -286,13 +286,13 @@ static inline bool vx_fast(const void* p, int64_t ld, int64_t width, int64_t esi
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * esize % 16 == 0 && width % 8 == 0 && ld >= width && ld < (1 << 21);
 }
 
-// row n of a W tile -> its row in the image (block * 16 + row of the block)
+// row n of a W tile -> its row in the image (block * 16 + row of the block), and back
 __device__ __forceinline__ int vx_row_w(int n) { return (n & ~31) + (n & 4) * 4 + (n >> 1 & 12) + (n & 3); }
-
+__device__ __forceinline__ int vx_row_n(int r) { return (r & ~31) + (r & 12) * 2 + (r >> 2 & 4) + (r & 3); }
 // stages R rows x BK k's with 256 threads: registers first (load), then the LDS image (store)
-template <typename T, int MODE, int R, bool FAST, bool IS_W>
+template <typename T, int MODE, int R, int BK, bool FAST, bool IS_W>
 struct VxStage {
-  static constexpr int BK = VxType<T>::BK, NPL = VxType<T>::NPL, NK = BK / 32, E = sizeof(T);
+  static constexpr int NPL = VxType<T>::NPL, NK = BK / 32, E = sizeof(T);
   static constexpr int PLANE = (R / 16) * vx_image_block<NK>();
   static constexpr int BYTES = PLANE * NPL;
   static constexpr int NI = R * BK / 8 / kTileThreads;            // KC: 8-value items per thread; KS: rows per thread
@@ -302,7 +302,7 @@ struct VxStage {
   VxCol8<T, MODE == KS ? W : 2> b;
   unsigned dead;                                                   // KS with a mask: bit i = k i of the eight reads as 0
 
-  // KC item i of a thread: row (of the tile) and k group. bf16: eight lanes read a row's 128 bytes; fp32: a lane's eight
+  // KC item i of a thread: row (of the image) and k group. bf16: eight lanes read a row's 128 bytes; fp32: a lane's eight
   // values are two loads, four lanes a row
   static __device__ __forceinline__ void item(int i, int tid, int& row, int& kc) {
     const int wave = tid >> 6, l = tid & 63, blk = i * (kTileThreads / 64) + wave;
@@ -326,6 +326,7 @@ struct VxStage {
       for (int i = 0; i < NI; ++i) {
         int row, kc;
         item(i, tid, row, kc);
+        if constexpr (IS_W) row = vx_row_n(row);
         if constexpr (FAST)
           a[i].load(vx_buffer(o.p + k0), row < o.rows && kc * 8 < kend - k0 ? row * (int)o.ld * E + kc * 8 * E : kVxOut);
         else
@@ -360,7 +361,6 @@ struct VxStage {
         int row, kc;
         item(i, tid, row, kc);
         a[i].planes(f);
-        if constexpr (IS_W) row = vx_row_w(row);
         vx_frag_store(img + vx_image_at<NK>(row >> 4, kc >> 2, (row & 15) + 16 * (kc & 3)), PLANE, f);
       }
     } else {
@@ -381,21 +381,22 @@ struct VxStage {
 };
 
 // LDS bytes of vx_gemm_loop
-template <typename T, int TM, int TN>
+template <typename T, int TM, int TN, int BK = VxType<T>::BK>
 constexpr int vx_gemm_lds() {
-  return (TM + TN) / 16 * vx_image_block<VxType<T>::BK / 32>() * VxType<T>::NPL;
+  return (TM + TN) / 16 * vx_image_block<BK / 32>() * VxType<T>::NPL;
 }
 
 // acc[mi][ni] += the TM x TN tile's product over k in [k0, kend); wave (wm, wn) of 2 x 2 owns TM/2 x TN/2. One LDS image,
 // two barriers per step: the next step's operands travel to registers while this one's are multiplied, and the two or
-// three workgroups of a CU cover each other's barriers (two images, or two and three steps in flight, were no faster at any
-// size: the steps are bound by the splitting and the LDS, not by latency). Ends with a barrier: the caller may reuse the LDS.
-template <typename T, int XM, int WM, int TM, int TN, bool FAST>
+// three workgroups of a CU cover each other's barriers and splitting. Measured against it: two images with one barrier a step and
+// the split of the next step among this one's products 4096^3 fp32 694 -> 869 us, 204800 x 384 -> 512 bf16 134 -> 170 us (one
+// workgroup less a CU); two and three steps in flight: no difference. Ends with a barrier: the caller may reuse the LDS.
+template <typename T, int XM, int WM, int TM, int TN, bool FAST, int BK = VxType<T>::BK>
 __device__ __forceinline__ void vx_gemm_loop(const VxOperand<T>& X, const VxOperand<T>& W, int k0, int kend, char* lds,
                                              vx_f32x4 (&acc)[TM / 32][TN / 32]) {
-  constexpr int BK = VxType<T>::BK, NPL = VxType<T>::NPL, NK = BK / 32;
-  using SX = VxStage<T, XM, TM, FAST, false>;
-  using SW = VxStage<T, WM, TN, FAST, true>;
+  constexpr int NPL = VxType<T>::NPL, NK = BK / 32;
+  using SX = VxStage<T, XM, TM, BK, FAST, false>;
+  using SW = VxStage<T, WM, TN, BK, FAST, true>;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   char *ix = lds, *iw = lds + SX::BYTES;
   SX sx;
@@ -419,14 +420,18 @@ __device__ __forceinline__ void vx_gemm_loop(const VxOperand<T>& X, const VxOper
       VxFrag<NPL> fx[TM / 32];
 #pragma unroll
       for (int mi = 0; mi < TM / 32; ++mi) vx_frag_load(px + mi * vx_image_block<NK>(), SX::PLANE, fx[mi]);
+      constexpr int G = TM / 32 >= 4 ? 1 : 2;     // W blocks at a time: four independent accumulators
 #pragma unroll
-      for (int ni = 0; ni < TN / 32; ++ni) {
-        VxFrag<NPL> fw;
-        vx_frag_load(pw + ni * vx_image_block<NK>(), SW::PLANE, fw);
+      for (int ni = 0; ni < TN / 32; ni += G) {
+        VxFrag<NPL> fw[G];
+#pragma unroll
+        for (int u = 0; u < G; ++u) vx_frag_load(pw + (ni + u) * vx_image_block<NK>(), SW::PLANE, fw[u]);
 #pragma unroll
         for (int pr = 0; pr < VxProducts<NPL>::N; ++pr)
 #pragma unroll
-          for (int mi = 0; mi < TM / 32; ++mi) acc[mi][ni] = vx_mma(pr, fw, fx[mi], acc[mi][ni]);
+          for (int u = 0; u < G; ++u)
+#pragma unroll
+            for (int mi = 0; mi < TM / 32; ++mi) acc[mi][ni + u] = vx_mma(pr, fw[u], fx[mi], acc[mi][ni + u]);
       }
     }
     __syncthreads();
