@@ -168,6 +168,10 @@ ATTN = [(1, 1, 1, 1, 1, 1, 1, 1), (1, 1, 480, 2, 2, 1, 192, 384), (2, 65, 33, 4,
         (1, 64, 32, 1, 1, 1, 32, 64), (2, 150, 300, 2, 2, 1, 192, 384), (1, 3, 5000, 2, 1, 1, 48, 48), (5, 1, 7, 3, 3, 1, 130, 257)]
 # enough query tiles for the 128-query form, in the smallest and the largest tile
 ATTN_WIDE = [(2, 2048, 70, 8, 8, 8, 16, 24), (4, 4096, 40, 2, 2, 1, 192, 384), (2, 2050, 65, 8, 2, 4, 96, 130)]
+# five and more tiles of 64 queries, every width class, lists of keys longer than one sweep
+ATTN_IMAGES = [(1, 300, 100, 2, 2, 1, 192, 384), (2, 333, 77, 4, 2, 1, 37, 53), (1, 321, 130, 2, 1, 2, 24, 48), (1, 400, 65, 1, 1, 1, 64, 64),
+               (2, 270, 200, 2, 2, 1, 128, 128), (1, 300, 260, 2, 2, 2, 90, 180), (1, 260, 33, 2, 2, 1, 60, 100),
+               (2, 300, 3001, 2, 1, 1, 48, 48), (1, 257, 1, 1, 1, 1, 8, 8)]
 MASKS = ["none", "some", "blank", "all"]
 
 
@@ -236,7 +240,7 @@ def attn_reference(q, k, v, km, do, scale=None):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("mask", MASKS)
-@pytest.mark.parametrize("shape", ATTN)
+@pytest.mark.parametrize("shape", ATTN + ATTN_IMAGES)
 def test_attention_and_gradients(shape, mask, dtype, dev):
     from vista_amd import ops
     q, k, v, km, do = make_attn(shape, dtype, dev, sum(shape), mask, poison=True)

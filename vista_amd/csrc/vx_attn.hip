@@ -21,6 +21,7 @@ struct AttnArgs {
   const uint8_t* mask;                       // [batch][mask_b] bytes, or null
   long long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h, mask_b;
   int sq, sk, h, gk, gv, d, dv;              // gk, gv: query heads per key / value head
+  const int *index, *place, *count;          // attn_live's lists of the keys that take part, or null (no mask, or few queries)
   float scale2, sign;                        // scale * log2(e) as scale2 > 0 (1 for scale 0) and a sign of 1, -1 or 0, so that the
                                              // maximum of the scores is that of the scaled ones and masked ones stay -inf
 };
@@ -42,9 +43,9 @@ struct AttnTile {
 
 // bits: which keys of tile t take part (lane l < KT speaks for key t * KT + l)
 template <typename T>
-__device__ __forceinline__ bool attn_key_live(const AttnArgs<T>& a, const uint8_t* mask, int t, int lane) {
+__device__ __forceinline__ bool attn_key_live(int keys, const uint8_t* mask, int t, int lane) {
   const int key = t * AttnTile<T>::KT + lane;
-  return lane < AttnTile<T>::KT && key < a.sk && (mask == nullptr || mask[key] != 0);
+  return lane < AttnTile<T>::KT && key < keys && (mask == nullptr || mask[key] != 0);
 }
 
 // A workgroup owns 16 * RT * QG queries of one head: QG groups of 16 * RT, each with CS waves. Everything is kept transposed --
@@ -79,11 +80,12 @@ void attn_fwd(const FwdArgs<T> a) {
   w /= a.tiles_q;
   const int split = (int)(w % a.splits);
   const int bh = (int)(w / a.splits), b = bh / a.h, h = bh % a.h;
-  const int tiles_k = (a.sk + KT - 1) / KT;
-  const int t0 = split * a.span, t1 = t0 + a.span < tiles_k ? t0 + a.span : tiles_k;
+  const int tiles_k = (a.sk + KT - 1) / KT;                                    // of the images
+  const int keys = IMG && a.count ? a.count[b] : a.sk, tiles = (keys + KT - 1) / KT;
+  const int t0 = split * a.span, t1 = t0 + a.span < tiles ? t0 + a.span : tiles;
   const T* kp = a.k + b * a.k_b + (h / a.gk) * a.k_h;
   const T* vp = a.v + b * a.v_b + (h / a.gv) * a.v_h;
-  const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  const uint8_t* mask = !IMG && a.mask ? a.mask + b * a.mask_b : nullptr;
   const int q0 = (tile_q * QG + wave / CS) * (16 * RT);
 
   VxFrag<NPL> qf[RT][KD];
@@ -189,7 +191,7 @@ void attn_fwd(const FwdArgs<T> a) {
   // the first tile from t on that has a key that takes part, and which of its keys do
   auto find = [&](int t, unsigned long long& live) {
     for (live = 0; t < t1; ++t) {
-      live = __ballot(attn_key_live(a, mask, t, lane));
+      live = __ballot(attn_key_live<T>(keys, mask, t, lane));
       if (live) break;
     }
     return t;
@@ -210,7 +212,7 @@ void attn_fwd(const FwdArgs<T> a) {
   }
   __syncthreads();
   while (cur) {
-    const bool ahead = tn + 1 < t1 && attn_key_live(a, mask, tn + 1, lane);
+    const bool ahead = tn + 1 < t1 && attn_key_live<T>(keys, mask, tn + 1, lane);
     vx_f32x4 s[RT][NK];
     {
       VxCol8<T, VW> vs[VI];
@@ -358,9 +360,57 @@ void attn_fwd(const FwdArgs<T> a) {
   }
 }
 
+// Which keys take part, once per call: index[b][j] = the j-th of them, place[b][key] = its j or -1, count[b]. Everything behind
+// works on the keys that take part alone, in their order, so a masked key costs nothing. One workgroup per batch, four keys a
+// thread and sweep.
+struct LiveArgs {
+  const uint8_t* mask;
+  long long mask_b;
+  int sk;
+  int *index, *place, *count;
+};
+__device__ __forceinline__ void live_keys(const LiveArgs& a, int b) {
+  __shared__ int sums[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint8_t* mask = a.mask + b * a.mask_b;
+  int *index = a.index + (long long)b * a.sk, *place = a.place + (long long)b * a.sk;
+  int base = 0;
+  for (int k0 = 0; k0 < a.sk; k0 += 1024) {
+    const int key = k0 + threadIdx.x * 4;
+    int live = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) live |= key + i < a.sk && mask[key + i] != 0 ? 1 << i : 0;
+    int upto = __popc(live);                   // inclusive sum over the wave's lanes
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += v;
+    }
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int j = base + upto - __popc(live), all = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i < wave) j += sums[i];
+      all += sums[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool on = live >> i & 1;
+      if (on) index[j] = key + i;
+      if (key + i < a.sk) place[key + i] = on ? j : -1;
+      j += on;
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) a.count[b] = base;
+}
+__global__ __launch_bounds__(256) void attn_live(const LiveArgs a) { live_keys(a, blockIdx.x); }
+
 // K and V as operand images: per head and tile of KT keys, planes of 1 KB fragments -- K: key block, 32-d step; V^T: column block,
 // 32-key step in the operand order of the keys. A thread makes one lane's 16 bytes of a fragment (all planes). Widths are padded
-// with 0 to the tile's, masked and missing keys are 0. It costs one pass over k and v; each tile of queries then saves the split
+// with 0 to the tile's, keys behind the last are 0. It costs one pass over k and v; each tile of queries then saves the split
 // and the transposition.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_pack(const AttnArgs<T> a, char* __restrict__ k_img, char* __restrict__ v_img, int tiles,
@@ -376,24 +426,32 @@ __global__ __launch_bounds__(256) void attn_pack(const AttnArgs<T> a, char* __re
   const int frag = (int)(ft % frags), t = (int)(tile_id % tiles);
   const long long head_id = tile_id / tiles;
   const int heads = is_k ? a.h / a.gk : a.h / a.gv, b = (int)(head_id / heads), head = (int)(head_id % heads);
-  const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  const int keys = a.count ? a.count[b] : a.sk;
+  if (t * KT >= keys) return;                  // no query reads this tile
+  const int* index = a.index ? a.index + (long long)b * a.sk : nullptr;
   VxFrag<NPL> f;
   if (is_k) {
     const int key = t * KT + frag / kd * 16 + c, d = frag % kd * 32 + g * 8;
-    const bool live = key < a.sk && (mask == nullptr || mask[key]);
+    const bool live = key < keys;
+    const int row = index && live ? index[key] : key;
     VxRow8<T> x;
-    x.load(a.k + b * a.k_b + head * a.k_h + key * a.k_s + d, live ? a.d - d : 0);
+    x.load(a.k + b * a.k_b + head * a.k_h + row * a.k_s + d, live ? a.d - d : 0);
     x.planes(f);
   } else {
     const int n = frag / NS * 16 + c, k0 = t * KT + frag % NS * 32 + g * 4;
     const T* p = a.v + b * a.v_b + head * a.v_h + (n < a.dv ? n : 0);
     float x[8];
+    int row[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int key = k0 + (j >> 2) * 16 + (j & 3);
-      const bool live = key < a.sk && n < a.dv && (mask == nullptr || mask[key]);
-      const float y = (float)p[(key < a.sk ? key : 0) * a.v_s];
-      x[j] = live ? y : 0.0f;
+      const int key = k0 + (j >> 2) * 16 + (j & 3), last = keys - 1;
+      row[j] = key < last ? key : last;
+      if (index) row[j] = index[row[j]];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float y = (float)p[row[j] * a.v_s];
+      x[j] = k0 + (j >> 2) * 16 + (j & 3) < keys && n < a.dv ? y : 0.0f;
     }
     vx_planes(x, f);
   }
@@ -472,16 +530,49 @@ struct BwdArgs : AttnArgs<T> {
   float *slab_k, *slab_v;                    // [splits][b*h][sk][d], [splits][b*h][sk][dv]
   float scale;
   int q0, rows, skp;                         // present chunk: queries [q0, q0 + rows); skp: sk rounded up to 8
+  long long kc_b, kc_h, vc_b, vc_h;          // gathered k, v: [b][head][sk][d], [b][head][sk][dv]
+  T *kc, *vc;
   int bh, split0, span;                      // first split of the chunk, queries of one split
   int tqp, tkp;                              // tiles of attn_pds: queries, keys
   int tq, tk, td, tdv;                       // tiles of attn_grads: queries, keys, columns of dK and dQ, columns of dV
   unsigned n_v, n_k, n_q;                    // workgroups per problem
 };
 
-// delta = sum_n go * out per query: one wave per row
+// k and v of the keys that take part, in their order (16 bytes a thread where the rows allow it)
 template <typename T>
-__global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long rows) {
-  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void attn_gather(const BwdArgs<T> a, int pieces_k, int pieces_v, long long items_k, long long items) {
+  constexpr int P = 16 / sizeof(T);
+  long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= items) return;
+  const bool is_k = i < items_k;
+  if (!is_k) i -= items_k;
+  const int pieces = is_k ? pieces_k : pieces_v, width = is_k ? a.d : a.dv, heads = is_k ? a.h / a.gk : a.h / a.gv;
+  const int n = (int)(i % pieces) * P;
+  i /= pieces;
+  const int j = (int)(i % a.sk);
+  i /= a.sk;
+  const int head = (int)(i % heads), b = (int)(i / heads);
+  if (j >= a.count[b]) return;
+  const int key = a.index[(long long)b * a.sk + j];
+  const T* from = (is_k ? a.k + b * a.k_b + key * a.k_s + head * a.k_h : a.v + b * a.v_b + key * a.v_s + head * a.v_h) + n;
+  T* to = (is_k ? a.kc + b * a.kc_b + head * a.kc_h : a.vc + b * a.vc_b + head * a.vc_h) + (long long)j * width + n;
+  if (width - n >= P) {
+    vx_u32x4u v;
+    __builtin_memcpy(&v, from, 16);
+    __builtin_memcpy(to, &v, 16);
+  } else {
+    for (int e = 0; e < width - n; ++e) to[e] = from[e];
+  }
+}
+
+// delta = sum_n go * out per query: one wave per row; with a mask the first workgroups make its lists
+template <typename T>
+__global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long rows, const LiveArgs live, unsigned batches) {
+  if (blockIdx.x < batches) {
+    live_keys(live, blockIdx.x);
+    return;
+  }
+  const long long r = (long long)(blockIdx.x - batches) * 4 + (threadIdx.x >> 6);
   if (r >= rows) return;
   const int lane = threadIdx.x & 63;
   const int bh = (int)(r / a.sq), row = (int)(r % a.sq), b = bh / a.h, h = bh % a.h;
@@ -509,22 +600,23 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) 
   w /= a.tkp;
   const int m0 = (int)(w % a.tqp) * TM;
   const int bh = (int)(w / a.tqp), b = bh / a.h, h = bh % a.h;
-  const int rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = a.sk - n0 < TN ? a.sk - n0 : TN;
+  const int keys = a.count ? a.count[b] : a.sk;
+  if (n0 >= keys) return;
+  const int rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = keys - n0 < TN ? keys - n0 : TN;
   const long long q = a.q0 + m0;
   vx_f32x4 s[TM / 32][TN / 32], dp[TM / 32][TN / 32];
   vx_acc_zero(s);
   vx_acc_zero(dp);
-  vx_gemm_loop<T, KC, KC, TM, TN, FAST, BK>({a.q + b * a.q_b + q * a.q_s + h * a.q_h, a.q_s, rows_m, nullptr},
-                                  {a.k + b * a.k_b + (h / a.gk) * a.k_h + n0 * a.k_s, a.k_s, rows_n, nullptr}, 0, a.d, lds, s);
-  vx_gemm_loop<T, KC, KC, TM, TN, FAST, BK>({a.go + b * a.go_b + q * a.go_s + h * a.go_h, a.go_s, rows_m, nullptr},
-                                  {a.v + b * a.v_b + (h / a.gv) * a.v_h + n0 * a.v_s, a.v_s, rows_n, nullptr}, 0, a.dv, lds, dp);
-  const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  vx_gemm_loop<T, KC, KC, TM, TN, FAST, BK>({a.q + b * a.q_b + q * a.q_s + h * a.q_h, a.q_s, rows_m},
+                                  {a.k + b * a.k_b + (h / a.gk) * a.k_h + n0 * a.k_s, a.k_s, rows_n}, 0, a.d, lds, s);
+  vx_gemm_loop<T, KC, KC, TM, TN, FAST, BK>({a.go + b * a.go_b + q * a.go_s + h * a.go_h, a.go_s, rows_m},
+                                  {a.v + b * a.v_b + (h / a.gv) * a.v_h + n0 * a.v_s, a.v_s, rows_n}, 0, a.dv, lds, dp);
   unsigned live[TN / 64];                      // of this lane's eight keys
   vx_acc_each<TM, TN>(s, [&](int mi, int, int j, int n, const vx_f32x4&, const vx_f32x4&) {
     if (mi) return;
     live[j] = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) live[j] |= n + i < rows_n && (mask == nullptr || mask[n0 + n + i] != 0) ? 1u << i : 0u;
+    for (int i = 0; i < 8; ++i) live[j] |= n + i < rows_n ? 1u << i : 0u;
   });
   float2 st[TM / 32];
   float delta[TM / 32];
@@ -570,12 +662,14 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
     const int m0 = (int)(w % a.tk) * TM;
     w /= a.tk;
     const int bh = (int)(w % a.bh), sp = (int)(w / a.bh), b = bh / a.h, h = bh % a.h;
+    const int keys = a.count ? a.count[b] : a.sk;
+    if (m0 >= keys) return;
     const int r0 = sp * a.span, len = a.rows - r0 < a.span ? a.rows - r0 : a.span;
-    const int rows_m = a.sk - m0 < TM ? a.sk - m0 : TM, rows_n = width - n0 < TN ? width - n0 : TN;
+    const int rows_m = keys - m0 < TM ? keys - m0 : TM, rows_n = width - n0 < TN ? width - n0 : TN;
     const long long q = a.q0 + r0;
-    const VxOperand<T> X{(is_v ? a.p : a.ds) + ((long long)bh * a.rows + r0) * a.skp + m0, a.skp, a.skp - m0, nullptr};
+    const VxOperand<T> X{(is_v ? a.p : a.ds) + ((long long)bh * a.rows + r0) * a.skp + m0, a.skp, a.skp - m0};
     const VxOperand<T> W{is_v ? a.go + b * a.go_b + q * a.go_s + h * a.go_h + n0 : a.q + b * a.q_b + q * a.q_s + h * a.q_h + n0,
-                         is_v ? a.go_s : a.q_s, rows_n, nullptr};
+                         is_v ? a.go_s : a.q_s, rows_n};
     vx_gemm_loop<T, KS, KS, TM, TN, FAST>(X, W, 0, len, lds, acc);
     float* slab = (is_v ? a.slab_v : a.slab_k) + ((long long)(a.split0 + sp) * a.bh + bh) * a.sk * width;
     vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
@@ -588,9 +682,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
     const int m0 = (int)(w % a.tq) * TM;
     const int bh = (int)(w / a.tq), b = bh / a.h, h = bh % a.h;
     const int rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = a.d - n0 < TN ? a.d - n0 : TN;
-    const VxOperand<T> X{a.ds + ((long long)bh * a.rows + m0) * a.skp, a.skp, rows_m, nullptr};
-    const VxOperand<T> W{a.k + b * a.k_b + (h / a.gk) * a.k_h + n0, a.k_s, rows_n, a.mask ? a.mask + b * a.mask_b : nullptr};
-    vx_gemm_loop<T, KC, KS, TM, TN, FAST>(X, W, 0, a.sk, lds, acc);   // the pad of dS is 0
+    const VxOperand<T> X{a.ds + ((long long)bh * a.rows + m0) * a.skp, a.skp, rows_m};
+    const VxOperand<T> W{a.k + b * a.k_b + (h / a.gk) * a.k_h + n0, a.k_s, rows_n};
+    vx_gemm_loop<T, KC, KS, TM, TN, FAST>(X, W, 0, a.count ? a.count[b] : a.sk, lds, acc);   // dS is 0 from there to its tile's end
     vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
       if (m < rows_m && n < rows_n)
         vx_store8(a.dq + (((long long)b * a.sq + a.q0 + m0 + m) * a.h + h) * a.d + n0 + n, v, w, rows_n - n);
@@ -612,11 +706,12 @@ __global__ __launch_bounds__(256) void attn_slab_sum(const BwdArgs<T> a, int spl
   r /= a.sk;
   const int heads = a.h / group, head = (int)(r % heads), b = (int)(r / heads);
   vx_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (a.mask == nullptr || a.mask[b * a.mask_b + key]) {
+  const int row = a.place ? a.place[(long long)b * a.sk + key] : key;
+  if (row >= 0) {
     const float* slab = is_v ? a.slab_v : a.slab_k;
     for (int j = 0; j < group; ++j)
       for (int sp = 0; sp < splits; ++sp)
-        s += vx_load4(slab + (((long long)sp * a.bh + b * a.h + head * group + j) * a.sk + key) * width + n, left);
+        s += vx_load4(slab + (((long long)sp * a.bh + b * a.h + head * group + j) * a.sk + row) * width + n, left);
   }
   vx_store4((is_v ? a.dvv : a.dk) + (((long long)b * a.sk + key) * heads + head) * width + n, s, left);
 }
@@ -674,10 +769,22 @@ int class_of(int64_t d, int64_t dv) {
   return i;
 }
 
+// attn_live's lists
+size_t live_bytes(const Shape& s) { return 2 * vx_align((size_t)s.b * s.sk * 4) + vx_align((size_t)s.b * 4); }
+template <typename T>
+LiveArgs live_args(AttnArgs<T>& a, const Shape& s, char* ws) {
+  const size_t list = vx_align((size_t)s.b * s.sk * 4);
+  const LiveArgs l{a.mask, a.mask_b, a.sk, (int*)ws, (int*)(ws + list), (int*)(ws + 2 * list)};
+  a.index = l.index;
+  a.place = l.place;
+  a.count = l.count;
+  return l;
+}
+
 struct FwdPlan {
   bool many, img;            // 128 queries per workgroup instead of 64; operand images
   int64_t tiles_q, splits, span, tiles_k;
-  size_t k_img, v_img;       // bytes
+  size_t k_img, v_img, live; // bytes
 };
 FwdPlan fwd_plan(const Shape& s, int32_t dtype) {
   FwdPlan p;
@@ -707,12 +814,13 @@ FwdPlan fwd_plan(const Shape& s, int32_t dtype) {
   const size_t row = dtype == VX_F32 ? 6 : 2;      // bytes of a value's planes
   p.k_img = p.img ? (size_t)s.b * s.hk * tiles_k * kt * kDims[c][0] * row : 0;
   p.v_img = p.img ? (size_t)s.b * s.hv * tiles_k * kt * kDims[c][1] * row : 0;
+  p.live = p.img ? live_bytes(s) : 0;
   return p;
 }
 size_t fwd_bytes(const Shape& s, int32_t dtype) {
   const FwdPlan p = fwd_plan(s, dtype);
   const size_t rows = p.splits > 1 ? (size_t)p.splits * s.b * s.h * s.sq : 0;
-  return p.k_img + p.v_img + vx_align(rows * s.dv * 4) + vx_align(rows * 8);
+  return p.k_img + p.v_img + p.live + vx_align(rows * s.dv * 4) + vx_align(rows * 8);
 }
 
 template <typename T, int C>
@@ -743,9 +851,14 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   const size_t rows = (size_t)p.splits * bh * sh.sq;
   a.k_img = ws;
   a.v_img = ws + p.k_img;
-  a.part = (float*)(ws + p.k_img + p.v_img);
-  a.part_ml = (float2*)(ws + p.k_img + p.v_img + vx_align(rows * sh.dv * 4));
+  char* lists = ws + p.k_img + p.v_img;
+  a.part = (float*)(lists + p.live);
+  a.part_ml = (float2*)(lists + p.live + vx_align(rows * sh.dv * 4));
   if (p.img && p.tiles_k) {
+    if (a.mask) {
+      attn_live<<<(unsigned)sh.b, 256, 0, s>>>(live_args(a, sh, lists));
+      VX_LAUNCH_CHECK();
+    }
     const int c = class_of(sh.d, sh.dv), kd = kDims[c][0] / 32, nv = kDims[c][1] / 16, kt = AttnTile<T>::KT;
     const int64_t ks = sh.b * sh.hk * p.tiles_k * (kt / 16) * kd * 64, all = ks + sh.b * sh.hv * p.tiles_k * nv * (kt / 32) * 64;
     VX_REQUIRE(vx_cdiv(all, 256) < (1LL << 31), "attn_fwd: too many keys");
@@ -775,8 +888,8 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
 
 struct BwdPlan {
   int64_t tp, tm, tn, skp, span, per_chunk, splits, chunk;  // queries per split, splits per chunk, all splits, queries per chunk
-  size_t delta, pds, slab_k, slab_v;                    // bytes
-  size_t total() const { return delta + 2 * pds + slab_k + slab_v; }
+  size_t delta, pds, slab_k, slab_v, live, kc, vc;      // bytes
+  size_t total() const { return delta + 2 * pds + slab_k + slab_v + live + kc + vc; }
 };
 // queries are cut into splits (one slab each) and the splits into chunks, whose probabilities and score gradients are in
 // memory at a time (at most kChunkBytes of both)
@@ -809,6 +922,9 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   p.pds = vx_align((size_t)bh * p.chunk * p.skp * e);
   p.slab_k = vx_align((size_t)p.splits * bh * s.sk * s.d * 4);
   p.slab_v = vx_align((size_t)p.splits * bh * s.sk * s.dv * 4);
+  p.live = live_bytes(s);
+  p.kc = vx_align((size_t)s.b * s.hk * s.sk * s.d * e);
+  p.vc = vx_align((size_t)s.b * s.hv * s.sk * s.dv * e);
   return p;
 }
 
@@ -840,9 +956,31 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   a.tk = (int)vx_cdiv(sh.sk, p.tm);
   a.td = (int)vx_cdiv(sh.d, p.tn);
   a.tdv = (int)vx_cdiv(sh.dv, p.tn);
-  VX_REQUIRE(vx_cdiv(rows, 4) < (1LL << 31), "attn_bwd: too many queries");
-  attn_delta<T><<<(unsigned)vx_cdiv(rows, 4), 256, 0, s>>>(a, rows);
+  char* at = ws + p.delta + 2 * p.pds + p.slab_k + p.slab_v;
+  const int64_t batches = a.mask ? sh.b : 0;
+  VX_REQUIRE(vx_cdiv(rows, 4) + batches < (1LL << 31), "attn_bwd: too many queries");
+  const LiveArgs live = a.mask ? live_args(a, sh, at) : LiveArgs{};
+  attn_delta<T><<<(unsigned)(vx_cdiv(rows, 4) + batches), 256, 0, s>>>(a, rows, live, (unsigned)batches);
   VX_LAUNCH_CHECK();
+  if (a.mask) {
+    a.kc = (T*)(at + p.live);
+    a.vc = (T*)(at + p.live + p.kc);
+    a.kc_h = sh.sk * sh.d;
+    a.kc_b = sh.hk * a.kc_h;
+    a.vc_h = sh.sk * sh.dv;
+    a.vc_b = sh.hv * a.vc_h;
+    constexpr int P = 16 / sizeof(T);
+    const int pk = (int)vx_cdiv(sh.d, P), pv = (int)vx_cdiv(sh.dv, P);
+    const int64_t ik = sh.b * sh.hk * sh.sk * pk, all = ik + sh.b * sh.hv * sh.sk * pv;
+    VX_REQUIRE(vx_cdiv(all, 256) < (1LL << 31), "attn_bwd: too many keys");
+    attn_gather<T><<<(unsigned)vx_cdiv(all, 256), 256, 0, s>>>(a, pk, pv, ik, all);
+    VX_LAUNCH_CHECK();
+    a.k = a.kc;
+    a.k_b = a.kc_b; a.k_s = sh.d; a.k_h = a.kc_h;
+    a.v = a.vc;
+    a.v_b = a.vc_b; a.v_s = sh.dv; a.v_h = a.vc_h;
+    a.mask = nullptr;
+  }
   const bool fast = args_fast(a) && heads_fast(a.go, a.go_b, a.go_s, a.go_h, sh.dv, sizeof(T));
   for (int64_t q0 = 0, split = 0; q0 < sh.sq; q0 += p.chunk, split += p.per_chunk) {
     a.q0 = (int)q0;

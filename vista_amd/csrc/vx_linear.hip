@@ -61,7 +61,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a
   const int rows_m = (int)(a.m - m0 < TM ? a.m - m0 : TM), rows_n = a.n - n0 < TN ? a.n - n0 : TN;
   vx_f32x4 acc[TM / 32][TN / 32];
   vx_acc_zero(acc);
-  const VxOperand<T> X{a.x + m0 * a.ldx, a.ldx, rows_m, nullptr}, W{a.w + (long long)n0 * a.ldw, a.ldw, rows_n, nullptr};
+  const VxOperand<T> X{a.x + m0 * a.ldx, a.ldx, rows_m}, W{a.w + (long long)n0 * a.ldw, a.ldw, rows_n};
   vx_gemm_loop<T, KC, KC, TM, TN, FAST, BK>(X, W, 0, a.k, lds, acc);
   vx_f32x4 bias[TN / 64][2];                   // of this lane's columns
   if (a.bias) {
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a
     const long long r0 = split * a.span;
     const int rows = (int)(a.m - r0 < a.span ? a.m - r0 : a.span);
     const int rows_n = a.n - n0 < TM ? a.n - n0 : TM, rows_k = a.k - k0 < TN ? a.k - k0 : TN;
-    const VxOperand<T> X{a.g + r0 * a.ldg + n0, a.ldg, rows_n, nullptr}, W{a.x + r0 * a.ldx + k0, a.ldx, rows_k, nullptr};
+    const VxOperand<T> X{a.g + r0 * a.ldg + n0, a.ldg, rows_n}, W{a.x + r0 * a.ldx + k0, a.ldx, rows_k};
     vx_gemm_loop<T, KS, KS, TM, TN, FAST>(X, W, 0, rows, lds, acc);
     float* slab = a.slab ? a.slab + (long long)split * a.n * a.k : nullptr;
     vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a
     const long long m0 = (long long)(t / a.tiles_xk) * TM;
     const int k0 = (int)(t % a.tiles_xk) * TN;
     const int rows_m = (int)(a.m - m0 < TM ? a.m - m0 : TM), rows_k = a.k - k0 < TN ? a.k - k0 : TN;
-    const VxOperand<T> X{a.g + m0 * a.ldg, a.ldg, rows_m, nullptr}, W{a.w + k0, a.ldw, rows_k, nullptr};
+    const VxOperand<T> X{a.g + m0 * a.ldg, a.ldg, rows_m}, W{a.w + k0, a.ldw, rows_k};
     vx_gemm_loop<T, KC, KS, TM, TN, FAST>(X, W, 0, a.n, lds, acc);
     const long long at0 = m0 * a.k + k0;
     vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {

@@ -182,10 +182,6 @@ struct VxCol8<float, W> {
       v[k][0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, at, uniform, 0));
     }
   }
-  __device__ __forceinline__ void clear(int k) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) v[k][j] = 0.0f;
-  }
   __device__ __forceinline__ void planes(int j, VxFrag<3>& f) const {
     const float x[8] = {v[0][j], v[1][j], v[2][j], v[3][j], v[4][j], v[5][j], v[6][j], v[7][j]};
     vx_planes(x, f);
@@ -227,10 +223,6 @@ struct VxCol8<__bf16, W> {
       v[k][0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, uniform, 0);
     }
   }
-  __device__ __forceinline__ void clear(int k) {
-#pragma unroll
-    for (int j = 0; j < W / 2; ++j) v[k][j] = 0u;
-  }
   __device__ __forceinline__ void planes(int j, VxFrag<1>& f) const {
     vx_u32x4 o;
     const unsigned sel = j & 1 ? 0x07060302u : 0x05040100u;
@@ -270,7 +262,7 @@ __device__ __forceinline__ void vx_frag_load(const char* p, int plane, VxFrag<NP
 // ---- GEMM ---------------------------------------------------------------------------------------------------------
 // operand tile: p points at (first row of the tile, k = 0)
 //   KC (k contiguous): element (r, k) at p[r * ld + k];  KS (k strided): element (r, k) at p[k * ld + r]
-// rows: rows that exist from the tile's first on; kmask (KS only): k's whose byte is 0 read as 0, whatever they hold.
+// rows: rows that exist from the tile's first on.
 // FAST operands are read by buffer loads: 16-byte aligned base and row stride, and (vx_fast) rows (KS) or the reduction (KC) in
 // multiples of 8, ld no smaller than a row, the offsets of a tile in 31 bits. The others are read element by element at
 // their edges, and every load waits for its own branch: measured 1.7 to 6 times the time of a FAST call.
@@ -280,7 +272,6 @@ struct VxOperand {
   const T* p;
   long long ld;
   int rows;
-  const uint8_t* kmask;
 };
 static inline bool vx_fast(const void* p, int64_t ld, int64_t width, int64_t esize) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * esize % 16 == 0 && width % 8 == 0 && ld >= width && ld < (1 << 21);
@@ -300,7 +291,6 @@ struct VxStage {
   static_assert(R * BK / 8 % kTileThreads == 0, "every thread stages the same amount");
   VxRow8<T> a[MODE == KC ? NI : 1];
   VxCol8<T, MODE == KS ? W : 2> b;
-  unsigned dead;                                                   // KS with a mask: bit i = k i of the eight reads as 0
 
   // KC item i of a thread: row (of the image) and k group. bf16: eight lanes read a row's 128 bytes; fp32: a lane's eight
   // values are two loads, four lanes a row
@@ -334,11 +324,6 @@ struct VxStage {
       }
     } else {
       const int r = tid % (R / W) * W, kg = group(tid) * 8;
-      if (o.kmask != nullptr) {
-        dead = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dead |= k0 + kg + i < kend && o.kmask[k0 + kg + i] ? 0u : 1u << i;
-      }
       if constexpr (FAST) {
         // the range ends with the reduction: k's past it read as 0
         const long long left = (long long)(kend - k0) * o.ld * E;
@@ -353,7 +338,7 @@ struct VxStage {
       }
     }
   }
-  __device__ __forceinline__ void store(const VxOperand<T>& o, char* img, int tid) {
+  __device__ __forceinline__ void store(char* img, int tid) const {
     VxFrag<NPL> f;
     if constexpr (MODE == KC) {
 #pragma unroll
@@ -365,11 +350,6 @@ struct VxStage {
       }
     } else {
       const int r = tid % (R / W) * W, kg = group(tid);
-      if (o.kmask != nullptr) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (dead >> i & 1) b.clear(i);
-      }
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         b.planes(j, f);
@@ -406,8 +386,8 @@ __device__ __forceinline__ void vx_gemm_loop(const VxOperand<T>& X, const VxOper
     sw.load(W, k0, kend, tid);
   }
   for (int k = k0; k < kend; k += BK) {
-    sx.store(X, ix, tid);
-    sw.store(W, iw, tid);
+    sx.store(ix, tid);
+    sw.store(iw, tid);
     __syncthreads();
     if (k + BK < kend) {
       sx.load(X, k + BK, kend, tid);
