@@ -147,36 +147,59 @@ __global__ __launch_bounds__(kTileThreads) void linear_few(const FwdArgs<T> a) {
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------
-// g = dy * act'(saved) (written where there is an activation) and the column sums of g per row chunk. A workgroup owns 128
-// columns (32 lanes x 4) and a chunk of rows (8 row lanes); sums in fp32 per thread, then over the 8 row lanes in order.
-constexpr int kActCols = 128, kActRowLanes = 8;
+// g = dy * act'(saved) (written where there is an activation) and the column sums of g per row chunk. A lane owns 16 bytes of
+// columns, `lanes` (a power of two, at most a wave) lanes a row, so that a wave reads whole rows; a workgroup owns `lanes` x 16 bytes
+// of columns and a chunk of rows. Sums in fp32 per thread, then over the workgroup's rows in order.
 template <typename T>
 __global__ __launch_bounds__(256) void act_bwd(const T* __restrict__ dy, long long ldy, const T* __restrict__ saved, long long m,
-                                               int n, int act, long long chunk, T* __restrict__ g, float* __restrict__ part) {
-  __shared__ vx_f32x4 sh[kActRowLanes][32];
-  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
-  const int c = blockIdx.x * kActCols + cl * 4;
+                                               int n, int act, long long chunk, int lanes, T* __restrict__ g, float* __restrict__ part) {
+  constexpr int V = 16 / sizeof(T), Q = V / 4, U = 2;              // columns and quads of a lane, rows in flight
+  __shared__ vx_f32x4 sh[256][Q];
+  const int cl = threadIdx.x & (lanes - 1), rl = threadIdx.x / lanes, rows = 256 / lanes;
+  const int c = (blockIdx.x * lanes + cl) * V;
   const long long r0 = (long long)blockIdx.y * chunk, r1 = r0 + chunk < m ? r0 + chunk : m;
-  vx_f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (c < n) {
-    for (long long r = r0 + rl; r < r1; r += kActRowLanes) {
-      vx_f32x4 v = vx_load4(dy + r * ldy + c, n - c);
-      if (act != kActNone) {
-        const vx_f32x4 s = vx_load4(saved + r * n + c, n - c);
+  vx_f32x4 sum[Q];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = act == kActRelu ? (s[i] > 0.0f ? v[i] : 0.0f) : v[i] * act_slope(s[i], act);
-        vx_store4(g + r * n + c, v, n - c);
+  for (int q = 0; q < Q; ++q) sum[q] = vx_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < n) {
+    for (long long r = r0 + rl; r < r1; r += U * rows) {
+      vx_f32x4 v[U][Q], s[U][Q];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long row = r + u * rows < r1 ? r + u * rows : r;
+        vx_loadq(dy + row * ldy + c, n - c, v[u]);
+        if (act != kActNone) vx_loadq(saved + row * n + c, n - c, s[u]);
       }
-      sum += v;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long row = r + u * rows;
+        if (row >= r1) break;
+        if (act != kActNone) {
+#pragma unroll
+          for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              v[u][q][i] = act == kActRelu ? (s[u][q][i] > 0.0f ? v[u][q][i] : 0.0f) : v[u][q][i] * act_slope(s[u][q][i], act);
+          if constexpr (Q == 2)
+            vx_store8(g + row * n + c, v[u][0], v[u][1], n - c);
+          else
+            vx_store4(g + row * n + c, v[u][0], n - c);
+        }
+#pragma unroll
+        for (int q = 0; q < Q; ++q) sum[q] += v[u][q];
+      }
     }
   }
   if (!part) return;
-  sh[rl][cl] = sum;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) sh[threadIdx.x][q] = sum[q];
   __syncthreads();
   if (rl == 0 && c < n) {
 #pragma unroll
-    for (int i = 1; i < kActRowLanes; ++i) sum += sh[i][cl];
-    vx_store4(part + (long long)blockIdx.y * n + c, sum, n - c);
+    for (int q = 0; q < Q; ++q) {
+      for (int i = 1; i < rows; ++i) sum[q] += sh[i * lanes + cl][q];
+      vx_store4(part + (long long)blockIdx.y * n + c + q * 4, sum[q], n - c - q * 4);
+    }
   }
 }
 
@@ -227,34 +250,59 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a
   }
 }
 
-// out[i] = sum over the slabs of slab[s * len + i], in a fixed order: lane group j of a workgroup (16 of 16 lanes, four values a
-// lane) adds the slabs j, j + 16, ..., then the 16 groups are added in order. Two such sums in one launch (dw, dbias).
+// out[i] = sum over the slabs of slab[s * len + i], in a fixed order. Two such sums in one launch: dw (few long slabs: a thread has
+// four values, eight slabs in flight) and dbias (many short ones: lane group j of a workgroup, 16 of 16 lanes, adds the slabs
+// j, j + 16, ..., then the 16 groups are added in order).
 template <typename T>
 __global__ __launch_bounds__(256) void slab_sum(const float* __restrict__ a, int count_a, long long len_a, T* __restrict__ out_a,
                                                 const float* __restrict__ b, int count_b, long long len_b,
                                                 T* __restrict__ out_b, unsigned blocks_a) {
   __shared__ vx_f32x4 sh[16][17];
-  const bool first = blockIdx.x < blocks_a;
-  const float* src = first ? a : b;
-  const int count = first ? count_a : count_b, cl = threadIdx.x & 15, grp = threadIdx.x >> 4;
-  const long long len = first ? len_a : len_b;
-  T* out = first ? out_a : out_b;
-  const long long i = ((long long)(first ? blockIdx.x : blockIdx.x - blocks_a) * 16 + cl) * 4;
-  const int left = len - i < 4 ? (int)(len - i) : 4;
+  constexpr int U = 8;
   vx_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (left > 0)
-    for (int c = grp; c < count; c += 16) s += vx_load4(src + c * len + i, left);
+  if (blockIdx.x < blocks_a) {
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= len_a) return;
+    const int left = len_a - i < 4 ? (int)(len_a - i) : 4, last = count_a - 1;
+    for (int c = 0; c < count_a; c += U) {
+      vx_f32x4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = vx_load4(a + (c + u < last ? c + u : last) * len_a + i, left);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (c + u > last) break;
+        s += v[u];
+      }
+    }
+    vx_store4(out_a + i, s, left);
+    return;
+  }
+  const int cl = threadIdx.x & 15, grp = threadIdx.x >> 4;
+  const long long i = ((long long)(blockIdx.x - blocks_a) * 16 + cl) * 4;
+  const int left = len_b - i < 4 ? (int)(len_b - i) : 4;
+  if (left > 0) {
+    for (int c = grp; c < count_b; c += 16 * U) {
+      vx_f32x4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = vx_load4(b + (c + u * 16 < count_b ? c + u * 16 : c) * len_b + i, left);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (c + u * 16 >= count_b) break;
+        s += v[u];
+      }
+    }
+  }
   sh[grp][cl] = s;
   __syncthreads();
   if (grp || left <= 0) return;
 #pragma unroll
   for (int j = 1; j < 16; ++j) s += sh[j][cl];
-  vx_store4(out + i, s, left);
+  vx_store4(out_b + i, s, left);
 }
 
 struct BwdPlan {
   bool big;
-  int64_t splits, span, chunks, chunk;
+  int64_t splits, span, chunks, chunk, lanes;      // lanes: of act_bwd, a row
 };
 BwdPlan bwd_plan(int64_t m, int64_t n, int64_t k, int32_t dtype) {
   BwdPlan p;
@@ -267,8 +315,12 @@ BwdPlan bwd_plan(int64_t m, int64_t n, int64_t k, int32_t dtype) {
   if (splits < 1) splits = 1;
   p.span = vx_cdiv(vx_cdiv(m, splits), bk) * bk;
   p.splits = vx_cdiv(m, p.span);
-  p.chunk = vx_cdiv(vx_cdiv(m, vx_cdiv(4 * cus, vx_cdiv(n, kActCols))), kActRowLanes) * kActRowLanes;
-  if (p.chunk < 4 * kActRowLanes) p.chunk = 4 * kActRowLanes;
+  const int64_t v = dtype == VX_F32 ? 4 : 8;
+  p.lanes = 1;
+  while (p.lanes < 64 && p.lanes * v < n) p.lanes *= 2;
+  const int64_t rows = 256 / p.lanes;
+  p.chunk = vx_cdiv(vx_cdiv(m, vx_cdiv(4 * cus, vx_cdiv(n, p.lanes * v))), rows) * rows;
+  if (p.chunk < 8 * rows) p.chunk = 8 * rows;
   p.chunks = vx_cdiv(m, p.chunk);
   return p;
 }
@@ -305,8 +357,8 @@ int32_t bwd_impl(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w,
   const T* g = dy;
   int64_t ldg = lddy;
   if (act != VX_ACT_NONE || dbias) {
-    const dim3 grid((unsigned)vx_cdiv(n, kActCols), (unsigned)p.chunks);
-    act_bwd<T><<<grid, 256, 0, s>>>(dy, lddy, saved, m, n, act, p.chunk, dpre, dbias ? part : nullptr);
+    const dim3 grid((unsigned)vx_cdiv(n, p.lanes * (16 / sizeof(T))), (unsigned)p.chunks);
+    act_bwd<T><<<grid, 256, 0, s>>>(dy, lddy, saved, m, n, act, p.chunk, (int)p.lanes, dpre, dbias ? part : nullptr);
     VX_LAUNCH_CHECK();
     if (act != VX_ACT_NONE) {
       g = dpre;
@@ -333,7 +385,7 @@ int32_t bwd_impl(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w,
     VX_LAUNCH_CHECK();
   }
   const int64_t len_w = dw && p.splits > 1 ? (int64_t)n * k : 0, len_b = dbias ? n : 0;
-  const unsigned ga = (unsigned)vx_cdiv(len_w, 64), gb = (unsigned)vx_cdiv(len_b, 64);
+  const unsigned ga = (unsigned)vx_cdiv(len_w, 1024), gb = (unsigned)vx_cdiv(len_b, 64);
   if (ga + gb) {
     slab_sum<T><<<ga + gb, 256, 0, s>>>(slab, (int)p.splits, len_w, dw, part, (int)p.chunks, len_b, dbias, ga);
     VX_LAUNCH_CHECK();

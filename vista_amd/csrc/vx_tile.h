@@ -458,6 +458,18 @@ __device__ __forceinline__ vx_f32x4 vx_load4(const __bf16* p, int n) {
   for (int i = 0; i < 4; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
   return v;
 }
+// 16 bytes of a row as quads
+__device__ __forceinline__ void vx_loadq(const float* p, int n, vx_f32x4 (&v)[1]) { v[0] = vx_load4(p, n); }
+__device__ __forceinline__ void vx_loadq(const __bf16* p, int n, vx_f32x4 (&v)[2]) {
+  if (n >= 8) {
+    const vx_u32x4 a = *reinterpret_cast<const vx_u32x4u*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = __uint_as_float(i & 1 ? a[i >> 1] & 0xffff0000u : a[i >> 1] << 16);
+    return;
+  }
+  v[0] = vx_load4(p, n);
+  v[1] = vx_load4(p + 4, n - 4);
+}
 __device__ __forceinline__ void vx_store4(float* p, const vx_f32x4& v, int n) {
   if (n >= 4) {
     *reinterpret_cast<vx_f32x4u*>(p) = v;
