@@ -61,9 +61,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a
   const int rows_m = (int)(a.m - m0 < TM ? a.m - m0 : TM), rows_n = a.n - n0 < TN ? a.n - n0 : TN;
   vx_f32x4 acc[TM / 32][TN / 32];
   vx_acc_zero(acc);
-  const VxOperand<T> X{a.x + m0 * a.ldx, a.ldx, rows_m}, W{a.w + (long long)n0 * a.ldw, a.ldw, rows_n};
-  vx_gemm_loop<T, KC, KC, TM, TN, FAST, BK>(X, W, 0, a.k, lds, acc);
-  vx_f32x4 bias[TN / 64][2];                   // of this lane's columns
+  vx_f32x4 bias[TN / 64][2];                   // of this lane's columns, there when the product is
   if (a.bias) {
     vx_acc_each<TM, TN>(acc, [&](int mi, int, int j, int n, const vx_f32x4&, const vx_f32x4&) {
       if (mi) return;
@@ -71,6 +69,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a
       bias[j][1] = vx_load4(a.bias + n0 + n + 4, rows_n - n - 4);
     });
   }
+  const VxOperand<T> X{a.x + m0 * a.ldx, a.ldx, rows_m}, W{a.w + (long long)n0 * a.ldw, a.ldw, rows_n};
+  vx_gemm_loop<T, KC, KC, TM, TN, FAST, BK>(X, W, 0, a.k, lds, acc);
   const long long at0 = m0 * a.n + n0;
   vx_acc_each<TM, TN>(acc, [&](int, int m, int j, int n, vx_f32x4 v, vx_f32x4 w) {
     const int left = rows_n - n;
@@ -151,13 +151,26 @@ __global__ __launch_bounds__(kTileThreads) void linear_few(const FwdArgs<T> a) {
 // columns, `lanes` (a power of two, at most a wave) lanes a row, so that a wave reads whole rows; a workgroup owns `lanes` x 16 bytes
 // of columns and a chunk of rows. Sums in fp32 per thread, then over the workgroup's rows in order.
 template <typename T>
-__global__ __launch_bounds__(256) void act_bwd(const T* __restrict__ dy, long long ldy, const T* __restrict__ saved, long long m,
-                                               int n, int act, long long chunk, int lanes, T* __restrict__ g, float* __restrict__ part) {
+struct ActArgs {
+  const T *dy, *saved;
+  T* g;
+  float* part;
+  long long ldy, m, chunk;
+  int n, act, lanes, cols;                     // cols: workgroups along the columns
+};
+template <typename T>
+__device__ __forceinline__ void act_rows(const ActArgs<T>& a, unsigned block, char* lds) {
   constexpr int V = 16 / sizeof(T), Q = V / 4, U = 2;              // columns and quads of a lane, rows in flight
-  __shared__ vx_f32x4 sh[256][Q];
+  vx_f32x4(*sh)[Q] = reinterpret_cast<vx_f32x4(*)[Q]>(lds);
+  const T *__restrict__ dy = a.dy, *__restrict__ saved = a.saved;
+  T* __restrict__ g = a.g;
+  float* __restrict__ part = a.part;
+  const long long ldy = a.ldy, m = a.m, chunk = a.chunk;
+  const int n = a.n, act = a.act, lanes = a.lanes;
+  const unsigned bx = block % a.cols, by = block / a.cols;
   const int cl = threadIdx.x & (lanes - 1), rl = threadIdx.x / lanes, rows = 256 / lanes;
-  const int c = (blockIdx.x * lanes + cl) * V;
-  const long long r0 = (long long)blockIdx.y * chunk, r1 = r0 + chunk < m ? r0 + chunk : m;
+  const int c = (bx * lanes + cl) * V;
+  const long long r0 = (long long)by * chunk, r1 = r0 + chunk < m ? r0 + chunk : m;
   vx_f32x4 sum[Q];
 #pragma unroll
   for (int q = 0; q < Q; ++q) sum[q] = vx_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -198,9 +211,14 @@ __global__ __launch_bounds__(256) void act_bwd(const T* __restrict__ dy, long lo
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       for (int i = 1; i < rows; ++i) sum[q] += sh[i * lanes + cl][q];
-      vx_store4(part + (long long)blockIdx.y * n + c + q * 4, sum[q], n - c - q * 4);
+      vx_store4(part + (long long)by * n + c + q * 4, sum[q], n - c - q * 4);
     }
   }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void act_bwd(const ActArgs<T> a) {
+  __shared__ __attribute__((aligned(16))) char lds[256 * 16 / sizeof(T) * 4];
+  act_rows(a, blockIdx.x, lds);
 }
 
 template <typename T>
@@ -213,11 +231,15 @@ struct BwdArgs {
   unsigned blocks_w, blocks_x;
 };
 
-// one launch for both gradients: workgroups [0, blocks_w) are tiles of dw = g^T x (reduction over the rows, split), the rest
-// tiles of dx = g w (reduction over n)
+// one launch for the gradients: workgroups [0, blocks_w) are tiles of dw = g^T x (reduction over the rows, split), the next blocks_x
+// tiles of dx = g w (reduction over n), the others (no activation: g = dy) the column sums
 template <typename T, int TM, int TN, bool FAST>
-__global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a) {
+__global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a, const ActArgs<T> sums) {
   __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
+  if (blockIdx.x >= a.blocks_w + a.blocks_x) {
+    act_rows(sums, blockIdx.x - a.blocks_w - a.blocks_x, lds);
+    return;
+  }
   vx_f32x4 acc[TM / 32][TN / 32];
   vx_acc_zero(acc);
   if (blockIdx.x < a.blocks_w) {
@@ -307,7 +329,9 @@ struct BwdPlan {
 BwdPlan bwd_plan(int64_t m, int64_t n, int64_t k, int32_t dtype) {
   BwdPlan p;
   const int64_t cus = vx_tile_cus(), bk = dtype == VX_F32 ? 32 : 64;
-  p.big = vx_cdiv(m, 128) * vx_cdiv(k, 128) >= cus;
+  // 128 x 128 tiles from here on; us of 64 / 128: fp32 6400 x 384 -> 384 (150 tiles of dx) 41 / 45, x 512 -> 384 (200) 50 / 47, 25600 x 384
+  // -> 512 151 / 143; bf16 6400 x 512 -> 384 27 / 27, 12800 x 384 -> 512 39 / 37, 102400 192 / 147
+  p.big = 4 * vx_cdiv(m, 128) * vx_cdiv(k, 128) >= 3 * cus;
   const int64_t t = p.big ? 128 : 64, tiles = vx_cdiv(n, t) * vx_cdiv(k, t);
   int64_t splits = vx_cdiv(2 * cus, tiles);
   const int64_t most = vx_cdiv(m, 8 * bk);
@@ -330,11 +354,15 @@ BwdPlan bwd_plan(int64_t m, int64_t n, int64_t k, int32_t dtype) {
 // 3.5 / 4.5, 5.8 / 5.9 (512, 640 workgroups); 512 rows 5.0 / 4.5.
 bool few_rule(int64_t m, int64_t n, int64_t cus, bool f32) { return vx_cdiv(m, 16) * vx_cdiv(n, 16) <= (f32 ? 4 : 2) * cus; }
 
+// 128 x 128 tiles instead of 64 x 64; us of 64 / 128: fp32 12800 x 512 -> 384 (300 tiles) 38 / 44, x 384 -> 512 (400) 40 / 38, 102400
+// 297 / 277; bf16 25600 x 384 -> 512 (800 tiles) 21.9 / 22.6, 102400 71 / 55
+bool big_rule(int64_t m, int64_t n, int64_t cus, bool f32) { return 2 * vx_cdiv(m, 128) * vx_cdiv(n, 128) >= (f32 ? 3 : 6) * cus; }
+
 template <typename T>
 int32_t fwd_impl(const FwdArgs<T>& args, hipStream_t s) {
   FwdArgs<T> a = args;
   const int64_t cus = vx_tile_cus();
-  const bool few = few_rule(a.m, a.n, cus, sizeof(T) == 4), use_big = vx_cdiv(a.m, 128) * vx_cdiv(a.n, 128) >= cus;
+  const bool few = few_rule(a.m, a.n, cus, sizeof(T) == 4), use_big = big_rule(a.m, a.n, cus, sizeof(T) == 4);
   const int64_t t = few ? 16 : use_big ? 128 : 64;
   a.tiles_n = (int)vx_cdiv(a.n, t);
   const int64_t grid = vx_cdiv(a.m, t) * a.tiles_n;
@@ -356,14 +384,16 @@ int32_t bwd_impl(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w,
   float* part = (float*)(ws + vx_align(p.splits > 1 ? (size_t)p.splits * n * k * 4 : 0));
   const T* g = dy;
   int64_t ldg = lddy;
-  if (act != VX_ACT_NONE || dbias) {
-    const dim3 grid((unsigned)vx_cdiv(n, p.lanes * (16 / sizeof(T))), (unsigned)p.chunks);
-    act_bwd<T><<<grid, 256, 0, s>>>(dy, lddy, saved, m, n, act, p.chunk, (int)p.lanes, dpre, dbias ? part : nullptr);
+  const int64_t cols = vx_cdiv(n, p.lanes * (16 / (int64_t)sizeof(T)));
+  const ActArgs<T> rows{dy, saved, dpre, dbias ? part : nullptr, lddy, m, p.chunk, n, act, (int)p.lanes, (int)cols};
+  int64_t sums = dbias ? cols * p.chunks : 0;        // workgroups of the column sums
+  VX_REQUIRE(cols * p.chunks < (1LL << 31), "linear_bwd: too many rows");
+  if (act != VX_ACT_NONE) {
+    act_bwd<T><<<(unsigned)(cols * p.chunks), 256, 0, s>>>(rows);
     VX_LAUNCH_CHECK();
-    if (act != VX_ACT_NONE) {
-      g = dpre;
-      ldg = n;
-    }
+    g = dpre;
+    ldg = n;
+    sums = 0;
   }
   const int64_t t = p.big ? 128 : 64;
   BwdArgs<T> a{};
@@ -374,14 +404,14 @@ int32_t bwd_impl(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w,
   a.tiles_w = (int)(vx_cdiv(n, t) * a.tiles_wk);
   a.tiles_xk = a.tiles_wk;
   const int64_t bw = dw ? a.tiles_w * p.splits : 0, bx = dx ? vx_cdiv(m, t) * a.tiles_xk : 0;
-  VX_REQUIRE(bw + bx < (1LL << 31), "linear_bwd: too many rows");
+  VX_REQUIRE(bw + bx + sums < (1LL << 31), "linear_bwd: too many rows");
   a.blocks_w = (unsigned)bw;
   a.blocks_x = (unsigned)bx;
-  if (bw + bx) {
+  if (bw + bx + sums) {
     const bool fast = vx_fast(a.g, a.ldg, n, sizeof(T)) && vx_fast(a.x, a.ldx, k, sizeof(T)) && vx_fast(a.w, a.ldw, k, sizeof(T));
     const auto kernel = p.big ? (fast ? linear_bwd<T, 128, 128, true> : linear_bwd<T, 128, 128, false>)
                               : (fast ? linear_bwd<T, 64, 64, true> : linear_bwd<T, 64, 64, false>);
-    kernel<<<(unsigned)(bw + bx), kTileThreads, 0, s>>>(a);
+    kernel<<<(unsigned)(bw + bx + sums), kTileThreads, 0, s>>>(a, rows);
     VX_LAUNCH_CHECK();
   }
   const int64_t len_w = dw && p.splits > 1 ? (int64_t)n * k : 0, len_b = dbias ? n : 0;
