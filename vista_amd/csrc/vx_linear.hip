@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a
       w += vx_load4(r + 4, left - 4);
     }
     const long long at = at0 + (long long)m * a.n + n;
-    if (a.pre) vx_store8(a.pre + at, v, w, left);
+    if (a.pre) vx_store8<true>(a.pre + at, v, w, left);
     if (a.act == kActRelu) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a
         w[i] = act_value(w[i], a.act);
       }
     }
-    vx_store8(a.y + at, v, w, left);
+    vx_store8<true>(a.y + at, v, w, left);   // 204800 x 384 -> 512 bf16: 143 -> 117 us
   });
 }
 

@@ -493,11 +493,25 @@ __device__ __forceinline__ void vx_store4(__bf16* p, const vx_f32x4& v, int n) {
     if (i < n) p[i] = (__bf16)v[i];
 }
 
-// eight neighbours, `n` of which exist
+// eight neighbours, `n` of which exist; ONCE: past the caches, for what this launch does not read again
+template <bool ONCE, typename V, typename P>
+__device__ __forceinline__ void vx_put(const V& v, P* p) {
+  if constexpr (ONCE)
+    __builtin_nontemporal_store(v, p);
+  else
+    *p = v;
+}
+template <bool ONCE = false>
 __device__ __forceinline__ void vx_store8(float* p, const vx_f32x4& a, const vx_f32x4& b, int n) {
+  if (n >= 8) {
+    vx_put<ONCE>(static_cast<vx_f32x4u>(a), reinterpret_cast<vx_f32x4u*>(p));
+    vx_put<ONCE>(static_cast<vx_f32x4u>(b), reinterpret_cast<vx_f32x4u*>(p + 4));
+    return;
+  }
   vx_store4(p, a, n);
   vx_store4(p + 4, b, n - 4);
 }
+template <bool ONCE = false>
 __device__ __forceinline__ void vx_store8(__bf16* p, const vx_f32x4& a, const vx_f32x4& b, int n) {
   if (n >= 8) {
     bf16x8 h;
@@ -506,7 +520,7 @@ __device__ __forceinline__ void vx_store8(__bf16* p, const vx_f32x4& a, const vx
       h[i] = (__bf16)a[i];
       h[4 + i] = (__bf16)b[i];
     }
-    *reinterpret_cast<vx_u32x4u*>(p) = __builtin_bit_cast(vx_u32x4u, h);
+    vx_put<ONCE>(__builtin_bit_cast(vx_u32x4u, h), reinterpret_cast<vx_u32x4u*>(p));
     return;
   }
   vx_store4(p, a, n);
