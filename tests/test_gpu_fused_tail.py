@@ -141,6 +141,49 @@ def test_linear_reads_strides_in_place(dev):
     assert all(torch.equal(a, b) for a, b in zip(one, two))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m", [1, 3, 31, 33, 1000, 6401])
+def test_linear_gradients_read_no_row_behind_the_last(m, dtype, dev):
+    """Operands at the front of a buffer whose other rows are NaN."""
+    from vista_amd import ops
+    x, w, _, s, dy = make_linear(m, 384, 512, dtype, dev, m, False, True)
+    want = ops.linear_bwd(dy, x, w, "relu", s)
+
+    def front(t):
+        buf = torch.full((m + 70, t.shape[1]), math.nan, dtype=dtype, device=dev)
+        buf[:m] = t
+        return buf[:m]
+
+    for a, b in zip(ops.linear_bwd(front(dy), front(x), w, "relu", front(s)), want):
+        assert torch.equal(a, b)
+    assert torch.equal(ops.linear_fwd(front(x), w)[0], ops.linear_fwd(x, w)[0])
+    one = ops.linear_bwd(dy, x[:1].expand(m, 384), w, "none")            # a repeated row: stride 0
+    for a, b in zip(one, ops.linear_bwd(dy, x[:1].expand(m, 384).contiguous(), w, "none")):
+        within(a, b.double(), 2 * gamma(max(m, 512), dtype) * 64 * (1 + b.double().abs()) + 4 * half_step(dtype) * b.double().abs(), "row")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(2, 70, 50, 4, 2, 2, 24, 40), (1, 300, 100, 2, 2, 1, 192, 384), (1, 300, 45, 2, 2, 1, 160, 200)])
+def test_attention_reads_no_row_behind_the_last(shape, dtype, dev):
+    from vista_amd import ops
+    q, k, v, km, do = make_attn(shape, dtype, dev, 2, "some")
+    want, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    grads = ops.attn_bwd(do, q, k, v, want, stats, km)
+    free, fstats = ops.attn_fwd(q, k, v, want_stats=True)
+    fgrads = ops.attn_bwd(do, q, k, v, free, fstats)
+
+    def front(t):
+        buf = torch.full((t.shape[0], t.shape[1] + 130, *t.shape[2:]), math.nan, dtype=dtype, device=dev)
+        buf[:, :t.shape[1]] = t
+        return buf[:, :t.shape[1]]
+
+    q2, k2, v2, do2 = (front(t) for t in (q, k, v, do))
+    for mask, first, back in ((km, want, grads), (None, free, fgrads)):
+        out, st = ops.attn_fwd(q2, k2, v2, mask, want_stats=True)
+        assert torch.equal(out, first)
+        assert all(torch.equal(a, b) for a, b in zip(ops.attn_bwd(do2, q2, k2, v2, out, st, mask), back))
+
+
 def test_linear_without_rows(dev):
     from vista_amd import ops
     w = torch.randn(5, 9, device=dev)
@@ -171,7 +214,8 @@ ATTN_WIDE = [(2, 2048, 70, 8, 8, 8, 16, 24), (4, 4096, 40, 2, 2, 1, 192, 384), (
 # five and more tiles of 64 queries, every width class, lists of keys longer than one sweep
 ATTN_IMAGES = [(1, 300, 100, 2, 2, 1, 192, 384), (2, 333, 77, 4, 2, 1, 37, 53), (1, 321, 130, 2, 1, 2, 24, 48), (1, 400, 65, 1, 1, 1, 64, 64),
                (2, 270, 200, 2, 2, 1, 128, 128), (1, 300, 260, 2, 2, 2, 90, 180), (1, 260, 33, 2, 2, 1, 60, 100),
-               (2, 300, 3001, 2, 1, 1, 48, 48), (1, 257, 1, 1, 1, 1, 8, 8)]
+               (2, 300, 3001, 2, 1, 1, 48, 48), (1, 257, 1, 1, 1, 1, 8, 8), (1, 290, 70, 2, 2, 1, 136, 264),
+               (1, 5000, 3, 2, 1, 1, 16, 16)]
 MASKS = ["none", "some", "blank", "all"]
 
 

@@ -157,7 +157,7 @@ void attn_fwd(const FwdArgs<T> a) {
         const bool here = bits >> kk & 1;
         const T* base = vp + (t * KT + kk) * a.v_s + nb;
         if constexpr (FAST)
-          vs[i].load(j, vx_buffer(base), here ? at : kVxOut, 0);
+          vs[i].load(j, vx_buffer(base), here ? at : kVxOut);
         else
           vs[i].load(j, base + vg * 4 * a.v_s + vl, here && u < V_UNITS ? a.dv - nb - vl : 0);
       }
@@ -709,9 +709,21 @@ __global__ __launch_bounds__(256) void attn_slab_sum(const BwdArgs<T> a, int spl
   const int row = a.place ? a.place[(long long)b * a.sk + key] : key;
   if (row >= 0) {
     const float* slab = is_v ? a.slab_v : a.slab_k;
-    for (int j = 0; j < group; ++j)
-      for (int sp = 0; sp < splits; ++sp)
-        s += vx_load4(slab + (((long long)sp * a.bh + b * a.h + head * group + j) * a.sk + row) * width + n, left);
+    constexpr int U = 8;                           // slabs in flight
+    const int last = group * splits - 1;
+    for (int i = 0; i <= last; i += U) {
+      vx_f32x4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = i + u < last ? i + u : last, j = at / splits, sp = at % splits;
+        v[u] = vx_load4(slab + (((long long)sp * a.bh + b * a.h + head * group + j) * a.sk + row) * width + n, left);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + u > last) break;
+        s += v[u];
+      }
+    }
   }
   vx_store4((is_v ? a.dvv : a.dk) + (((long long)b * a.sk + key) * heads + head) * width + n, s, left);
 }
@@ -903,7 +915,8 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   const int64_t t128 = vx_cdiv(s.sq, 128) * vx_cdiv(s.sk, 128) * bh;
   p.tp = 2 * t128 >= 3 * cus ? 128 : 64;
   p.tm = t128 >= 2 * cus ? 128 : 64;
-  p.tn = s.d > 128 ? 192 : p.tm;           // wide heads: 192 and 384 columns without a ragged tile, and less staging per product
+  // wide heads: 192 and 384 columns without a ragged tile, and less staging per product (a lane stages 3 or 6 columns at a time)
+  p.tn = s.d > 128 && s.d % 24 == 0 && s.dv % 24 == 0 ? 192 : p.tm;
   const int64_t tiles = vx_cdiv(s.sk, p.tm) * (vx_cdiv(s.dv, p.tn) + vx_cdiv(s.d, p.tn)) * bh;
   int64_t splits = 2 * cus / (tiles > 0 ? tiles : 1);
   if (splits < vx_cdiv(s.sq, 2 * s.sk)) splits = vx_cdiv(s.sq, 2 * s.sk);       // no workgroup much longer than those of dQ
@@ -981,7 +994,7 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
     a.v_b = a.vc_b; a.v_s = sh.dv; a.v_h = a.vc_h;
     a.mask = nullptr;
   }
-  const bool fast = args_fast(a) && heads_fast(a.go, a.go_b, a.go_s, a.go_h, sh.dv, sizeof(T));
+  const bool fast = args_fast(a) && heads_fast(a.go, a.go_b, a.go_s, a.go_h, sh.dv, sizeof(T)) && p.skp < (1 << 21);
   for (int64_t q0 = 0, split = 0; q0 < sh.sq; q0 += p.chunk, split += p.per_chunk) {
     a.q0 = (int)q0;
     a.rows = (int)(sh.sq - q0 < p.chunk ? sh.sq - q0 : p.chunk);

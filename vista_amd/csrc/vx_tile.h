@@ -165,21 +165,21 @@ struct VxCol8<float, W> {
       for (int j = 0; j < W; ++j) v[k][j] = j < n ? p[j] : 0.0f;
     }
   }
-  __device__ __forceinline__ void load(int k, vx_rsrc b, int at, int uniform) {
+  __device__ __forceinline__ void load(int k, vx_rsrc b, int at) {
     if constexpr (W == 4) {
-      const vx_u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(b, at, uniform, 0);
+      const vx_u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[k][j] = __uint_as_float(a[j]);
     } else if constexpr (W == 3) {
-      const vx_u32x3 a = __builtin_amdgcn_raw_buffer_load_b96(b, at, uniform, 0);
+      const vx_u32x3 a = __builtin_amdgcn_raw_buffer_load_b96(b, at, 0, 0);
 #pragma unroll
       for (int j = 0; j < 3; ++j) v[k][j] = __uint_as_float(a[j]);
     } else if constexpr (W == 2) {
-      const vx_u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(b, at, uniform, 0);
+      const vx_u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0);
       v[k][0] = __uint_as_float(a[0]);
       v[k][1] = __uint_as_float(a[1]);
     } else {
-      v[k][0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, at, uniform, 0));
+      v[k][0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0));
     }
   }
   __device__ __forceinline__ void planes(int j, VxFrag<3>& f) const {
@@ -210,17 +210,17 @@ struct VxCol8<__bf16, W> {
       }
     }
   }
-  __device__ __forceinline__ void load(int k, vx_rsrc b, int at, int uniform) {
+  __device__ __forceinline__ void load(int k, vx_rsrc b, int at) {
     if constexpr (W == 4) {
-      const vx_u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(b, at, uniform, 0);
+      const vx_u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0);
       v[k][0] = a[0];
       v[k][1] = a[1];
     } else if constexpr (W == 6) {
-      const vx_u32x3 a = __builtin_amdgcn_raw_buffer_load_b96(b, at, uniform, 0);
+      const vx_u32x3 a = __builtin_amdgcn_raw_buffer_load_b96(b, at, 0, 0);
 #pragma unroll
       for (int j = 0; j < 3; ++j) v[k][j] = a[j];
     } else {
-      v[k][0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, uniform, 0);
+      v[k][0] = __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0);
     }
   }
   __device__ __forceinline__ void planes(int j, VxFrag<1>& f) const {
@@ -264,8 +264,8 @@ __device__ __forceinline__ void vx_frag_load(const char* p, int plane, VxFrag<NP
 //   KC (k contiguous): element (r, k) at p[r * ld + k];  KS (k strided): element (r, k) at p[k * ld + r]
 // rows: rows that exist from the tile's first on.
 // FAST operands are read by buffer loads: 16-byte aligned base and row stride, and (vx_fast) rows (KS) or the reduction (KC) in
-// multiples of 8, ld no smaller than a row, the offsets of a tile in 31 bits. The others are read element by element at
-// their edges, and every load waits for its own branch: measured 1.7 to 6 times the time of a FAST call.
+// multiples of 8, ld no smaller than a row, the offsets of a tile in 31 bits; KS tiles of 192 rows want multiples of 24. The
+// others are read element by element at their edges, and every load waits for its own branch.
 constexpr int KC = 0, KS = 1;
 template <typename T>
 struct VxOperand {
@@ -325,12 +325,12 @@ struct VxStage {
     } else {
       const int r = tid % (R / W) * W, kg = group(tid) * 8;
       if constexpr (FAST) {
-        // the range ends with the reduction: k's past it read as 0
+        // the range ends with the reduction: k's past it read as 0 (the whole offset is the lane's: the check sees all of it)
         const long long left = (long long)(kend - k0) * o.ld * E;
         const vx_rsrc buf = vx_buffer(o.p + (long long)k0 * o.ld, left < (long long)kVxRange ? (unsigned)left : kVxRange);
         const int at = r < o.rows ? kg * (int)o.ld * E + r * E : kVxOut;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) b.load(i, buf, at, i * (int)o.ld * E);
+        for (int i = 0; i < 8; ++i) b.load(i, buf, at + i * (int)o.ld * E);
       } else {
         const T* p = o.p + (long long)(k0 + kg) * o.ld + r;
 #pragma unroll
