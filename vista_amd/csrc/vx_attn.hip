@@ -369,11 +369,12 @@ struct LiveArgs {
   int sk;
   int *index, *place, *count;
 };
-__device__ __forceinline__ void live_keys(const LiveArgs& a, int b) {
+// the whole workgroup (256 threads); GLOBAL: writes the lists; local (if not null): the keys in their order; returns the count
+template <bool GLOBAL>
+__device__ __forceinline__ int live_keys(const LiveArgs& a, int b, int* local) {
   __shared__ int sums[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint8_t* mask = a.mask + b * a.mask_b;
-  int *index = a.index + (long long)b * a.sk, *place = a.place + (long long)b * a.sk;
   int base = 0;
   for (int k0 = 0; k0 < a.sk; k0 += 1024) {
     const int key = k0 + threadIdx.x * 4;
@@ -397,38 +398,57 @@ __device__ __forceinline__ void live_keys(const LiveArgs& a, int b) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const bool on = live >> i & 1;
-      if (on) index[j] = key + i;
-      if (key + i < a.sk) place[key + i] = on ? j : -1;
+      if (local && on) local[j] = key + i;
+      if constexpr (GLOBAL) {
+        if (on) a.index[(long long)b * a.sk + j] = key + i;
+        if (key + i < a.sk) a.place[(long long)b * a.sk + key + i] = on ? j : -1;
+      }
       j += on;
     }
     base += all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) a.count[b] = base;
+  return base;
 }
-__global__ __launch_bounds__(256) void attn_live(const LiveArgs a) { live_keys(a, blockIdx.x); }
+__device__ __forceinline__ void live_lists(const LiveArgs& a, int b) {
+  const int n = live_keys<true>(a, b, nullptr);
+  if (threadIdx.x == 0) a.count[b] = n;
+}
+__global__ __launch_bounds__(256) void attn_live(const LiveArgs a) { live_lists(a, blockIdx.x); }
 
 // K and V as operand images: per head and tile of KT keys, planes of 1 KB fragments -- K: key block, 32-d step; V^T: column block,
 // 32-key step in the operand order of the keys. A thread makes one lane's 16 bytes of a fragment (all planes). Widths are padded
 // with 0 to the tile's, keys behind the last are 0. It costs one pass over k and v; each tile of queries then saves the split
 // and the transposition.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_pack(const AttnArgs<T> a, char* __restrict__ k_img, char* __restrict__ v_img, int tiles,
-                                                 int kd, int nv, long long k_slots, long long slots) {
+// OWN: with a mask of at most kOwnKeys keys every workgroup finds the keys by itself, which saves the launch of attn_live.
+constexpr int kOwnKeys = 2048;
+template <typename T, bool OWN>
+__global__ __launch_bounds__(256) void attn_pack(const AttnArgs<T> a, const LiveArgs own, char* __restrict__ k_img, char* __restrict__ v_img,
+                                                 int tiles, int kd, int nv, long long k_slots, long long slots, unsigned per) {
   constexpr int NPL = VxType<T>::NPL, KT = AttnTile<T>::KT, NS = KT / 32, NK = KT / 16;
-  long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  __shared__ int list[OWN ? kOwnKeys : 1];
+  const int b = blockIdx.x / per;              // `per` workgroups a batch
+  const unsigned block = blockIdx.x % per;
+  int keys = a.sk;
+  const int* index = nullptr;
+  if constexpr (OWN) {
+    keys = live_keys<false>(own, b, list);
+    index = list;
+    if (block == 0 && threadIdx.x == 0) own.count[b] = keys;
+  } else if (a.count) {
+    keys = a.count[b];
+    index = a.index + (long long)b * a.sk;
+  }
+  long long i = (long long)block * 256 + threadIdx.x;
   if (i >= slots) return;
   const bool is_k = i < k_slots;
   if (!is_k) i -= k_slots;
   const int lane = (int)(i & 63), c = lane & 15, g = lane >> 4;
-  const int frags = is_k ? NK * kd : nv * NS;
-  const long long ft = i >> 6, tile_id = ft / frags;
-  const int frag = (int)(ft % frags), t = (int)(tile_id % tiles);
-  const long long head_id = tile_id / tiles;
-  const int heads = is_k ? a.h / a.gk : a.h / a.gv, b = (int)(head_id / heads), head = (int)(head_id % heads);
-  const int keys = a.count ? a.count[b] : a.sk;
+  const int frags = is_k ? NK * kd : nv * NS, heads = is_k ? a.h / a.gk : a.h / a.gv;
+  const long long ft = i >> 6, ht = ft / frags;
+  const int frag = (int)(ft % frags), t = (int)(ht % tiles), head = (int)(ht / tiles);
+  const long long tile_id = (long long)b * heads * tiles + ht;
   if (t * KT >= keys) return;                  // no query reads this tile
-  const int* index = a.index ? a.index + (long long)b * a.sk : nullptr;
   VxFrag<NPL> f;
   if (is_k) {
     const int key = t * KT + frag / kd * 16 + c, d = frag % kd * 32 + g * 8;
@@ -569,7 +589,7 @@ __global__ __launch_bounds__(256) void attn_gather(const BwdArgs<T> a, int piece
 template <typename T>
 __global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long rows, const LiveArgs live, unsigned batches) {
   if (blockIdx.x < batches) {
-    live_keys(live, blockIdx.x);
+    live_lists(live, blockIdx.x);
     return;
   }
   const long long r = (long long)(blockIdx.x - batches) * 4 + (threadIdx.x >> 6);
@@ -867,14 +887,21 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   a.part = (float*)(lists + p.live);
   a.part_ml = (float2*)(lists + p.live + vx_align(rows * sh.dv * 4));
   if (p.img && p.tiles_k) {
-    if (a.mask) {
-      attn_live<<<(unsigned)sh.b, 256, 0, s>>>(live_args(a, sh, lists));
-      VX_LAUNCH_CHECK();
-    }
     const int c = class_of(sh.d, sh.dv), kd = kDims[c][0] / 32, nv = kDims[c][1] / 16, kt = AttnTile<T>::KT;
-    const int64_t ks = sh.b * sh.hk * p.tiles_k * (kt / 16) * kd * 64, all = ks + sh.b * sh.hv * p.tiles_k * nv * (kt / 32) * 64;
-    VX_REQUIRE(vx_cdiv(all, 256) < (1LL << 31), "attn_fwd: too many keys");
-    attn_pack<T><<<(unsigned)vx_cdiv(all, 256), 256, 0, s>>>(a, ws, ws + p.k_img, (int)p.tiles_k, kd, nv, ks, all);
+    const int64_t ks = sh.hk * p.tiles_k * (kt / 16) * kd * 64, all = ks + sh.hv * p.tiles_k * nv * (kt / 32) * 64;     // of a batch
+    const int64_t per = vx_cdiv(all, 256);
+    VX_REQUIRE(per * sh.b < (1LL << 31), "attn_fwd: too many keys");
+    const bool own = a.mask && sh.sk <= kOwnKeys;
+    LiveArgs live{};
+    if (a.mask) {
+      live = live_args(a, sh, lists);
+      if (!own) {
+        attn_live<<<(unsigned)sh.b, 256, 0, s>>>(live);
+        VX_LAUNCH_CHECK();
+      }
+    }
+    const auto pack = own ? attn_pack<T, true> : attn_pack<T, false>;
+    pack<<<(unsigned)(per * sh.b), 256, 0, s>>>(a, live, ws, ws + p.k_img, (int)p.tiles_k, kd, nv, ks, all, (unsigned)per);
     VX_LAUNCH_CHECK();
   }
   switch (class_of(sh.d, sh.dv)) {

@@ -36,7 +36,7 @@ def attention(q, k, v, key_mask=None, scale=None):
     key and value heads are shared by consecutive query heads. key_mask: bool [b, sk], True where the key takes part; a masked key
     has no part in the output or any gradient, whatever it holds, and a query without keys gives zeros. scale defaults to
     dim ** -0.5; dim <= 192, v_dim <= 384."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _AttentionFn.apply(q, k, v, key_mask, scale)
     return ops.attn_fwd(q, k, v, key_mask, scale)[0]
 
@@ -61,16 +61,16 @@ class _LinearFn(torch.autograd.Function):
 def linear_act(x, weight, bias=None, residual=None, act="none"):
     """act(x w^T + bias + residual) over the last dimension of x [..., fin]; weight [fout, fin], bias [fout], residual
     [..., fout]. act: none, relu, gelu (erf form), silu; it comes after the residual, as in the sparse convolutions' epilogue."""
+    grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                        or (residual is not None and residual.requires_grad))
+    if x.dim() == 2:
+        return _LinearFn.apply(x, weight, bias, residual, act) if grad else ops.linear_fwd(x, weight, bias, residual, act)[0]
     if x.dim() < 1 or (residual is not None and residual.shape[:-1] != x.shape[:-1]):
         raise ValueError("x must be [..., fin] and residual [..., fout] with the same leading dimensions")
-    lead = x.shape[:-1]
-    x2 = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
-    r2 = residual.reshape(-1, residual.shape[-1]) if residual is not None and residual.dim() != 2 else residual
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        y = _LinearFn.apply(x2, weight, bias, r2, act)
-    else:
-        y = ops.linear_fwd(x2, weight, bias, r2, act)[0]
-    return y if x.dim() == 2 else y.view(*lead, weight.shape[0])
+    x2 = x.reshape(-1, x.shape[-1])
+    r2 = residual.reshape(-1, residual.shape[-1]) if residual is not None else None
+    y = _LinearFn.apply(x2, weight, bias, r2, act) if grad else ops.linear_fwd(x2, weight, bias, r2, act)[0]
+    return y.view(*x.shape[:-1], weight.shape[0])
 
 
 def _conv1x1(conv, x, residual=None):

@@ -614,19 +614,18 @@ def _launch(dev, fn, *args):
 
 def _check_tensors(first, name, others, names):
     """`first` is a float32 / bfloat16 HIP tensor; the `others` (None: absent) share its device and dtype."""
-    if not isinstance(first, torch.Tensor) or not first.is_cuda:
-        _need_gpu(first, name)
-    if first.dtype not in _DT:
-        raise ValueError(f"unsupported {name} dtype {first.dtype}: float32 or bfloat16")
+    _need_gpu(first, name)
+    dtype, device = first.dtype, first.device
+    if dtype not in _DT:
+        raise ValueError(f"unsupported {name} dtype {dtype}: float32 or bfloat16")
     for t, n in zip(others, names):
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            _need_gpu(t, n)
-        if t.device != first.device:
-            raise ValueError(f"{n} is on {t.device}, {name} on {first.device}")
-        if t.dtype != first.dtype:
-            raise ValueError(f"{n} is {t.dtype}, {name} {first.dtype}: they must share a dtype")
+        _need_gpu(t, n)
+        if t.device != device:
+            raise ValueError(f"{n} is on {t.device}, {name} on {device}")
+        if t.dtype != dtype:
+            raise ValueError(f"{n} is {t.dtype}, {name} {dtype}: they must share a dtype")
 
 
 def _act_code(act):
