@@ -324,6 +324,21 @@ def test_attention_gradients_in_chunks_of_queries(k_len, dev):
         within(got, *ref[name], name)
 
 
+@pytest.mark.parametrize("k_len,live", [(2, 2), (5, 3), (16, 10), (40, 26), (128, 128)])
+def test_bf16_gradients_over_few_keys_lose_nothing(k_len, live, dev):
+    """Over at most 128 keys P and dS are 16-bit operands and delta is summed from P dP itself: what is left beside the gradients' own
+    rounding to bf16 (2-norm, rms about 2^-9 of each value) is 2^-17 of the operands: 1.05 of it with room for the sample."""
+    from vista_amd import ops
+    q, k, v, _, do = make_attn((1, 600, k_len, 2, 2, 1, 64, 96), BF16, dev, k_len, "none")
+    km = (torch.arange(k_len, device=dev) < live)[None]
+    out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    ref = attn_reference(q, k, v, km, do)
+    for name, got in zip(("dq", "dk", "dv"), ops.attn_bwd(do, q, k, v, out, stats, km)):
+        want = ref[name][0]
+        rounding = (want.to(BF16).double() - want).norm()
+        assert (got.double() - want).norm() <= 1.05 * rounding, name
+
+
 def test_attention_of_large_scores(dev):
     """Scores of some hundreds: the running maximum keeps every exponent in range; scale 0 and below zero are scales too."""
     from vista_amd import ops

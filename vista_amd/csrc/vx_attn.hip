@@ -6,7 +6,7 @@
 // fp32 operands run as three exact bf16 planes (six products, fp32 accumulation), bf16 ones directly (vx_tile.h). Softmax
 // statistics, probabilities and sums over queries are fp32; for bf16 tensors the probabilities and score gradients are rounded
 // to bf16 where they become matrix operands (at most half a step, 2^-8 of each value: independent errors, so that their sum is off
-// by about as much as the output's own rounding).
+// by about as much as the output's own rounding), in the backward pass over at most 128 keys to 16 bits.
 // A masked key has no part in anything, whatever its rows hold; a query without keys gives zeros. No atomics: bitwise
 // reproducible.
 #include "vx_tile.h"
@@ -230,7 +230,7 @@ void attn_fwd(const FwdArgs<T> a) {
 #pragma unroll
         for (int k = 0; k < OWN; ++k) vx_frag_load(ik + frag_at(K_BLOCK, half * OWN + k, kd), K_PLANE, kf[k]);
 #pragma unroll
-        for (int pr = 0; pr < VxProducts<NPL>::N; ++pr)
+        for (int pr = 0; pr < VxProducts<NPL, NPL>::N; ++pr)
 #pragma unroll
           for (int k = 0; k < OWN; ++k)
 #pragma unroll
@@ -317,7 +317,7 @@ void attn_fwd(const FwdArgs<T> a) {
 #pragma unroll
         for (int u = 0; u < G; ++u) vx_frag_load(iv + frag_at(V_BLOCK, half * NV + nv + u, ns), V_PLANE, vf[u]);
 #pragma unroll
-        for (int pr = 0; pr < VxProducts<NPL>::N; ++pr)
+        for (int pr = 0; pr < VxProducts<NPL, NPL>::N; ++pr)
 #pragma unroll
           for (int u = 0; u < G; ++u)
 #pragma unroll
@@ -545,7 +545,7 @@ struct BwdArgs : AttnArgs<T> {
   long long go_b, go_s, go_h;
   const float2* stats;
   float* delta;                              // [b*h][sq]
-  T *p, *ds;                                 // [b*h][rows][skp] of the present chunk of queries
+  void *p, *ds;                              // [b*h][rows][skp] of the present chunk of queries: T, or fp32 where the keys fit one tile
   T *dq, *dk, *dvv;                          // [b][sq][h][d], [b][sk][h/gk][d], [b][sk][h/gv][dv]
   float *slab_k, *slab_v;                    // [splits][b*h][sk][d], [splits][b*h][sk][dv]
   float scale;
@@ -585,6 +585,15 @@ __global__ __launch_bounds__(256) void attn_gather(const BwdArgs<T> a, int piece
   }
 }
 
+template <bool A, typename X, typename Y>
+struct VxPick {
+  typedef X type;
+};
+template <typename X, typename Y>
+struct VxPick<false, X, Y> {
+  typedef Y type;
+};
+
 // delta = sum_n go * out per query: one wave per row; with a mask the first workgroups make its lists
 template <typename T>
 __global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long rows, const LiveArgs live, unsigned batches) {
@@ -611,7 +620,11 @@ __global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long 
 constexpr int kPdsN = 128;                   // keys of an attn_pds tile
 // P and dS of a TM-query x TN-key tile: scores and dP = go v^T are two products with one epilogue,
 // P = 2^(scale2 s - max) / sum, dS = scale P (dP - delta).
-template <typename T, int TM, int TN, bool FAST>
+// ONE: all keys are in the tile. delta is then the tile's own sum of P dP, and both go out in fp32: over few keys the rounding of a
+// bf16 output inside delta and of P and dS to bf16 would not average out (2^-9 each of terms that nearly cancel).
+template <typename T, bool ONE>
+using AttnProb = typename VxPick<ONE, float, T>::type;
+template <typename T, int TM, int TN, bool FAST, bool ONE>
 __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) {
   constexpr int BK = TM <= 64 ? 64 : VxType<T>::BK;
   __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN, BK>()];
@@ -644,7 +657,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) 
     if (j) return;
     const long long r = (long long)bh * a.sq + a.q0 + m0 + (m < rows_m ? m : 0);
     st[mi] = a.stats[r];
-    delta[mi] = a.delta[r];
+    delta[mi] = ONE ? 0.0f : a.delta[r];
   });
   const long long at0 = ((long long)bh * a.rows + m0) * a.skp + n0;
 #pragma unroll
@@ -654,23 +667,47 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const bool on = live[ni / 2] >> (ni % 2 * 4 + i) & 1;
-        const float p = on ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[mi][ni][i] * a.sign, a.scale2, -st[mi].x)) * st[mi].y : 0.0f;
-        dp[mi][ni][i] = on ? p * (dp[mi][ni][i] - delta[mi]) * a.scale : 0.0f;
-        s[mi][ni][i] = p;
+        s[mi][ni][i] = on ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[mi][ni][i] * a.sign, a.scale2, -st[mi].x)) * st[mi].y : 0.0f;
+        dp[mi][ni][i] = on ? dp[mi][ni][i] : 0.0f;
+        if constexpr (ONE) delta[mi] = __builtin_fmaf(s[mi][ni][i], dp[mi][ni][i], delta[mi]);
       }
+  if constexpr (ONE) {                         // over the lane groups, then over the two waves of a row
+    float* sh = reinterpret_cast<float*>(lds);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int mi = 0; mi < TM / 32; ++mi) {
+      delta[mi] += __shfl_xor(delta[mi], 16, 64);
+      delta[mi] += __shfl_xor(delta[mi], 32, 64);
+      if (lane < 16) sh[(wave * (TM / 32) + mi) * 16 + lane] = delta[mi];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int mi = 0; mi < TM / 32; ++mi)
+      delta[mi] = sh[((wave & 2) * (TM / 32) + mi) * 16 + (lane & 15)] + sh[((wave | 1) * (TM / 32) + mi) * 16 + (lane & 15)];
+  }
+#pragma unroll
+  for (int mi = 0; mi < TM / 32; ++mi)
+#pragma unroll
+    for (int ni = 0; ni < TN / 32; ++ni)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dp[mi][ni][i] = s[mi][ni][i] * (dp[mi][ni][i] - delta[mi]) * a.scale;
+  using P = AttnProb<T, ONE>;
   vx_acc_each<TM, TN>(s, [&](int mi, int m, int j, int n, const vx_f32x4& v, const vx_f32x4& w) {
     if (m >= rows_m || n0 + n >= a.skp) return;
     const long long at = at0 + (long long)m * a.skp + n;
-    vx_store8(a.p + at, v, w, 8);
-    vx_store8(a.ds + at, dp[mi][2 * j], dp[mi][2 * j + 1], 8);
+    vx_store8((P*)a.p + at, v, w, 8);
+    vx_store8((P*)a.ds + at, dp[mi][2 * j], dp[mi][2 * j + 1], 8);
   });
 }
 
 // the three gradients of a chunk in one launch: dV slabs = P^T go, dK slabs = dS^T q (reduction over the queries of a split),
 // dQ = dS k (reduction over the keys)
-template <typename T, int TM, int TN, bool FAST>
+// ONE: P and dS are fp32; beside bf16 operands they are two planes
+template <typename T, int TM, int TN, bool FAST, bool ONE>
 __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a) {
-  __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
+  using P = AttnProb<T, ONE>;
+  constexpr int BK = VxType<T>::BK, PX = sizeof(T) == 2 && ONE ? 2 : VxType<T>::NPL;
+  __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN, BK, PX>()];
   vx_f32x4 acc[TM / 32][TN / 32];
   vx_acc_zero(acc);
   if (blockIdx.x < a.n_v + a.n_k) {
@@ -687,10 +724,10 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
     const int r0 = sp * a.span, len = a.rows - r0 < a.span ? a.rows - r0 : a.span;
     const int rows_m = keys - m0 < TM ? keys - m0 : TM, rows_n = width - n0 < TN ? width - n0 : TN;
     const long long q = a.q0 + r0;
-    const VxOperand<T> X{(is_v ? a.p : a.ds) + ((long long)bh * a.rows + r0) * a.skp + m0, a.skp, a.skp - m0};
+    const VxOperand<P> X{(const P*)(is_v ? a.p : a.ds) + ((long long)bh * a.rows + r0) * a.skp + m0, a.skp, a.skp - m0};
     const VxOperand<T> W{is_v ? a.go + b * a.go_b + q * a.go_s + h * a.go_h + n0 : a.q + b * a.q_b + q * a.q_s + h * a.q_h + n0,
                          is_v ? a.go_s : a.q_s, rows_n};
-    vx_gemm_loop<T, KS, KS, TM, TN, FAST>(X, W, 0, len, lds, acc);
+    vx_gemm_loop<T, KS, KS, TM, TN, FAST, BK, P, PX>(X, W, 0, len, lds, acc);
     float* slab = (is_v ? a.slab_v : a.slab_k) + ((long long)(a.split0 + sp) * a.bh + bh) * a.sk * width;
     vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
       if (m < rows_m && n < rows_n) vx_store8(slab + (long long)(m0 + m) * width + n0 + n, v, w, rows_n - n);
@@ -702,9 +739,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
     const int m0 = (int)(w % a.tq) * TM;
     const int bh = (int)(w / a.tq), b = bh / a.h, h = bh % a.h;
     const int rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = a.d - n0 < TN ? a.d - n0 : TN;
-    const VxOperand<T> X{a.ds + ((long long)bh * a.rows + m0) * a.skp, a.skp, rows_m};
+    const VxOperand<P> X{(const P*)a.ds + ((long long)bh * a.rows + m0) * a.skp, a.skp, rows_m};
     const VxOperand<T> W{a.k + b * a.k_b + (h / a.gk) * a.k_h + n0, a.k_s, rows_n};
-    vx_gemm_loop<T, KC, KS, TM, TN, FAST>(X, W, 0, a.count ? a.count[b] : a.sk, lds, acc);   // dS is 0 from there to its tile's end
+    vx_gemm_loop<T, KC, KS, TM, TN, FAST, BK, P, PX>(X, W, 0, a.count ? a.count[b] : a.sk, lds, acc);   // dS is 0 from there to its tile's end
     vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
       if (m < rows_m && n < rows_n)
         vx_store8(a.dq + (((long long)b * a.sq + a.q0 + m0 + m) * a.h + h) * a.d + n0 + n, v, w, rows_n - n);
@@ -926,6 +963,7 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
 }
 
 struct BwdPlan {
+  bool one;                                             // all keys fit one tile of attn_pds
   int64_t tp, tm, tn, skp, span, per_chunk, splits, chunk;  // queries per split, splits per chunk, all splits, queries per chunk
   size_t delta, pds, slab_k, slab_v, live, kc, vc;      // bytes
   size_t total() const { return delta + 2 * pds + slab_k + slab_v + live + kc + vc; }
@@ -935,21 +973,22 @@ struct BwdPlan {
 constexpr size_t kChunkBytes = (size_t)1 << 30;
 BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   BwdPlan p;
-  const int64_t cus = vx_tile_cus(), bh = s.b * s.h, e = dtype == VX_F32 ? 4 : 2, bk = dtype == VX_F32 ? 32 : 64;
+  p.one = s.sk <= kPdsN;
+  const int64_t cus = vx_tile_cus(), bh = s.b * s.h, e = dtype == VX_F32 ? 4 : 2, ep = p.one ? 4 : e, bk = dtype == VX_F32 ? 32 : 64;
   p.skp = vx_cdiv(s.sk, 8) * 8;
   // query rows of a tile; 4 x 2 heads, 1600 x 480, 192 / 384 wide, fp32 (416 tiles of 128): attn_pds 71 us with 64, 62 with 128,
   // attn_grads 82 and 84
   const int64_t t128 = vx_cdiv(s.sq, 128) * vx_cdiv(s.sk, 128) * bh;
-  p.tp = 2 * t128 >= 3 * cus ? 128 : 64;
-  p.tm = t128 >= 2 * cus ? 128 : 64;
+  p.tp = !p.one && 2 * t128 >= 3 * cus ? 128 : 64;
+  p.tm = !p.one && t128 >= 2 * cus ? 128 : 64;
   // wide heads: 192 and 384 columns without a ragged tile, and less staging per product (a lane stages 3 or 6 columns at a time)
-  p.tn = s.d > 128 && s.d % 24 == 0 && s.dv % 24 == 0 ? 192 : p.tm;
+  p.tn = !p.one && s.d > 128 && s.d % 24 == 0 && s.dv % 24 == 0 ? 192 : p.tm;
   const int64_t tiles = vx_cdiv(s.sk, p.tm) * (vx_cdiv(s.dv, p.tn) + vx_cdiv(s.d, p.tn)) * bh;
   int64_t splits = 2 * cus / (tiles > 0 ? tiles : 1);
   if (splits < vx_cdiv(s.sq, 2 * s.sk)) splits = vx_cdiv(s.sq, 2 * s.sk);       // no workgroup much longer than those of dQ
   const int64_t most = vx_cdiv(s.sq, 4 * bk);
   if (splits > most) splits = most;
-  int64_t fit = (int64_t)(kChunkBytes / 2) / (bh * p.skp * e);       // queries of a chunk
+  int64_t fit = (int64_t)(kChunkBytes / 2) / (bh * p.skp * ep);      // queries of a chunk
   if (fit < p.tm) fit = p.tm;
   if (splits < vx_cdiv(s.sq, fit)) splits = vx_cdiv(s.sq, fit);
   if (splits < 1) splits = 1;
@@ -959,7 +998,7 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   if (p.per_chunk > p.splits) p.per_chunk = p.splits;
   p.chunk = p.per_chunk * p.span < s.sq ? p.per_chunk * p.span : s.sq;
   p.delta = vx_align((size_t)bh * s.sq * 4);
-  p.pds = vx_align((size_t)bh * p.chunk * p.skp * e);
+  p.pds = vx_align((size_t)bh * p.chunk * p.skp * ep);
   p.slab_k = vx_align((size_t)p.splits * bh * s.sk * s.d * 4);
   p.slab_v = vx_align((size_t)p.splits * bh * s.sk * s.dv * 4);
   p.live = live_bytes(s);
@@ -970,11 +1009,12 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
 
 template <typename T, bool FAST>
 int32_t bwd_chunk(const BwdArgs<T>& a, const BwdPlan& p, unsigned pds, unsigned grads, hipStream_t s) {
-  const auto probs = p.tp == 128 ? attn_pds<T, 128, kPdsN, FAST> : attn_pds<T, 64, kPdsN, FAST>;
+  const auto probs = p.one ? attn_pds<T, 64, kPdsN, FAST, true> : p.tp == 128 ? attn_pds<T, 128, kPdsN, FAST, false> : attn_pds<T, 64, kPdsN, FAST, false>;
   probs<<<pds, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
-  const auto sums = p.tm == 128 ? (p.tn == 192 ? attn_grads<T, 128, 192, FAST> : attn_grads<T, 128, 128, FAST>)
-                                : (p.tn == 192 ? attn_grads<T, 64, 192, FAST> : attn_grads<T, 64, 64, FAST>);
+  const auto sums = p.one ? attn_grads<T, 64, 64, FAST, true>
+                    : p.tm == 128 ? (p.tn == 192 ? attn_grads<T, 128, 192, FAST, false> : attn_grads<T, 128, 128, FAST, false>)
+                                  : (p.tn == 192 ? attn_grads<T, 64, 192, FAST, false> : attn_grads<T, 64, 64, FAST, false>);
   sums<<<grads, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
   return VX_OK;
@@ -985,8 +1025,8 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   const BwdPlan p = bwd_plan(sh, dtype);
   const int64_t bh = sh.b * sh.h, rows = bh * sh.sq;
   a.delta = (float*)ws;
-  a.p = (T*)(ws + p.delta);
-  a.ds = (T*)(ws + p.delta + p.pds);
+  a.p = ws + p.delta;
+  a.ds = ws + p.delta + p.pds;
   a.slab_k = (float*)(ws + p.delta + 2 * p.pds);
   a.slab_v = (float*)(ws + p.delta + 2 * p.pds + p.slab_k);
   a.skp = (int)p.skp;
@@ -1000,8 +1040,11 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   const int64_t batches = a.mask ? sh.b : 0;
   VX_REQUIRE(vx_cdiv(rows, 4) + batches < (1LL << 31), "attn_bwd: too many queries");
   const LiveArgs live = a.mask ? live_args(a, sh, at) : LiveArgs{};
-  attn_delta<T><<<(unsigned)(vx_cdiv(rows, 4) + batches), 256, 0, s>>>(a, rows, live, (unsigned)batches);
-  VX_LAUNCH_CHECK();
+  const int64_t sums = p.one ? 0 : rows;             // (attn_pds makes its own delta over one tile)
+  if (batches + sums) {
+    attn_delta<T><<<(unsigned)(vx_cdiv(sums, 4) + batches), 256, 0, s>>>(a, sums, live, (unsigned)batches);
+    VX_LAUNCH_CHECK();
+  }
   if (a.mask) {
     a.kc = (T*)(at + p.live);
     a.vc = (T*)(at + p.live + p.kc);

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(kTileThreads) void linear_few(const FwdArgs<T> a) {
       x[u].planes(fx);
       w[u].planes(fw);
 #pragma unroll
-      for (int pr = 0; pr < VxProducts<NPL>::N; ++pr) acc = vx_mma(pr, fw, fx, acc);
+      for (int pr = 0; pr < VxProducts<NPL, NPL>::N; ++pr) acc = vx_mma(pr, fw, fx, acc);
     }
   }
   sh[wave][lane] = acc;

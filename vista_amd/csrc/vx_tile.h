@@ -51,24 +51,29 @@ struct VxFrag {
   bf16x8 p[NPL];
 };
 
-// the plane products of c += w * x, in order (fp32: six, down to 2^-21 of |w x|, smallest first). Callers loop over independent
-// accumulators inside a product, so that no matrix instruction waits for the one before it.
-template <int NPL>
+// the plane products of c += w * x, in order: three planes each (fp32): six, down to 2^-21 of |w x|, smallest first; one and two
+// (bf16 and an fp32 intermediate rounded to 16 bits): both. Callers loop over independent accumulators inside a product, so that
+// no matrix instruction waits for the one before it.
+template <int PW, int PX>
 struct VxProducts;
 template <>
-struct VxProducts<1> {
+struct VxProducts<1, 1> {
   static constexpr int N = 1, W[1] = {0}, X[1] = {0};
 };
 template <>
-struct VxProducts<3> {
+struct VxProducts<1, 2> {
+  static constexpr int N = 2, W[2] = {0, 0}, X[2] = {1, 0};
+};
+template <>
+struct VxProducts<3, 3> {
   static constexpr int N = 6, W[6] = {2, 0, 1, 1, 0, 0}, X[6] = {0, 2, 1, 0, 1, 0};
 };
-template <int NPL>
-__device__ __forceinline__ vx_f32x4 vx_mma(int product, const VxFrag<NPL>& w, const VxFrag<NPL>& x, vx_f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[VxProducts<NPL>::W[product]], x.p[VxProducts<NPL>::X[product]], c, 0, 0, 0);
+template <int PW, int PX>
+__device__ __forceinline__ vx_f32x4 vx_mma(int product, const VxFrag<PW>& w, const VxFrag<PX>& x, vx_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[VxProducts<PW, PX>::W[product]], x.p[VxProducts<PW, PX>::X[product]], c, 0, 0, 0);
 }
 
-// eight fp32 values -> operand planes (bf16: rounded to nearest even)
+// eight fp32 values -> operand planes (three: exact; one and two: rounded to nearest even, to 8 and 16 bits)
 __device__ __forceinline__ void vx_planes(const float (&v)[8], VxFrag<3>& f) {
   const Planes p = split8s(v);
   f.p[0] = p.h;
@@ -78,6 +83,13 @@ __device__ __forceinline__ void vx_planes(const float (&v)[8], VxFrag<3>& f) {
 __device__ __forceinline__ void vx_planes(const float (&v)[8], VxFrag<1>& f) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) f.p[0][i] = (__bf16)v[i];
+}
+__device__ __forceinline__ void vx_planes(const float (&v)[8], VxFrag<2>& f) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    f.p[0][i] = (__bf16)v[i];
+    f.p[1][i] = (__bf16)(v[i] - (float)f.p[0][i]);
+  }
 }
 
 // ---- buffer loads -------------------------------------------------------------------------------------------------
@@ -118,7 +130,8 @@ struct VxRow8<float> {
       v[4 + i] = __uint_as_float(y[i]);
     }
   }
-  __device__ __forceinline__ void planes(VxFrag<3>& f) const { vx_planes(v, f); }
+  template <int PL>
+  __device__ __forceinline__ void planes(VxFrag<PL>& f) const { vx_planes(v, f); }
 };
 template <>
 struct VxRow8<__bf16> {
@@ -182,7 +195,8 @@ struct VxCol8<float, W> {
       v[k][0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0));
     }
   }
-  __device__ __forceinline__ void planes(int j, VxFrag<3>& f) const {
+  template <int PL>
+  __device__ __forceinline__ void planes(int j, VxFrag<PL>& f) const {
     const float x[8] = {v[0][j], v[1][j], v[2][j], v[3][j], v[4][j], v[5][j], v[6][j], v[7][j]};
     vx_planes(x, f);
   }
@@ -281,9 +295,9 @@ static inline bool vx_fast(const void* p, int64_t ld, int64_t width, int64_t esi
 __device__ __forceinline__ int vx_row_w(int n) { return (n & ~31) + (n & 4) * 4 + (n >> 1 & 12) + (n & 3); }
 __device__ __forceinline__ int vx_row_n(int r) { return (r & ~31) + (r & 12) * 2 + (r >> 2 & 4) + (r & 3); }
 // stages R rows x BK k's with 256 threads: registers first (load), then the LDS image (store)
-template <typename T, int MODE, int R, int BK, bool FAST, bool IS_W>
+template <typename T, int NPL, int MODE, int R, int BK, bool FAST, bool IS_W>
 struct VxStage {
-  static constexpr int NPL = VxType<T>::NPL, NK = BK / 32, E = sizeof(T);
+  static constexpr int NK = BK / 32, E = sizeof(T);
   static constexpr int PLANE = (R / 16) * vx_image_block<NK>();
   static constexpr int BYTES = PLANE * NPL;
   static constexpr int NI = R * BK / 8 / kTileThreads;            // KC: 8-value items per thread; KS: rows per thread
@@ -361,9 +375,9 @@ struct VxStage {
 };
 
 // LDS bytes of vx_gemm_loop
-template <typename T, int TM, int TN, int BK = VxType<T>::BK>
+template <typename T, int TM, int TN, int BK = VxType<T>::BK, int PX = VxType<T>::NPL>
 constexpr int vx_gemm_lds() {
-  return (TM + TN) / 16 * vx_image_block<BK / 32>() * VxType<T>::NPL;
+  return (TM * PX + TN * VxType<T>::NPL) / 16 * vx_image_block<BK / 32>();
 }
 
 // acc[mi][ni] += the TM x TN tile's product over k in [k0, kend); wave (wm, wn) of 2 x 2 owns TM/2 x TN/2. One LDS image,
@@ -371,12 +385,13 @@ constexpr int vx_gemm_lds() {
 // three workgroups of a CU cover each other's barriers and splitting. Measured against it: two images with one barrier a step and
 // the split of the next step among this one's products 4096^3 fp32 694 -> 869 us, 204800 x 384 -> 512 bf16 134 -> 170 us (one
 // workgroup less a CU); two and three steps in flight: no difference. Ends with a barrier: the caller may reuse the LDS.
-template <typename T, int XM, int WM, int TM, int TN, bool FAST, int BK = VxType<T>::BK>
-__device__ __forceinline__ void vx_gemm_loop(const VxOperand<T>& X, const VxOperand<T>& W, int k0, int kend, char* lds,
+// TX, PX: the type and planes of X where they are not those of W
+template <typename T, int XM, int WM, int TM, int TN, bool FAST, int BK = VxType<T>::BK, typename TX = T, int PX = VxType<T>::NPL>
+__device__ __forceinline__ void vx_gemm_loop(const VxOperand<TX>& X, const VxOperand<T>& W, int k0, int kend, char* lds,
                                              vx_f32x4 (&acc)[TM / 32][TN / 32]) {
   constexpr int NPL = VxType<T>::NPL, NK = BK / 32;
-  using SX = VxStage<T, XM, TM, BK, FAST, false>;
-  using SW = VxStage<T, WM, TN, BK, FAST, true>;
+  using SX = VxStage<TX, PX, XM, TM, BK, FAST, false>;
+  using SW = VxStage<T, NPL, WM, TN, BK, FAST, true>;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   char *ix = lds, *iw = lds + SX::BYTES;
   SX sx;
@@ -397,7 +412,7 @@ __device__ __forceinline__ void vx_gemm_loop(const VxOperand<T>& X, const VxOper
     for (int ks = 0; ks < NK; ++ks) {
       const char* px = ix + vx_image_at<NK>(wm * (TM / 32), ks, lane);
       const char* pw = iw + vx_image_at<NK>(wn * (TN / 32), ks, lane);
-      VxFrag<NPL> fx[TM / 32];
+      VxFrag<PX> fx[TM / 32];
 #pragma unroll
       for (int mi = 0; mi < TM / 32; ++mi) vx_frag_load(px + mi * vx_image_block<NK>(), SX::PLANE, fx[mi]);
       constexpr int G = TM / 32 >= 4 ? 1 : 2;     // W blocks at a time: four independent accumulators
@@ -407,7 +422,7 @@ __device__ __forceinline__ void vx_gemm_loop(const VxOperand<T>& X, const VxOper
 #pragma unroll
         for (int u = 0; u < G; ++u) vx_frag_load(pw + (ni + u) * vx_image_block<NK>(), SW::PLANE, fw[u]);
 #pragma unroll
-        for (int pr = 0; pr < VxProducts<NPL>::N; ++pr)
+        for (int pr = 0; pr < VxProducts<NPL, PX>::N; ++pr)
 #pragma unroll
           for (int u = 0; u < G; ++u)
 #pragma unroll
