@@ -54,6 +54,10 @@ __device__ __forceinline__ void linear_finish(const FwdArgs<T>& a, long long m, 
 template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a) {
   constexpr int BK = TM <= 64 ? 64 : VxType<T>::BK;        // 64 against 32 of fp32: 6400 x 384 -> 384 24 -> 21 us
+  // y of the small tiles goes past the caches: it would push out the rows of x that the next column tiles read. us past / through them:
+  // 64 x 64 6400 x 384 -> 384 17.4 / 18.2, bf16 60000 x 128 -> 512 24 / 35, 16896 x 384 -> 384 13.7 / 14.7; 128 x 128 204800 x 384 -> 512
+  // bf16 154 / 136, fp32 470 / 470
+  constexpr bool ONCE = TM <= 64;
   __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN, BK>()];
   const unsigned t = vx_xcd_tile(blockIdx.x, gridDim.x);
   const long long m0 = (long long)(t / a.tiles_n) * TM;
@@ -85,7 +89,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a
       w += vx_load4(r + 4, left - 4);
     }
     const long long at = at0 + (long long)m * a.n + n;
-    if (a.pre) vx_store8<true>(a.pre + at, v, w, left);
+    if (a.pre) vx_store8<ONCE>(a.pre + at, v, w, left);
     if (a.act == kActRelu) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -99,7 +103,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a
         w[i] = act_value(w[i], a.act);
       }
     }
-    vx_store8<true>(a.y + at, v, w, left);   // 204800 x 384 -> 512 bf16: 143 -> 117 us
+    vx_store8<ONCE>(a.y + at, v, w, left);
   });
 }
 
@@ -354,15 +358,22 @@ BwdPlan bwd_plan(int64_t m, int64_t n, int64_t k, int32_t dtype) {
 // 3.5 / 4.5, 5.8 / 5.9 (512, 640 workgroups); 512 rows 5.0 / 4.5.
 bool few_rule(int64_t m, int64_t n, int64_t cus, bool f32) { return vx_cdiv(m, 16) * vx_cdiv(n, 16) <= (f32 ? 4 : 2) * cus; }
 
-// 128 x 128 tiles instead of 64 x 64; us of 64 / 128: fp32 12800 x 512 -> 384 (300 tiles) 38 / 44, x 384 -> 512 (400) 40 / 38, 102400
-// 297 / 277; bf16 25600 x 384 -> 512 (800 tiles) 21.9 / 22.6, 102400 71 / 55
-bool big_rule(int64_t m, int64_t n, int64_t cus, bool f32) { return 2 * vx_cdiv(m, 128) * vx_cdiv(n, 128) >= (f32 ? 3 : 6) * cus; }
+// 128 x 128 tiles instead of 64 x 64: half the reads per output, but fewer workgroups to hide a short sum's stores behind. us of 64 / 128:
+// fp32 12800 x 512 -> 384 (300 tiles of 128) 38 / 45, 14400 x 384 -> 512 (452) 44 / 40, 60000 x 256 -> 512 (1876) 119 / 109, but 128 -> 512
+// 66 / 74; bf16 of a long sum by tiles too, 16896 x 512 -> 384 (396) 16 / 16, 36000 (846) 37 / 31, of a shorter one from where the L2s
+// (32 MiB in all) no longer keep x for its next column tile: 60000 x 256 -> 512 (29 MiB) 40 / 38, 100000 x 128 -> 512 (24) 40 / 45,
+// 36000 x 384 -> 384 (26) 22 / 27, 52000 (38) 42 / 31
+bool big_rule(int64_t m, int64_t n, int64_t k, int64_t cus, bool f32) {
+  const int64_t tiles = vx_cdiv(m, 128) * vx_cdiv(n, 128);
+  if (f32) return k >= 192 && 2 * tiles >= 3 * cus;
+  return k >= 512 ? tiles >= 3 * cus : m * k * 2 >= 29 << 20;
+}
 
 template <typename T>
 int32_t fwd_impl(const FwdArgs<T>& args, hipStream_t s) {
   FwdArgs<T> a = args;
   const int64_t cus = vx_tile_cus();
-  const bool few = few_rule(a.m, a.n, cus, sizeof(T) == 4), use_big = big_rule(a.m, a.n, cus, sizeof(T) == 4);
+  const bool few = few_rule(a.m, a.n, cus, sizeof(T) == 4), use_big = big_rule(a.m, a.n, a.k, cus, sizeof(T) == 4);
   const int64_t t = few ? 16 : use_big ? 128 : 64;
   a.tiles_n = (int)vx_cdiv(a.n, t);
   const int64_t grid = vx_cdiv(a.m, t) * a.tiles_n;
