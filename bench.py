@@ -49,6 +49,8 @@ def parse(argv=None):
     ap.add_argument("--full-net", action="store_true",
                     help="BASELINE configs[2]: MultiViewBackbone + dense tail (necks, cross-view attention, OHS head; "
                          "stock PyTorch-ROCm ops) on the VISTA geometry")
+    ap.add_argument("--fused-tail", action="store_true",
+                    help="with --full-net: the cross-view attention block on the libvx kernels (vista_amd.fused_tail)")
     ap.add_argument("--postprocess", action="store_true",
                     help="with --full-net: add box decode + score filter + rotated NMS (head.predict) to the step")
     ap.add_argument("--streams", type=int, default=1,
@@ -407,6 +409,9 @@ def run_infer(a, dev, rank, world, dist, backend, barrier):
         det.backbone = None         # the sparse part runs through the fused engine above
         dtype = torch.float32 if a.dtype == "fp32" else torch.bfloat16
         det = fuse_for_inference(det).to(dev).to(dtype)
+        if a.fused_tail:
+            from vista_amd.fused_tail import fuse_cross_attention
+            det = fuse_cross_attention(det)
         tail = det.dense_tail
         if a.postprocess:
             from vista_amd.postprocess import VISTA_TEST_CFG
@@ -434,6 +439,7 @@ def run_infer(a, dev, rank, world, dist, backend, barrier):
                                f"inputs resident in HBM (BASELINE.json {cfg_name})",
                    "frames_per_gpu": a.batch, "points_per_frame": int(np.mean([f.shape[0] for f in frames])),
                    "parallelism": f"frame-sharded x{world}",
+                   **({"dense_tail": "cross-view attention block on libvx kernels"} if a.full_net and a.fused_tail else {}),
                    "dispatch": "eager per-layer launches" if a.eager else engine.dispatch_name()
                    + (", two plans in flight: geometry graph of step k + 1 beside the feature graph of step k"
                       if a.pipeline and not a.full_net and a.streams == 1 else "")},

@@ -360,7 +360,8 @@ int32_t vx_nms_bev(const float* d_boxes, int32_t num_boxes, float thresh, int32_
  *                gradient; without one that is d_dy itself); d_dx [m][k] = g w, d_dw [n][k] = g^T x, d_dbias [n] = column
  *                sums of g; each of the three may be NULL
  * Row strides are in elements, >= 0 (0 repeats a row), the last dimension is contiguous. m < 2^31; n, k <= 2^20. m = 0 gives
- * zero parameter gradients. No atomics: bitwise reproducible. VX_ACT_GELU is the erf form.
+ * zero parameter gradients. No atomics: bitwise reproducible. VX_ACT_GELU is the erf form. An infinity or NaN in an fp32 operand
+ * gives NaN (not an infinity) in every output it reaches: its planes are not numbers.
  * ------------------------------------------------------------------------------------------- */
 #define VX_ACT_NONE 0
 #define VX_ACT_RELU 1
@@ -388,7 +389,9 @@ int32_t vx_linear_bwd(const void* d_dy, int64_t lddy, const void* d_x, int64_t l
  *          needs (maximum of log2(e) * scale * score, 1 / sum)
  * vx_attn_bwd  d_dout with its own strides HOST int64[3] (batch, position, head), d_out and d_stats of the forward pass ->
  *          d_dq [batch][q_len][heads][dim], d_dk [batch][k_len][k_heads][dim], d_dv [batch][k_len][v_heads][v_dim]
- * Statistics, probabilities and sums are fp32; matrix arithmetic as in vx_linear_*. No atomics: bitwise reproducible.
+ * Statistics, probabilities and sums are fp32; matrix arithmetic as in vx_linear_*. VX_BF16 probabilities and score gradients are
+ * rounded to bf16 where they become operands (over at most 128 keys the backward pass keeps 16 bits of them). Infinities and NaN
+ * in rows that take part give NaN; in masked rows they are never read. No atomics: bitwise reproducible.
  * ------------------------------------------------------------------------------------------- */
 #define VX_ATTN_MAX_DIM 192
 #define VX_ATTN_MAX_VDIM 384

@@ -563,6 +563,25 @@ def test_fused_block_runs_the_operators_together(heads, dev):
             close(a.grad, b.grad, name)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_fused_neck_at_full_size(dtype, dev):
+    """The detector's own neck (1600 queries over 480 keys, 384 channels, one head): the fused block and the stock one on the same
+    maps. fp32: 1e-4 of the largest value; bf16: sixteen roundings of half a step (2^-8) of it lie between a map and the same map."""
+    from vista_amd.dense_tail import Cross_Attention_Decouple
+    from vista_amd.fused_tail import fuse_cross_attention
+    import copy
+    torch.manual_seed(7)
+    stock = Cross_Attention_Decouple(384, 384, 384, 1, (160, 160), (40, 40), (160, 12), (40, 12), 512).eval().to(dev)
+    fused = fuse_cross_attention(copy.deepcopy(stock)).to(dtype)
+    bev, rv = torch.randn(2, 384, 160, 160, device=dev), torch.randn(2, 384, 160, 12, device=dev)
+    with torch.no_grad():
+        want, _ = stock((bev, rv), need_maps=False)
+        got, _ = fused((bev.to(dtype), rv.to(dtype)), need_maps=False)
+    for a, b in zip(got, want):
+        tol = 1e-4 if dtype == F32 else 16 * 2.0 ** -8
+        assert a.dtype == dtype and (a.float() - b).abs().max() <= tol * b.abs().max()
+
+
 def test_fused_block_with_maps_runs_the_stock_path(dev):
     from vista_amd.fused_tail import fuse_cross_attention
     m, bev, rv = block(dev)

@@ -6,7 +6,8 @@ ConvAttentionLayer_Decouple and FeedFowardLayer of a module to run on them:
   attention   det3d/models/necks/attention.py:55-124   both read-outs as two query / key heads over one value head
   linear_act  attention.py:36-41 (1x1 value / out convolutions, identity added in the epilogue), :127-146 (feed-forward)
 Gradients are exact formulas of the saved tensors (once differentiable). Both run on the caller's stream, allocate through
-torch's caching allocator only, and can be captured in a HIP graph.
+torch's caching allocator only, and can be captured in a HIP graph; before a backward pass is captured, drop every eager graph of
+the same leaves (torch ties a leaf's gradient accumulation to the stream on which it was first seen).
 """
 import torch
 from torch import nn
