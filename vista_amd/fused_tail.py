@@ -19,17 +19,19 @@ from .dense_tail import ConvAttentionLayer_Decouple, FeedFowardLayer
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_mask, scale):
-        out, stats = ops.attn_fwd(q, k, v, key_mask, scale, want_stats=True)
+        q, k, v, key_mask, geo = ops._attn_args(q, k, v, key_mask)
+        out, stats = ops._attn_fwd_run(q, k, v, key_mask, geo, scale, True)
         ctx.save_for_backward(q, k, v, key_mask, out, stats)
-        ctx.scale = scale
+        ctx.geo, ctx.scale = geo, scale
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, key_mask, out, stats = ctx.saved_tensors
-        grads = ops.attn_bwd(dout, q, k, v, out, stats, key_mask, ctx.scale)
-        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None)
+        # dout has out's shape, dtype and device: the engine sees to that
+        dq, dk, dv = ops._attn_bwd_run(dout, q, k, v, key_mask, ctx.geo, out, stats, ctx.scale)
+        return dq, dk, dv, None, None
 
 
 def attention(q, k, v, key_mask=None, scale=None):

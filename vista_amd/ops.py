@@ -764,7 +764,10 @@ def attn_fwd(q, k, v, key_mask=None, scale=None, want_stats=False):
     Query head i reads key head i // (h / hk) and value head i // (h / hv); key_mask bool [b, sk], True where the key takes part;
     a query without keys gives zeros. scale defaults to d ** -0.5. stats (want_stats) is what attn_bwd needs. Any strides with
     a contiguous last dimension are read in place."""
-    q, k, v, key_mask, geo = _attn_args(q, k, v, key_mask)
+    return _attn_fwd_run(*_attn_args(q, k, v, key_mask), scale, want_stats)
+
+
+def _attn_fwd_run(q, k, v, key_mask, geo, scale, want_stats):
     dev = q.device
     out = torch.empty(geo.out, dtype=q.dtype, device=dev)
     stats = torch.empty(geo.stats, dtype=torch.float32, device=dev) if want_stats else None
@@ -787,6 +790,11 @@ def attn_bwd(dout, q, k, v, out, stats, key_mask=None, scale=None):
     _need_gpu(stats, "stats")
     if stats.dtype != torch.float32 or stats.shape != geo.stats or not stats.is_contiguous() or stats.device != dev:
         raise ValueError("stats must be what attn_fwd(want_stats=True) returned")
+    return _attn_bwd_run(dout, q, k, v, key_mask, geo, out, stats, scale)
+
+
+def _attn_bwd_run(dout, q, k, v, key_mask, geo, out, stats, scale):
+    dev = q.device
     dout = _heads_last(dout)
     dout_strides = (ctypes.c_int64 * 3)(*dout.stride()[:3])
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
