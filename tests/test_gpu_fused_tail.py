@@ -312,6 +312,21 @@ def test_attention_many_queries(shape, dtype, dev):
         within(got, *ref[name], name)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("k_len", [1023, 1025, 2047, 2048, 2049])
+def test_attention_around_the_longest_short_mask(k_len, dtype, dev):
+    """Lists of 1024 keys a sweep; masks of at most 2048 keys are listed by the workgroups that use them."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((2, 270, k_len, 2, 2, 1, 40, 72), dtype, dev, k_len, "some", poison=True)
+    km[0, :], km[0, -1] = False, True                   # the last key alone
+    k[0, -1], v[0, -1] = 0.5, 0.25
+    ref = attn_reference(q, k, v, km, do)
+    out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    within(out, *ref["out"], "out")
+    for name, got in zip(("dq", "dk", "dv"), ops.attn_bwd(do, q, k, v, out, stats, km)):
+        within(got, *ref[name], name)
+
+
 @pytest.mark.parametrize("k_len", [2000, 5001])
 def test_attention_gradients_in_chunks_of_queries(k_len, dev):
     """Many queries: one chunk of several splits (2000 keys), and more probabilities than the workspace holds at once (5001)."""
