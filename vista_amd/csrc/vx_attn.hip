@@ -57,6 +57,8 @@ __device__ __forceinline__ bool attn_key_live(int keys, const uint8_t* mask, int
 // A tile: V(t) travels under S(t), K(t + 1) under O += P V(t); each LDS image is rewritten only after the barrier behind its last
 // reader. IMG: both come as finished images (attn_pack) and go straight to LDS; else (few queries) through registers, where
 // they are split and V is transposed.
+// Two heads of 192 / 384, masked: 4 x 1600 x 480 fp32 46 us (200 workgroups, the matrix pipe and LDS reads in turn: 153 TFLOP/s over all
+// keys), 25600 x 1920 bf16 143 us (790), fp32 475 us (238); 8 heads of 48, 2 x 2037 x 2037 bf16 40 us, bound by the exponentials.
 template <typename T, int DP, int DVP, int RT, int QG, int CS, bool IMG, bool FAST>
 __global__ __launch_bounds__(64 * QG * CS, QG * CS == 8 ? 2 : DVP > 192 || (DVP > 64 && VxType<T>::NPL == 3) ? 1 : 2)
 void attn_fwd(const FwdArgs<T> a) {
@@ -259,7 +261,8 @@ void attn_fwd(const FwdArgs<T> a) {
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int k = 0; k < NK; ++k)
-          s[rt][k] = *reinterpret_cast<const vx_f32x4*>(swap + (((wave & ~1) + k / OWN) * OWN * RT + rt * OWN + k % OWN) * kFragBytes + lane * 16);
+          s[rt][k] = *reinterpret_cast<const vx_f32x4*>(swap + (((wave & ~1) + k / OWN) * OWN * RT + rt * OWN + k % OWN) * kFragBytes +
+                                                        lane * 16);
     }
     VxFrag<NPL> pf[RT][NS];
     if (cur != ~0ull >> (64 - KT)) {           // some keys take no part
@@ -419,7 +422,7 @@ __global__ __launch_bounds__(256) void attn_live(const LiveArgs a) { live_lists(
 // K and V as operand images: per head and tile of KT keys, planes of 1 KB fragments -- K: key block, 32-d step; V^T: column block,
 // 32-key step in the operand order of the keys. A thread makes one lane's 16 bytes of a fragment (all planes). Widths are padded
 // with 0 to the tile's, keys behind the last are 0. It costs one pass over k and v; each tile of queries then saves the split
-// and the transposition.
+// and the transposition. 4 x 480 keys, (2 x 192 + 384) wide, fp32: 8.6 us, bound by V's column reads; 1920 keys bf16 8.7 us.
 // OWN: with a mask of at most kOwnKeys keys every workgroup finds the keys by itself, which saves the launch of attn_live.
 constexpr int kOwnKeys = 2048;
 template <typename T, bool OWN>
@@ -481,7 +484,8 @@ __global__ __launch_bounds__(256) void attn_pack(const AttnArgs<T> a, const Live
 }
 
 // joins the splits of a row: weights 2^(m_s - m). A workgroup has 256 / J quads of output values, J lanes each: lane j adds the
-// splits j, j + J, ..., four of them in flight (few rows: what counts is latency), then the J sums are added in order.
+// splits j, j + J, ..., four of them in flight (few rows: what counts is latency), then the J sums are added in order. 2 rows of 15
+// splits of 384: 4.0 us, of which the launch is most.
 template <typename T, int J>
 __global__ __launch_bounds__(256) void attn_join(const FwdArgs<T> a, long long items, int quads) {
   constexpr int U = 4, Q = 256 / J;
@@ -605,7 +609,7 @@ struct VxPick<false, X, Y> {
 
 // delta = sum_n go * out per query: one wave per row. With a mask the first `head` workgroups make its lists; OWN (at most kOwnKeys keys):
 // they gather the keys as well, each with a list of its own, which saves a launch (a step of 4 x 1600 x 480, 2 heads of 192 / 384, fp32:
-// 187 -> 182 us). One read of go and out: 4 x 2 x 1600 x 384 fp32 39 MB 9 us, 2 x 25600 x 384 157 MB 27 us (5.8 TB/s)
+// 187 -> 182 us). One read of go and out: 4 x 2 x 1600 x 384 fp32 39 MB 11 us with the gather, 2 x 25600 x 384 157 MB 28 us
 template <typename T, bool OWN>
 __global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long rows, const LiveArgs live, const GatherArgs gather,
                                                   unsigned head) {
@@ -642,7 +646,10 @@ constexpr int kPdsN = 128;                   // keys of an attn_pds tile
 // P and dS of a TM-query x TN-key tile: scores and dP = go v^T are two products with one epilogue,
 // P = 2^(scale2 s - max) / sum, dS = scale P (dP - delta).
 // ONE: all keys are in the tile. delta is then the tile's own sum of P dP, and both go out in fp32: over few keys the rounding of a
-// bf16 output inside delta and of P and dS to bf16 would not average out (2^-9 each of terms that nearly cancel).
+// bf16 output inside delta and of P and dS to bf16 would not average out (2^-9 each of terms that nearly cancel): relative 2-norm of
+// dq and dk over 16 keys 0.0025 so, 0.0020 with fp32, 0.0017 their own rounding.
+// Bound by the split into planes and LDS reads in fp32: 4 x 2 x 1600 x 480, 192 / 384 57 us, 25600 x 1920 483 us; bf16 3 x 4 x 777 x 301,
+// 96 / 192 10.7 us, where 468 workgroups of 64 x 128 are two rounds.
 template <typename T, bool ONE>
 using AttnProb = typename VxPick<ONE, float, T>::type;
 template <typename T, int TM, int TN, bool FAST, bool ONE>
@@ -724,6 +731,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) 
 // the three gradients of a chunk in one launch: dV slabs = P^T go, dK slabs = dS^T q (reduction over the queries of a split),
 // dQ = dS k (reduction over the keys)
 // ONE: P and dS are fp32; beside bf16 operands they are two planes
+// 4 x 2 x 1600 x 480, 192 / 384 fp32 66 us, 25600 x 1920 565 us: as attn_pds; dV and dK read both operands along their rows, transposed
+// on the way to LDS. bf16 3 x 4 x 777 x 301, 96 / 192 11.2 us
 template <typename T, int TM, int TN, bool FAST, bool ONE>
 __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a) {
   using P = AttnProb<T, ONE>;
@@ -762,7 +771,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
     const int rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = a.d - n0 < TN ? a.d - n0 : TN;
     const VxOperand<P> X{(const P*)a.ds + ((long long)bh * a.rows + m0) * a.skp, a.skp, rows_m};
     const VxOperand<T> W{a.k + b * a.k_b + (h / a.gk) * a.k_h + n0, a.k_s, rows_n};
-    vx_gemm_loop<T, KC, KS, TM, TN, FAST, BK, P, PX>(X, W, 0, a.count ? a.count[b] : a.sk, lds, acc);   // dS is 0 from there to its tile's end
+    const int keys = a.count ? a.count[b] : a.sk;    // dS is 0 from there to its tile's end
+    vx_gemm_loop<T, KC, KS, TM, TN, FAST, BK, P, PX>(X, W, 0, keys, lds, acc);
     vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
       if (m < rows_m && n < rows_n)
         vx_store8(a.dq + (((long long)b * a.sq + a.q0 + m0 + m) * a.h + h) * a.d + n0 + n, v, w, rows_n - n);
@@ -770,7 +780,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
   }
 }
 
-// dk, dv = sums of the slabs over a head's query heads and the splits, in that order; masked keys get zeros
+// dk, dv = sums of the slabs over a head's query heads and the splits, in that order; masked keys get zeros. One read of the slabs:
+// 4 x 480 keys of 2 x 192 and 384, 10.6 us
 template <typename T>
 __global__ __launch_bounds__(256) void attn_slab_sum(const BwdArgs<T> a, int splits, unsigned blocks_v, long long items_v,
                                                      long long items_k) {
@@ -1030,7 +1041,9 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
 
 template <typename T, bool FAST>
 int32_t bwd_chunk(const BwdArgs<T>& a, const BwdPlan& p, unsigned pds, unsigned grads, hipStream_t s) {
-  const auto probs = p.one ? attn_pds<T, 64, kPdsN, FAST, true> : p.tp == 128 ? attn_pds<T, 128, kPdsN, FAST, false> : attn_pds<T, 64, kPdsN, FAST, false>;
+  const auto probs = p.one          ? attn_pds<T, 64, kPdsN, FAST, true>
+                     : p.tp == 128 ? attn_pds<T, 128, kPdsN, FAST, false>
+                                   : attn_pds<T, 64, kPdsN, FAST, false>;
   probs<<<pds, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
   const auto sums = p.one ? attn_grads<T, 64, 64, FAST, true>
