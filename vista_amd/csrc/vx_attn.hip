@@ -1001,7 +1001,7 @@ struct BwdPlan {
   size_t total() const { return delta + 2 * pds + slab_k + slab_v + live + kc + vc; }
 };
 // queries are cut into splits (one slab each) and the splits into chunks, whose probabilities and score gradients are in
-// memory at a time (at most kChunkBytes of both)
+// memory at a time (at most kChunkBytes of both, but a tile of queries of every head at least)
 constexpr size_t kChunkBytes = (size_t)1 << 30;
 BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   BwdPlan p;

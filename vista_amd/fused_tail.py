@@ -145,7 +145,8 @@ class FusedFeedForward(nn.Module):
 def fuse_cross_attention(module):
     """Rewrite `module` in place: every ConvAttentionLayer_Decouple and FeedFowardLayer in it runs on the fused kernels
     (inference and training; HIP tensors only from then on, unless attention maps are asked for). Parameters, buffers and
-    state_dict keys are unchanged. Returns `module`, or its replacement when it is such a layer itself."""
+    state_dict keys are unchanged; hooks on a rewritten layer are not carried over. Returns `module`, or its replacement when it
+    is such a layer itself."""
     swap = {ConvAttentionLayer_Decouple: FusedConvAttention, FeedFowardLayer: FusedFeedForward}
     if type(module) in swap:
         return swap[type(module)](module).train(module.training)
