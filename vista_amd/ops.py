@@ -672,8 +672,8 @@ def linear_fwd(x, weight, bias=None, residual=None, act="none", want_pre=False):
             raise ValueError(f"residual must be [{m}, {n}], got {tuple(residual.shape)}")
         residual = _rows(residual)
         ldr = residual.stride(0)
-    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    pre = torch.empty_like(y) if want_pre else None
+    y = x.new_empty((m, n))
+    pre = x.new_empty((m, n)) if want_pre else None
     rc = _launch(x.device, L.lib().vx_linear_fwd, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), _at(bias),
                  _at(residual), ldr, m, n, k, code, y.data_ptr(), _at(pre), _DT[x.dtype])
     if rc:
@@ -696,10 +696,10 @@ def linear_bwd(dy, x, weight, act="none", saved=None, want_dx=True, want_dw=True
         saved = saved.contiguous()
     x, weight, g = _rows(x), _rows(weight), _rows(dy)
     dev, dt = x.device, x.dtype
-    dpre = torch.empty((m, n), dtype=dt, device=dev) if code else dy
-    dx = torch.empty((m, k), dtype=dt, device=dev) if want_dx else None
-    dw = torch.empty((n, k), dtype=dt, device=dev) if want_dw else None
-    db = torch.empty((n,), dtype=dt, device=dev) if want_dbias else None
+    dpre = x.new_empty((m, n)) if code else dy
+    dx = x.new_empty((m, k)) if want_dx else None
+    dw = x.new_empty((n, k)) if want_dw else None
+    db = x.new_empty((n,)) if want_dbias else None
     wsb = _linear_bwd_bytes(dev.index, m, n, k, _DT[dt])
     ws = _ws(wsb, dev)
     rc = _launch(dev, L.lib().vx_linear_bwd, g.data_ptr(), g.stride(0), x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0),
@@ -769,7 +769,7 @@ def attn_fwd(q, k, v, key_mask=None, scale=None, want_stats=False):
 
 def _attn_fwd_run(q, k, v, key_mask, geo, scale, want_stats):
     dev = q.device
-    out = torch.empty(geo.out, dtype=q.dtype, device=dev)
+    out = q.new_empty(geo.out)
     stats = torch.empty(geo.stats, dtype=torch.float32, device=dev) if want_stats else None
     ws = _ws(geo.fwd_bytes, dev) if geo.fwd_bytes else None
     rc = _launch(dev, L.lib().vx_attn_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(key_mask), geo.shape, geo.strides,
@@ -797,7 +797,7 @@ def _attn_bwd_run(dout, q, k, v, key_mask, geo, out, stats, scale):
     dev = q.device
     dout = _heads_last(dout)
     dout_strides = (ctypes.c_int64 * 3)(*dout.stride()[:3])
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+    dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
     ws = _ws(geo.bwd_bytes, dev)
     rc = _launch(dev, L.lib().vx_attn_bwd, dout.data_ptr(), dout_strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(key_mask),
                  geo.shape, geo.strides, out.data_ptr(), stats.data_ptr(), geo.scale if scale is None else float(scale), dq.data_ptr(),
