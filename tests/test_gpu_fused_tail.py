@@ -532,6 +532,62 @@ def test_captured_and_replayed(dev):
             assert all(torch.equal(a, b) for a, b in zip(held, want)), i
 
 
+def test_captured_training_step(dev):
+    """Attention into a layer, differentiated by autograd inside a capture, on leaves that no eager graph knows; replays on new inputs
+    between eager steps on copies of the leaves."""
+    from vista_amd.fused_tail import attention, linear_act
+    q, k, v, km, _ = make_attn((2, 70, 150, 2, 2, 1, 24, 48), F32, dev, 3, "some")
+    _, w, b, _, dy = make_linear(140, 96, 64, F32, dev, 4, True, False)
+
+    def step(q, k, v, w, b):
+        leaves = [t.requires_grad_(True) for t in (q, k, v, w, b)]
+        y = linear_act(attention(q, k, v, km).view(140, 96), w, b, act="silu")
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    inputs = [t.detach() for t in (q, k, v, w, b)]
+    eager = lambda: [t.clone() for t in step(*(i.detach().clone() for i in inputs))]  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        held = step(*(i.detach() for i in inputs))
+    gen = torch.Generator(device=dev).manual_seed(78)
+    for i in range(4):
+        for t in (*inputs, dy):
+            t.copy_(torch.randn(t.shape, generator=gen, device=dev))
+        want = eager()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), i
+
+
+def test_two_streams_at_once(dev):
+    """The same operands on two streams whose work overlaps: no call shares a workspace with another."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((2, 500, 300, 2, 2, 1, 96, 192), BF16, dev, 5, "some")
+    x, w, _, s, dy = make_linear(3000, 128, 96, BF16, dev, 6, False, True)
+
+    def step():
+        out, st = ops.attn_fwd(q, k, v, km, want_stats=True)
+        return (out, *ops.attn_bwd(do, q, k, v, out, st, km), *ops.linear_bwd(dy, x, w, "relu", s))
+
+    want = step()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(8):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for r in got for a, b in zip(r, want))
+
+
 # ------------------------------------------------------------------------------------------------ the block
 def block(dev, heads=1):
     from vista_amd import dense_tail as dt
