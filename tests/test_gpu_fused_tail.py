@@ -312,6 +312,34 @@ def test_attention_many_queries(shape, dtype, dev):
         within(got, *ref[name], name)
 
 
+def stale(*sizes, dev):
+    """Leaves NaN in the memory that the next tensors of these sizes get: a row that a kernel does not write shows."""
+    held = [torch.full((n,), math.nan, dtype=F32, device=dev) for n in sizes for _ in range(4)]
+    del held
+
+
+# batch x heads x query tiles enough for the 128-query form, but few queries of each
+ATTN_MANY_SHORT = [(64, 100, 20, 8, 8, 8, 64, 64), (16, 512, 33, 8, 8, 8, 48, 48), (128, 128, 20, 2, 2, 1, 192, 384),
+                   (6, 500, 40, 6, 6, 6, 150, 300), (90, 65, 17, 8, 4, 2, 24, 30), (70, 257, 21, 8, 8, 8, 33, 65), (130, 256, 9, 4, 4, 4, 96, 128),
+                   (128, 320, 30, 2, 2, 1, 190, 380)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("mask", ["none", "blank"])
+@pytest.mark.parametrize("shape", ATTN_MANY_SHORT)
+def test_attention_of_many_short_sequences_writes_every_row(shape, mask, dtype, dev):
+    """Many heads of 65 to 512 queries each: every row of out and stats is written, whatever tile the launch takes."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn(shape, dtype, dev, sum(shape), mask, poison=True)
+    ref = attn_reference(q, k, v, km, do)
+    stale(ref["out"][0].numel() * q.element_size() // 4, shape[0] * shape[3] * shape[1] * 2, dev=dev)
+    out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    within(out, *ref["out"], "out")
+    assert not torch.isnan(stats).any()
+    for name, got in zip(("dq", "dk", "dv"), ops.attn_bwd(do, q, k, v, out, stats, km)):
+        within(got, *ref[name], name)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("k_len", [1023, 1025, 2047, 2048, 2049])
 def test_attention_around_the_longest_short_mask(k_len, dtype, dev):

@@ -897,7 +897,12 @@ FwdPlan fwd_plan(const Shape& s, int32_t dtype) {
   // one wave a SIMD) and is not built.
   const int64_t n128 = vx_cdiv(s.sq, 128) * bh, n64 = vx_cdiv(s.sq, 64) * bh;
   const int c = class_of(s.d, s.dv);
-  if (c == kClasses - 1)
+  // images pay from about five tiles of 64 queries on; us with / without, 480 and 4096 keys, 4 x 2 heads of 192 / 384 fp32: 64 queries
+  // 31 / 25, 58 / 42; 256 32 / 34, 93 / 92; 512 38 / 44, 145 / 164; 2 x 8 heads of 64 / 64 bf16: 64 13 / 10, 23 / 15; 512 16 / 14, 49 / 48
+  p.img = vx_cdiv(s.sq, 64) > 4;
+  if (!p.img)                // the form without images has 64 queries a workgroup, however many heads there are
+    p.many = false;
+  else if (c == kClasses - 1)
     p.many = 1.45 * vx_cdiv(n128, cus) < vx_cdiv(n64, cus);
   else
     p.many = n128 >= 2 * cus && !(dtype == VX_F32 && c >= kWideF32);
@@ -909,9 +914,6 @@ FwdPlan fwd_plan(const Shape& s, int32_t dtype) {
   p.span = tiles_k ? vx_cdiv(tiles_k, splits) : 1;
   p.splits = tiles_k ? vx_cdiv(tiles_k, p.span) : 1;
   p.tiles_k = tiles_k;
-  // images pay from about five tiles of queries on; us with / without, 480 and 4096 keys, 4 x 2 heads of 192 / 384 fp32: 64 queries
-  // 31 / 25, 58 / 42; 256 32 / 34, 93 / 92; 512 38 / 44, 145 / 164; 2 x 8 heads of 64 / 64 bf16: 64 13 / 10, 23 / 15; 512 16 / 14, 49 / 48
-  p.img = p.tiles_q > 4;
   const size_t row = dtype == VX_F32 ? 6 : 2;      // bytes of a value's planes
   p.k_img = p.img ? (size_t)s.b * s.hk * tiles_k * kt * kDims[c][0] * row : 0;
   p.v_img = p.img ? (size_t)s.b * s.hv * tiles_k * kt * kDims[c][1] * row : 0;
@@ -924,14 +926,21 @@ size_t fwd_bytes(const Shape& s, int32_t dtype) {
   return p.k_img + p.v_img + p.live + vx_align(rows * s.dv * 4) + vx_align(rows * 8);
 }
 
+// refuses a plan whose tiles are not those of the launched form: rows would stay unwritten
+int32_t covers(int64_t tiles, int64_t rows, int64_t sq) {
+  VX_REQUIRE(tiles * rows >= sq && (tiles - 1) * rows < sq, "attn_fwd: %lld tiles of %lld queries for %lld", (long long)tiles,
+             (long long)rows, (long long)sq);
+  return VX_OK;
+}
 template <typename T, int C>
-void launch_fwd(const FwdArgs<T>& a, const FwdPlan& p, unsigned grid, hipStream_t s) {
+int32_t launch_fwd(const FwdArgs<T>& a, const FwdPlan& p, unsigned grid, hipStream_t s) {
   constexpr int DP = kDims[C][0], DVP = kDims[C][1];
   constexpr bool WIDE = C == kClasses - 1, F32 = sizeof(T) == 4, MANY = WIDE || !F32 || C < kWideF32;
   constexpr int RT = 1, QG = 4, CS = WIDE ? 2 : 1;       // 64 queries; wide heads: two waves a query group
   // 128 queries: 32 a wave, but 16 and twice the waves for wide fp32 heads, whose registers hold no more
   constexpr int RT2 = WIDE && F32 ? 1 : 2, QG2 = WIDE && F32 ? 8 : 4, CS2 = WIDE && F32 ? 1 : CS;
-  if (p.img && p.many) {
+  if (int32_t rc = covers(p.tiles_q, MANY && p.img && p.many ? 16 * RT2 * QG2 : 16 * RT * QG, a.sq)) return rc;
+  if (MANY && p.img && p.many) {
     if constexpr (MANY) attn_fwd<T, DP, DVP, RT2, QG2, CS2, true, false><<<grid, 64 * QG2 * CS2, 0, s>>>(a);
   } else if (p.img) {
     attn_fwd<T, DP, DVP, RT, QG, CS, true, false><<<grid, 64 * QG * CS, 0, s>>>(a);
@@ -939,6 +948,8 @@ void launch_fwd(const FwdArgs<T>& a, const FwdPlan& p, unsigned grid, hipStream_
     const auto kernel = args_fast(a) ? attn_fwd<T, DP, DVP, RT, QG, CS, false, true> : attn_fwd<T, DP, DVP, RT, QG, CS, false, false>;
     kernel<<<grid, 64 * CS * QG, 0, s>>>(a);
   }
+  VX_LAUNCH_CHECK();
+  return VX_OK;
 }
 
 template <typename T>
@@ -973,15 +984,16 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
     pack<<<(unsigned)(per * sh.b), 256, 0, s>>>(a, live, ws, ws + p.k_img, (int)p.tiles_k, kd, nv, ks, all, (unsigned)per);
     VX_LAUNCH_CHECK();
   }
+  int32_t rc;
   switch (class_of(sh.d, sh.dv)) {
-    case 0: launch_fwd<T, 0>(a, p, (unsigned)grid, s); break;
-    case 1: launch_fwd<T, 1>(a, p, (unsigned)grid, s); break;
-    case 2: launch_fwd<T, 2>(a, p, (unsigned)grid, s); break;
-    case 3: launch_fwd<T, 3>(a, p, (unsigned)grid, s); break;
-    case 4: launch_fwd<T, 4>(a, p, (unsigned)grid, s); break;
-    default: launch_fwd<T, 5>(a, p, (unsigned)grid, s); break;
+    case 0: rc = launch_fwd<T, 0>(a, p, (unsigned)grid, s); break;
+    case 1: rc = launch_fwd<T, 1>(a, p, (unsigned)grid, s); break;
+    case 2: rc = launch_fwd<T, 2>(a, p, (unsigned)grid, s); break;
+    case 3: rc = launch_fwd<T, 3>(a, p, (unsigned)grid, s); break;
+    case 4: rc = launch_fwd<T, 4>(a, p, (unsigned)grid, s); break;
+    default: rc = launch_fwd<T, 5>(a, p, (unsigned)grid, s); break;
   }
-  VX_LAUNCH_CHECK();
+  if (rc) return rc;
   if (p.splits > 1) {
     const int quads = (a.dv + 3) / 4;
     const int64_t items = bh * sh.sq * quads;
