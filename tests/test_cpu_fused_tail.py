@@ -104,3 +104,42 @@ def test_fuse_cross_attention_keeps_keys_and_parameters():
     assert [type(c).__name__ for c in m.modules()] == kinds
     ffn = fused_tail.fuse_cross_attention(dense_tail.FeedFowardLayer(8, 16).eval())
     assert isinstance(ffn, fused_tail.FusedFeedForward) and not ffn.training
+
+
+def entry_points():
+    t = lambda *s: torch.randn(s)  # noqa: E731
+    q, k, v, st = t(1, 2, 1, 4), t(1, 2, 1, 4), t(1, 2, 1, 4), t(1, 2, 2)
+    x, w, dy = t(2, 3), t(4, 3), t(2, 4)
+    return [(fused_tail.attention, (q, k, v)), (ops.attn_fwd, (q, k, v)), (ops.attn_bwd, (q, q, k, v, q, st)),
+            (fused_tail.linear_act, (x, w)), (ops.linear_fwd, (x, w)), (ops.linear_bwd, (dy, x, w))]
+
+
+@pytest.mark.parametrize("at", range(6))
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_recording_is_refused(at, grad):
+    """A trace would keep the allocation of the output and lose the launch: uninitialised memory."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, args = entry_points()[at]
+    with torch.set_grad_enabled(grad):
+        with pytest.raises(_lib.VxError, match="traced"):
+            torch.jit.trace(lambda *a: f(*a), args, check_trace=False)
+        with pytest.raises(_lib.VxError, match="traced"):
+            make_fx(lambda *a: f(*a))(*args)
+    with pytest.raises(_lib.VxError, match="CUDA"):          # outside of one: no CPU path, as ever
+        f(*args)
+
+
+@pytest.mark.parametrize("at", range(6))
+@pytest.mark.parametrize("arg", [0, 1])
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_tangent_is_refused(at, arg, grad):
+    """Forward-mode derivatives: with no input that requires gradients the output came without a tangent."""
+    from torch.autograd import forward_ad
+    f, args = entry_points()[at]
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        dual = list(args)
+        dual[arg] = forward_ad.make_dual(args[arg], torch.ones_like(args[arg]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            f(*dual)
+        with pytest.raises(_lib.VxError, match="CUDA"):
+            f(*args)

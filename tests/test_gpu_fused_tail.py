@@ -616,6 +616,23 @@ def test_two_streams_at_once(dev):
     assert all(torch.equal(a, b) for r in got for a, b in zip(r, want))
 
 
+def test_forward_over_reverse_and_compiled_callers(dev):
+    """A tangent that reaches the backward pass is refused; a compiled caller runs the same kernels (or refuses, but never returns
+    unwritten memory)."""
+    from torch.autograd import forward_ad
+    from vista_amd.fused_tail import attention, linear_act
+    q, k, v, km, do = make_attn((2, 40, 30, 2, 2, 1, 16, 32), F32, dev, 1, "some")
+    x, w, b, r, dy = make_linear(20, 16, 24, F32, dev, 1, True, True)
+    for f, args, cot in ((lambda *a: attention(*a, key_mask=km), (q, k, v), do), (linear_act, (x, w, b, r), dy)):
+        leaves = [a.clone().requires_grad_(True) for a in args]
+        out = f(*leaves)
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+            torch.autograd.grad(out, leaves, forward_ad.make_dual(cot, torch.ones_like(cot)))
+        with torch.no_grad():
+            want = f(*args) * 2
+            assert torch.equal(torch.compile(lambda *a: f(*a) * 2, backend="eager")(*args), want)
+
+
 # ------------------------------------------------------------------------------------------------ the block
 def block(dev, heads=1):
     from vista_amd import dense_tail as dt

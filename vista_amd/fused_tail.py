@@ -29,7 +29,7 @@ class _AttentionFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, key_mask, out, stats = ctx.saved_tensors
-        # dout has out's shape, dtype and device: the engine sees to that
+        ops._check_seen(dout)        # (out's shape, dtype and device: the engine sees to that)
         dq, dk, dv = ops._attn_bwd_run(dout, q, k, v, key_mask, ctx.geo, out, stats, ctx.scale)
         return dq, dk, dv, None, None
 

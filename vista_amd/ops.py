@@ -8,6 +8,7 @@ import functools
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -612,8 +613,22 @@ def _launch(dev, fn, *args):
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def _check_seen(*tensors):
+    """torch sees these launches through autograd alone. Refused is what would lose them without a word: a recording of torch calls
+    (torch.jit.trace, make_fx), which keeps the empty output, and forward-mode derivatives, whose tangent ends here."""
+    recorded = torch.jit.is_tracing()
+    if torch._C._len_torch_dispatch_stack():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        recorded = recorded or get_proxy_mode() is not None
+    if recorded:
+        raise L.VxError("libvx launches cannot be traced: the recorded program would return memory that nothing writes")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors if t is not None):
+        raise NotImplementedError("forward-mode derivatives are not implemented: the output would have no tangent")
+
+
 def _check_tensors(first, name, others, names):
     """`first` is a float32 / bfloat16 HIP tensor; the `others` (None: absent) share its device and dtype."""
+    _check_seen(first, *others)
     _need_gpu(first, name)
     dtype, device = first.dtype, first.device
     if dtype not in _DT:
@@ -782,6 +797,7 @@ def _attn_fwd_run(q, k, v, key_mask, geo, scale, want_stats):
 def attn_bwd(dout, q, k, v, out, stats, key_mask=None, scale=None):
     """Gradients of attn_fwd from its own out and stats -> (dq, dk, dv), shaped as q, k and v; the probabilities are recomputed.
     Gradients of masked keys are 0."""
+    _check_seen(dout)
     q, k, v, key_mask, geo = _attn_args(q, k, v, key_mask)
     _check_tensors(q, "q", (dout, out), ("dout", "out"))
     dev = q.device
