@@ -143,3 +143,50 @@ def test_a_tangent_is_refused(at, arg, grad):
             f(*dual)
         with pytest.raises(_lib.VxError, match="CUDA"):
             f(*args)
+
+
+def layers():
+    torch.manual_seed(0)
+    return dense_tail.ConvAttentionLayer_Decouple(16, 2), dense_tail.FeedFowardLayer(16, 24)
+
+
+DIRECT = [(0, "v_conv"), (0, "out_sem_conv"), (0, "out_geo_conv"), (1, "linear1"), (1, "linear2"), (1, "activation")]
+
+
+@pytest.mark.parametrize("kind", ["register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook",
+                                  "register_full_backward_pre_hook"])
+@pytest.mark.parametrize("which,child", DIRECT + [(0, None), (1, None)])
+def test_fusing_refuses_hooks(which, child, kind):
+    both = torch.nn.ModuleList(layers())
+    m = both[which] if child is None else getattr(both[which], child)
+    handle = getattr(m, kind)(lambda *a: None)
+    with pytest.raises(ValueError, match="hooks"):
+        fused_tail.fuse_cross_attention(both)
+    assert [type(c) for c in both] == [dense_tail.ConvAttentionLayer_Decouple, dense_tail.FeedFowardLayer]      # nothing changed
+    handle.remove()
+    both[0].q_sem_conv.register_forward_hook(lambda *a: None)       # called as ever: no reason to refuse
+    both[1].norm.register_forward_hook(lambda *a: None)
+    fused_tail.fuse_cross_attention(both)
+    assert [type(c) for c in both] == [fused_tail.FusedConvAttention, fused_tail.FusedFeedForward]
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("which,child", DIRECT[:5])
+def test_weights_made_in_a_hook_are_never_stale(which, child):
+    """weight_norm makes the weight in a forward pre-hook. Refused when it is there before; when it comes later the layer's own forward
+    runs (on the CPU here), with the weight of the present weight_g."""
+    x = torch.randn(2, 16, 3, 4) if which == 0 else torch.randn(12, 2, 16)
+    call = (lambda m: m(x, x, x, need_maps=False)[0]) if which == 0 else (lambda m: [m(x)])
+    stock, plain = layers()[which], layers()[which]
+    fused = fused_tail.fuse_cross_attention(layers()[which])
+    for m in (stock, fused, plain):
+        torch.nn.utils.weight_norm(getattr(m, child))
+    with pytest.raises(ValueError, match="hooks"):
+        fused_tail.fuse_cross_attention(plain)
+    for m in (stock, fused):
+        with torch.no_grad():
+            getattr(m, child).weight_g.mul_(1.7)
+    assert all(torch.equal(a, b) for a, b in zip(call(stock), call(fused)))
+    if which == 0:
+        with pytest.raises(ValueError, match="key_mask"):
+            fused(x, x, x, need_maps=False, key_mask=torch.ones(2, 12, dtype=torch.bool))

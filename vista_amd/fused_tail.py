@@ -76,6 +76,10 @@ def linear_act(x, weight, bias=None, residual=None, act="none"):
     return y.view(*x.shape[:-1], weight.shape[0])
 
 
+def _hooked(module):
+    return bool(module._forward_pre_hooks or module._forward_hooks or module._backward_pre_hooks or module._backward_hooks)
+
+
 def _conv1x1(conv, x, residual=None):
     """A 1x1 nn.Conv2d over tokens [..., c] instead of a map [b, c, h, w]."""
     return linear_act(x, conv.weight.flatten(1), conv.bias, residual)
@@ -83,7 +87,10 @@ def _conv1x1(conv, x, residual=None):
 
 class FusedConvAttention(nn.Module):
     """ConvAttentionLayer_Decouple on `attention` and `linear_act`; shares the layer's submodules, so parameters and
-    state_dict keys are the layer's. The attention maps are not formed: need_maps=True runs the layer's own forward."""
+    state_dict keys are the layer's. The attention maps are not formed: need_maps=True runs the layer's own forward, and so do hooks on
+    a submodule of `direct`, whose weight is read without a call of it (weight_norm, prune and the like make the weight in a hook)."""
+
+    direct = ("v_conv", "out_sem_conv", "out_geo_conv")
 
     def __init__(self, layer):
         super().__init__()
@@ -93,10 +100,11 @@ class FusedConvAttention(nn.Module):
 
     def forward(self, query, key, value, q_pos_emb=None, k_pos_emb=None, need_maps=True, key_mask=None):
         """-> ([tokens[HW_q, B, C]] x2, [None, None]); key_mask bool [B, HW_kv], True where the key block takes part."""
-        if need_maps:
+        if need_maps or any(_hooked(self._modules[name]) for name in self.direct):
             if key_mask is not None:
-                raise ValueError("key_mask is supported without attention maps only (need_maps=False)")
-            return ConvAttentionLayer_Decouple.forward(self, query, key, value, q_pos_emb, k_pos_emb, True)
+                raise ValueError("key_mask is supported without attention maps (need_maps=False) and without hooks on "
+                                 f"{', '.join(self.direct)} only")
+            return ConvAttentionLayer_Decouple.forward(self, query, key, value, q_pos_emb, k_pos_emb, need_maps)
         identity = query
         if q_pos_emb is not None:
             query = query + q_pos_emb
@@ -127,7 +135,10 @@ class FusedConvAttention(nn.Module):
 
 
 class FusedFeedForward(nn.Module):
-    """FeedFowardLayer on `linear_act`: ReLU in the first product's epilogue, the residual in the second's."""
+    """FeedFowardLayer on `linear_act`: ReLU in the first product's epilogue, the residual in the second's. Hooks on a submodule of
+    `direct`: the layer's own forward, which calls them."""
+
+    direct = ("linear1", "linear2", "activation")
 
     def __init__(self, layer):
         super().__init__()
@@ -135,6 +146,8 @@ class FusedFeedForward(nn.Module):
             self.add_module(name, child)
 
     def forward(self, view):
+        if any(_hooked(self._modules[name]) for name in self.direct):
+            return FeedFowardLayer.forward(self, view)
         flip = view.dim() == 3 and not view.is_contiguous()     # FusedConvAttention's tokens: rows in memory order
         x = view.transpose(0, 1) if flip else view
         h = linear_act(x, self.linear1.weight, self.linear1.bias, act="relu")
@@ -142,15 +155,27 @@ class FusedFeedForward(nn.Module):
         return y.transpose(0, 1) if flip else y
 
 
+_SWAP = {ConvAttentionLayer_Decouple: FusedConvAttention, FeedFowardLayer: FusedFeedForward}
+
+
 def fuse_cross_attention(module):
     """Rewrite `module` in place: every ConvAttentionLayer_Decouple and FeedFowardLayer in it runs on the fused kernels
     (inference and training; HIP tensors only from then on, unless attention maps are asked for). Parameters, buffers and
-    state_dict keys are unchanged; hooks on a rewritten layer are not carried over. Returns `module`, or its replacement when it
-    is such a layer itself."""
-    swap = {ConvAttentionLayer_Decouple: FusedConvAttention, FeedFowardLayer: FusedFeedForward}
-    if type(module) in swap:
-        return swap[type(module)](module).train(module.training)
+    state_dict keys are unchanged. A layer with hooks, or with hooks on a submodule that the fused form does not call, is refused before
+    anything is changed; hooks that such a submodule gets later run the layer's own forward. Returns `module`, or its replacement
+    when it is such a layer itself."""
+    for name, layer in module.named_modules():
+        if type(layer) in _SWAP:
+            for at, m in [("", layer)] + [("." + c, layer._modules[c]) for c in _SWAP[type(layer)].direct]:
+                if _hooked(m):
+                    raise ValueError(f"{name or type(layer).__name__}{at} has hooks, which the fused layer would not call")
+    return _rewrite(module)
+
+
+def _rewrite(module):
+    if type(module) in _SWAP:
+        return _SWAP[type(module)](module).train(module.training)
     for name, child in list(module._modules.items()):
         if child is not None:
-            module._modules[name] = fuse_cross_attention(child)
+            module._modules[name] = _rewrite(child)
     return module
