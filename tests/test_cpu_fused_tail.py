@@ -190,3 +190,24 @@ def test_weights_made_in_a_hook_are_never_stale(which, child):
     if which == 0:
         with pytest.raises(ValueError, match="key_mask"):
             fused(x, x, x, need_maps=False, key_mask=torch.ones(2, 12, dtype=torch.bool))
+
+
+def test_fusing_keeps_what_a_layer_holds():
+    """Training flags of single submodules, submodules under two names, parameters and buffers of the layer itself, attributes, and a
+    layer that stands in two places."""
+    att, ffn = layers()
+    att.geo_norm = att.sem_norm
+    att.out_sem_conv.eval()
+    att.register_parameter("gain", torch.nn.Parameter(torch.ones(3)))
+    att.register_buffer("seen", torch.zeros(2))
+    att.note = "kept"
+    net = torch.nn.ModuleList([att, ffn, torch.nn.Sequential(ffn)])
+    keys, flags = list(net.state_dict()), {n: m.training for n, m in net.named_modules()}
+    ids = {n: id(p) for n, p in net.named_parameters()}
+    fused_tail.fuse_cross_attention(net)
+    assert type(net[0]) is fused_tail.FusedConvAttention and type(net[1]) is fused_tail.FusedFeedForward
+    assert list(net.state_dict()) == keys and {n: m.training for n, m in net.named_modules()} == flags
+    assert {n: id(p) for n, p in net.named_parameters()} == ids
+    assert net[0].geo_norm is net[0].sem_norm and net[0].note == "kept" and net[1] is net[2][0]
+    net[0].extra = torch.nn.Identity()                      # what the replacement gets later is its own
+    assert "extra" not in att._modules

@@ -80,6 +80,12 @@ def _hooked(module):
     return bool(module._forward_pre_hooks or module._forward_hooks or module._backward_pre_hooks or module._backward_hooks)
 
 
+def _become(module, layer):
+    """All that `layer` holds -- submodules (one that stands under two names too), parameters and buffers of its own, training flags,
+    attributes -- in containers of `module`'s own."""
+    module.__dict__.update((k, v.copy() if isinstance(v, (dict, set)) else v) for k, v in layer.__dict__.items())
+
+
 def _conv1x1(conv, x, residual=None):
     """A 1x1 nn.Conv2d over tokens [..., c] instead of a map [b, c, h, w]."""
     return linear_act(x, conv.weight.flatten(1), conv.bias, residual)
@@ -93,10 +99,7 @@ class FusedConvAttention(nn.Module):
     direct = ("v_conv", "out_sem_conv", "out_geo_conv")
 
     def __init__(self, layer):
-        super().__init__()
-        for name, child in layer.named_children():
-            self.add_module(name, child)
-        self.channels, self.numhead, self.head_dim = layer.channels, layer.numhead, layer.head_dim
+        _become(self, layer)
 
     def forward(self, query, key, value, q_pos_emb=None, k_pos_emb=None, need_maps=True, key_mask=None):
         """-> ([tokens[HW_q, B, C]] x2, [None, None]); key_mask bool [B, HW_kv], True where the key block takes part."""
@@ -141,9 +144,7 @@ class FusedFeedForward(nn.Module):
     direct = ("linear1", "linear2", "activation")
 
     def __init__(self, layer):
-        super().__init__()
-        for name, child in layer.named_children():
-            self.add_module(name, child)
+        _become(self, layer)
 
     def forward(self, view):
         if any(_hooked(self._modules[name]) for name in self.direct):
@@ -169,13 +170,16 @@ def fuse_cross_attention(module):
             for at, m in [("", layer)] + [("." + c, layer._modules[c]) for c in _SWAP[type(layer)].direct]:
                 if _hooked(m):
                     raise ValueError(f"{name or type(layer).__name__}{at} has hooks, which the fused layer would not call")
-    return _rewrite(module)
+    return _rewrite(module, {})
 
 
-def _rewrite(module):
+def _rewrite(module, done):
+    """`done`: layer -> its replacement, for layers that stand in several places."""
     if type(module) in _SWAP:
-        return _SWAP[type(module)](module).train(module.training)
+        if module not in done:
+            done[module] = _SWAP[type(module)](module)
+        return done[module]
     for name, child in list(module._modules.items()):
         if child is not None:
-            module._modules[name] = _rewrite(child)
+            module._modules[name] = _rewrite(child, done)
     return module
