@@ -211,3 +211,49 @@ def test_fusing_keeps_what_a_layer_holds():
     assert net[0].geo_norm is net[0].sem_norm and net[0].note == "kept" and net[1] is net[2][0]
     net[0].extra = torch.nn.Identity()                      # what the replacement gets later is its own
     assert "extra" not in att._modules
+
+
+def test_layers_that_the_kernels_do_not_compute_are_left_alone():
+    """Heads wider than the kernels' (512 channels in one head: 256 / 512; 384 with unreduced keys: 384 / 384), and submodules of another
+    kind: the layer stays, or, replaced after the rewriting, runs its own forward."""
+    wide = torch.nn.ModuleList([dense_tail.ConvAttentionLayer_Decouple(512, 1), dense_tail.ConvAttentionLayer_Decouple(384, 1, 1),
+                                dense_tail.ConvAttentionLayer_Decouple(384, 1), dense_tail.ConvAttentionLayer_Decouple(512, 2)])
+    fused_tail.fuse_cross_attention(wide)
+    own, fused = dense_tail.ConvAttentionLayer_Decouple, fused_tail.FusedConvAttention
+    assert [type(m) for m in wide] == [own, own, fused, fused]
+
+    class Scaled(torch.nn.Linear):
+        def forward(self, x):
+            return super().forward(x) * 2
+
+    def change(i, m):
+        if i < 2:
+            m[1].activation = (torch.nn.GELU(), torch.nn.Identity())[i]
+        elif i == 2:
+            m[1].linear1 = Scaled(16, 24)
+        elif i == 3:
+            m[1].linear2 = torch.nn.Sequential(torch.nn.Linear(24, 16))
+        else:
+            name = ("v_conv", "out_geo_conv", "out_sem_conv")[i - 4]
+            setattr(m[0], name, torch.nn.Conv2d(16, 16, 3, 1, 1) if i < 6 else torch.nn.Sequential(torch.nn.Conv2d(16, 16, 1)))
+
+    x = torch.randn(2, 16, 3, 4)
+    call = lambda m, i: m[0](x, x, x, need_maps=False)[0] if i >= 4 else [m[1](x.flatten(2).permute(2, 0, 1))]  # noqa: E731
+    for i in range(7):
+        torch.manual_seed(i)
+        stock = torch.nn.ModuleList(layers())
+        change(i, stock)
+        want = call(stock, i)
+        before = [type(m) for m in stock]
+        fused_tail.fuse_cross_attention(stock)
+        kinds = [type(m) for m in stock]
+        assert kinds[i < 4] is before[i < 4] and kinds[i >= 4] is not before[i >= 4]
+        assert all(torch.equal(a, b) for a, b in zip(call(stock, i), want))
+        late = fused_tail.fuse_cross_attention(torch.nn.ModuleList(layers()))
+        change(i, late)
+        late.load_state_dict(stock.state_dict())
+        assert all(torch.equal(a, b) for a, b in zip(call(late, i), want))
+    norm = torch.nn.utils.parametrizations.weight_norm
+    m = torch.nn.ModuleList(layers())
+    norm(m[0].v_conv), norm(m[1].linear1)                    # made at each read of the weight: no hook, never stale
+    assert [type(c) for c in fused_tail.fuse_cross_attention(m)] == [fused, fused_tail.FusedFeedForward]

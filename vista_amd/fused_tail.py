@@ -12,7 +12,7 @@ the same leaves (torch ties a leaf's gradient accumulation to the stream on whic
 import torch
 from torch import nn
 
-from . import ops
+from . import _lib, ops
 from .dense_tail import ConvAttentionLayer_Decouple, FeedFowardLayer
 
 
@@ -80,6 +80,15 @@ def _hooked(module):
     return bool(module._forward_pre_hooks or module._forward_hooks or module._backward_pre_hooks or module._backward_hooks)
 
 
+def _plain_conv1x1(m):
+    return (isinstance(m, nn.Conv2d) and type(m).forward is nn.Conv2d.forward and m.kernel_size == (1, 1) and m.stride == (1, 1)
+            and m.padding == (0, 0) and m.groups == 1)
+
+
+def _plain_linear(m):
+    return isinstance(m, nn.Linear) and type(m).forward is nn.Linear.forward
+
+
 def _become(module, layer):
     """All that `layer` holds -- submodules (one that stands under two names too), parameters and buffers of its own, training flags,
     attributes -- in containers of `module`'s own."""
@@ -94,19 +103,26 @@ def _conv1x1(conv, x, residual=None):
 class FusedConvAttention(nn.Module):
     """ConvAttentionLayer_Decouple on `attention` and `linear_act`; shares the layer's submodules, so parameters and
     state_dict keys are the layer's. The attention maps are not formed: need_maps=True runs the layer's own forward, and so do hooks on
-    a submodule of `direct`, whose weight is read without a call of it (weight_norm, prune and the like make the weight in a hook)."""
+    a submodule of `direct`, whose weight is read without a call of it (weight_norm, prune and the like make the weight in a hook), and
+    a submodule there that is no 1x1 convolution."""
 
     direct = ("v_conv", "out_sem_conv", "out_geo_conv")
+
+    @classmethod
+    def computes(cls, layer):
+        """Whether the kernels can stand in for the layer's own forward."""
+        return (all(_plain_conv1x1(getattr(layer, name, None)) for name in cls.direct) and layer.head_dim <= _lib.VX_ATTN_MAX_DIM
+                and layer.v_conv.out_channels // layer.numhead <= _lib.VX_ATTN_MAX_VDIM)
 
     def __init__(self, layer):
         _become(self, layer)
 
     def forward(self, query, key, value, q_pos_emb=None, k_pos_emb=None, need_maps=True, key_mask=None):
         """-> ([tokens[HW_q, B, C]] x2, [None, None]); key_mask bool [B, HW_kv], True where the key block takes part."""
-        if need_maps or any(_hooked(self._modules[name]) for name in self.direct):
+        if need_maps or not _direct(self):
             if key_mask is not None:
-                raise ValueError("key_mask is supported without attention maps (need_maps=False) and without hooks on "
-                                 f"{', '.join(self.direct)} only")
+                raise ValueError("key_mask is supported without attention maps (need_maps=False) and where the kernels compute the "
+                                 f"layer (no hooks on {', '.join(self.direct)}) only")
             return ConvAttentionLayer_Decouple.forward(self, query, key, value, q_pos_emb, k_pos_emb, need_maps)
         identity = query
         if q_pos_emb is not None:
@@ -139,15 +155,20 @@ class FusedConvAttention(nn.Module):
 
 class FusedFeedForward(nn.Module):
     """FeedFowardLayer on `linear_act`: ReLU in the first product's epilogue, the residual in the second's. Hooks on a submodule of
-    `direct`: the layer's own forward, which calls them."""
+    `direct`, or another kind of submodule there: the layer's own forward, which calls them."""
 
     direct = ("linear1", "linear2", "activation")
+
+    @classmethod
+    def computes(cls, layer):
+        act = getattr(layer, "activation", None)
+        return all(_plain_linear(getattr(layer, name, None)) for name in cls.direct[:2]) and type(act) is nn.ReLU
 
     def __init__(self, layer):
         _become(self, layer)
 
     def forward(self, view):
-        if any(_hooked(self._modules[name]) for name in self.direct):
+        if not _direct(self):
             return FeedFowardLayer.forward(self, view)
         flip = view.dim() == 3 and not view.is_contiguous()     # FusedConvAttention's tokens: rows in memory order
         x = view.transpose(0, 1) if flip else view
@@ -156,17 +177,26 @@ class FusedFeedForward(nn.Module):
         return y.transpose(0, 1) if flip else y
 
 
+def _direct(fused):
+    return fused.computes(fused) and not any(_hooked(fused._modules[name]) for name in fused.direct)
+
+
 _SWAP = {ConvAttentionLayer_Decouple: FusedConvAttention, FeedFowardLayer: FusedFeedForward}
+
+
+def _fusable(module):
+    return type(module) in _SWAP and _SWAP[type(module)].computes(module)
 
 
 def fuse_cross_attention(module):
     """Rewrite `module` in place: every ConvAttentionLayer_Decouple and FeedFowardLayer in it runs on the fused kernels
     (inference and training; HIP tensors only from then on, unless attention maps are asked for). Parameters, buffers and
     state_dict keys are unchanged. A layer with hooks, or with hooks on a submodule that the fused form does not call, is refused before
-    anything is changed; hooks that such a submodule gets later run the layer's own forward. Returns `module`, or its replacement
+    anything is changed; hooks that such a submodule gets later run the layer's own forward. A layer that the kernels do not compute
+    (heads wider than `attention` takes, another activation, submodules of another kind) is left as it is. Returns `module`, or its replacement
     when it is such a layer itself."""
     for name, layer in module.named_modules():
-        if type(layer) in _SWAP:
+        if _fusable(layer):
             for at, m in [("", layer)] + [("." + c, layer._modules[c]) for c in _SWAP[type(layer)].direct]:
                 if _hooked(m):
                     raise ValueError(f"{name or type(layer).__name__}{at} has hooks, which the fused layer would not call")
@@ -175,7 +205,7 @@ def fuse_cross_attention(module):
 
 def _rewrite(module, done):
     """`done`: layer -> its replacement, for layers that stand in several places."""
-    if type(module) in _SWAP:
+    if _fusable(module):
         if module not in done:
             done[module] = _SWAP[type(module)](module)
         return done[module]
