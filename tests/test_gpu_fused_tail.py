@@ -720,6 +720,22 @@ def test_fused_block_with_maps_runs_the_stock_path(dev):
             blk(q, kv, kv, key_mask=mask)
 
 
+def test_fused_layers_return_the_layout_of_the_stock_ones(dev):
+    """Tokens [HW, B, C], contiguous: a caller's .view() works on them; a feed-forward layer of transposed tokens likewise."""
+    from vista_amd.dense_tail import ConvAttentionLayer_Decouple, FeedFowardLayer
+    from vista_amd.fused_tail import fuse_cross_attention
+    att, ffn = ConvAttentionLayer_Decouple(24, 2).to(dev), FeedFowardLayer(24, 40).to(dev)
+    fatt, fffn = fuse_cross_attention(att), fuse_cross_attention(ffn)
+    q, kv = torch.randn(3, 24, 5, 4, device=dev), torch.randn(3, 24, 2, 7, device=dev)
+    for a, b in zip(att(q, kv, kv, need_maps=False)[0], fatt(q, kv, kv, need_maps=False)[0]):
+        assert b.shape == a.shape and b.stride() == a.stride() and b.is_contiguous()
+        within(b, a.double(), 1e-4 * a.abs().max().double().expand_as(a), "tokens")
+        for v in (b, b.transpose(0, 1), b[:, :1]):
+            y, z = ffn(v), fffn(v)
+            assert z.stride() == y.stride()
+            within(z, y.double(), 1e-4 * y.abs().max().double().expand_as(y), "ffn")
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals(dev):
     from vista_amd import ops

@@ -145,11 +145,10 @@ class FusedConvAttention(nn.Module):
         v = _conv1x1(self.v_conv, tokens(value)).view(b, -1, n, c // n)
         r = attention(heads(self.q_sem_conv(query), self.q_geo_conv(query)), heads(self.k_sem_conv(key), self.k_geo_conv(key)),
                       v, key_mask, float(self.head_dim) ** -0.5).view(b, sq, n, 2, c // n)
-        rows = tokens(identity)
+        rows = identity.flatten(2).permute(2, 0, 1).contiguous()
         outs = []
         for i, (conv, norm) in enumerate(((self.out_sem_conv, self.sem_norm), (self.out_geo_conv, self.geo_norm))):
-            y = norm(_conv1x1(conv, r[:, :, :, i].reshape(b, sq, c), rows))
-            outs.append(y.transpose(0, 1))
+            outs.append(norm(_conv1x1(conv, r[:, :, :, i].transpose(0, 1).reshape(sq, b, c), rows)))
         return outs, [None, None]
 
 
@@ -170,11 +169,8 @@ class FusedFeedForward(nn.Module):
     def forward(self, view):
         if not _direct(self):
             return FeedFowardLayer.forward(self, view)
-        flip = view.dim() == 3 and not view.is_contiguous()     # FusedConvAttention's tokens: rows in memory order
-        x = view.transpose(0, 1) if flip else view
-        h = linear_act(x, self.linear1.weight, self.linear1.bias, act="relu")
-        y = self.norm(linear_act(h, self.linear2.weight, self.linear2.bias, x))
-        return y.transpose(0, 1) if flip else y
+        h = linear_act(view, self.linear1.weight, self.linear1.bias, act="relu")
+        return self.norm(linear_act(h, self.linear2.weight, self.linear2.bias, view))
 
 
 def _direct(fused):
