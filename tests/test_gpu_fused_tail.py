@@ -736,6 +736,52 @@ def test_fused_layers_return_the_layout_of_the_stock_ones(dev):
             within(z, y.double(), 1e-4 * y.abs().max().double().expand_as(y), "ffn")
 
 
+@pytest.mark.parametrize("half", [BF16, torch.float16])
+@pytest.mark.parametrize("masked", [False, True])
+def test_fused_block_under_autocast(half, masked, dev):
+    """The stock block runs under autocast, so the fused one does: outputs and gradients against the block in float64, no farther than the
+    stock block's own and sixteen roundings of half a bf16 step of the largest value. Autocast to float16 runs the stock form."""
+    import copy
+    from vista_amd.dense_tail import CrossAttenBlock_Decouple
+    from vista_amd.fused_tail import fuse_cross_attention
+    torch.manual_seed(5)
+    stock = CrossAttenBlock_Decouple(48, 2, 64).to(dev)
+    fused = fuse_cross_attention(copy.deepcopy(stock))
+    exact = copy.deepcopy(stock).double()
+    bev, rv = torch.randn(3, 48, 10, 9, device=dev), torch.randn(3, 48, 10, 4, device=dev)
+    if masked:                                             # the layer's own argument: a stock layer has none
+        km = torch.rand(3, 40, device=dev) > 0.3
+        with torch.autocast("cuda", half):
+            if half == BF16:
+                a = fused.cross_atten(bev, rv, rv, need_maps=False, key_mask=km)[0]
+            else:
+                with pytest.raises(ValueError, match="key_mask"):
+                    fused.cross_atten(bev, rv, rv, need_maps=False, key_mask=km)
+                return
+        for x, y in zip(a, fused.cross_atten(bev, rv, rv, need_maps=False, key_mask=km)[0]):
+            assert x.dtype == F32 and (x - y).abs().max() <= 16 * 2.0 ** -8 * y.abs().max()
+        return
+    cot = [torch.randn(3, 48, 10, 9, device=dev) for _ in range(2)]
+
+    def step(m, cast):
+        dt = next(m.parameters()).dtype
+        x, y = (t.to(dt).requires_grad_(True) for t in (bev, rv))
+        with torch.autocast("cuda", half, enabled=cast):
+            out, _ = m(x, y, need_maps=False)
+        got = torch.autograd.grad(out, (x, y), [c.to(o.dtype) for c, o in zip(cot, out)], retain_graph=True)
+        par = torch.autograd.grad(out, list(m.parameters()), [c.to(o.dtype) for c, o in zip(cot, out)])
+        return [(o.detach().dtype, o.detach().double()) for o in (*out, *got, *par)]
+
+    names = ["sem", "geo", "bev", "rv"] + [n for n, _ in stock.named_parameters()]
+    for name, (t, a), (u, b), (_, c) in zip(names, step(fused, True), step(stock, True), step(exact, False)):
+        assert t == u, name
+        size = c.abs().max().clamp(min=1.0 if ".k_" in name else 0.0)            # (gradients of the biases of k are exactly zero)
+        if half == BF16:
+            assert (a - c).abs().max() <= (b - c).abs().max() + 16 * 2.0 ** -8 * size, name
+        else:
+            assert (a - b).abs().max() <= 2.0 ** -8 * size, name
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals(dev):
     from vista_amd import ops

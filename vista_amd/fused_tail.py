@@ -95,9 +95,23 @@ def _become(module, layer):
     module.__dict__.update((k, v.copy() if isinstance(v, (dict, set)) else v) for k, v in layer.__dict__.items())
 
 
+def _autocast():
+    """The type that autocast asks for, or None outside of it."""
+    return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else None
+
+
+def _layer(x, weight, bias, residual=None, act="none"):
+    """linear_act as one of autocast's operators: its product in bfloat16 there, the residual added in its own type."""
+    if _autocast() is None:
+        return linear_act(x, weight, bias, residual, act)
+    half = [t.to(torch.bfloat16) if t is not None else None for t in (x, weight, bias)]
+    y = linear_act(*half, act=act)
+    return y if residual is None else residual + y
+
+
 def _conv1x1(conv, x, residual=None):
     """A 1x1 nn.Conv2d over tokens [..., c] instead of a map [b, c, h, w]."""
-    return linear_act(x, conv.weight.flatten(1), conv.bias, residual)
+    return _layer(x, conv.weight.flatten(1), conv.bias, residual)
 
 
 class FusedConvAttention(nn.Module):
@@ -169,12 +183,12 @@ class FusedFeedForward(nn.Module):
     def forward(self, view):
         if not _direct(self):
             return FeedFowardLayer.forward(self, view)
-        h = linear_act(view, self.linear1.weight, self.linear1.bias, act="relu")
-        return self.norm(linear_act(h, self.linear2.weight, self.linear2.bias, view))
+        h = _layer(view, self.linear1.weight, self.linear1.bias, act="relu")
+        return self.norm(_layer(h, self.linear2.weight, self.linear2.bias, view))
 
 
 def _direct(fused):
-    return fused.computes(fused) and not any(_hooked(fused._modules[name]) for name in fused.direct)
+    return fused.computes(fused) and _autocast() in (None, torch.bfloat16) and not any(_hooked(fused._modules[name]) for name in fused.direct)
 
 
 _SWAP = {ConvAttentionLayer_Decouple: FusedConvAttention, FeedFowardLayer: FusedFeedForward}
@@ -189,7 +203,8 @@ def fuse_cross_attention(module):
     (inference and training; HIP tensors only from then on, unless attention maps are asked for). Parameters, buffers and
     state_dict keys are unchanged. A layer with hooks, or with hooks on a submodule that the fused form does not call, is refused before
     anything is changed; hooks that such a submodule gets later run the layer's own forward. A layer that the kernels do not compute
-    (heads wider than `attention` takes, another activation, submodules of another kind) is left as it is. Returns `module`, or its replacement
+    (heads wider than `attention` takes, another activation, submodules of another kind) is left as it is. Under autocast to bfloat16
+    the products run in bfloat16, under another autocast the layer's own forward does. Returns `module`, or its replacement
     when it is such a layer itself."""
     for name, layer in module.named_modules():
         if _fusable(layer):
