@@ -367,6 +367,24 @@ def test_attention_gradients_in_chunks_of_queries(k_len, dev):
         within(got, *ref[name], name)
 
 
+def off_by_its_rounding(got, want, what, room):
+    """A bf16 result whose value before the rounding is good to 2^-15: the 2-norm of its error is that of the rounding alone, r (rms some
+    2^-9 / sqrt 3 of each value), times sqrt(1 + (2^-15 / r)^2) < 1.001; `room` for the values that the rounding itself leaves exact."""
+    rounding = (want.to(BF16).double() - want).norm()
+    assert (got.double() - want).norm() <= room * rounding, (what, ((got.double() - want).norm() / rounding).item())
+
+
+@pytest.mark.parametrize("scale", [None, 1.0])
+@pytest.mark.parametrize("shape", [(1, 3, 700, 2, 2, 1, 64, 96), (2, 200, 150, 2, 2, 1, 48, 48), (2, 700, 300, 4, 2, 1, 96, 192),
+                                   (1, 600, 900, 2, 2, 1, 192, 384), (8, 1100, 140, 8, 8, 8, 64, 64)])
+def test_bf16_attention_is_rounded_once(shape, scale, dev):
+    """Every width of tile, few and many queries, split and joined keys; flat and peaked (scale 1) rows."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn(shape, BF16, dev, 21, "some")
+    ref = attn_reference(q, k, v, km, do, scale)
+    off_by_its_rounding(ops.attn_fwd(q, k, v, km, scale)[0], ref["out"][0], "out", 1.02)
+
+
 @pytest.mark.parametrize("k_len,live", [(2, 2), (5, 3), (16, 10), (40, 26), (128, 128)])
 def test_bf16_gradients_over_few_keys_lose_nothing(k_len, live, dev):
     """Over at most 128 keys P and dS are 16-bit operands and delta is summed from P dP itself: what is left beside the gradients' own

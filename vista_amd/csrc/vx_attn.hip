@@ -4,9 +4,9 @@
 // Forward: one pass over the keys with a running maximum and sum per query; probabilities never leave the registers.
 // Backward: probabilities recomputed from the saved (maximum, 1 / sum); see attn_pds below.
 // fp32 operands run as three exact bf16 planes (six products, fp32 accumulation), bf16 ones directly (vx_tile.h). Softmax
-// statistics, probabilities and sums over queries are fp32; for bf16 tensors the probabilities and score gradients are rounded
-// to bf16 where they become matrix operands (at most half a step, 2^-8 of each value: independent errors, so that their sum is off
-// by about as much as the output's own rounding), in the backward pass over at most 128 keys to 16 bits.
+// statistics, probabilities and sums over queries are fp32; for bf16 tensors the probabilities are rounded to 16 bits (two planes) where
+// they become operands of P v: to 8 bits, their errors would be about as large as the output's own rounding (2-norm 0.0024 of the output
+// instead of 0.0017). In the backward pass P and dS are rounded to bf16, over at most 128 keys to 16 bits.
 // A masked key has no part in anything, whatever its rows hold; a query without keys gives zeros. No atomics: bitwise
 // reproducible.
 #include "vx_tile.h"
@@ -62,7 +62,7 @@ __device__ __forceinline__ bool attn_key_live(int keys, const uint8_t* mask, int
 template <typename T, int DP, int DVP, int RT, int QG, int CS, bool IMG, bool FAST>
 __global__ __launch_bounds__(64 * QG * CS, QG * CS == 8 ? 2 : DVP > 192 || (DVP > 64 && VxType<T>::NPL == 3) ? 1 : 2)
 void attn_fwd(const FwdArgs<T> a) {
-  constexpr int NPL = VxType<T>::NPL, KT = AttnTile<T>::KT, NS = KT / 32;     // NS: 32-key steps of a tile
+  constexpr int NPL = VxType<T>::NPL, PP = VxType<T>::NPL_F32, KT = AttnTile<T>::KT, NS = KT / 32;     // NS: 32-key steps of a tile
   constexpr int KD = DP / 32, NV = DVP / 16 / CS, NK = KT / 16, OWN = NK / CS, E = sizeof(T), NW = QG * CS;
   constexpr int K_FRAGS = NK * KD;
   constexpr int K_BLOCK = IMG ? KD * kFragBytes : vx_image_block<KD>(), V_BLOCK = IMG ? NS * kFragBytes : vx_image_block<NS>();
@@ -264,7 +264,7 @@ void attn_fwd(const FwdArgs<T> a) {
           s[rt][k] = *reinterpret_cast<const vx_f32x4*>(swap + (((wave & ~1) + k / OWN) * OWN * RT + rt * OWN + k % OWN) * kFragBytes +
                                                         lane * 16);
     }
-    VxFrag<NPL> pf[RT][NS];
+    VxFrag<PP> pf[RT][NS];
     if (cur != ~0ull >> (64 - KT)) {           // some keys take no part
       const unsigned long long bits = cur >> (g * 4);
 #pragma unroll
@@ -320,7 +320,7 @@ void attn_fwd(const FwdArgs<T> a) {
 #pragma unroll
         for (int u = 0; u < G; ++u) vx_frag_load(iv + frag_at(V_BLOCK, half * NV + nv + u, ns), V_PLANE, vf[u]);
 #pragma unroll
-        for (int pr = 0; pr < VxProducts<NPL, NPL>::N; ++pr)
+        for (int pr = 0; pr < VxProducts<NPL, PP>::N; ++pr)
 #pragma unroll
           for (int u = 0; u < G; ++u)
 #pragma unroll

@@ -38,11 +38,13 @@ struct VxType;
 template <>
 struct VxType<float> {
   static constexpr int NPL = 3;   // bf16 planes per value
+  static constexpr int NPL_F32 = 3;   // ... of an fp32 intermediate that meets such values in a product
   static constexpr int BK = 32;   // reduction values per staged step of a GEMM (64: small tiles of k-contiguous operands)
 };
 template <>
 struct VxType<__bf16> {
   static constexpr int NPL = 1;
+  static constexpr int NPL_F32 = 2;
   static constexpr int BK = 64;
 };
 
