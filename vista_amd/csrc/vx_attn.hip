@@ -5,8 +5,8 @@
 // Backward: probabilities recomputed from the saved (maximum, 1 / sum); see attn_pds below.
 // fp32 operands run as three exact bf16 planes (six products, fp32 accumulation), bf16 ones directly (vx_tile.h). Softmax
 // statistics, probabilities and sums over queries are fp32; for bf16 tensors the probabilities are rounded to 16 bits (two planes) where
-// they become operands of P v: to 8 bits, their errors would be about as large as the output's own rounding (2-norm 0.0024 of the output
-// instead of 0.0017). In the backward pass P and dS are rounded to bf16, over at most 128 keys to 16 bits.
+// they become operands: to 8 bits, their errors would be about as large as the output's own rounding (2-norm 0.0024 of the output
+// instead of 0.0017). The backward pass keeps P and dS in fp32; as operands beside bf16 ones they are two planes as well.
 // A masked key has no part in anything, whatever its rows hold; a query without keys gives zeros. No atomics: bitwise
 // reproducible.
 #include "vx_tile.h"
@@ -549,7 +549,7 @@ struct BwdArgs : AttnArgs<T> {
   long long go_b, go_s, go_h;
   const float2* stats;
   float* delta;                              // [b*h][sq]
-  void *p, *ds;                              // [b*h][rows][skp] of the present chunk of queries: T, or fp32 where the keys fit one tile
+  float *p, *ds;                             // [b*h][rows][skp] of the present chunk of queries
   T *dq, *dk, *dvv;                          // [b][sq][h][d], [b][sk][h/gk][d], [b][sk][h/gv][dv]
   float *slab_k, *slab_v;                    // [splits][b*h][sk][d], [splits][b*h][sk][dv]
   float scale;
@@ -598,15 +598,6 @@ __global__ __launch_bounds__(256) void attn_gather(const BwdArgs<T> a, const Gat
   gather_piece(a, g, b, (long long)(blockIdx.x % g.per) * 256 + threadIdx.x, a.count[b], a.index + (long long)b * a.sk);
 }
 
-template <bool A, typename X, typename Y>
-struct VxPick {
-  typedef X type;
-};
-template <typename X, typename Y>
-struct VxPick<false, X, Y> {
-  typedef Y type;
-};
-
 // delta = sum_n go * out per query: one wave per row. With a mask the first `head` workgroups make its lists; OWN (at most kOwnKeys keys):
 // they gather the keys as well, each with a list of its own, which saves a launch (a step of 4 x 1600 x 480, 2 heads of 192 / 384, fp32:
 // 187 -> 182 us). One read of go and out: 4 x 2 x 1600 x 384 fp32 39 MB 11 us with the gather, 2 x 25600 x 384 157 MB 28 us
@@ -645,13 +636,11 @@ __global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long 
 constexpr int kPdsN = 128;                   // keys of an attn_pds tile
 // P and dS of a TM-query x TN-key tile: scores and dP = go v^T are two products with one epilogue,
 // P = 2^(scale2 s - max) / sum, dS = scale P (dP - delta).
-// ONE: all keys are in the tile. delta is then the tile's own sum of P dP, and both go out in fp32: over few keys the rounding of a
-// bf16 output inside delta and of P and dS to bf16 would not average out (2^-9 each of terms that nearly cancel): relative 2-norm of
-// dq and dk over 16 keys 0.0025 so, 0.0020 with fp32, 0.0017 their own rounding.
+// Both go out in fp32: rounded to bf16 they would make the error of dq and dk 1.4 times that of their own rounding (3 x 777 x 301).
+// ONE: all keys are in the tile. delta is then the tile's own sum of P dP: over few keys the rounding of a bf16 output inside delta would
+// not average out (terms that nearly cancel): relative 2-norm of dq and dk over 16 keys 0.0020 so, 0.0017 their own rounding.
 // Bound by the split into planes and LDS reads in fp32: 4 x 2 x 1600 x 480, 192 / 384 57 us, 25600 x 1920 483 us; bf16 3 x 4 x 777 x 301,
 // 96 / 192 10.7 us, where 468 workgroups of 64 x 128 are two rounds.
-template <typename T, bool ONE>
-using AttnProb = typename VxPick<ONE, float, T>::type;
 template <typename T, int TM, int TN, bool FAST, bool ONE>
 __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) {
   constexpr int BK = TM <= 64 ? 64 : VxType<T>::BK;
@@ -719,24 +708,22 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) 
     for (int ni = 0; ni < TN / 32; ++ni)
 #pragma unroll
       for (int i = 0; i < 4; ++i) dp[mi][ni][i] = s[mi][ni][i] * (dp[mi][ni][i] - delta[mi]) * a.scale;
-  using P = AttnProb<T, ONE>;
   vx_acc_each<TM, TN>(s, [&](int mi, int m, int j, int n, const vx_f32x4& v, const vx_f32x4& w) {
     if (m >= rows_m || n0 + n >= a.skp) return;
     const long long at = at0 + (long long)m * a.skp + n;
-    vx_store8((P*)a.p + at, v, w, 8);
-    vx_store8((P*)a.ds + at, dp[mi][2 * j], dp[mi][2 * j + 1], 8);
+    vx_store8(a.p + at, v, w, 8);
+    vx_store8(a.ds + at, dp[mi][2 * j], dp[mi][2 * j + 1], 8);
   });
 }
 
 // the three gradients of a chunk in one launch: dV slabs = P^T go, dK slabs = dS^T q (reduction over the queries of a split),
 // dQ = dS k (reduction over the keys)
-// ONE: P and dS are fp32; beside bf16 operands they are two planes
+// P and dS are fp32; beside bf16 operands they are two planes
 // 4 x 2 x 1600 x 480, 192 / 384 fp32 66 us, 25600 x 1920 565 us: as attn_pds; dV and dK read both operands along their rows, transposed
 // on the way to LDS. bf16 3 x 4 x 777 x 301, 96 / 192 11.2 us
-template <typename T, int TM, int TN, bool FAST, bool ONE>
+template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a) {
-  using P = AttnProb<T, ONE>;
-  constexpr int BK = VxType<T>::BK, PX = sizeof(T) == 2 && ONE ? 2 : VxType<T>::NPL;
+  constexpr int BK = VxType<T>::BK, PX = VxType<T>::NPL_F32;
   __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN, BK, PX>()];
   vx_f32x4 acc[TM / 32][TN / 32];
   vx_acc_zero(acc);
@@ -754,10 +741,10 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
     const int r0 = sp * a.span, len = a.rows - r0 < a.span ? a.rows - r0 : a.span;
     const int rows_m = keys - m0 < TM ? keys - m0 : TM, rows_n = width - n0 < TN ? width - n0 : TN;
     const long long q = a.q0 + r0;
-    const VxOperand<P> X{(const P*)(is_v ? a.p : a.ds) + ((long long)bh * a.rows + r0) * a.skp + m0, a.skp, a.skp - m0};
+    const VxOperand<float> X{(is_v ? a.p : a.ds) + ((long long)bh * a.rows + r0) * a.skp + m0, a.skp, a.skp - m0};
     const VxOperand<T> W{is_v ? a.go + b * a.go_b + q * a.go_s + h * a.go_h + n0 : a.q + b * a.q_b + q * a.q_s + h * a.q_h + n0,
                          is_v ? a.go_s : a.q_s, rows_n};
-    vx_gemm_loop<T, KS, KS, TM, TN, FAST, BK, P, PX>(X, W, 0, len, lds, acc);
+    vx_gemm_loop<T, KS, KS, TM, TN, FAST, BK, float, PX>(X, W, 0, len, lds, acc);
     float* slab = (is_v ? a.slab_v : a.slab_k) + ((long long)(a.split0 + sp) * a.bh + bh) * a.sk * width;
     vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
       if (m < rows_m && n < rows_n) vx_store8(slab + (long long)(m0 + m) * width + n0 + n, v, w, rows_n - n);
@@ -769,10 +756,10 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
     const int m0 = (int)(w % a.tq) * TM;
     const int bh = (int)(w / a.tq), b = bh / a.h, h = bh % a.h;
     const int rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = a.d - n0 < TN ? a.d - n0 : TN;
-    const VxOperand<P> X{(const P*)a.ds + ((long long)bh * a.rows + m0) * a.skp, a.skp, rows_m};
+    const VxOperand<float> X{a.ds + ((long long)bh * a.rows + m0) * a.skp, a.skp, rows_m};
     const VxOperand<T> W{a.k + b * a.k_b + (h / a.gk) * a.k_h + n0, a.k_s, rows_n};
     const int keys = a.count ? a.count[b] : a.sk;    // dS is 0 from there to its tile's end
-    vx_gemm_loop<T, KC, KS, TM, TN, FAST, BK, P, PX>(X, W, 0, keys, lds, acc);
+    vx_gemm_loop<T, KC, KS, TM, TN, FAST, BK, float, PX>(X, W, 0, keys, lds, acc);
     vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
       if (m < rows_m && n < rows_n)
         vx_store8(a.dq + (((long long)b * a.sq + a.q0 + m0 + m) * a.h + h) * a.d + n0 + n, v, w, rows_n - n);
@@ -1018,7 +1005,7 @@ constexpr size_t kChunkBytes = (size_t)1 << 30;
 BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   BwdPlan p;
   p.one = s.sk <= kPdsN;
-  const int64_t cus = vx_tile_cus(), bh = s.b * s.h, e = dtype == VX_F32 ? 4 : 2, ep = p.one ? 4 : e, bk = dtype == VX_F32 ? 32 : 64;
+  const int64_t cus = vx_tile_cus(), bh = s.b * s.h, e = dtype == VX_F32 ? 4 : 2, bk = dtype == VX_F32 ? 32 : 64;
   p.skp = vx_cdiv(s.sk, 8) * 8;
   // query rows of a tile; 4 x 2 heads, 1600 x 480, 192 / 384 wide, fp32 (416 tiles of 128): attn_pds 71 us with 64, 62 with 128,
   // attn_grads 82 and 84
@@ -1032,7 +1019,7 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   if (splits < vx_cdiv(s.sq, 2 * s.sk)) splits = vx_cdiv(s.sq, 2 * s.sk);       // no workgroup much longer than those of dQ
   const int64_t most = vx_cdiv(s.sq, 4 * bk);
   if (splits > most) splits = most;
-  int64_t fit = (int64_t)(kChunkBytes / 2) / (bh * p.skp * ep);      // queries of a chunk
+  int64_t fit = (int64_t)(kChunkBytes / 2) / (bh * p.skp * 4);       // queries of a chunk
   if (fit < p.tm) fit = p.tm;
   if (splits < vx_cdiv(s.sq, fit)) splits = vx_cdiv(s.sq, fit);
   if (splits < 1) splits = 1;
@@ -1042,7 +1029,7 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   if (p.per_chunk > p.splits) p.per_chunk = p.splits;
   p.chunk = p.per_chunk * p.span < s.sq ? p.per_chunk * p.span : s.sq;
   p.delta = vx_align((size_t)bh * s.sq * 4);
-  p.pds = vx_align((size_t)bh * p.chunk * p.skp * ep);
+  p.pds = vx_align((size_t)bh * p.chunk * p.skp * 4);
   p.slab_k = vx_align((size_t)p.splits * bh * s.sk * s.d * 4);
   p.slab_v = vx_align((size_t)p.splits * bh * s.sk * s.dv * 4);
   p.live = live_bytes(s);
@@ -1058,9 +1045,8 @@ int32_t bwd_chunk(const BwdArgs<T>& a, const BwdPlan& p, unsigned pds, unsigned 
                                    : attn_pds<T, 64, kPdsN, FAST, false>;
   probs<<<pds, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
-  const auto sums = p.one ? attn_grads<T, 64, 64, FAST, true>
-                    : p.tm == 128 ? (p.tn == 192 ? attn_grads<T, 128, 192, FAST, false> : attn_grads<T, 128, 128, FAST, false>)
-                                  : (p.tn == 192 ? attn_grads<T, 64, 192, FAST, false> : attn_grads<T, 64, 64, FAST, false>);
+  const auto sums = p.tm == 128 ? (p.tn == 192 ? attn_grads<T, 128, 192, FAST> : attn_grads<T, 128, 128, FAST>)
+                                : (p.tn == 192 ? attn_grads<T, 64, 192, FAST> : attn_grads<T, 64, 64, FAST>);
   sums<<<grads, kTileThreads, 0, s>>>(a);
   VX_LAUNCH_CHECK();
   return VX_OK;
@@ -1071,8 +1057,8 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   const BwdPlan p = bwd_plan(sh, dtype);
   const int64_t bh = sh.b * sh.h, rows = bh * sh.sq;
   a.delta = (float*)ws;
-  a.p = ws + p.delta;
-  a.ds = ws + p.delta + p.pds;
+  a.p = (float*)(ws + p.delta);
+  a.ds = (float*)(ws + p.delta + p.pds);
   a.slab_k = (float*)(ws + p.delta + 2 * p.pds);
   a.slab_v = (float*)(ws + p.delta + 2 * p.pds + p.slab_k);
   a.skp = (int)p.skp;
