@@ -389,8 +389,11 @@ int32_t vx_linear_bwd(const void* d_dy, int64_t lddy, const void* d_x, int64_t l
  *          needs (maximum of log2(e) * scale * score, 1 / sum)
  * vx_attn_bwd  d_dout with its own strides HOST int64[3] (batch, position, head), d_out and d_stats of the forward pass ->
  *          d_dq [batch][q_len][heads][dim], d_dk [batch][k_len][k_heads][dim], d_dv [batch][k_len][v_heads][v_dim]
- * Statistics, probabilities and sums are fp32; matrix arithmetic as in vx_linear_*. VX_BF16 probabilities and score gradients are
- * rounded to bf16 where they become operands (over at most 128 keys the backward pass keeps 16 bits of them). Infinities and NaN
+ * vx_attn_fwd_rest, vx_attn_bwd_rest  the same with d_rest: vx_attn_rest_bytes bytes (0 where the backward pass has no use for
+ *          it: VX_F32, or at most 128 keys) or NULL. It carries what the rounding of d_out to bf16 left behind to the backward pass,
+ *          whose row sums of d_dout * out would lack it: gradients of rows that few keys dominate lose two bits without it
+ * Statistics, probabilities, score gradients and sums are fp32; matrix arithmetic as in vx_linear_*: beside VX_BF16 operands
+ * probabilities and score gradients are rounded to 16 bits. Infinities and NaN
  * in rows that take part give NaN; in masked rows they are never read. No atomics: bitwise reproducible.
  * ------------------------------------------------------------------------------------------- */
 #define VX_ATTN_MAX_DIM 192
@@ -399,7 +402,15 @@ size_t vx_attn_fwd_workspace_bytes(const int64_t* shape, int32_t dtype);
 int32_t vx_attn_fwd(const void* d_q, const void* d_k, const void* d_v, const uint8_t* d_key_mask, const int64_t* shape,
                     const int64_t* strides, float scale, void* d_out, float* d_stats, int32_t dtype, void* d_workspace,
                     size_t workspace_bytes, void* stream);
+size_t vx_attn_rest_bytes(const int64_t* shape, int32_t dtype);
+int32_t vx_attn_fwd_rest(const void* d_q, const void* d_k, const void* d_v, const uint8_t* d_key_mask, const int64_t* shape,
+                         const int64_t* strides, float scale, void* d_out, float* d_stats, void* d_rest, int32_t dtype,
+                         void* d_workspace, size_t workspace_bytes, void* stream);
 size_t vx_attn_bwd_workspace_bytes(const int64_t* shape, int32_t dtype);
+int32_t vx_attn_bwd_rest(const void* d_dout, const int64_t* dout_strides, const void* d_q, const void* d_k, const void* d_v,
+                         const uint8_t* d_key_mask, const int64_t* shape, const int64_t* strides, const void* d_out,
+                         const float* d_stats, const void* d_rest, float scale, void* d_dq, void* d_dk, void* d_dv, int32_t dtype,
+                         void* d_workspace, size_t workspace_bytes, void* stream);
 int32_t vx_attn_bwd(const void* d_dout, const int64_t* dout_strides, const void* d_q, const void* d_k, const void* d_v,
                     const uint8_t* d_key_mask, const int64_t* shape, const int64_t* strides, const void* d_out,
                     const float* d_stats, float scale, void* d_dq, void* d_dk, void* d_dv, int32_t dtype,

@@ -257,3 +257,18 @@ def test_layers_that_the_kernels_do_not_compute_are_left_alone():
     m = torch.nn.ModuleList(layers())
     norm(m[0].v_conv), norm(m[1].linear1)                    # made at each read of the weight: no hook, never stale
     assert [type(c) for c in fused_tail.fuse_cross_attention(m)] == [fused, fused_tail.FusedFeedForward]
+
+
+def test_rest_of_the_output():
+    """What the forward pass hands to the backward one beside the statistics: bf16 of more than 128 keys alone; refusals as without it."""
+    lib = _lib.lib()
+    size = lambda dtype, *s: lib.vx_attn_rest_bytes(i64(*s), dtype)  # noqa: E731
+    assert size(1, 3, 50, 129, 4, 2, 1, 64, 129) == 3 * 50 * 4 * 129 * 2
+    assert size(1, 3, 50, 128, 4, 2, 1, 64, 129) == 0 and size(0, 3, 50, 129, 4, 2, 1, 64, 129) == 0
+    assert size(1, 3, 50, 129, 4, 3, 1, 64, 129) == 0 and size(2, 3, 50, 129, 4, 2, 1, 64, 129) == 0
+    one = i64(*(1,) * 10)
+    assert lib.vx_attn_fwd_rest(FAKE, FAKE, FAKE, None, i64(*GOOD), one, 1.0, None, None, FAKE, 1, FAKE, 1 << 40, None) == ERR_ARG
+    assert lib.vx_attn_bwd_rest(FAKE, i64(1, 1, 1), FAKE, FAKE, FAKE, None, i64(*GOOD), one, None, FAKE, FAKE, 1.0, FAKE, FAKE, FAKE, 1,
+                                FAKE, 1 << 40, None) == ERR_ARG
+    assert lib.vx_attn_bwd_rest(FAKE, i64(1, 1, 1), FAKE, FAKE, FAKE, None, i64(*GOOD), one, FAKE, FAKE, FAKE, 1.0, FAKE, FAKE, FAKE, 1,
+                                FAKE, 8, None) == ERR_WS

@@ -389,12 +389,13 @@ def test_bf16_attention_is_rounded_once(shape, scale, dev):
 @pytest.mark.parametrize("shape", [(1, 100, 200, 2, 2, 1, 64, 96), (3, 777, 301, 4, 2, 1, 96, 192), (1, 3000, 500, 2, 2, 1, 192, 384),
                                    (4, 2000, 260, 4, 4, 4, 64, 64), (1, 700, 1000, 2, 2, 1, 144, 168)])
 def test_bf16_attention_gradients_are_rounded_once(shape, scale, dev):
-    """More than 128 keys, every tile of the backward pass; dv, whose error is that of P."""
+    """More than 128 keys, every tile of the backward pass, flat rows and (scale 1) rows that few keys dominate."""
     from vista_amd import ops
     q, k, v, km, do = make_attn(shape, BF16, dev, 22, "some")
     ref = attn_reference(q, k, v, km, do, scale)
     out, stats = ops.attn_fwd(q, k, v, km, scale, want_stats=True)
-    off_by_its_rounding(ops.attn_bwd(do, q, k, v, out, stats, km, scale)[2], ref["dv"][0], "dv", 1.02)
+    for name, got in zip(("dq", "dk", "dv"), ops.attn_bwd(do, q, k, v, out, stats, km, scale)):
+        off_by_its_rounding(got, ref[name][0], name, 1.02)
 
 
 @pytest.mark.parametrize("k_len,live", [(2, 2), (5, 3), (16, 10), (40, 26), (128, 128)])

@@ -107,6 +107,11 @@ SIGNATURES = {
     "vx_attn_fwd_workspace_bytes": (c_size_t, [c_i64p, c_int32]),
     "vx_attn_fwd": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_i64p, c_i64p, ctypes.c_float, c_void_p, c_void_p,
                               c_int32, c_void_p, c_size_t, c_void_p]),
+    "vx_attn_rest_bytes": (c_size_t, [c_i64p, c_int32]),
+    "vx_attn_fwd_rest": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_i64p, c_i64p, ctypes.c_float, c_void_p, c_void_p,
+                                   c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),
+    "vx_attn_bwd_rest": (c_int32, [c_void_p, c_i64p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64p, c_i64p, c_void_p, c_void_p,
+                                   c_void_p, ctypes.c_float, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),
     "vx_attn_bwd_workspace_bytes": (c_size_t, [c_i64p, c_int32]),
     "vx_attn_bwd": (c_int32, [c_void_p, c_i64p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64p, c_i64p, c_void_p, c_void_p,
                               ctypes.c_float, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),

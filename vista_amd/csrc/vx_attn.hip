@@ -29,12 +29,24 @@ struct AttnArgs {
 template <typename T>
 struct FwdArgs : AttnArgs<T> {
   const char *k_img, *v_img;                 // attn_pack's images, tile after tile of each key / value head
-  T* out;                                    // [b][sq][h][dv]
+  T *out, *rest;                             // [b][sq][h][dv]; rest: what the rounding of out to bf16 left behind, or null
   float2* stats;                             // [b*h][sq] {max of scale2 * score, 1 / sum} or null
   float* part;                               // [splits][b*h][sq][dv] when the keys are split
   float2* part_ml;                           // [splits][b*h][sq]
   int tiles_q, splits, span;                 // span: key tiles of one split
 };
+
+// values n .. n + 3 of an output row, `left` of which exist
+template <typename T>
+__device__ __forceinline__ void attn_put(const FwdArgs<T>& a, long long at, vx_f32x4 v, int left) {
+  vx_store4(a.out + at, v, left);
+  if constexpr (sizeof(T) == 2) {
+    if (!a.rest) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] -= (float)(T)v[i];
+    vx_store4(a.rest + at, v, left);
+  }
+}
 
 template <typename T>
 struct AttnTile {
@@ -356,9 +368,9 @@ void attn_fwd(const FwdArgs<T> a) {
     } else {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       if (a.stats && g == 0 && half == 0) a.stats[(long long)bh * a.sq + row] = make_float2(m[rt], inv);
-      T* op = a.out + (((long long)b * a.sq + row) * a.h + h) * a.dv;
+      const long long at = (((long long)b * a.sq + row) * a.h + h) * a.dv + n0;
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv) vx_store4(op + n0 + nv * 16, o[rt][nv] * inv, a.dv - n0 - nv * 16);
+      for (int nv = 0; nv < NV; ++nv) attn_put(a, at + nv * 16, o[rt][nv] * inv, a.dv - n0 - nv * 16);
     }
   }
 }
@@ -538,14 +550,14 @@ __global__ __launch_bounds__(256) void attn_join(const FwdArgs<T> a, long long i
   if (!here) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int bh = (int)(rowid / a.sq), row = (int)(rowid % a.sq), b = bh / a.h, h = bh % a.h;
-  vx_store4(a.out + (((long long)b * a.sq + row) * a.h + h) * a.dv + n, o * inv, a.dv - n);
+  attn_put(a, (((long long)b * a.sq + row) * a.h + h) * a.dv + n, o * inv, a.dv - n);
   if (a.stats && n == 0) a.stats[rowid] = make_float2(m, inv);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------
 template <typename T>
 struct BwdArgs : AttnArgs<T> {
-  const T *out, *go;                         // out [b][sq][h][dv]; go by strides
+  const T *out, *rest, *go;                  // out [b][sq][h][dv] and its rest or null; go by strides
   long long go_b, go_s, go_h;
   const float2* stats;
   float* delta;                              // [b*h][sq]
@@ -598,7 +610,8 @@ __global__ __launch_bounds__(256) void attn_gather(const BwdArgs<T> a, const Gat
   gather_piece(a, g, b, (long long)(blockIdx.x % g.per) * 256 + threadIdx.x, a.count[b], a.index + (long long)b * a.sk);
 }
 
-// delta = sum_n go * out per query: one wave per row. With a mask the first `head` workgroups make its lists; OWN (at most kOwnKeys keys):
+// delta = sum_n go * out per query, out with its rest: a row that one key dominates has dP of that key next to delta, and a bf16 out alone
+// would leave 3 times the gradients' own rounding (scores of 200 to 1000 keys with standard deviation 8). One wave per row. With a mask the first `head` workgroups make its lists; OWN (at most kOwnKeys keys):
 // they gather the keys as well, each with a list of its own, which saves a launch (a step of 4 x 1600 x 480, 2 heads of 192 / 384, fp32:
 // 187 -> 182 us). One read of go and out: 4 x 2 x 1600 x 384 fp32 39 MB 11 us with the gather, 2 x 25600 x 384 157 MB 28 us
 template <typename T, bool OWN>
@@ -622,10 +635,12 @@ __global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long 
   const int lane = threadIdx.x & 63;
   const int bh = (int)(r / a.sq), row = (int)(r % a.sq), b = bh / a.h, h = bh % a.h;
   const T* go = a.go + b * a.go_b + row * a.go_s + h * a.go_h;
-  const T* o = a.out + (((long long)b * a.sq + row) * a.h + h) * a.dv;
+  const long long o = (((long long)b * a.sq + row) * a.h + h) * a.dv;
   float s = 0.0f;
   for (int n = lane * 4; n < a.dv; n += 256) {
-    const vx_f32x4 x = vx_load4(go + n, a.dv - n) * vx_load4(o + n, a.dv - n);
+    vx_f32x4 y = vx_load4(a.out + o + n, a.dv - n);
+    if (sizeof(T) == 2 && a.rest) y += vx_load4(a.rest + o + n, a.dv - n);
+    const vx_f32x4 x = vx_load4(go + n, a.dv - n) * y;
     s += (x[0] + x[1]) + (x[2] + x[3]);
   }
 #pragma unroll
@@ -1142,9 +1157,15 @@ extern "C" size_t vx_attn_fwd_workspace_bytes(const int64_t* shape, int32_t dtyp
   return s.b && s.sq ? fwd_bytes(s, dtype) : 0;
 }
 
-extern "C" int32_t vx_attn_fwd(const void* d_q, const void* d_k, const void* d_v, const uint8_t* d_key_mask, const int64_t* shape,
-                               const int64_t* strides, float scale, void* d_out, float* d_stats, int32_t dtype, void* d_workspace,
-                               size_t workspace_bytes, void* stream) {
+extern "C" size_t vx_attn_rest_bytes(const int64_t* shape, int32_t dtype) {
+  if (check("attn_fwd", shape, dtype)) return 0;
+  const Shape s = shape_of(shape);       // fp32: nothing is left behind; keys in one tile: attn_pds makes its own delta
+  return dtype == VX_F32 || s.sk <= kPdsN ? 0 : (size_t)s.b * s.sq * s.h * s.dv * 2;
+}
+
+extern "C" int32_t vx_attn_fwd_rest(const void* d_q, const void* d_k, const void* d_v, const uint8_t* d_key_mask, const int64_t* shape,
+                                    const int64_t* strides, float scale, void* d_out, float* d_stats, void* d_rest, int32_t dtype,
+                                    void* d_workspace, size_t workspace_bytes, void* stream) {
   if (int32_t rc = check("attn_fwd", shape, dtype)) return rc;
   const Shape s = shape_of(shape);
   if (s.b == 0 || s.sq == 0) return VX_OK;
@@ -1166,8 +1187,16 @@ extern "C" int32_t vx_attn_fwd(const void* d_q, const void* d_k, const void* d_v
   FwdArgs<__bf16> a{};
   fill_args(a, s, strides, d_q, d_k, d_v, d_key_mask, scale);
   a.out = (__bf16*)d_out;
+  a.rest = (__bf16*)d_rest;
   a.stats = (float2*)d_stats;
   return fwd_impl(a, s, dtype, (char*)d_workspace, st);
+}
+
+extern "C" int32_t vx_attn_fwd(const void* d_q, const void* d_k, const void* d_v, const uint8_t* d_key_mask, const int64_t* shape,
+                               const int64_t* strides, float scale, void* d_out, float* d_stats, int32_t dtype, void* d_workspace,
+                               size_t workspace_bytes, void* stream) {
+  return vx_attn_fwd_rest(d_q, d_k, d_v, d_key_mask, shape, strides, scale, d_out, d_stats, nullptr, dtype, d_workspace, workspace_bytes,
+                          stream);
 }
 
 extern "C" size_t vx_attn_bwd_workspace_bytes(const int64_t* shape, int32_t dtype) {
@@ -1179,11 +1208,12 @@ extern "C" size_t vx_attn_bwd_workspace_bytes(const int64_t* shape, int32_t dtyp
 template <typename T>
 static int32_t attn_bwd_typed(const Shape& s, const void* d_dout, const int64_t* dout_strides, const void* d_q, const void* d_k,
                               const void* d_v, const uint8_t* d_key_mask, const int64_t* strides, const void* d_out,
-                              const float* d_stats, float scale, void* d_dq, void* d_dk, void* d_dv, int32_t dtype, void* ws,
-                              hipStream_t st) {
+                              const float* d_stats, const void* d_rest, float scale, void* d_dq, void* d_dk, void* d_dv, int32_t dtype,
+                              void* ws, hipStream_t st) {
   BwdArgs<T> a{};
   fill_args(a, s, strides, d_q, d_k, d_v, d_key_mask, scale);
   a.out = (const T*)d_out;
+  a.rest = (const T*)d_rest;
   a.go = (const T*)d_dout;
   a.go_b = dout_strides[0];
   a.go_s = dout_strides[1];
@@ -1196,10 +1226,10 @@ static int32_t attn_bwd_typed(const Shape& s, const void* d_dout, const int64_t*
   return bwd_impl(a, s, dtype, (char*)ws, st);
 }
 
-extern "C" int32_t vx_attn_bwd(const void* d_dout, const int64_t* dout_strides, const void* d_q, const void* d_k, const void* d_v,
-                               const uint8_t* d_key_mask, const int64_t* shape, const int64_t* strides, const void* d_out,
-                               const float* d_stats, float scale, void* d_dq, void* d_dk, void* d_dv, int32_t dtype,
-                               void* d_workspace, size_t workspace_bytes, void* stream) {
+extern "C" int32_t vx_attn_bwd_rest(const void* d_dout, const int64_t* dout_strides, const void* d_q, const void* d_k, const void* d_v,
+                                    const uint8_t* d_key_mask, const int64_t* shape, const int64_t* strides, const void* d_out,
+                                    const float* d_stats, const void* d_rest, float scale, void* d_dq, void* d_dk, void* d_dv,
+                                    int32_t dtype, void* d_workspace, size_t workspace_bytes, void* stream) {
   if (int32_t rc = check("attn_bwd", shape, dtype)) return rc;
   const Shape s = shape_of(shape);
   const hipStream_t st = (hipStream_t)stream;
@@ -1223,9 +1253,15 @@ extern "C" int32_t vx_attn_bwd(const void* d_dout, const int64_t* dout_strides, 
     vx_set_error("attn_bwd: workspace too small");
     return VX_ERR_WORKSPACE;
   }
-  if (dtype == VX_F32)
-    return attn_bwd_typed<float>(s, d_dout, dout_strides, d_q, d_k, d_v, d_key_mask, strides, d_out, d_stats, scale, d_dq, d_dk, d_dv,
-                                 dtype, d_workspace, st);
-  return attn_bwd_typed<__bf16>(s, d_dout, dout_strides, d_q, d_k, d_v, d_key_mask, strides, d_out, d_stats, scale, d_dq, d_dk, d_dv,
-                                dtype, d_workspace, st);
+  const auto typed = dtype == VX_F32 ? attn_bwd_typed<float> : attn_bwd_typed<__bf16>;
+  return typed(s, d_dout, dout_strides, d_q, d_k, d_v, d_key_mask, strides, d_out, d_stats, d_rest, scale, d_dq, d_dk, d_dv, dtype,
+               d_workspace, st);
+}
+
+extern "C" int32_t vx_attn_bwd(const void* d_dout, const int64_t* dout_strides, const void* d_q, const void* d_k, const void* d_v,
+                               const uint8_t* d_key_mask, const int64_t* shape, const int64_t* strides, const void* d_out,
+                               const float* d_stats, float scale, void* d_dq, void* d_dk, void* d_dv, int32_t dtype,
+                               void* d_workspace, size_t workspace_bytes, void* stream) {
+  return vx_attn_bwd_rest(d_dout, dout_strides, d_q, d_k, d_v, d_key_mask, shape, strides, d_out, d_stats, nullptr, scale, d_dq, d_dk,
+                          d_dv, dtype, d_workspace, workspace_bytes, stream);
 }

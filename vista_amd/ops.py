@@ -741,7 +741,10 @@ class _AttnGeometry:
         self.shape = (ctypes.c_int64 * 8)(b, sq, sk, h, hk, hv, d, dv)
         self.strides = (ctypes.c_int64 * 10)(*q_st[:3], *k_st[:3], *v_st[:3], mask_st)
         self.scale = d ** -0.5
-        self.out, self.stats = (b, sq, h, dv), (b * h, sq, 2)
+        self.out = (b, sq, h, dv)
+        rest = L.lib().vx_attn_rest_bytes(self.shape, dtype)       # behind the statistics, in the same tensor
+        self.rest = b * h * sq * 8 if rest else None
+        self.stats = (-(-(b * h * sq * 8 + rest) // 4),) if rest else (b * h, sq, 2)
         with torch.cuda.device(device):
             self.fwd_bytes = L.lib().vx_attn_fwd_workspace_bytes(self.shape, dtype)
             self.bwd_bytes = L.lib().vx_attn_bwd_workspace_bytes(self.shape, dtype)
@@ -777,7 +780,8 @@ def _attn_args(q, k, v, key_mask):
 def attn_fwd(q, k, v, key_mask=None, scale=None, want_stats=False):
     """softmax(scale q k^T) v over q [b, sq, h, d], k [b, sk, hk, d], v [b, sk, hv, dv] -> (out [b, sq, h, dv], stats | None).
     Query head i reads key head i // (h / hk) and value head i // (h / hv); key_mask bool [b, sk], True where the key takes part;
-    a query without keys gives zeros. scale defaults to d ** -0.5. stats (want_stats) is what attn_bwd needs. Any strides with
+    a query without keys gives zeros. scale defaults to d ** -0.5. stats (want_stats) is what attn_bwd needs, a float32 tensor of
+    its own layout. Any strides with
     a contiguous last dimension are read in place."""
     return _attn_fwd_run(*_attn_args(q, k, v, key_mask), scale, want_stats)
 
@@ -787,10 +791,11 @@ def _attn_fwd_run(q, k, v, key_mask, geo, scale, want_stats):
     out = q.new_empty(geo.out)
     stats = torch.empty(geo.stats, dtype=torch.float32, device=dev) if want_stats else None
     ws = _ws(geo.fwd_bytes, dev) if geo.fwd_bytes else None
-    rc = _launch(dev, L.lib().vx_attn_fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(key_mask), geo.shape, geo.strides,
-                 geo.scale if scale is None else float(scale), out.data_ptr(), _at(stats), _DT[q.dtype], _at(ws), geo.fwd_bytes)
+    rest = stats.data_ptr() + geo.rest if want_stats and geo.rest is not None else None
+    rc = _launch(dev, L.lib().vx_attn_fwd_rest, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(key_mask), geo.shape, geo.strides,
+                 geo.scale if scale is None else float(scale), out.data_ptr(), _at(stats), rest, _DT[q.dtype], _at(ws), geo.fwd_bytes)
     if rc:
-        L.check(rc, "vx_attn_fwd")
+        L.check(rc, "vx_attn_fwd_rest")
     return out, stats
 
 
@@ -815,9 +820,10 @@ def _attn_bwd_run(dout, q, k, v, key_mask, geo, out, stats, scale):
     dout_strides = (ctypes.c_int64 * 3)(*dout.stride()[:3])
     dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
     ws = _ws(geo.bwd_bytes, dev)
-    rc = _launch(dev, L.lib().vx_attn_bwd, dout.data_ptr(), dout_strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(key_mask),
-                 geo.shape, geo.strides, out.data_ptr(), stats.data_ptr(), geo.scale if scale is None else float(scale), dq.data_ptr(),
-                 dk.data_ptr(), dv.data_ptr(), _DT[q.dtype], ws.data_ptr(), geo.bwd_bytes)
+    rest = stats.data_ptr() + geo.rest if geo.rest is not None else None
+    rc = _launch(dev, L.lib().vx_attn_bwd_rest, dout.data_ptr(), dout_strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(key_mask),
+                 geo.shape, geo.strides, out.data_ptr(), stats.data_ptr(), rest, geo.scale if scale is None else float(scale),
+                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _DT[q.dtype], ws.data_ptr(), geo.bwd_bytes)
     if rc:
-        L.check(rc, "vx_attn_bwd")
+        L.check(rc, "vx_attn_bwd_rest")
     return dq, dk, dv
