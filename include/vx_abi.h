@@ -359,6 +359,8 @@ int32_t vx_nms_bev(const float* d_boxes, int32_t num_boxes, float thresh, int32_
  *                VX_ACT_NONE. g = dy * act'(saved) -> d_dpre [m][n] (required with an activation: it is also the residual's
  *                gradient; without one that is d_dy itself); d_dx [m][k] = g w, d_dw [n][k] = g^T x, d_dbias [n] = column
  *                sums of g; each of the three may be NULL
+ * vx_linear_bwd_act_workspace_bytes  the workspace for one activation; vx_linear_bwd_workspace_bytes is enough for each (with
+ *                VX_BF16, VX_ACT_GELU and _SILU keep g in fp32 for the two products: m * n * 4 bytes more)
  * Row strides are in elements, >= 0 (0 repeats a row), the last dimension is contiguous. m < 2^31; n, k <= 2^20. m = 0 gives
  * zero parameter gradients. No atomics: bitwise reproducible. VX_ACT_GELU is the erf form. An infinity or NaN in an fp32 operand
  * gives NaN (not an infinity) in every output it reaches: its planes are not numbers.
@@ -370,6 +372,7 @@ int32_t vx_nms_bev(const float* d_boxes, int32_t num_boxes, float thresh, int32_
 int32_t vx_linear_fwd(const void* d_x, int64_t ldx, const void* d_weight, int64_t ldw, const void* d_bias,
                       const void* d_residual, int64_t ldr, int64_t m, int32_t n, int32_t k, int32_t act, void* d_y,
                       void* d_pre, int32_t dtype, void* stream);
+size_t vx_linear_bwd_act_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t act, int32_t dtype);
 size_t vx_linear_bwd_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t dtype);
 int32_t vx_linear_bwd(const void* d_dy, int64_t lddy, const void* d_x, int64_t ldx, const void* d_weight, int64_t ldw,
                       const void* d_saved, int64_t m, int32_t n, int32_t k, int32_t act, void* d_dpre, void* d_dx,

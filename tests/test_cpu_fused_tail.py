@@ -272,3 +272,13 @@ def test_rest_of_the_output():
                                 FAKE, 1 << 40, None) == ERR_ARG
     assert lib.vx_attn_bwd_rest(FAKE, i64(1, 1, 1), FAKE, FAKE, FAKE, None, i64(*GOOD), one, FAKE, FAKE, FAKE, 1.0, FAKE, FAKE, FAKE, 1,
                                 FAKE, 8, None) == ERR_WS
+
+
+def test_layer_gradients_workspace_follows_the_activation():
+    lib = _lib.lib()
+    m, n, k = 1000, 96, 64
+    size = [[lib.vx_linear_bwd_act_workspace_bytes(m, n, k, act, dtype) for act in range(4)] for dtype in (0, 1)]
+    assert len(set(size[0])) == 1 and size[1][0] == size[1][1] and size[1][2] == size[1][3] == size[1][0] + m * n * 4
+    assert [lib.vx_linear_bwd_workspace_bytes(m, n, k, dtype) for dtype in (0, 1)] == [size[0][0], size[1][2]]
+    call = lambda act, room: lib.vx_linear_bwd(FAKE, n, FAKE, k, FAKE, k, FAKE, m, n, k, act, FAKE, FAKE, FAKE, FAKE, 1, FAKE, room, None)  # noqa: E731
+    assert call(2, size[1][2] - 1) == ERR_WS and call(3, size[1][0]) == ERR_WS and call(1, size[1][1] - 1) == ERR_WS

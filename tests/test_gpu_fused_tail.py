@@ -204,6 +204,25 @@ def test_linear_nan_and_inf_stay_in_their_row(dev):
     assert torch.equal(y[keep], clean[keep]) and torch.isnan(y[17]).all()
 
 
+def off_by_its_rounding(got, want, what, room):
+    """A bf16 result whose value before the rounding is good to 2^-15: the 2-norm of its error is that of the rounding alone, r (rms some
+    2^-9 / sqrt 3 of each value), times sqrt(1 + (2^-15 / r)^2) < 1.001; `room` for the values that the rounding itself leaves exact."""
+    rounding = (want.to(BF16).double() - want).norm()
+    assert (got.double() - want).norm() <= room * rounding, (what, ((got.double() - want).norm() / rounding).item())
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("m,k,n", [(50, 70, 90), (3000, 128, 96), (20000, 128, 256)])
+def test_bf16_layer_gradients_are_rounded_once(m, k, n, act, dev):
+    """dx and dw of a smooth activation: g = dy act'(pre) goes into both products unrounded."""
+    from vista_amd import ops
+    x, w, _, s, dy = make_linear(m, k, n, BF16, dev, m, False, True)
+    dx, dw, db, dpre = ops.linear_bwd(dy, x, w, act, s)
+    g = dy.double() * slope64(s.double(), act)
+    for name, got, want in (("dpre", dpre, g), ("dx", dx, g @ w.double()), ("dw", dw, g.t() @ x.double()), ("dbias", db, g.sum(0))):
+        off_by_its_rounding(got, want, name, 1.02)
+
+
 # ------------------------------------------------------------------------------------------------ attention
 # batch, q_len, k_len, heads, k_heads, v_heads, dim, v_dim
 ATTN = [(1, 1, 1, 1, 1, 1, 1, 1), (1, 1, 480, 2, 2, 1, 192, 384), (2, 65, 33, 4, 2, 1, 37, 53), (1, 130, 100, 2, 2, 1, 24, 48),
@@ -365,13 +384,6 @@ def test_attention_gradients_in_chunks_of_queries(k_len, dev):
     within(out, *ref["out"], "out")
     for name, got in zip(("dq", "dk", "dv"), ops.attn_bwd(do, q, k, v, out, stats, km)):
         within(got, *ref[name], name)
-
-
-def off_by_its_rounding(got, want, what, room):
-    """A bf16 result whose value before the rounding is good to 2^-15: the 2-norm of its error is that of the rounding alone, r (rms some
-    2^-9 / sqrt 3 of each value), times sqrt(1 + (2^-15 / r)^2) < 1.001; `room` for the values that the rounding itself leaves exact."""
-    rounding = (want.to(BF16).double() - want).norm()
-    assert (got.double() - want).norm() <= room * rounding, (what, ((got.double() - want).norm() / rounding).item())
 
 
 @pytest.mark.parametrize("scale", [None, 1.0])

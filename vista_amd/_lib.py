@@ -101,6 +101,7 @@ SIGNATURES = {
                              c_void_p]),
     "vx_linear_fwd": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32,
                                 c_int32, c_void_p, c_void_p, c_int32, c_void_p]),
+    "vx_linear_bwd_act_workspace_bytes": (c_size_t, [c_int64, c_int32, c_int32, c_int32, c_int32]),
     "vx_linear_bwd_workspace_bytes": (c_size_t, [c_int64, c_int32, c_int32, c_int32]),
     "vx_linear_bwd": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32,
                                 c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),

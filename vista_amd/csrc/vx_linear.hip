@@ -5,6 +5,8 @@
 // fp32 operands run as three exact bf16 planes (six products, fp32 accumulation), bf16 ones directly; both in the tiles of
 // vx_tile.h. A reduction split over workgroups leaves fp32 slabs that one kernel adds in a fixed order: no atomics, bitwise
 // reproducible.
+#include <type_traits>
+
 #include "vx_tile.h"
 
 namespace {
@@ -155,7 +157,9 @@ __global__ __launch_bounds__(kTileThreads) void linear_few(const FwdArgs<T> a) {
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------
-// g = dy * act'(saved) (written where there is an activation) and the column sums of g per row chunk. A lane owns 16 bytes of
+// g = dy * act'(saved) (written where there is an activation) and the column sums of g per row chunk. wide: g unrounded for the two
+// products, where its rounding to bf16 is one (gelu, silu: it would make the error of dx and dw 1.4 times that of their own rounding;
+// relu's g is dy or 0). A lane owns 16 bytes of
 // columns, `lanes` (a power of two, at most a wave) lanes a row, so that a wave reads whole rows; a workgroup owns `lanes` x 16 bytes
 // of columns and a chunk of rows. Sums in fp32 per thread, then over the workgroup's rows in order. One pass: 102399 x 512 bf16, two
 // reads and a write, 64 us (4.9 TB/s of the 5.1 that a copy reaches).
@@ -163,7 +167,7 @@ template <typename T>
 struct ActArgs {
   const T *dy, *saved;
   T* g;
-  float* part;
+  float *wide, *part;                          // wide: [m][n] or null
   long long ldy, m, chunk;
   int n, act, lanes, cols;                     // cols: workgroups along the columns
 };
@@ -206,6 +210,8 @@ __device__ __forceinline__ void act_rows(const ActArgs<T>& a, unsigned block, ch
             vx_store8(g + row * n + c, v[u][0], v[u][1], n - c);
           else
             vx_store4(g + row * n + c, v[u][0], n - c);
+          if constexpr (Q == 2)
+            if (a.wide) vx_store8(a.wide + row * n + c, v[u][0], v[u][1], n - c);
         }
 #pragma unroll
         for (int q = 0; q < Q; ++q) sum[q] += v[u][q];
@@ -230,9 +236,10 @@ __global__ __launch_bounds__(256) void act_bwd(const ActArgs<T> a) {
   act_rows(a, blockIdx.x, lds);
 }
 
-template <typename T>
+template <typename T, typename G>
 struct BwdArgs {
-  const T *g, *x, *w;
+  const G* g;
+  const T *x, *w;
   T *dx, *dw;
   float* slab;          // [splits][n][k] when splits > 1
   long long ldg, ldx, ldw, m, span;   // span: rows of one split
@@ -243,9 +250,11 @@ struct BwdArgs {
 // one launch for the gradients: workgroups [0, blocks_w) are tiles of dw = g^T x (reduction over the rows, split), the next blocks_x
 // tiles of dx = g w (reduction over n), the others (no activation: g = dy) the column sums. 6400 x 512 -> 384 fp32 38 us (131 TFLOP/s),
 // 102399 x 384 -> 512 bf16 132 us (610): dw's operands are transposed on their way to LDS
-template <typename T, int TM, int TN, bool FAST>
-__global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a, const ActArgs<T> sums) {
-  __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN>()];
+// G: the type of g, fp32 beside bf16 operands where act_bwd wrote it so (two planes)
+template <typename T, typename G, int TM, int TN, bool FAST>
+__global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T, G> a, const ActArgs<T> sums) {
+  constexpr int BK = VxType<T>::BK, PG = sizeof(G) == sizeof(T) ? VxType<T>::NPL : VxType<T>::NPL_F32;
+  __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN, BK, PG>()];
   if (blockIdx.x >= a.blocks_w + a.blocks_x) {
     act_rows(sums, blockIdx.x - a.blocks_w - a.blocks_x, lds);
     return;
@@ -259,8 +268,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a
     const long long r0 = split * a.span;
     const int rows = (int)(a.m - r0 < a.span ? a.m - r0 : a.span);
     const int rows_n = a.n - n0 < TM ? a.n - n0 : TM, rows_k = a.k - k0 < TN ? a.k - k0 : TN;
-    const VxOperand<T> X{a.g + r0 * a.ldg + n0, a.ldg, rows_n}, W{a.x + r0 * a.ldx + k0, a.ldx, rows_k};
-    vx_gemm_loop<T, KS, KS, TM, TN, FAST>(X, W, 0, rows, lds, acc);
+    const VxOperand<G> X{a.g + r0 * a.ldg + n0, a.ldg, rows_n};
+    const VxOperand<T> W{a.x + r0 * a.ldx + k0, a.ldx, rows_k};
+    vx_gemm_loop<T, KS, KS, TM, TN, FAST, BK, G, PG>(X, W, 0, rows, lds, acc);
     float* slab = a.slab ? a.slab + (long long)split * a.n * a.k : nullptr;
     vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
       const int left = rows_k - n;
@@ -273,8 +283,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T> a
     const long long m0 = (long long)(t / a.tiles_xk) * TM;
     const int k0 = (int)(t % a.tiles_xk) * TN;
     const int rows_m = (int)(a.m - m0 < TM ? a.m - m0 : TM), rows_k = a.k - k0 < TN ? a.k - k0 : TN;
-    const VxOperand<T> X{a.g + m0 * a.ldg, a.ldg, rows_m}, W{a.w + k0, a.ldw, rows_k};
-    vx_gemm_loop<T, KC, KS, TM, TN, FAST>(X, W, 0, a.n, lds, acc);
+    const VxOperand<G> X{a.g + m0 * a.ldg, a.ldg, rows_m};
+    const VxOperand<T> W{a.w + k0, a.ldw, rows_k};
+    vx_gemm_loop<T, KC, KS, TM, TN, FAST, BK, G, PG>(X, W, 0, a.n, lds, acc);
     const long long at0 = m0 * a.k + k0;
     vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
       if (m < rows_m && n < rows_k) vx_store8(a.dx + at0 + (long long)m * a.k + n, v, w, rows_k - n);
@@ -393,44 +404,65 @@ int32_t fwd_impl(const FwdArgs<T>& args, hipStream_t s) {
   return VX_OK;
 }
 
+// bytes of the workspace: slabs of dw, column sums of row chunks, g unrounded
+bool wide_g(int32_t act, int32_t dtype) { return dtype == VX_BF16 && (act == VX_ACT_GELU || act == VX_ACT_SILU); }
+size_t slab_bytes(const BwdPlan& p, int64_t n, int64_t k) { return vx_align(p.splits > 1 ? (size_t)p.splits * n * k * 4 : 0); }
+size_t part_bytes(const BwdPlan& p, int64_t n) { return vx_align((size_t)p.chunks * n * 4); }
+size_t bwd_bytes(int64_t m, int64_t n, int64_t k, int32_t act, int32_t dtype) {
+  const BwdPlan p = bwd_plan(m, n, k, dtype);
+  return slab_bytes(p, n, k) + part_bytes(p, n) + (wide_g(act, dtype) ? vx_align((size_t)m * n * 4) : 0);
+}
+
+// dw, dx and, without an activation, the column sums
+template <typename T, typename G>
+int32_t launch_bwd(BwdArgs<T, G>& a, const BwdPlan& p, const ActArgs<T>& rows, int64_t sums, hipStream_t s) {
+  const int64_t t = p.big ? 128 : 64;
+  a.span = p.span;
+  a.tiles_wk = (int)vx_cdiv(a.k, t);
+  a.tiles_w = (int)(vx_cdiv(a.n, t) * a.tiles_wk);
+  a.tiles_xk = a.tiles_wk;
+  const int64_t bw = a.dw ? a.tiles_w * p.splits : 0, bx = a.dx ? vx_cdiv(a.m, t) * a.tiles_xk : 0;
+  VX_REQUIRE(bw + bx + sums < (1LL << 31), "linear_bwd: too many rows");
+  a.blocks_w = (unsigned)bw;
+  a.blocks_x = (unsigned)bx;
+  if (bw + bx + sums == 0) return VX_OK;
+  const bool fast = vx_fast(a.g, a.ldg, a.n, sizeof(G)) && vx_fast(a.x, a.ldx, a.k, sizeof(T)) && vx_fast(a.w, a.ldw, a.k, sizeof(T));
+  const auto kernel = p.big ? (fast ? linear_bwd<T, G, 128, 128, true> : linear_bwd<T, G, 128, 128, false>)
+                            : (fast ? linear_bwd<T, G, 64, 64, true> : linear_bwd<T, G, 64, 64, false>);
+  kernel<<<(unsigned)(bw + bx + sums), kTileThreads, 0, s>>>(a, rows);
+  VX_LAUNCH_CHECK();
+  return VX_OK;
+}
+
 template <typename T>
 int32_t bwd_impl(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w, int64_t ldw, const T* saved, int64_t m, int32_t n,
                  int32_t k, int32_t act, T* dpre, T* dx, T* dw, T* dbias, char* ws, int32_t dtype, hipStream_t s) {
   const BwdPlan p = bwd_plan(m, n, k, dtype);
-  float* slab = (float*)ws;
-  float* part = (float*)(ws + vx_align(p.splits > 1 ? (size_t)p.splits * n * k * 4 : 0));
-  const T* g = dy;
-  int64_t ldg = lddy;
+  float *slab = (float*)ws, *part = (float*)(ws + slab_bytes(p, n, k));
+  float* wide = wide_g(act, dtype) && (dx || dw) ? (float*)(ws + slab_bytes(p, n, k) + part_bytes(p, n)) : nullptr;
   const int64_t cols = vx_cdiv(n, p.lanes * (16 / (int64_t)sizeof(T)));
-  const ActArgs<T> rows{dy, saved, dpre, dbias ? part : nullptr, lddy, m, p.chunk, n, act, (int)p.lanes, (int)cols};
-  int64_t sums = dbias ? cols * p.chunks : 0;        // workgroups of the column sums
+  const ActArgs<T> rows{dy, saved, dpre, wide, dbias ? part : nullptr, lddy, m, p.chunk, n, act, (int)p.lanes, (int)cols};
   VX_REQUIRE(cols * p.chunks < (1LL << 31), "linear_bwd: too many rows");
   if (act != VX_ACT_NONE) {
     act_bwd<T><<<(unsigned)(cols * p.chunks), 256, 0, s>>>(rows);
     VX_LAUNCH_CHECK();
-    g = dpre;
-    ldg = n;
-    sums = 0;
   }
-  const int64_t t = p.big ? 128 : 64;
-  BwdArgs<T> a{};
-  a.g = g; a.x = x; a.w = w; a.dx = dx; a.dw = dw;
-  a.slab = p.splits > 1 ? slab : nullptr;
-  a.ldg = ldg; a.ldx = ldx; a.ldw = ldw; a.m = m; a.span = p.span; a.n = n; a.k = k;
-  a.tiles_wk = (int)vx_cdiv(k, t);
-  a.tiles_w = (int)(vx_cdiv(n, t) * a.tiles_wk);
-  a.tiles_xk = a.tiles_wk;
-  const int64_t bw = dw ? a.tiles_w * p.splits : 0, bx = dx ? vx_cdiv(m, t) * a.tiles_xk : 0;
-  VX_REQUIRE(bw + bx + sums < (1LL << 31), "linear_bwd: too many rows");
-  a.blocks_w = (unsigned)bw;
-  a.blocks_x = (unsigned)bx;
-  if (bw + bx + sums) {
-    const bool fast = vx_fast(a.g, a.ldg, n, sizeof(T)) && vx_fast(a.x, a.ldx, k, sizeof(T)) && vx_fast(a.w, a.ldw, k, sizeof(T));
-    const auto kernel = p.big ? (fast ? linear_bwd<T, 128, 128, true> : linear_bwd<T, 128, 128, false>)
-                              : (fast ? linear_bwd<T, 64, 64, true> : linear_bwd<T, 64, 64, false>);
-    kernel<<<(unsigned)(bw + bx + sums), kTileThreads, 0, s>>>(a, rows);
-    VX_LAUNCH_CHECK();
-  }
+  const auto products = [&](const auto* g, int64_t ldg, int64_t sums) {
+    using G = std::remove_const_t<std::remove_pointer_t<decltype(g)>>;
+    BwdArgs<T, G> a{};
+    a.g = g; a.x = x; a.w = w; a.dx = dx; a.dw = dw;
+    a.slab = p.splits > 1 ? slab : nullptr;
+    a.ldg = ldg; a.ldx = ldx; a.ldw = ldw; a.m = m; a.n = n; a.k = k;
+    return launch_bwd(a, p, rows, sums, s);
+  };
+  int32_t rc;
+  if (act == VX_ACT_NONE)
+    rc = products(dy, lddy, dbias ? cols * p.chunks : 0);          // the column sums run beside the products
+  else if (wide)
+    rc = products((const float*)wide, n, 0);
+  else
+    rc = products((const T*)dpre, n, 0);
+  if (rc) return rc;
   const int64_t len_w = dw && p.splits > 1 ? (int64_t)n * k : 0, len_b = dbias ? n : 0;
   const unsigned ga = (unsigned)vx_cdiv(len_w, 1024), gb = (unsigned)vx_cdiv(len_b, 64);
   if (ga + gb) {
@@ -474,10 +506,12 @@ extern "C" int32_t vx_linear_fwd(const void* d_x, int64_t ldx, const void* d_wei
                            (__bf16*)d_y, (__bf16*)d_pre, ldx, ldw, ldr, m, n, k, act, 0}, (hipStream_t)stream);
 }
 
+extern "C" size_t vx_linear_bwd_act_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t act, int32_t dtype) {
+  return m <= 0 || n <= 0 || k <= 0 ? 0 : bwd_bytes(m, n, k, act, dtype);
+}
+
 extern "C" size_t vx_linear_bwd_workspace_bytes(int64_t m, int32_t n, int32_t k, int32_t dtype) {
-  if (m <= 0 || n <= 0 || k <= 0) return 0;
-  const BwdPlan p = bwd_plan(m, n, k, dtype);
-  return vx_align(p.splits > 1 ? (size_t)p.splits * n * k * 4 : 0) + vx_align((size_t)p.chunks * n * 4);
+  return vx_linear_bwd_act_workspace_bytes(m, n, k, VX_ACT_GELU, dtype);
 }
 
 extern "C" int32_t vx_linear_bwd(const void* d_dy, int64_t lddy, const void* d_x, int64_t ldx, const void* d_weight, int64_t ldw,
@@ -498,7 +532,7 @@ extern "C" int32_t vx_linear_bwd(const void* d_dy, int64_t lddy, const void* d_x
   VX_REQUIRE(d_dy && d_x && d_weight, "linear_bwd: null pointer");
   VX_REQUIRE(lddy >= 0 && ldx >= 0 && ldw >= 0, "linear_bwd: negative row stride");
   VX_REQUIRE(act == VX_ACT_NONE || (d_saved && d_dpre), "linear_bwd: an activation needs d_saved and d_dpre");
-  if (workspace_bytes < vx_linear_bwd_workspace_bytes(m, n, k, dtype) || !d_workspace) {
+  if (workspace_bytes < bwd_bytes(m, n, k, act, dtype) || !d_workspace) {
     vx_set_error("linear_bwd: workspace too small");
     return VX_ERR_WORKSPACE;
   }

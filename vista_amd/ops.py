@@ -665,9 +665,9 @@ def _linear_sizes(x, weight):
 
 
 @functools.lru_cache(maxsize=1024)
-def _linear_bwd_bytes(device, m, n, k, dtype):
+def _linear_bwd_bytes(device, m, n, k, act, dtype):
     with torch.cuda.device(device):
-        return L.lib().vx_linear_bwd_workspace_bytes(m, n, k, dtype)
+        return L.lib().vx_linear_bwd_act_workspace_bytes(m, n, k, act, dtype)
 
 
 def linear_fwd(x, weight, bias=None, residual=None, act="none", want_pre=False):
@@ -715,7 +715,7 @@ def linear_bwd(dy, x, weight, act="none", saved=None, want_dx=True, want_dw=True
     dx = x.new_empty((m, k)) if want_dx else None
     dw = x.new_empty((n, k)) if want_dw else None
     db = x.new_empty((n,)) if want_dbias else None
-    wsb = _linear_bwd_bytes(dev.index, m, n, k, _DT[dt])
+    wsb = _linear_bwd_bytes(dev.index, m, n, k, code, _DT[dt])
     ws = _ws(wsb, dev)
     rc = _launch(dev, L.lib().vx_linear_bwd, g.data_ptr(), g.stride(0), x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0),
                  _at(saved) if code else None, m, n, k, code, dpre.data_ptr() if code else None, _at(dx), _at(dw), _at(db), _DT[dt],
