@@ -282,3 +282,27 @@ def test_layer_gradients_workspace_follows_the_activation():
     assert [lib.vx_linear_bwd_workspace_bytes(m, n, k, dtype) for dtype in (0, 1)] == [size[0][0], size[1][2]]
     call = lambda act, room: lib.vx_linear_bwd(FAKE, n, FAKE, k, FAKE, k, FAKE, m, n, k, act, FAKE, FAKE, FAKE, FAKE, 1, FAKE, room, None)  # noqa: E731
     assert call(2, size[1][2] - 1) == ERR_WS and call(3, size[1][0]) == ERR_WS and call(1, size[1][1] - 1) == ERR_WS
+
+
+SHAPES = [(4, 25600, 25600, 2, 2, 1, 192, 384), (8, 25600, 25600, 8, 8, 8, 48, 48), (1, 1024, 57000, 16, 16, 16, 8, 8),
+          (1, 25600, 1920, 2, 2, 1, 192, 384), (1, 400000, 1920, 2, 2, 1, 192, 384), (4, 1600, 480, 2, 2, 1, 192, 384),
+          (1, 200000, 16, 8, 8, 8, 64, 64), (64, 65, 5001, 8, 4, 2, 40, 60), (1, 3100, 60001, 1, 1, 1, 16, 24), (2, 3000, 129, 16, 16, 16, 32, 32),
+          *((4, n, k, 2, 2, 1, 192, 384) for n in (200000, 800000) for k in (200, 2000, 20000))]
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_backward_workspace_keeps_its_limits(shape, dtype):
+    """Term by term: P and dS of one chunk (1 GiB, or 128 queries of every head where that is more), the slabs of ONE chunk, delta, the
+    lists of keys and gathered k and v. Slabs: 2 a CU of at most 128 x 192 tiles in all (512 * 128 * 192 floats), or a split for every
+    2 k_len queries of a chunk, rounded up. None of it but delta grows with the number of chunks."""
+    b, sq, sk, h, hk, hv, d, dv = shape
+    bh, skp, e = b * h, -(-sk // 8) * 8, (4, 2)[dtype]
+    chunk = max(1 << 30, 2 * bh * 128 * skp * 4)
+    slabs = max(512 * 128 * 192 * 4, bh * (d + dv) * 4 * (min(sq, max(2 ** 29 // (bh * skp * 4), 128)) // 2 + sk))
+    rest = bh * sq * 4 + 8 * b * sk + 4 * b + b * sk * (hk * d + hv * dv) * e
+    size = _lib.lib().vx_attn_bwd_workspace_bytes(i64(*shape), dtype)
+    assert size <= chunk + slabs + rest + 9 * 256
+    small = 2 * bh * min(sq, 128) * skp * 4 + bh * sk * (d + dv) * 4 + rest                       # (it is a real amount)
+    assert size >= small // 2
+

@@ -410,6 +410,19 @@ def test_bf16_attention_gradients_are_rounded_once(shape, scale, dev):
         off_by_its_rounding(got, ref[name][0], name, 1.02)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_gradients_over_many_chunks(dtype, dev):
+    """Few queries over very many keys: four chunks of equal length whose last is shorter; dk and dv are summed over all of them."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((1, 3100, 60001, 1, 1, 1, 16, 24), dtype, dev, 16, "some", poison=True)
+    ref = attn_reference(q, k, v, km, do)
+    out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    within(out, *ref["out"], "out")
+    stale(1 << 28, dev=dev)
+    for name, got in zip(("dq", "dk", "dv"), ops.attn_bwd(do, q, k, v, out, stats, km)):
+        within(got, *ref[name], name)
+
+
 @pytest.mark.parametrize("k_len,live", [(2, 2), (5, 3), (16, 10), (40, 26), (128, 128)])
 def test_bf16_gradients_over_few_keys_lose_nothing(k_len, live, dev):
     """Over at most 128 keys P and dS are 16-bit operands and delta is summed from P dP itself: what is left beside the gradients' own

@@ -568,7 +568,8 @@ struct BwdArgs : AttnArgs<T> {
   int q0, rows, skp;                         // present chunk: queries [q0, q0 + rows); skp: sk rounded up to 8
   long long kc_b, kc_h, vc_b, vc_h;          // gathered k, v: [b][head][sk][d], [b][head][sk][dv]
   T *kc, *vc;
-  int bh, split0, span;                      // first split of the chunk, queries of one split
+  int bh, span;                              // queries of one split
+  bool add;                                  // a later chunk: the slabs hold the sums of the earlier ones
   int tqp, tkp;                              // tiles of attn_pds: queries, keys
   int tq, tk, td, tdv;                       // tiles of attn_grads: queries, keys, columns of dK and dQ, columns of dV
   unsigned n_v, n_k, n_q;                    // workgroups per problem
@@ -760,9 +761,15 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
     const VxOperand<T> W{is_v ? a.go + b * a.go_b + q * a.go_s + h * a.go_h + n0 : a.q + b * a.q_b + q * a.q_s + h * a.q_h + n0,
                          is_v ? a.go_s : a.q_s, rows_n};
     vx_gemm_loop<T, KS, KS, TM, TN, FAST, BK, float, PX>(X, W, 0, len, lds, acc);
-    float* slab = (is_v ? a.slab_v : a.slab_k) + ((long long)(a.split0 + sp) * a.bh + bh) * a.sk * width;
-    vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, const vx_f32x4& v, const vx_f32x4& w) {
-      if (m < rows_m && n < rows_n) vx_store8(slab + (long long)(m0 + m) * width + n0 + n, v, w, rows_n - n);
+    float* slab = (is_v ? a.slab_v : a.slab_k) + ((long long)sp * a.bh + bh) * a.sk * width;
+    vx_acc_each<TM, TN>(acc, [&](int, int m, int, int n, vx_f32x4 v, vx_f32x4 w) {
+      if (m >= rows_m || n >= rows_n) return;
+      float* at = slab + (long long)(m0 + m) * width + n0 + n;
+      if (a.add) {
+        v += vx_load4(at, rows_n - n);
+        w += vx_load4(at + 4, rows_n - n - 4);
+      }
+      vx_store8(at, v, w, rows_n - n);
     });
   } else {
     unsigned w = vx_xcd_tile(blockIdx.x - a.n_v - a.n_k, a.n_q);
@@ -1010,12 +1017,12 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
 
 struct BwdPlan {
   bool one;                                             // all keys fit one tile of attn_pds
-  int64_t tp, tm, tn, skp, span, per_chunk, splits, chunk;  // queries per split, splits per chunk, all splits, queries per chunk
+  int64_t tp, tm, tn, skp, span, splits, chunk;         // queries per split, splits and queries per chunk
   size_t delta, pds, slab_k, slab_v, live, kc, vc;      // bytes
   size_t total() const { return delta + 2 * pds + slab_k + slab_v + live + kc + vc; }
 };
-// queries are cut into splits (one slab each) and the splits into chunks, whose probabilities and score gradients are in
-// memory at a time (at most kChunkBytes of both, but a tile of queries of every head at least)
+// queries are cut into chunks, whose probabilities and score gradients are in memory at a time (at most kChunkBytes of both, but a
+// tile of queries of every head at least), and a chunk into splits, one slab each; later chunks add to the slabs of the first
 constexpr size_t kChunkBytes = (size_t)1 << 30;
 BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   BwdPlan p;
@@ -1029,20 +1036,18 @@ BwdPlan bwd_plan(const Shape& s, int32_t dtype) {
   p.tm = !p.one && t128 >= 2 * cus ? 128 : 64;
   // wide heads: 192 and 384 columns without a ragged tile, and less staging per product (a lane stages 3 or 6 columns at a time)
   p.tn = !p.one && s.d > 128 && s.d % 24 == 0 && s.dv % 24 == 0 ? 192 : p.tm;
+  int64_t fit = (int64_t)(kChunkBytes / 2) / (bh * p.skp * 4) / p.tm * p.tm;      // queries of a chunk
+  if (fit < p.tm) fit = p.tm;
+  const int64_t chunks = vx_cdiv(s.sq, fit);
+  p.chunk = chunks == 1 ? s.sq : vx_cdiv(vx_cdiv(s.sq, chunks), p.tm) * p.tm;     // equal ones; no more than fit, a multiple of tm
   const int64_t tiles = vx_cdiv(s.sk, p.tm) * (vx_cdiv(s.dv, p.tn) + vx_cdiv(s.d, p.tn)) * bh;
   int64_t splits = 2 * cus / (tiles > 0 ? tiles : 1);
-  if (splits < vx_cdiv(s.sq, 2 * s.sk)) splits = vx_cdiv(s.sq, 2 * s.sk);       // no workgroup much longer than those of dQ
-  const int64_t most = vx_cdiv(s.sq, 4 * bk);
+  if (splits < vx_cdiv(p.chunk, 2 * s.sk)) splits = vx_cdiv(p.chunk, 2 * s.sk);   // no workgroup much longer than those of dQ
+  const int64_t most = vx_cdiv(p.chunk, 4 * bk);
   if (splits > most) splits = most;
-  int64_t fit = (int64_t)(kChunkBytes / 2) / (bh * p.skp * 4);       // queries of a chunk
-  if (fit < p.tm) fit = p.tm;
-  if (splits < vx_cdiv(s.sq, fit)) splits = vx_cdiv(s.sq, fit);
   if (splits < 1) splits = 1;
-  p.span = vx_cdiv(vx_cdiv(s.sq, splits), p.tm) * p.tm;
-  p.splits = vx_cdiv(s.sq, p.span);
-  p.per_chunk = fit / p.span < 1 ? 1 : fit / p.span;
-  if (p.per_chunk > p.splits) p.per_chunk = p.splits;
-  p.chunk = p.per_chunk * p.span < s.sq ? p.per_chunk * p.span : s.sq;
+  p.span = vx_cdiv(vx_cdiv(p.chunk, splits), p.tm) * p.tm;
+  p.splits = vx_cdiv(p.chunk, p.span);
   p.delta = vx_align((size_t)bh * s.sq * 4);
   p.pds = vx_align((size_t)bh * p.chunk * p.skp * 4);
   p.slab_k = vx_align((size_t)p.splits * bh * s.sk * s.d * 4);
@@ -1124,10 +1129,10 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
     a.mask = nullptr;
   }
   const bool fast = args_fast(a) && heads_fast(a.go, a.go_b, a.go_s, a.go_h, sh.dv, sizeof(T)) && p.skp < (1 << 21);
-  for (int64_t q0 = 0, split = 0; q0 < sh.sq; q0 += p.chunk, split += p.per_chunk) {
+  for (int64_t q0 = 0; q0 < sh.sq; q0 += p.chunk) {
     a.q0 = (int)q0;
     a.rows = (int)(sh.sq - q0 < p.chunk ? sh.sq - q0 : p.chunk);
-    a.split0 = (int)split;
+    a.add = q0 > 0;
     a.tq = (int)vx_cdiv(a.rows, p.tm);
     const int64_t here = vx_cdiv(a.rows, p.span);
     const int64_t nv = here * bh * a.tk * a.tdv, nk = here * bh * a.tk * a.td, nq = (int64_t)a.tq * a.td * bh;
