@@ -396,8 +396,9 @@ int32_t vx_linear_bwd(const void* d_dy, int64_t lddy, const void* d_x, int64_t l
  *          it: VX_F32, or at most 128 keys) or NULL. It carries what the rounding of d_out to bf16 left behind to the backward pass,
  *          whose row sums of d_dout * out would lack it: gradients of rows that few keys dominate lose two bits without it
  * Statistics, probabilities, score gradients and sums are fp32; matrix arithmetic as in vx_linear_*: beside VX_BF16 operands
- * probabilities and score gradients are rounded to 16 bits. Infinities and NaN
- * in rows that take part give NaN; in masked rows they are never read. No atomics: bitwise reproducible.
+ * probabilities and score gradients are rounded to 16 bits. NaN in rows that take part gives
+ * NaN, and so do infinities with VX_F32; with VX_BF16 they follow the formula (a score of -inf has weight 0). A query whose scores all
+ * leave the range of fp32 gives NaN. What masked rows hold has no effect. No atomics: bitwise reproducible.
  * ------------------------------------------------------------------------------------------- */
 #define VX_ATTN_MAX_DIM 192
 #define VX_ATTN_MAX_VDIM 384

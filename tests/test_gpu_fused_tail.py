@@ -450,6 +450,33 @@ def test_attention_of_large_scores(dev):
             within(got, *ref[name], name)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(1, 5, 40, 2, 2, 1, 32, 48), (1, 3, 3000, 1, 1, 1, 64, 64), (2, 300, 200, 2, 2, 1, 48, 96)])
+def test_scores_past_the_range_are_no_missing_keys(shape, dtype, dev):
+    """A query whose scores all overflow (to -inf, or to +inf when scaled) has keys: NaN, not the zeros of a query without any; the
+    other queries do not see it. Direct, split and packed keys."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn(shape, dtype, dev, 31, "some")
+    km[:, -1] = True
+    k[..., 0] = k[..., 0].abs() + 0.5
+    q[:, 1] = 0.0
+    q[:, 1, :, 0] = -1e38                                  # scores of -1e37 and below, all of one sign
+    kk = k * 100.0                                         # ... past -3.4e38: -inf
+    rest = torch.ones(shape[1], dtype=torch.bool, device=dev)
+    rest[1] = False
+    out, st = ops.attn_fwd(q, kk, v, km, 0.01 * shape[6] ** -0.5, want_stats=True)
+    assert torch.isnan(out[:, 1]).all() and torch.isfinite(out[:, rest]).all()
+    dq, dk, dv = ops.attn_bwd(do, q, kk, v, out, st, km, 0.01 * shape[6] ** -0.5)
+    assert torch.isnan(dq[:, 1]).all() and torch.isfinite(dq[:, rest]).all()
+    q[:, 1, :, 0] = 1e37                                   # finite scores, above the range when scaled
+    k[..., 0] = 2.0
+    out, st = ops.attn_fwd(q, k, v, km, 1e3, want_stats=True)
+    assert torch.isnan(out[:, 1]).all() and torch.isfinite(out[:, rest]).all()
+    km[0] = False                                          # without keys: zeros all the same
+    out, st = ops.attn_fwd(q, k, v, km, 1e3, want_stats=True)
+    assert not out[0].any() and not ops.attn_bwd(do, q, k, v, out, st, km, 1e3)[0][0].any()
+
+
 def test_attention_without_keys_or_queries(dev):
     from vista_amd import ops
     q, k, v = (torch.randn(2, n, 2, 16, device=dev) for n in (5, 0, 0))

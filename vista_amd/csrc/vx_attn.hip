@@ -7,8 +7,11 @@
 // statistics, probabilities and sums over queries are fp32; for bf16 tensors the probabilities are rounded to 16 bits (two planes) where
 // they become operands: to 8 bits, their errors would be about as large as the output's own rounding (2-norm 0.0024 of the output
 // instead of 0.0017). The backward pass keeps P and dS in fp32; as operands beside bf16 ones they are two planes as well.
-// A masked key has no part in anything, whatever its rows hold; a query without keys gives zeros. No atomics: bitwise
+// A masked key has no part in anything, whatever its rows hold; a query without keys gives zeros, one whose scores all leave fp32's range
+// NaN. No atomics: bitwise
 // reproducible.
+#include <float.h>
+
 #include "vx_tile.h"
 
 namespace {
@@ -213,6 +216,7 @@ void attn_fwd(const FwdArgs<T> a) {
 
   unsigned long long cur, nxt = 0;
   int t = find(t0, cur), tn = t1;
+  const bool any = cur != 0;                   // this workgroup has keys
   if (cur) {
     tn = find(t + 1, nxt);
     if constexpr (IMG) {
@@ -362,11 +366,12 @@ void attn_fwd(const FwdArgs<T> a) {
     const int n0 = half * NV * 16 + g * 4;
     if (a.splits > 1) {
       const long long at = ((long long)split * gridDim.x / (a.tiles_q * a.splits) + bh) * a.sq + row;
-      if (g == 0 && half == 0) a.part_ml[at] = make_float2(m[rt], sum);
+      // keys whose scores are all -inf count as keys: attn_join tells them from none by the maximum
+      if (g == 0 && half == 0) a.part_ml[at] = make_float2(any && m[rt] == -INFINITY ? -FLT_MAX : m[rt], sum);
 #pragma unroll
       for (int nv = 0; nv < NV; ++nv) vx_store4(a.part + at * a.dv + n0 + nv * 16, o[rt][nv], a.dv - n0 - nv * 16);
     } else {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const float inv = any ? 1.0f / sum : 0.0f;         // a sum of 0 over keys: every score left the range, 0 / 0 = NaN
       if (a.stats && g == 0 && half == 0) a.stats[(long long)bh * a.sq + row] = make_float2(m[rt], inv);
       const long long at = (((long long)b * a.sq + row) * a.h + h) * a.dv + n0;
 #pragma unroll
@@ -548,7 +553,7 @@ __global__ __launch_bounds__(256) void attn_join(const FwdArgs<T> a, long long i
     }
   }
   if (!here) return;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;    // no keys in any split
   const int bh = (int)(rowid / a.sq), row = (int)(rowid % a.sq), b = bh / a.h, h = bh % a.h;
   attn_put(a, (((long long)b * a.sq + row) * a.h + h) * a.dv + n, o * inv, a.dv - n);
   if (a.stats && n == 0) a.stats[rowid] = make_float2(m, inv);
