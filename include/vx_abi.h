@@ -391,7 +391,8 @@ int32_t vx_linear_bwd(const void* d_dy, int64_t lddy, const void* d_x, int64_t l
  * vx_attn_fwd  d_out [batch][q_len][heads][v_dim]; d_stats f32[batch * heads][q_len][2] or NULL: what the backward pass
  *          needs (maximum of log2(e) * scale * score, 1 / sum)
  * vx_attn_bwd  d_dout with its own strides HOST int64[3] (batch, position, head), d_out and d_stats of the forward pass ->
- *          d_dq [batch][q_len][heads][dim], d_dk [batch][k_len][k_heads][dim], d_dv [batch][k_len][v_heads][v_dim]
+ *          d_dq [batch][q_len][heads][dim], d_dk [batch][k_len][k_heads][dim], d_dv [batch][k_len][v_heads][v_dim]; each of the three may
+ *          be NULL: its products are left out
  * vx_attn_fwd_rest, vx_attn_bwd_rest  the same with d_rest: vx_attn_rest_bytes bytes (0 where the backward pass has no use for
  *          it: VX_F32, or at most 128 keys) or NULL. It carries what the rounding of d_out to bf16 left behind to the backward pass,
  *          whose row sums of d_dout * out would lack it: gradients of rows that few keys dominate lose two bits without it

@@ -306,3 +306,10 @@ def test_backward_workspace_keeps_its_limits(shape, dtype):
     small = 2 * bh * min(sq, 128) * skp * 4 + bh * sk * (d + dv) * 4 + rest                       # (it is a real amount)
     assert size >= small // 2
 
+
+
+def test_no_gradient_wanted_launches_nothing():
+    lib = _lib.lib()
+    call = lambda dout: lib.vx_attn_bwd(dout, i64(1, 1, 1), FAKE, FAKE, FAKE, None, i64(*GOOD), i64(*(1,) * 10), FAKE, FAKE, 1.0,  # noqa: E731
+                                        None, None, None, 0, FAKE, 1 << 40, None)
+    assert call(FAKE) == 0 and call(None) == ERR_ARG

@@ -595,6 +595,40 @@ def test_autograd_returns_what_is_asked(dev):
         gk.sum().backward()
 
 
+@pytest.mark.parametrize("shape", [(2, 200, 150, 4, 2, 1, 48, 96), (1, 70, 40, 2, 2, 1, 33, 50), (1, 3000, 60000, 1, 1, 1, 16, 24)])
+def test_only_wanted_gradients_are_made(shape, dev):
+    """Each subset of the three, from the plain call and through autograd: the bits of the full call, None for the others."""
+    from vista_amd import ops
+    from vista_amd.fused_tail import attention
+    q, k, v, km, do = make_attn(shape, F32, dev, 1, "some")
+    out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    full = ops.attn_bwd(do, q, k, v, out, stats, km)
+    calls = []
+    real, ops._launch = ops._launch, lambda d, fn, *a: (calls.append((fn.__name__, a)), real(d, fn, *a))[1]
+    try:
+        for bits in range(8):
+            want = [bool(bits >> i & 1) for i in range(3)]
+            got = ops.attn_bwd(do, q, k, v, out, stats, km, None, *want)
+            assert all((g is None) if not w else torch.equal(g, f) for g, f, w in zip(got, full, want))
+            leaves = [t.clone().requires_grad_(w) for t, w in zip((q, k, v), want)]
+            calls.clear()
+            y = attention(*leaves, key_mask=km)
+            assert y.requires_grad == any(want)
+            if not any(want):
+                continue
+            y.backward(do)
+            assert all((t.grad is None) if not w else torch.equal(t.grad, f) for t, f, w in zip(leaves, full, want))
+            (args,) = [a for name, a in calls if "bwd" in name]
+            assert [a is not None for a in args[12:15]] == want          # no room, and no work, for the others
+    finally:
+        ops._launch = real
+    z = torch.zeros(2, 0, 2, 16, device=dev)
+    q0 = torch.randn(2, 5, 2, 16, device=dev)
+    o0, s0 = ops.attn_fwd(q0, z, z, want_stats=True)
+    dq, dk, dv = ops.attn_bwd(torch.ones_like(o0), q0, z, z, o0, s0, want_dk=False)
+    assert not dq.any() and dk is None and dv.shape == z.shape
+
+
 def test_on_another_stream(dev):
     from vista_amd import ops
     q, k, v, km, do = make_attn((2, 200, 100, 2, 2, 1, 48, 96), F32, dev, 1, "some")

@@ -567,7 +567,7 @@ struct BwdArgs : AttnArgs<T> {
   const float2* stats;
   float* delta;                              // [b*h][sq]
   float *p, *ds;                             // [b*h][rows][skp] of the present chunk of queries
-  T *dq, *dk, *dvv;                          // [b][sq][h][d], [b][sk][h/gk][d], [b][sk][h/gv][dv]
+  T *dq, *dk, *dvv;                          // [b][sq][h][d], [b][sk][h/gk][d], [b][sk][h/gv][dv]; null: not wanted
   float *slab_k, *slab_v;                    // [splits][b*h][sk][d], [splits][b*h][sk][dv]
   float scale;
   int q0, rows, skp;                         // present chunk: queries [q0, q0 + rows); skp: sk rounded up to 8
@@ -1140,7 +1140,8 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
     a.add = q0 > 0;
     a.tq = (int)vx_cdiv(a.rows, p.tm);
     const int64_t here = vx_cdiv(a.rows, p.span);
-    const int64_t nv = here * bh * a.tk * a.tdv, nk = here * bh * a.tk * a.td, nq = (int64_t)a.tq * a.td * bh;
+    const int64_t nv = a.dvv ? here * bh * a.tk * a.tdv : 0, nk = a.dk ? here * bh * a.tk * a.td : 0;
+    const int64_t nq = a.dq ? (int64_t)a.tq * a.td * bh : 0;
     const int64_t pds = (int64_t)a.tkp * vx_cdiv(a.rows, p.tp) * bh, grads = nv + nk + nq;
     VX_REQUIRE(pds < (1LL << 31) && grads < (1LL << 31), "attn_bwd: too many tiles");
     a.n_v = (unsigned)nv;
@@ -1152,8 +1153,9 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
     if (rc) return rc;
   }
   const int64_t iv = sh.b * sh.hv * sh.sk * vx_cdiv(sh.dv, 4), ik = sh.b * sh.hk * sh.sk * vx_cdiv(sh.d, 4);
-  const int64_t gv = vx_cdiv(iv, 256), gk = vx_cdiv(ik, 256);
+  const int64_t gv = a.dvv ? vx_cdiv(iv, 256) : 0, gk = a.dk ? vx_cdiv(ik, 256) : 0;
   VX_REQUIRE(gv + gk < (1LL << 31), "attn_bwd: too many keys");
+  if (gv + gk == 0) return VX_OK;
   attn_slab_sum<T><<<(unsigned)(gv + gk), 256, 0, s>>>(a, (int)p.splits, (unsigned)gv, iv, ik);
   VX_LAUNCH_CHECK();
   return VX_OK;
@@ -1247,22 +1249,22 @@ extern "C" int32_t vx_attn_bwd_rest(const void* d_dout, const int64_t* dout_stri
   if (s.b == 0 || s.sq == 0 || s.sk == 0) {          // nothing attends: zero gradients
     const size_t nq = (size_t)s.b * s.sq * s.h * s.d * e, nk = (size_t)s.b * s.sk * s.hk * s.d * e,
                  nv = (size_t)s.b * s.sk * s.hv * s.dv * e;
-    if (nq)
+    if (nq && d_dq)
       if (int32_t rc = vx_fill_async(d_dq, 0, nq, st)) return rc;
-    if (nk)
+    if (nk && d_dk)
       if (int32_t rc = vx_fill_async(d_dk, 0, nk, st)) return rc;
-    if (nv)
+    if (nv && d_dv)
       if (int32_t rc = vx_fill_async(d_dv, 0, nv, st)) return rc;
     return VX_OK;
   }
-  VX_REQUIRE(strides && dout_strides && d_dout && d_q && d_k && d_v && d_out && d_stats && d_dq && d_dk && d_dv,
-             "attn_bwd: null pointer");
+  VX_REQUIRE(strides && dout_strides && d_dout && d_q && d_k && d_v && d_out && d_stats, "attn_bwd: null pointer");
   for (int i = 0; i < 10; ++i) VX_REQUIRE(strides[i] >= 0, "attn_bwd: negative stride");
   for (int i = 0; i < 3; ++i) VX_REQUIRE(dout_strides[i] >= 0, "attn_bwd: negative stride");
   if (workspace_bytes < bwd_plan(s, dtype).total() || !d_workspace) {
     vx_set_error("attn_bwd: workspace too small");
     return VX_ERR_WORKSPACE;
   }
+  if (!d_dq && !d_dk && !d_dv) return VX_OK;
   const auto typed = dtype == VX_F32 ? attn_bwd_typed<float> : attn_bwd_typed<__bf16>;
   return typed(s, d_dout, dout_strides, d_q, d_k, d_v, d_key_mask, strides, d_out, d_stats, d_rest, scale, d_dq, d_dk, d_dv, dtype,
                d_workspace, st);

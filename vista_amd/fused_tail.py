@@ -30,7 +30,7 @@ class _AttentionFn(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, key_mask, out, stats = ctx.saved_tensors
         ops._check_seen(dout)        # (out's shape, dtype and device: the engine sees to that)
-        dq, dk, dv = ops._attn_bwd_run(dout, q, k, v, key_mask, ctx.geo, out, stats, ctx.scale)
+        dq, dk, dv = ops._attn_bwd_run(dout, q, k, v, key_mask, ctx.geo, out, stats, ctx.scale, ctx.needs_input_grad[:3])
         return dq, dk, dv, None, None
 
 

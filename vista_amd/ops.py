@@ -799,9 +799,9 @@ def _attn_fwd_run(q, k, v, key_mask, geo, scale, want_stats):
     return out, stats
 
 
-def attn_bwd(dout, q, k, v, out, stats, key_mask=None, scale=None):
-    """Gradients of attn_fwd from its own out and stats -> (dq, dk, dv), shaped as q, k and v; the probabilities are recomputed.
-    Gradients of masked keys are 0."""
+def attn_bwd(dout, q, k, v, out, stats, key_mask=None, scale=None, want_dq=True, want_dk=True, want_dv=True):
+    """Gradients of attn_fwd from its own out and stats -> (dq, dk, dv), shaped as q, k and v; an unwanted one is None. The
+    probabilities are recomputed. Gradients of masked keys are 0."""
     _check_seen(dout)
     q, k, v, key_mask, geo = _attn_args(q, k, v, key_mask)
     _check_tensors(q, "q", (dout, out), ("dout", "out"))
@@ -811,19 +811,19 @@ def attn_bwd(dout, q, k, v, out, stats, key_mask=None, scale=None):
     _need_gpu(stats, "stats")
     if stats.dtype != torch.float32 or stats.shape != geo.stats or not stats.is_contiguous() or stats.device != dev:
         raise ValueError("stats must be what attn_fwd(want_stats=True) returned")
-    return _attn_bwd_run(dout, q, k, v, key_mask, geo, out, stats, scale)
+    return _attn_bwd_run(dout, q, k, v, key_mask, geo, out, stats, scale, (want_dq, want_dk, want_dv))
 
 
-def _attn_bwd_run(dout, q, k, v, key_mask, geo, out, stats, scale):
+def _attn_bwd_run(dout, q, k, v, key_mask, geo, out, stats, scale, want):
     dev = q.device
     dout = _heads_last(dout)
     dout_strides = (ctypes.c_int64 * 3)(*dout.stride()[:3])
-    dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
+    dq, dk, dv = (q.new_empty(t.shape) if w else None for t, w in zip((q, k, v), want))
     ws = _ws(geo.bwd_bytes, dev)
     rest = stats.data_ptr() + geo.rest if geo.rest is not None else None
     rc = _launch(dev, L.lib().vx_attn_bwd_rest, dout.data_ptr(), dout_strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(key_mask),
                  geo.shape, geo.strides, out.data_ptr(), stats.data_ptr(), rest, geo.scale if scale is None else float(scale),
-                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _DT[q.dtype], ws.data_ptr(), geo.bwd_bytes)
+                 _at(dq), _at(dk), _at(dv), _DT[q.dtype], ws.data_ptr(), geo.bwd_bytes)
     if rc:
         L.check(rc, "vx_attn_bwd_rest")
     return dq, dk, dv
