@@ -361,7 +361,8 @@ int32_t vx_nms_bev(const float* d_boxes, int32_t num_boxes, float thresh, int32_
  *                sums of g; each of the three may be NULL
  * vx_linear_bwd_act_workspace_bytes  the workspace for one activation; vx_linear_bwd_workspace_bytes is enough for each (with
  *                VX_BF16, VX_ACT_GELU and _SILU keep g in fp32 for the two products: m * n * 4 bytes more)
- * Row strides are in elements, >= 0 (0 repeats a row), the last dimension is contiguous. m < 2^31; n, k <= 2^20. m = 0 gives
+ * Row strides are in elements, >= 0 (0 repeats a row), the last dimension is contiguous. m < 2^31; n, k <= 2^20; a call
+ * whose tiles (64 x 64 at least) would need a launch of 2^32 work items or more is refused. m = 0 gives
  * zero parameter gradients. No atomics: bitwise reproducible. VX_ACT_GELU is the erf form. An infinity or NaN in an fp32 operand
  * gives NaN (not an infinity) in every output it reaches: its planes are not numbers.
  * ------------------------------------------------------------------------------------------- */

@@ -313,3 +313,18 @@ def test_no_gradient_wanted_launches_nothing():
     call = lambda dout: lib.vx_attn_bwd(dout, i64(1, 1, 1), FAKE, FAKE, FAKE, None, i64(*GOOD), i64(*(1,) * 10), FAKE, FAKE, 1.0,  # noqa: E731
                                         None, None, None, 0, FAKE, 1 << 40, None)
     assert call(FAKE) == 0 and call(None) == ERR_ARG
+
+
+def test_launches_past_the_limit_are_refused():
+    """One launch has fewer than 2^32 work items: what would need more (and a tensor of that size could be there) is refused by name."""
+    lib = _lib.lib()
+    rows = (1 << 31) - 1                                   # 2^24 tiles of 128 rows, 256 work items each
+    assert lib.vx_linear_fwd(FAKE, 1, FAKE, 1, None, None, 0, rows, 1, 1, 0, FAKE, None, 0, None) == ERR_ARG
+    assert b"too many" in lib.vx_last_error()
+    assert lib.vx_linear_bwd(FAKE, 1, FAKE, 1, FAKE, 1, None, rows, 1, 1, 0, None, FAKE, None, None, 0, FAKE, 1 << 40, None) == ERR_ARG
+    assert b"too many" in lib.vx_last_error()
+    many = (1 << 23, 100, 20, 1, 1, 1, 4, 4)
+    assert fwd(many) == ERR_ARG and b"too many" in lib.vx_last_error()
+    assert lib.vx_attn_bwd(FAKE, i64(1, 1, 1), FAKE, FAKE, FAKE, None, i64(*many), i64(*(1,) * 10), FAKE, FAKE, 1.0, FAKE, FAKE, FAKE, 0,
+                           FAKE, 1 << 45, None) == ERR_ARG
+    assert b"too many" in lib.vx_last_error()

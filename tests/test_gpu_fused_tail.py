@@ -423,6 +423,18 @@ def test_attention_gradients_over_many_chunks(dtype, dev):
         within(got, *ref[name], name)
 
 
+def test_attention_gradients_of_very_many_rows(dev):
+    """More rows than the waves of one launch that sums dout * out: 64 x 16 x 4200 of them. The first and the last batch by themselves."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((64, 4200, 130, 16, 1, 1, 8, 8), BF16, dev, 17, "some")
+    out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    grads = ops.attn_bwd(do, q, k, v, out, stats, km)
+    for b in (slice(0, 1), slice(63, 64)):
+        ref = attn_reference(q[b], k[b], v[b], km[b], do[b])
+        for name, got in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+            within(got[b], *ref[name], name)
+
+
 @pytest.mark.parametrize("k_len,live", [(2, 2), (5, 3), (16, 10), (40, 26), (128, 128)])
 def test_bf16_gradients_over_few_keys_lose_nothing(k_len, live, dev):
     """Over at most 128 keys P and dS are 16-bit operands and delta is summed from P dP itself: what is left beside the gradients' own

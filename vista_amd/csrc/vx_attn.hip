@@ -636,22 +636,22 @@ __global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long 
     }
     return;
   }
-  const long long r = (long long)(blockIdx.x - head) * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
   const int lane = threadIdx.x & 63;
-  const int bh = (int)(r / a.sq), row = (int)(r % a.sq), b = bh / a.h, h = bh % a.h;
-  const T* go = a.go + b * a.go_b + row * a.go_s + h * a.go_h;
-  const long long o = (((long long)b * a.sq + row) * a.h + h) * a.dv;
-  float s = 0.0f;
-  for (int n = lane * 4; n < a.dv; n += 256) {
-    vx_f32x4 y = vx_load4(a.out + o + n, a.dv - n);
-    if (sizeof(T) == 2 && a.rest) y += vx_load4(a.rest + o + n, a.dv - n);
-    const vx_f32x4 x = vx_load4(go + n, a.dv - n) * y;
-    s += (x[0] + x[1]) + (x[2] + x[3]);
-  }
+  for (long long r = (long long)(blockIdx.x - head) * 4 + (threadIdx.x >> 6); r < rows; r += (long long)(gridDim.x - head) * 4) {
+    const int bh = (int)(r / a.sq), row = (int)(r % a.sq), b = bh / a.h, h = bh % a.h;
+    const T* go = a.go + b * a.go_b + row * a.go_s + h * a.go_h;
+    const long long o = (((long long)b * a.sq + row) * a.h + h) * a.dv;
+    float s = 0.0f;
+    for (int n = lane * 4; n < a.dv; n += 256) {
+      vx_f32x4 y = vx_load4(a.out + o + n, a.dv - n);
+      if (sizeof(T) == 2 && a.rest) y += vx_load4(a.rest + o + n, a.dv - n);
+      const vx_f32x4 x = vx_load4(go + n, a.dv - n) * y;
+      s += (x[0] + x[1]) + (x[2] + x[3]);
+    }
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
-  if (lane == 0) a.delta[r] = s;
+    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
+    if (lane == 0) a.delta[r] = s;
+  }
 }
 
 constexpr int kPdsN = 128;                   // keys of an attn_pds tile
@@ -970,7 +970,7 @@ template <typename T>
 int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStream_t s) {
   const FwdPlan p = fwd_plan(sh, dtype);
   const int64_t bh = sh.b * sh.h, grid = p.tiles_q * p.splits * bh;
-  VX_REQUIRE(grid < (1LL << 31), "attn_fwd: too many tiles");
+  VX_REQUIRE(vx_launchable(grid, 512), "attn_fwd: too many tiles");      // (the largest workgroup has 512)
   a.tiles_q = (int)p.tiles_q;
   a.splits = (int)p.splits;
   a.span = (int)p.span;
@@ -984,7 +984,7 @@ int32_t fwd_impl(FwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
     const int c = class_of(sh.d, sh.dv), kd = kDims[c][0] / 32, nv = kDims[c][1] / 16, kt = AttnTile<T>::KT;
     const int64_t ks = sh.hk * p.tiles_k * (kt / 16) * kd * 64, all = ks + sh.hv * p.tiles_k * nv * (kt / 32) * 64;     // of a batch
     const int64_t per = vx_cdiv(all, 256);
-    VX_REQUIRE(per * sh.b < (1LL << 31), "attn_fwd: too many keys");
+    VX_REQUIRE(vx_launchable(per * sh.b, 256), "attn_fwd: too many keys");
     const bool own = a.mask && sh.sk <= kOwnKeys;
     LiveArgs live{};
     if (a.mask) {
@@ -1112,14 +1112,16 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
     gather.pieces_v = (int)vx_cdiv(sh.dv, P);
     gather.items_k = sh.hk * sh.sk * gather.pieces_k;
     gather.items = gather.items_k + sh.hv * sh.sk * gather.pieces_v;
-    VX_REQUIRE(vx_cdiv(gather.items, 256) * sh.b < (1LL << 31), "attn_bwd: too many keys");
+    VX_REQUIRE(vx_launchable(vx_cdiv(gather.items, 256) * sh.b, 256), "attn_bwd: too many keys");
     gather.per = (unsigned)vx_cdiv(gather.items, 256);
     head = own ? gather.per * sh.b : sh.b;
   }
-  VX_REQUIRE(vx_cdiv(rows, 4) + head < (1LL << 31), "attn_bwd: too many queries");
+  int64_t waves = vx_cdiv(sums, 4);
+  if (waves > 1 << 20) waves = 1 << 20;              // (a wave then has more than one row)
+  VX_REQUIRE(vx_launchable(waves + head, 256), "attn_bwd: too many keys");
   if (head + sums) {
     const auto delta = own ? attn_delta<T, true> : attn_delta<T, false>;
-    delta<<<(unsigned)(vx_cdiv(sums, 4) + head), 256, 0, s>>>(a, sums, live, gather, (unsigned)head);
+    delta<<<(unsigned)(waves + head), 256, 0, s>>>(a, sums, live, gather, (unsigned)head);
     VX_LAUNCH_CHECK();
   }
   if (a.mask) {
@@ -1143,7 +1145,7 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
     const int64_t nv = a.dvv ? here * bh * a.tk * a.tdv : 0, nk = a.dk ? here * bh * a.tk * a.td : 0;
     const int64_t nq = a.dq ? (int64_t)a.tq * a.td * bh : 0;
     const int64_t pds = (int64_t)a.tkp * vx_cdiv(a.rows, p.tp) * bh, grads = nv + nk + nq;
-    VX_REQUIRE(pds < (1LL << 31) && grads < (1LL << 31), "attn_bwd: too many tiles");
+    VX_REQUIRE(vx_launchable(pds, kTileThreads) && vx_launchable(grads, kTileThreads), "attn_bwd: too many tiles");
     a.n_v = (unsigned)nv;
     a.n_k = (unsigned)nk;
     a.n_q = (unsigned)nq;
@@ -1154,7 +1156,7 @@ int32_t bwd_impl(BwdArgs<T>& a, const Shape& sh, int32_t dtype, char* ws, hipStr
   }
   const int64_t iv = sh.b * sh.hv * sh.sk * vx_cdiv(sh.dv, 4), ik = sh.b * sh.hk * sh.sk * vx_cdiv(sh.d, 4);
   const int64_t gv = a.dvv ? vx_cdiv(iv, 256) : 0, gk = a.dk ? vx_cdiv(ik, 256) : 0;
-  VX_REQUIRE(gv + gk < (1LL << 31), "attn_bwd: too many keys");
+  VX_REQUIRE(vx_launchable(gv + gk, 256), "attn_bwd: too many keys");
   if (gv + gk == 0) return VX_OK;
   attn_slab_sum<T><<<(unsigned)(gv + gk), 256, 0, s>>>(a, (int)p.splits, (unsigned)gv, iv, ik);
   VX_LAUNCH_CHECK();

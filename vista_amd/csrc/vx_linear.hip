@@ -394,7 +394,7 @@ int32_t fwd_impl(const FwdArgs<T>& args, hipStream_t s) {
   const int64_t t = few ? 16 : use_big ? 128 : 64;
   a.tiles_n = (int)vx_cdiv(a.n, t);
   const int64_t grid = vx_cdiv(a.m, t) * a.tiles_n;
-  VX_REQUIRE(grid < (1LL << 31), "linear_fwd: too many rows");
+  VX_REQUIRE(vx_launchable(grid, kTileThreads), "linear_fwd: too many rows");
   const bool fast = vx_fast(a.x, a.ldx, a.k, sizeof(T)) && vx_fast(a.w, a.ldw, a.k, sizeof(T));
   const auto kernel = few ? (fast ? linear_few<T, true> : linear_few<T, false>)
                           : use_big ? (fast ? linear_fwd<T, 128, 128, true> : linear_fwd<T, 128, 128, false>)
@@ -422,7 +422,7 @@ int32_t launch_bwd(BwdArgs<T, G>& a, const BwdPlan& p, const ActArgs<T>& rows, i
   a.tiles_w = (int)(vx_cdiv(a.n, t) * a.tiles_wk);
   a.tiles_xk = a.tiles_wk;
   const int64_t bw = a.dw ? a.tiles_w * p.splits : 0, bx = a.dx ? vx_cdiv(a.m, t) * a.tiles_xk : 0;
-  VX_REQUIRE(bw + bx + sums < (1LL << 31), "linear_bwd: too many rows");
+  VX_REQUIRE(vx_launchable(bw + bx + sums, kTileThreads), "linear_bwd: too many rows");
   a.blocks_w = (unsigned)bw;
   a.blocks_x = (unsigned)bx;
   if (bw + bx + sums == 0) return VX_OK;
@@ -442,7 +442,7 @@ int32_t bwd_impl(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w,
   float* wide = wide_g(act, dtype) && (dx || dw) ? (float*)(ws + slab_bytes(p, n, k) + part_bytes(p, n)) : nullptr;
   const int64_t cols = vx_cdiv(n, p.lanes * (16 / (int64_t)sizeof(T)));
   const ActArgs<T> rows{dy, saved, dpre, wide, dbias ? part : nullptr, lddy, m, p.chunk, n, act, (int)p.lanes, (int)cols};
-  VX_REQUIRE(cols * p.chunks < (1LL << 31), "linear_bwd: too many rows");
+  VX_REQUIRE(vx_launchable(cols * p.chunks, 256), "linear_bwd: too many rows");
   if (act != VX_ACT_NONE) {
     act_bwd<T><<<(unsigned)(cols * p.chunks), 256, 0, s>>>(rows);
     VX_LAUNCH_CHECK();

@@ -544,5 +544,8 @@ __device__ __forceinline__ void vx_store8(__bf16* p, const vx_f32x4& a, const vx
   vx_store4(p + 4, b, n - 4);
 }
 
+// whether a launch of `blocks` workgroups of `threads` has fewer than the 2^32 work items that one may have
+static inline bool vx_launchable(int64_t blocks, int threads) { return blocks < (1LL << 32) / threads; }
+
 // compute units of the current device (cached per device; 256 if it cannot be asked)
 int vx_tile_cus();
