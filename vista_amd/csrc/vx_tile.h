@@ -511,8 +511,16 @@ __device__ __forceinline__ void vx_store4(__bf16* p, const vx_f32x4& v, int n) {
 }
 
 // eight neighbours, `n` of which exist; ONCE: past the caches, for what this launch does not read again
-template <bool ONCE, typename V, typename P>
-__device__ __forceinline__ void vx_put(const V& v, P* p) {
+// (one function a type: a template's parameter would take the vector without its element alignment)
+template <bool ONCE>
+__device__ __forceinline__ void vx_put(const vx_f32x4u& v, vx_f32x4u* p) {
+  if constexpr (ONCE)
+    __builtin_nontemporal_store(v, p);
+  else
+    *p = v;
+}
+template <bool ONCE>
+__device__ __forceinline__ void vx_put(const vx_u32x4u& v, vx_u32x4u* p) {
   if constexpr (ONCE)
     __builtin_nontemporal_store(v, p);
   else
