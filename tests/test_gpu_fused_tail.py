@@ -552,6 +552,59 @@ def test_same_inputs_same_bits(dev):
     assert all(torch.equal(i, j) for i, j in zip(a, b))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(1, 3, (1 << 21) + 9, 1, 1, 1, 8, 8), (70000, 2, 5, 2, 1, 2, 4, 6), (1, 2000, 2, 64, 16, 4, 8, 12)])
+def test_attention_of_extreme_shapes(shape, dtype, dev):
+    """Rows of scores longer than the fast loads' strides, more batches than 16 bits, many heads that share keys."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn(shape, dtype, dev, 41, "some", poison=True)
+    ref = attn_reference(q, k, v, km, do)
+    out, stats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    within(out, *ref["out"], "out")
+    for name, got in zip(("dq", "dk", "dv"), ops.attn_bwd(do, q, k, v, out, stats, km)):
+        within(got, *ref[name], name)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,k,n", [(5, 1 << 20, 9), (9, 8, 1 << 20), (300, 70000, 70)])
+def test_linear_of_extreme_shapes(m, k, n, dtype, dev):
+    from vista_amd import ops
+    x, w, b, r, dy = make_linear(m, k, n, dtype, dev, 42, True, True)
+    a = x.double() @ w.double().t() + b.double() + r.double()
+    size = x.double().abs() @ w.double().abs().t() + b.double().abs() + r.double().abs()
+    off = gamma(k, dtype) * size
+    within(ops.linear_fwd(x, w, b, r)[0], a, off + half_step(dtype) * (a.abs() + off), "y")
+    dx, dw, db, _ = ops.linear_bwd(dy, x, w)
+    for name, got, want, off in (("dx", dx, dy.double() @ w.double(), gamma(n, dtype) * (dy.double().abs() @ w.double().abs())),
+                                 ("dw", dw, dy.double().t() @ x.double(), gamma(m, dtype) * (dy.double().abs().t() @ x.double().abs())),
+                                 ("db", db, dy.double().sum(0), 2.0 ** -20 * dy.double().abs().sum(0))):
+        within(got, want, off + half_step(dtype) * (want.abs() + off) + 1e-38, name)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_broadcast_inputs(dtype, dev):
+    """One query for all batches, one key head and one value row for all: strides 0, and gradients summed over them by autograd."""
+    from vista_amd.fused_tail import attention
+    q, k, v, km, do = make_attn((3, 70, 150, 4, 2, 2, 24, 40), dtype, dev, 43, "some")
+    q1, k1, v1 = q[:1].clone(), k[:, :, :1].clone(), v[:, :1].clone()
+    views = lambda a, b, c: (a.expand_as(q), b.expand_as(k), c.expand_as(v))  # noqa: E731
+    leaves = [t.requires_grad_(True) for t in (q1, k1, v1)]
+    whole = [t.detach().contiguous().requires_grad_(True) for t in views(*leaves)]
+    one, two = attention(*views(*leaves), key_mask=km), attention(*whole, key_mask=km)
+    assert torch.equal(one, two)
+    got = torch.autograd.grad(one, leaves, do)
+    full = torch.autograd.grad(two, whole, do)
+    for g, f, dim in zip(got, full, (0, 2, 1)):
+        assert torch.equal(g, f.sum(dim, keepdim=True))
+    x = q.detach().requires_grad_(True)                     # the same tensor three times, differentiated twice
+    y = attention(x, x, x)
+    a = torch.autograd.grad(y, x, y.detach(), retain_graph=True)[0]
+    assert torch.equal(a, torch.autograd.grad(y, x, y.detach())[0])
+    parts = [t.detach().clone().requires_grad_(True) for t in (q, q, q)]
+    grads = torch.autograd.grad(attention(*parts), parts, y.detach())
+    within(a, sum(g.double() for g in grads), 4 * half_step(dtype) * sum(g.double().abs() for g in grads), "shared")
+
+
 # ------------------------------------------------------------------------------------------------ autograd, streams, graphs
 def test_gradients_against_differences(dev):
     """<gradient, direction> of attention and of a gelu layer against central differences of the float64 formulas: the
@@ -684,6 +737,42 @@ def test_captured_and_replayed(dev):
         want = [t.clone() for t in step()]
         for gr, held in graphs:
             gr.replay()
+        torch.cuda.synchronize()
+        for gr, held in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(held, want)), i
+
+
+def test_captured_and_replayed_bf16(dev):
+    """The same with the rest of the output behind the statistics and g of a smooth activation in the workspace; two graphs, two streams."""
+    from vista_amd import ops
+    q, k, v, km, do = make_attn((2, 330, 170, 2, 2, 1, 48, 97), BF16, dev, 1, "some")
+    x, w, b, r, dy = make_linear(700, 64, 96, BF16, dev, 2, True, True)
+
+    def step():
+        out, st = ops.attn_fwd(q, k, v, km, want_stats=True)
+        y, pre = ops.linear_fwd(x, w, b, r, "silu", want_pre=True)
+        return (out, *ops.attn_bwd(do, q, k, v, out, st, km), y, *ops.linear_bwd(dy, x, w, "silu", pre))
+
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs = []
+    for side in streams:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            held = step()
+        graphs.append((gr, held))
+    gen = torch.Generator(device=dev).manual_seed(79)
+    for i in range(4):
+        for t in (q, k, v, do, x, dy):
+            t.copy_(torch.randn(t.shape, generator=gen, device=dev))
+        want = [t.clone() for t in step()]
+        for side, (gr, held) in zip(streams, graphs):       # both at once
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                gr.replay()
         torch.cuda.synchronize()
         for gr, held in graphs:
             assert all(torch.equal(a, b) for a, b in zip(held, want)), i
