@@ -59,9 +59,10 @@ __device__ __forceinline__ void linear_finish(const FwdArgs<T>& a, long long m, 
 template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a) {
   constexpr int BK = TM <= 64 ? 64 : VxType<T>::BK;        // 64 against 32 of fp32: 6400 x 384 -> 384 21 against 24 us
-  // y of the small tiles goes past the caches: it would push out the rows of x that the next column tiles read. us past / through them:
-  // 64 x 64 6400 x 384 -> 384 17.4 / 18.2, bf16 60000 x 128 -> 512 24 / 35, 16896 x 384 -> 384 13.7 / 14.7; 128 x 128 204800 x 384 -> 512
-  // bf16 154 / 136, fp32 470 / 470
+  // y of the small tiles goes past the caches: it would push out the rows of x that the next column tiles read. Measured with the layer
+  // that reads y behind it (384 -> 512 -> 384, bf16; us of the pair, past / through): 64 x 64 tiles, 6400 rows 17.8 / 18.1, 16896 35.0 /
+  // 38.1 (128 -> 512 of 60000 rows alone 24 / 35); 128 x 128 tiles, 60000 rows 93.8 / 85.4, 204800 305 / 308 (alone 121 / 142: what the layer gains the next one loses). fp32:
+  // within 2 % either way, 6400 to 204800 rows
   constexpr bool ONCE = TM <= 64;
   __shared__ __attribute__((aligned(16))) char lds[vx_gemm_lds<T, TM, TN, BK>()];
   const unsigned t = vx_xcd_tile(blockIdx.x, gridDim.x);
