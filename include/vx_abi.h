@@ -351,7 +351,8 @@ int32_t vx_nms_bev(const float* d_boxes, int32_t num_boxes, float thresh, int32_
  * Dense layer with its epilogue, y = act(x w^T + bias + residual), and its backward pass: the 1x1 convolutions and
  * feed-forward layers of the cross-view attention block (det3d/models/necks/attention.py:36-41,77-84,127-146). The activation
  * comes after the residual, as in vx_spconv_fwd's epilogue. Every pointer but the workspace is of `dtype`
- * (VX_F32: exact three-plane split on the bf16 matrix pipe, as vx_spconv_* with six products; VX_BF16); accumulation fp32.
+ * (VX_F32: operands split exactly into three bf16 planes, six of the nine plane products on the bf16 matrix pipe, as
+ * vx_spconv_* with six products: what is left out of a product is below 2^-21 of it; VX_BF16); accumulation fp32.
  *
  * vx_linear_fwd  d_x [m][k] rows ldx apart, d_weight [n][k] rows ldw apart, d_bias [n] or NULL, d_residual [m][n] rows ldr
  *                apart or NULL -> d_y [m][n]; d_pre [m][n] or NULL receives the sum before the activation

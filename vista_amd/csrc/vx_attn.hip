@@ -72,8 +72,10 @@ __device__ __forceinline__ bool attn_key_live(int keys, const uint8_t* mask, int
 // A tile: V(t) travels under S(t), K(t + 1) under O += P V(t); each LDS image is rewritten only after the barrier behind its last
 // reader. IMG: both come as finished images (attn_pack) and go straight to LDS; else (few queries) through registers, where
 // they are split and V is transposed.
-// Two heads of 192 / 384, masked: 4 x 1600 x 480 fp32 46 us (200 workgroups, the matrix pipe and LDS reads in turn: 153 TFLOP/s over all
-// keys), 25600 x 1920 bf16 143 us (790), fp32 475 us (238); 8 heads of 48, 2 x 2037 x 2037 bf16 40 us, bound by the exponentials.
+// Two heads of 192 / 384, 65 % of the keys live: 4 x 1600 x 480 fp32 46 us (200 workgroups on 256 CUs; 100 TFLOP/s of the live keys; without
+// a mask 63 us, 113), 25600 x 1920 bf16 182 us (405; 143 us with P in one plane), fp32 467 us (158); 8 heads of 48, 2 x 2037 x 2037
+// bf16 47 us. No pipe is full: counters say matrix pipe, vector pipe and LDS busy 11, 8 and 6 of 48 us, 50, 52 and 23 of 182, 180, 74
+// and 92 of 491, 10, 21 and 8 of 48; waves wait 33 to 48 % of their cycles, at the two barriers a tile and for what the next one loads.
 template <typename T, int DP, int DVP, int RT, int QG, int CS, bool IMG, bool FAST>
 __global__ __launch_bounds__(64 * QG * CS, QG * CS == 8 ? 2 : DVP > 192 || (DVP > 64 && VxType<T>::NPL == 3) ? 1 : 2)
 void attn_fwd(const FwdArgs<T> a) {
@@ -617,9 +619,11 @@ __global__ __launch_bounds__(256) void attn_gather(const BwdArgs<T> a, const Gat
 }
 
 // delta = sum_n go * out per query, out with its rest: a row that one key dominates has dP of that key next to delta, and a bf16 out alone
-// would leave 3 times the gradients' own rounding (scores of 200 to 1000 keys with standard deviation 8). One wave per row. With a mask the first `head` workgroups make its lists; OWN (at most kOwnKeys keys):
+// would leave 3 times the gradients' own rounding (scores of 200 to 1000 keys with standard deviation 8). One wave per row, more rows a
+// wave past 2^22 of them. With a mask the first `head` workgroups make its lists; OWN (at most kOwnKeys keys):
 // they gather the keys as well, each with a list of its own, which saves a launch (a step of 4 x 1600 x 480, 2 heads of 192 / 384, fp32:
-// 187 -> 182 us). One read of go and out: 4 x 2 x 1600 x 384 fp32 39 MB 11 us with the gather, 2 x 25600 x 384 157 MB 28 us
+// 187 -> 182 us). One read of go and out (and rest): 4 x 2 x 1600 x 384 fp32 39 MB 11 us with the gather, 2 x 25600 x 384 157 MB 29 us,
+// bf16 118 MB 35 us
 template <typename T, bool OWN>
 __global__ __launch_bounds__(256) void attn_delta(const BwdArgs<T> a, long long rows, const LiveArgs live, const GatherArgs gather,
                                                   unsigned head) {
@@ -660,8 +664,9 @@ constexpr int kPdsN = 128;                   // keys of an attn_pds tile
 // Both go out in fp32: rounded to bf16 they would make the error of dq and dk 1.4 times that of their own rounding (3 x 777 x 301).
 // ONE: all keys are in the tile. delta is then the tile's own sum of P dP: over few keys the rounding of a bf16 output inside delta would
 // not average out (terms that nearly cancel): relative 2-norm of dq and dk over 16 keys 0.0020 so, 0.0017 their own rounding.
-// Bound by the split into planes and LDS reads in fp32: 4 x 2 x 1600 x 480, 192 / 384 57 us, 25600 x 1920 483 us; bf16 3 x 4 x 777 x 301,
-// 96 / 192 10.7 us, where 468 workgroups of 64 x 128 are two rounds.
+// 4 x 2 x 1600 x 480, 192 / 384, fp32 57 us, 25600 x 1920 487 us: matrix pipe 14 and 180 of it, vector pipe (split into planes) 13 and 162,
+// LDS 7 and 90, one after the other behind two barriers a step. bf16 25600 x 1920 209 us, of which the writes of P and dS (0.5 GB) are
+// half; 3 x 4 x 777 x 301, 96 / 192 12.0 us, where 468 workgroups of 64 x 128 are two rounds.
 template <typename T, int TM, int TN, bool FAST, bool ONE>
 __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) {
   constexpr int BK = TM <= 64 ? 64 : VxType<T>::BK;
@@ -740,8 +745,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_pds(const BwdArgs<T> a) 
 // the three gradients of a chunk in one launch: dV slabs = P^T go, dK slabs = dS^T q (reduction over the queries of a split),
 // dQ = dS k (reduction over the keys)
 // P and dS are fp32; beside bf16 operands they are two planes
-// 4 x 2 x 1600 x 480, 192 / 384 fp32 66 us, 25600 x 1920 565 us: as attn_pds; dV and dK read both operands along their rows, transposed
-// on the way to LDS. bf16 3 x 4 x 777 x 301, 96 / 192 11.2 us
+// 4 x 2 x 1600 x 480, 192 / 384 fp32 66 us, 25600 x 1920 567 us: as attn_pds (matrix pipe 15 and 240 of it, vector pipe 14 and 155, LDS 14
+// and 150, a third of that bank conflicts); dV and dK read both operands along their rows, transposed on the way to LDS. bf16 25600 x
+// 1920 265 us, 3 x 4 x 777 x 301, 96 / 192 15.6 us
 template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a) {
   constexpr int BK = VxType<T>::BK, PX = VxType<T>::NPL_F32;
@@ -795,7 +801,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void attn_grads(const BwdArgs<T> a
 }
 
 // dk, dv = sums of the slabs over a head's query heads and the splits, in that order; masked keys get zeros. One read of the slabs:
-// 4 x 480 keys of 2 x 192 and 384, 10.6 us
+// 4 x 480 keys of 2 x 192 and 384, 6.5 us
 template <typename T>
 __global__ __launch_bounds__(256) void attn_slab_sum(const BwdArgs<T> a, int splits, unsigned blocks_v, long long items_v,
                                                      long long items_k) {
@@ -905,14 +911,14 @@ FwdPlan fwd_plan(const Shape& s, int32_t dtype) {
   FwdPlan p;
   const int64_t cus = vx_tile_cus(), bh = s.b * s.h, kt = dtype == VX_F32 ? 32 : 64, tiles_k = vx_cdiv(s.sk, kt);
   // 128 queries a workgroup share a staged tile, 64 fill the CUs sooner. us of 64 / 128 at 1024 keys, 8 heads, n 128-query tiles:
-  // 192 / 384 wide, fp32: n = 128 125 / 180, 256 239 / 206, 2048 1887 / 1489; bf16: 50 / 64, 87 / 68, 633 / 480: a tile takes 1.45
-  // times as long, so whole rounds over the CUs decide. 64 / 64, fp32: 256 70 / 76, 512 104 / 101, 2048 358 / 317; bf16: 28 / 31,
-  // 38 / 37, 117 / 109: two workgroups of 64 fit a CU. 96 / 192 and 128 / 128, fp32: 128 loses everywhere (831 / 973, 746 / 845:
+  // 192 / 384 wide, fp32: n = 128 125 / 180, 256 239 / 206, 2048 1887 / 1489; bf16: 63 / 75, 107 / 88, 699 / 556: a tile takes 1.45
+  // times as long, so whole rounds over the CUs decide. 64 / 64, fp32: 256 70 / 76, 512 104 / 101, 2048 358 / 317; bf16: 29 / 33,
+  // 43 / 41, 138 / 128: two workgroups of 64 fit a CU. 96 / 192 and 128 / 128, fp32: 128 loses everywhere (831 / 973, 746 / 845:
   // one wave a SIMD) and is not built.
   const int64_t n128 = vx_cdiv(s.sq, 128) * bh, n64 = vx_cdiv(s.sq, 64) * bh;
   const int c = class_of(s.d, s.dv);
   // images pay from about five tiles of 64 queries on; us with / without, 480 and 4096 keys, 4 x 2 heads of 192 / 384 fp32: 64 queries
-  // 31 / 25, 58 / 42; 256 32 / 34, 93 / 92; 512 38 / 44, 145 / 164; 2 x 8 heads of 64 / 64 bf16: 64 13 / 10, 23 / 15; 512 16 / 14, 49 / 48
+  // 33 / 25, 60 / 42; 256 34 / 33, 98 / 92; 512 41 / 42, 152 / 165; 2 x 8 heads of 64 / 64 bf16: 64 14 / 11, 26 / 16; 512 18 / 15, 55 / 54
   p.img = vx_cdiv(s.sq, 64) > 4;
   if (!p.img)                // the form without images has 64 queries a workgroup, however many heads there are
     p.many = false;

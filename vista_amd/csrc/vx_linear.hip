@@ -2,7 +2,7 @@
 // feed-forward layers of the cross-view attention block: det3d/models/necks/attention.py:36-41, :77-84, :127-146).
 // The activation comes after the residual, as in the epilogue of the sparse convolutions.
 //
-// fp32 operands run as three exact bf16 planes (six products, fp32 accumulation), bf16 ones directly; both in the tiles of
+// fp32 operands run as three exact bf16 planes (six of the nine products, fp32 accumulation), bf16 ones directly; both in the tiles of
 // vx_tile.h. A reduction split over workgroups leaves fp32 slabs that one kernel adds in a fixed order: no atomics, bitwise
 // reproducible.
 #include <type_traits>
@@ -53,9 +53,10 @@ __device__ __forceinline__ void linear_finish(const FwdArgs<T>& a, long long m, 
   vx_store4(a.y + at, v, left);
 }
 
-// A workgroup owns TM x TN outputs. fp32 is bound by the six products' matrix time and their LDS reads: 6400 x 384 -> 384 17 us
-// (600 workgroups, 111 TFLOP/s), 204800 x 384 -> 512 470 (171); bf16 by staging through registers between the products: 136 us
-// (592 TFLOP/s, 2.7 TB/s).
+// A workgroup owns TM x TN outputs. fp32 6400 x 384 -> 384 18 us (600 workgroups, 2.3 rounds on 256 CUs, 105 TFLOP/s; counters: matrix
+// pipe and LDS 4.5 us each, vector pipe 6, the waves wait for loads and at the barriers of twelve steps), 204800 x 384 -> 512 495 us
+// (163); bf16 141 us (571 TFLOP/s, 2.6 TB/s; matrix pipe, vector pipe and LDS 32 us each, one after the other in six steps of
+// 64: staging through registers between the products).
 template <typename T, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void linear_fwd(const FwdArgs<T> a) {
   constexpr int BK = TM <= 64 ? 64 : VxType<T>::BK;        // 64 against 32 of fp32: 6400 x 384 -> 384 21 against 24 us
@@ -160,10 +161,9 @@ __global__ __launch_bounds__(kTileThreads) void linear_few(const FwdArgs<T> a) {
 // ---- backward -------------------------------------------------------------------------------------------------------
 // g = dy * act'(saved) (written where there is an activation) and the column sums of g per row chunk. wide: g unrounded for the two
 // products, where its rounding to bf16 is one (gelu, silu: it would make the error of dx and dw 1.4 times that of their own rounding;
-// relu's g is dy or 0). A lane owns 16 bytes of
-// columns, `lanes` (a power of two, at most a wave) lanes a row, so that a wave reads whole rows; a workgroup owns `lanes` x 16 bytes
+// relu's g is dy or 0). A lane owns 16 bytes of columns, `lanes` (a power of two, at most a wave) lanes a row, so that a wave reads whole rows; a workgroup owns `lanes` x 16 bytes
 // of columns and a chunk of rows. Sums in fp32 per thread, then over the workgroup's rows in order. One pass: 102399 x 512 bf16, two
-// reads and a write, 64 us (4.9 TB/s of the 5.1 that a copy reaches).
+// reads and a write, 64 us (4.9 TB/s of the 5.1 that a copy reaches); gelu, with g in fp32 as well, 112 us (4.7).
 template <typename T>
 struct ActArgs {
   const T *dy, *saved;
@@ -249,9 +249,10 @@ struct BwdArgs {
 };
 
 // one launch for the gradients: workgroups [0, blocks_w) are tiles of dw = g^T x (reduction over the rows, split), the next blocks_x
-// tiles of dx = g w (reduction over n), the others (no activation: g = dy) the column sums. 6400 x 512 -> 384 fp32 38 us (131 TFLOP/s),
-// 102399 x 384 -> 512 bf16 132 us (610): dw's operands are transposed on their way to LDS
-// G: the type of g, fp32 beside bf16 operands where act_bwd wrote it so (two planes)
+// tiles of dx = g w (reduction over n), the others (no activation: g = dy) the column sums. 6400 x 512 -> 384 fp32 39 us (129 TFLOP/s),
+// 102399 x 384 -> 512 bf16 129 us (624; LDS 44 us of it, a quarter of that bank conflicts, matrix pipe 32): dw's operands are transposed on
+// their way to LDS.
+// G: the type of g, fp32 beside bf16 operands where act_bwd wrote it so (two planes): 207 us
 template <typename T, typename G, int TM, int TN, bool FAST>
 __global__ __launch_bounds__(kTileThreads, 2) void linear_bwd(const BwdArgs<T, G> a, const ActArgs<T> sums) {
   constexpr int BK = VxType<T>::BK, PG = sizeof(G) == sizeof(T) ? VxType<T>::NPL : VxType<T>::NPL_F32;
