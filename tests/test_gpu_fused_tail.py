@@ -582,6 +582,54 @@ def test_linear_of_extreme_shapes(m, k, n, dtype, dev):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+def test_c_entries_without_the_rest(dtype, dev):
+    """vx_attn_fwd and vx_attn_bwd as they were: statistics of two floats a row, no rest; a workspace of the stated size and no more."""
+    import ctypes
+    from vista_amd import _lib, ops
+    lib, code = _lib.lib(), 0 if dtype == F32 else 1
+    shape = (2, 300, 170, 4, 2, 1, 40, 60)
+    q, k, v, km, do = make_attn(shape, dtype, dev, 44, "some")
+    want, wstats = ops.attn_fwd(q, k, v, km, want_stats=True)
+    ref = attn_reference(q, k, v, km, do)
+    i64 = lambda *s: (ctypes.c_int64 * len(s))(*s)  # noqa: E731
+    strides = i64(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], km.stride(0))
+    room = lambda n: torch.full((n + 256,), 255, dtype=torch.uint8, device=dev)  # noqa: E731
+    stream = torch.cuda.current_stream().cuda_stream
+    out, stats = torch.empty_like(want), torch.full((8 * 300 * 2 + 64,), 7.0, device=dev)
+    n = lib.vx_attn_fwd_workspace_bytes(i64(*shape), code)
+    ws = room(n)
+    assert lib.vx_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), km.data_ptr(), i64(*shape), strides, 40 ** -0.5, out.data_ptr(),
+                           stats.data_ptr(), code, ws.data_ptr(), n, stream) == 0
+    assert torch.equal(out, want) and torch.equal(stats[:4800], wstats.flatten()[:4800])
+    assert (stats[4800:] == 7.0).all() and (ws[n:] == 255).all()
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    n = lib.vx_attn_bwd_workspace_bytes(i64(*shape), code)
+    ws = room(n)
+    assert lib.vx_attn_bwd(do.data_ptr(), i64(*do.stride()[:3]), q.data_ptr(), k.data_ptr(), v.data_ptr(), km.data_ptr(), i64(*shape), strides,
+                           out.data_ptr(), stats.data_ptr(), 40 ** -0.5, *(g.data_ptr() for g in grads), code, ws.data_ptr(), n, stream) == 0
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        within(got, *ref[name], name)
+    assert (ws[n:] == 255).all()
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layer_gradients_stay_in_their_workspace(dtype, act, dev):
+    from vista_amd import _lib, ops
+    lib, code = _lib.lib(), 0 if dtype == F32 else 1
+    m, k, n = 1001, 70, 90
+    x, w, _, s, dy = make_linear(m, k, n, dtype, dev, 45, False, True)
+    want = ops.linear_bwd(dy, x, w, act, s)
+    size = lib.vx_linear_bwd_act_workspace_bytes(m, n, k, _lib.VX_ACT[act], code)
+    ws = torch.full((size + 256,), 255, dtype=torch.uint8, device=dev)
+    dx, dw, db, dpre = (torch.empty_like(t) for t in (x, w, want[2], dy))
+    assert lib.vx_linear_bwd(dy.data_ptr(), n, x.data_ptr(), k, w.data_ptr(), k, s.data_ptr(), m, n, k, _lib.VX_ACT[act], dpre.data_ptr(),
+                             dx.data_ptr(), dw.data_ptr(), db.data_ptr(), code, ws.data_ptr(), size,
+                             torch.cuda.current_stream().cuda_stream) == 0
+    assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), want)) and (ws[size:] == 255).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_broadcast_inputs(dtype, dev):
     """One query for all batches, one key head and one value row for all: strides 0, and gradients summed over them by autograd."""
     from vista_amd.fused_tail import attention
